@@ -32,6 +32,10 @@ DTYPE_SIZE = {0: 1, 1: 2, 2: 4, 3: 2, 4: 4, 5: 8, 6: 8, 7: 1, 8: 2, 9: 4, 10: 8,
 COLL_ALLREDUCE, COLL_REDUCESCATTER, COLL_ALLGATHER, COLL_ALLTOALLV, COLL_BROADCAST, COLL_REDUCE, COLL_SCATTER = range(7)
 ALGO_RING, ALGO_MESH, ALGO_RHD, ALGO_PAIRWISE = range(4)
 
+HCCL_DATA_TYPE_FP8E4M3 = 14          # 8-bit rows of the experts' operators; refused by every collective
+# HcclAmdScaleType (include/hccl/hccl_amd_experts.h)
+HCCL_AMD_SCALE_NONE, HCCL_AMD_SCALE_FP32, HCCL_AMD_SCALE_E8M0 = 0, 1, 2
+
 # Every symbol include/hccl/hccl.h and include/hccl/hccl_amd_ext.h declare.
 EXPORTS = [
     "HcclAllReduce", "HcclReduceScatter", "HcclAllGather", "HcclAlltoAllV", "HcclAlltoAll", "HcclAlltoAllVC", "HcclReduceScatterV",
@@ -42,6 +46,11 @@ EXPORTS = [
     "HcclCommInitRootInfoConfig", "HcclBroadcast", "HcclScatter", "HcclSend", "HcclRecv", "HcclReduce",
     "HcclBatchSendRecv", "HcclCommSetMemoryRange", "HcclCommUnsetMemoryRange", "HcclCommActivateCommMemory",
     "HcclCommDeactivateCommMemory", "HcclAmdSetParam", "HcclAmdGetLastOpInfo", "HcclAmdGetLastOpForm", "HcclAmdDescribePlan", "HcclAmdReduceScatterNoAlloc",
+]
+# Every symbol include/hccl/hccl_amd_experts.h declares.
+EXPERT_EXPORTS = [
+    "HcclAmdExpertRouteWorkspace", "HcclAmdExpertRoute", "HcclAmdExpertRouteGrad", "HcclAmdExpertPack", "HcclAmdExpertCombine",
+    "HcclAmdExpertCombineGrad", "HcclAmdBlockQuantWeights", "HcclAmdBlockQuantColumns", "HcclAmdBlockMatmul", "HcclAmdBlockMatmulGradWeight",
 ]
 
 
@@ -192,6 +201,17 @@ def lib():
     L.HcclAmdGetLastOpForm.argtypes = [vp, ctypes.POINTER(ctypes.c_int32)]
     L.HcclAmdDescribePlan.argtypes = [i32, i32, u32, u64, i32, u64, u64, u64, ctypes.POINTER(u64), ctypes.c_char_p,
                                       ctypes.c_size_t, ctypes.POINTER(ctypes.c_size_t)]
+    f32 = ctypes.c_float
+    L.HcclAmdExpertRouteWorkspace.argtypes = [u64, u32, ctypes.POINTER(u64)]
+    L.HcclAmdExpertRoute.argtypes = [vp, i32, u64, u32, u64, u32, u32, vp, f32, vp, vp, vp, vp, vp, vp, vp, u64, vp]
+    L.HcclAmdExpertRouteGrad.argtypes = [vp, i32, u64, u32, u64, u32, u32, vp, f32, vp, vp, vp, vp, vp, u64, vp]
+    L.HcclAmdExpertPack.argtypes = [vp, i32, u64, u64, u64, u32, vp, i32, vp, u64, u64, vp, u64, vp]
+    L.HcclAmdExpertCombine.argtypes = [vp, i32, u64, u64, u64, u64, u32, vp, vp, vp, u64, vp]
+    L.HcclAmdExpertCombineGrad.argtypes = [vp, u64, vp, i32, u64, u64, u64, u64, u32, vp, vp, vp, u64, vp, vp]
+    L.HcclAmdBlockQuantWeights.argtypes = [vp, i32, u32, u64, u64, u64, i32, vp, vp, vp, vp, vp]
+    L.HcclAmdBlockQuantColumns.argtypes = [vp, i32, u64, u64, u64, u32, vp, i32, vp, u64, vp, vp]
+    L.HcclAmdBlockMatmul.argtypes = [vp, u64, vp, u64, u64, u32, vp, vp, vp, vp, u32, u64, u64, i32, vp, i32, u64, vp]
+    L.HcclAmdBlockMatmulGradWeight.argtypes = [vp, vp, vp, vp, u64, u64, u64, u64, i32, u32, vp, vp, u32, vp, i32, u32, vp]
     _call = _native_call(L) or _through_ctypes
     _lib = L
     return L
@@ -453,3 +473,72 @@ def describe_plan(coll, algo, p, count, dtype, ccl_bytes=200 << 20, align=128, i
             continue
         _check("HcclAmdDescribePlan", rc)
         return json.loads(buf.value.decode())
+
+
+# ---- operators around the all-to-all-v (include/hccl/hccl_amd_experts.h); strides 0: rows without a gap -----------------
+
+def expert_route_workspace(tokens, experts):
+    """Bytes of device workspace expert_route needs."""
+    need = ctypes.c_uint64()
+    _check("HcclAmdExpertRouteWorkspace", lib().HcclAmdExpertRouteWorkspace(tokens, experts, ctypes.byref(need)))
+    return need.value
+
+
+def expert_route(logits, dtype, tokens, experts, topk, expert_of, weights, row_of, counts, offsets, loss, workspace, workspace_bytes, stream,
+                 renorm=False, mask=None, loss_scale=1.0, stride=0):
+    """The topk experts of every token, their weights, rows in expert order, per-expert counts and the balance loss."""
+    _check("HcclAmdExpertRoute", lib().HcclAmdExpertRoute(logits, dtype, tokens, experts, stride, topk, 1 if renorm else 0, mask, loss_scale, expert_of,
+                                                          weights, row_of, counts, offsets, loss, workspace, workspace_bytes, stream))
+
+
+def expert_route_grad(logits, dtype, tokens, experts, topk, expert_of, counts, weight_grad, loss_grad, logit_grad, stream, renorm=False, mask=None,
+                      loss_scale=1.0, stride=0, grad_stride=0):
+    _check("HcclAmdExpertRouteGrad", lib().HcclAmdExpertRouteGrad(logits, dtype, tokens, experts, stride, topk, 1 if renorm else 0, mask, loss_scale,
+                                                                  expert_of, counts, weight_grad, loss_grad, logit_grad, grad_stride, stream))
+
+
+def expert_pack(x, dtype, tokens, width, topk, row_of, out, rows, stream, scales=None, scale_type=HCCL_AMD_SCALE_NONE, x_stride=0, out_stride=0,
+                scale_stride=0):
+    """Tokens into expert order: copied, or (scale_type) as 8-bit rows with a scale per 128 values."""
+    _check("HcclAmdExpertPack", lib().HcclAmdExpertPack(x, dtype, tokens, width, x_stride, topk, row_of, scale_type, out, rows, out_stride, scales,
+                                                        scale_stride, stream))
+
+
+def expert_combine(x, dtype, rows, width, tokens, topk, row_of, weights, y, stream, x_stride=0, y_stride=0):
+    """Rows back to their tokens, weighted and summed (weights None: the gradient of expert_pack)."""
+    _check("HcclAmdExpertCombine", lib().HcclAmdExpertCombine(x, dtype, rows, width, x_stride, tokens, topk, row_of, weights, y, y_stride, stream))
+
+
+def expert_combine_grad(y_grad, x, dtype, rows, width, tokens, topk, row_of, weights, x_grad, weight_grad, stream, y_grad_stride=0, x_stride=0,
+                        x_grad_stride=0):
+    _check("HcclAmdExpertCombineGrad", lib().HcclAmdExpertCombineGrad(y_grad, y_grad_stride, x, dtype, rows, width, x_stride, tokens, topk, row_of,
+                                                                      weights, x_grad, x_grad_stride, weight_grad, stream))
+
+
+def block_quant_weights(w, dtype, experts, n, k, scale_type, q, scales, q_t, scales_t, stream, stride=0):
+    """Weights in 8 bits with a scale per 128 x 128, as they are and / or transposed."""
+    _check("HcclAmdBlockQuantWeights", lib().HcclAmdBlockQuantWeights(w, dtype, experts, n, k, stride, scale_type, q, scales, q_t, scales_t, stream))
+
+
+def block_columns(rows, groups):
+    """Columns that hold any `groups` groups of `rows` rows in all, each padded to a multiple of 128."""
+    return (rows // 128 + groups) * 128
+
+
+def block_quant_columns(x, dtype, rows, width, groups, offsets, scale_type, q_t, columns, scales, stream, stride=0):
+    _check("HcclAmdBlockQuantColumns", lib().HcclAmdBlockQuantColumns(x, dtype, rows, width, stride, groups, offsets, scale_type, q_t, columns, scales,
+                                                                      stream))
+
+
+def block_matmul(a, a_scales, rows, w, w_scales, experts, n, k, scale_type, y, y_dtype, stream, groups=1, offsets=None, expert_of_group=None,
+                 a_stride=0, a_scale_stride=0, y_stride=0):
+    """8-bit rows, group by group, times their experts' 8-bit weights."""
+    _check("HcclAmdBlockMatmul", lib().HcclAmdBlockMatmul(a, a_stride, a_scales, a_scale_stride, rows, groups, offsets, expert_of_group, w, w_scales,
+                                                          experts, n, k, scale_type, y, y_dtype, y_stride, stream))
+
+
+def block_matmul_grad_weight(y_grad_t, y_grad_scales, x_t, x_scales, columns, rows, n, k, scale_type, groups, offsets, experts, w_grad, grad_dtype,
+                             stream, expert_of_group=None, accumulate=False):
+    _check("HcclAmdBlockMatmulGradWeight", lib().HcclAmdBlockMatmulGradWeight(y_grad_t, y_grad_scales, x_t, x_scales, columns, rows, n, k, scale_type,
+                                                                              groups, offsets, expert_of_group, experts, w_grad, grad_dtype,
+                                                                              1 if accumulate else 0, stream))

@@ -27,6 +27,9 @@ COMMON = ["-O3", "-std=c++17", "-fPIC", "-ffp-contract=off", "-I", os.path.join(
 DEVICE = ["--offload-arch=gfx950", "-Xclang", "-target-feature", "-Xclang", "-packed-fp32-ops"]
 DTYPES = list(range(12)) + [255]
 DEVICE_SOURCES = ["noalloc.hip"]
+# the operators around the all-to-all-v: a directory of their own, with headers that nothing else reads
+EXPERT_SOURCES = ["route.hip", "exchange.hip", "quant.hip", "product.hip"]
+EXPERT_HEADER = "hccl_amd_experts.h"
 HOST_SOURCES = ["plan.cc", "plan_schedules.cc", "plan_lower.cc", "plan_fuse.cc", "plan_template.cc", "ranktable.cc", "exec.cc", "direct.cc", "a2av.cc", "api.cc", "api_rendezvous.cc", "api_comm.cc", "api_ext.cc", "kernels_table.cc"]
 
 
@@ -49,7 +52,11 @@ def build(force=False, jobs=None):
     os.makedirs(OBJ, exist_ok=True)
     os.makedirs(LIBDIR, exist_ok=True)
     headers = [os.path.join(CSRC, f) for f in os.listdir(CSRC) if f.endswith(".h")]
-    headers += [os.path.join(ROOT, "include", "hccl", f) for f in os.listdir(os.path.join(ROOT, "include", "hccl"))]
+    public = os.path.join(ROOT, "include", "hccl")
+    headers += [os.path.join(public, f) for f in os.listdir(public) if f != EXPERT_HEADER]
+    experts = os.path.join(CSRC, "experts")
+    expert_headers = [os.path.join(experts, f) for f in os.listdir(experts) if f.endswith(".h")]
+    expert_headers += [os.path.join(public, EXPERT_HEADER), os.path.join(public, "hccl_types.h"), os.path.join(CSRC, "log.h")]
     jobs = jobs or min(8, os.cpu_count() or 4)
     tasks, objs = [], []
     for dt in DTYPES:
@@ -63,6 +70,12 @@ def build(force=False, jobs=None):
         objs.append(obj)
         src = os.path.join(CSRC, name)
         if force or _newer(obj, [src] + headers):
+            tasks.append([HIPCC] + COMMON + DEVICE + ["-c", src, "-o", obj])
+    for name in EXPERT_SOURCES:
+        obj = os.path.join(OBJ, "experts_" + name.replace(".hip", ".o"))
+        objs.append(obj)
+        src = os.path.join(experts, name)
+        if force or _newer(obj, [src] + expert_headers):
             tasks.append([HIPCC] + COMMON + DEVICE + ["-c", src, "-o", obj])
     for name in HOST_SOURCES:
         obj = os.path.join(OBJ, name.replace(".cc", ".o"))

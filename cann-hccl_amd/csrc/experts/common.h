@@ -1,0 +1,222 @@
+// What the operators of an expert-parallel layer share: checks of arguments, element types, 8-bit blocks, the way from a
+// workgroup's number to its group of rows.
+#pragma once
+#include <hip/hip_runtime.h>
+
+#include <cstdint>
+
+#include "hccl/hccl_amd_experts.h"
+#include "log.h"
+
+namespace hcclamd {
+namespace experts {
+
+#define EXPERTS_CHK_PTR(p)                                      \
+    do {                                                        \
+        if ((p) == nullptr) {                                   \
+            HCCL_LOG_ERROR("%s: %s is null", __func__, #p);     \
+            return HCCL_E_PTR;                                  \
+        }                                                       \
+    } while (0)
+
+#define EXPERTS_CHK(cond)                                       \
+    do {                                                        \
+        if (!(cond)) {                                          \
+            HCCL_LOG_ERROR("%s: needs %s", __func__, #cond);    \
+            return HCCL_E_PARA;                                 \
+        }                                                       \
+    } while (0)
+
+#define EXPERTS_CHK_TYPE(cond)                                          \
+    do {                                                                \
+        if (!(cond)) {                                                  \
+            HCCL_LOG_ERROR("%s: type not supported", __func__);         \
+            return HCCL_E_NOT_SUPPORT;                                  \
+        }                                                               \
+    } while (0)
+
+constexpr uint64_t kMaxSize = (uint64_t(1) << 31) - 1;    // tokens, rows, widths; products of them are held in 64 bits
+constexpr uint64_t kMaxGroupedRows = uint64_t(1) << 28;   // rows that are cut into units group by group (FindUnit)
+
+inline uint64_t Up128(uint64_t n) { return (n + 127) / 128 * 128; }
+inline uint64_t Blocks(uint64_t n) { return (n + 127) / 128; }
+inline bool Float(HcclDataType t) { return t == HCCL_DATA_TYPE_FP32 || t == HCCL_DATA_TYPE_FP16 || t == HCCL_DATA_TYPE_BFP16; }
+inline uint64_t SizeOf(HcclDataType t) { return t == HCCL_DATA_TYPE_FP32 ? 4 : 2; }
+inline bool Scaled(HcclAmdScaleType s) { return s == HCCL_AMD_SCALE_FP32 || s == HCCL_AMD_SCALE_E8M0; }
+inline bool Aligned(const void *p, uint64_t to) { return reinterpret_cast<uintptr_t>(p) % to == 0; }
+inline bool AlignedTo(HcclDataType t, const void *p) { return Aligned(p, SizeOf(t)); }
+inline bool ScaleAligned(HcclAmdScaleType s, const void *p) { return s != HCCL_AMD_SCALE_FP32 || Aligned(p, 4); }
+
+inline HcclResult Launched(const char *fn)
+{
+    const hipError_t e = hipGetLastError();
+    if (e == hipSuccess) {
+        return HCCL_SUCCESS;
+    }
+    HCCL_LOG_ERROR("%s: %s", fn, hipGetErrorString(e));
+    return HCCL_E_RUNTIME;
+}
+
+// ---- element types ---------------------------------------------------------------------------------------
+
+typedef float Float4 __attribute__((ext_vector_type(4)));
+typedef int32_t Int4 __attribute__((ext_vector_type(4)));
+typedef int32_t Int8 __attribute__((ext_vector_type(8)));
+typedef uint32_t Word2 __attribute__((ext_vector_type(2)));
+typedef uint32_t Word4 __attribute__((ext_vector_type(4)));
+
+// N consecutive elements from p; kWide: p is aligned to 16 bytes (or to all of them, if they are fewer).
+template <bool kWide, int N, typename T>
+__device__ __forceinline__ void Load(const T *p, float (&v)[N])
+{
+    if constexpr (kWide) {
+        typedef T Vec __attribute__((ext_vector_type(N), aligned(N * sizeof(T) < 16 ? N * sizeof(T) : 16)));
+        const Vec x = *reinterpret_cast<const Vec *>(p);
+#pragma unroll
+        for (int i = 0; i < N; i++) {
+            v[i] = float(x[i]);
+        }
+    } else {
+#pragma unroll
+        for (int i = 0; i < N; i++) {
+            v[i] = float(p[i]);
+        }
+    }
+}
+
+template <bool kWide, int N, typename T>
+__device__ __forceinline__ void Store(T *p, const float (&v)[N])
+{
+    if constexpr (kWide) {
+        typedef T Vec __attribute__((ext_vector_type(N), aligned(N * sizeof(T) < 16 ? N * sizeof(T) : 16)));
+        Vec x;
+#pragma unroll
+        for (int i = 0; i < N; i++) {
+            x[i] = T(v[i]);
+        }
+        *reinterpret_cast<Vec *>(p) = x;
+    } else {
+#pragma unroll
+        for (int i = 0; i < N; i++) {
+            p[i] = T(v[i]);
+        }
+    }
+}
+
+// ---- 8-bit blocks --------------------------------------------------------------------------------------------
+
+constexpr float kLeastMax = 0x1p-96f;
+constexpr float kLargest = 448.0f;
+
+// A value's part in its block's maximum: infinities and NaN have none.
+__device__ __forceinline__ float FiniteSize(float v)
+{
+    const float a = __builtin_fabsf(v);
+    return a < __builtin_inff() ? a : 0.0f;
+}
+
+// What a block's values are multiplied by, from its maximum, and its scale as it is stored.
+template <HcclAmdScaleType kScale>
+struct BlockScale;
+
+template <>
+struct BlockScale<HCCL_AMD_SCALE_FP32> {
+    typedef float Stored;
+    float times;
+    float stored;
+    __device__ __forceinline__ explicit BlockScale(float top)
+    {
+        top = top > kLeastMax ? top : kLeastMax;
+        times = kLargest / top;
+        stored = top / kLargest;
+    }
+};
+
+template <>
+struct BlockScale<HCCL_AMD_SCALE_E8M0> {
+    typedef uint8_t Stored;
+    float times;
+    uint8_t stored;
+    __device__ __forceinline__ explicit BlockScale(float top)
+    {
+        top = top > kLeastMax ? top : kLeastMax;
+        // top = m * 2^p with m in [1, 2): 448 = 1.75 * 2^8, so the power is p - 8, one more where m > 1.75; the comparison
+        // of the mantissa's bits rounds up by a carry
+        const uint32_t bits = __float_as_uint(top) + 0x1fffffu;
+        const int power = int(bits >> 23) - 127 - 8;
+        times = __uint_as_float(uint32_t(127 - power) << 23);
+        stored = uint8_t(power + 127);
+    }
+};
+
+// Four values as four 8-bit ones, lowest byte first.  A scaled value is at most 448 * (1 + 2^-22), which rounds to 448.
+__device__ __forceinline__ uint32_t Quantise4(float a, float b, float c, float d)
+{
+    int w = __builtin_amdgcn_cvt_pk_fp8_f32(a, b, 0, false);
+    w = __builtin_amdgcn_cvt_pk_fp8_f32(c, d, w, true);
+    return uint32_t(w);
+}
+
+// Infinities must become NaN whatever the conversion's overflow mode does, and so must their product with `times`.
+__device__ __forceinline__ float Scaled8(float v, float times)
+{
+    return __builtin_fabsf(v) < __builtin_inff() ? v * times : __builtin_nanf("");
+}
+
+// ---- groups of rows ----------------------------------------------------------------------------------------
+
+// The rows [first, last) of unit `unit` of `per` rows: groups are cut into units one after the other, the last of a group
+// may be shorter.  `before`: how many units lie in front of the group's.
+struct Unit {
+    int group;        // -1: there is no such unit
+    int first, last;  // rows
+    int groupFirst, groupLast;
+    int before;
+};
+
+// Called by all 64 lanes of a wave.  Offsets that are not ascending or not within [0, rows] are brought there, so that
+// whatever they hold no row outside is named.  per >= 16, rows <= 2^28.
+__device__ __forceinline__ Unit FindUnit(const int32_t *__restrict__ offsets, int groups, int rows, int unit, int per)
+{
+    if (offsets == nullptr) {
+        const int64_t first = int64_t(unit) * per;
+        Unit u{first < rows ? 0 : -1, int(first), 0, 0, rows, 0};
+        u.last = rows - first < per ? rows : int(first + per);
+        return u;
+    }
+    const int lane = int(__lane_id());
+    int64_t before = 0;   // (64 groups of at most 2^24 units fit 32 bits, all groups do not where their rows overlap)
+    for (int g0 = 0; g0 < groups; g0 += 64) {
+        const int g = g0 + lane;
+        int lo = 0, hi = 0;
+        if (g < groups) {
+            lo = min(max(offsets[g], 0), rows);
+            hi = min(max(offsets[g + 1], lo), rows);
+        }
+        const int mine = (hi - lo + per - 1) / per;
+        int sum = mine;   // inclusive prefix over the lanes
+#pragma unroll
+        for (int d = 1; d < 64; d <<= 1) {
+            const int other = __shfl_up(sum, d, 64);
+            sum += lane >= d ? other : 0;
+        }
+        const int64_t start = before + sum - mine;
+        const unsigned long long has = __ballot(unit >= start && unit < start + mine);
+        if (has != 0) {
+            const int at = __ffsll(has) - 1;
+            Unit u;
+            u.group = g0 + at;
+            u.groupFirst = __shfl(lo, at, 64);
+            u.groupLast = __shfl(hi, at, 64);
+            u.before = int(before) + __shfl(sum - mine, at, 64);
+            u.first = u.groupFirst + (unit - u.before) * per;
+            u.last = min(u.first + per, u.groupLast);
+            return u;
+        }
+        before += __shfl(sum, 63, 64);
+    }
+    return Unit{-1, 0, 0, 0, 0, 0};
+}
+
+}  // namespace experts
+}  // namespace hcclamd

@@ -1,0 +1,395 @@
+// Products of 8-bit operands with a scale for each block of 128: HcclAmdBlockMatmul and HcclAmdBlockMatmulGradWeight.
+//
+//   y[r][c] = sum over blocks b of ra[r][b] * ca[c][b] * sum over the 128 values of b of rows[r][.] * cols[c][.]
+//
+// rows: a group's rows, or the output gradient's columns; cols: an expert's weights, or the columns of the experts' inputs.  The
+// matrix instruction takes 16 x 16 x 128: one block of 128 to an instruction.  Its first operand is `cols`, so that a lane
+// holds four neighbouring values of one row of the result.  Scales that are powers of two go into the instruction itself;
+// 32-bit ones multiply its result, which is then added in 32 bits.
+#include <type_traits>
+
+#include "common.h"
+
+namespace hcclamd {
+namespace experts {
+namespace {
+
+constexpr int kThreads = 256;
+constexpr int kWaves = kThreads / 64;
+
+struct ProductArgs {
+    const uint8_t *rows, *cols;
+    const void *rowScales, *colScales;
+    const int32_t *offsets;
+    const int32_t *expertOfGroup;
+    void *out;
+    int64_t rowPitch, colPitch, outPitch;   // bytes, bytes, elements
+    int64_t rowScalePitch;                  // matmul: scales from one row to the next
+    int numRows;                            // matmul: rows of all groups; gradient: n
+    int numCols;                            // matmul: n; gradient: k
+    int blocks;                             // matmul: blocks of 128 along k
+    int groups, experts;
+    int groupedRows;                        // gradient: rows of all groups
+    int colTiles;
+    bool accumulate;
+};
+
+// The 8-bit matrix instructions keep fewer than 32 bits inside: on blocks of normally distributed values their results are
+// 1.3e-5 off (2-norm), those of the 16-bit ones 1.5e-8.  8-bit values fit 16-bit ones exactly, and so does their product with a
+// power of two; converting costs an instruction per two values and halves the rate (2.2 for 4.4 PFLOP/s).
+typedef __bf16 Half8 __attribute__((ext_vector_type(8)));
+
+struct Wide32 {     // a lane's 32 values of a block
+    Half8 v[4];
+};
+
+__device__ __forceinline__ Wide32 Widen(const Int8 &x, float scale)
+{
+    Wide32 w;
+#pragma unroll
+    for (int i = 0; i < 8; i++) {
+        const auto lo = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(uint32_t(x[i]), scale, false);
+        const auto hi = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(uint32_t(x[i]), scale, true);
+        w.v[i / 2][i % 2 * 4 + 0] = lo[0];
+        w.v[i / 2][i % 2 * 4 + 1] = lo[1];
+        w.v[i / 2][i % 2 * 4 + 2] = hi[0];
+        w.v[i / 2][i % 2 * 4 + 3] = hi[1];
+    }
+    return w;
+}
+
+__device__ __forceinline__ Float4 MfmaWide(const Wide32 &cols, const Wide32 &rows, Float4 sum)
+{
+#pragma unroll
+    for (int i = 0; i < 4; i++) {
+        sum = __builtin_amdgcn_mfma_f32_16x16x32_bf16(cols.v[i], rows.v[i], sum, 0, 0, 0);
+    }
+    return sum;
+}
+
+__device__ __forceinline__ float PowerOf(uint8_t scale) { return __uint_as_float(scale == 0 ? 0x400000u : uint32_t(scale) << 23); }
+
+// What values are multiplied by as they are widened, and what is left for their sum.
+__device__ __forceinline__ float Inside(uint8_t scale) { return PowerOf(scale); }
+__device__ __forceinline__ float Inside(float) { return 1.0f; }
+
+// A lane's 32 of the 128 bytes of a block: those at 16 * (lane / 16) and 64 behind.  Which of a block's values meet in which
+// lane does not matter, as long as both operands are cut alike.
+__device__ __forceinline__ Int8 LoadLane(const uint8_t *p)
+{
+    const Int4 lo = *reinterpret_cast<const Int4 *>(p), hi = *reinterpret_cast<const Int4 *>(p + 64);
+    return Int8{lo.x, lo.y, lo.z, lo.w, hi.x, hi.y, hi.z, hi.w};
+}
+
+__device__ __forceinline__ Float4 Zero4() { return Float4{0.0f, 0.0f, 0.0f, 0.0f}; }
+
+template <typename T>
+__device__ __forceinline__ void StoreFour(T *out, const float (&v)[4], int col, int numCols, bool accumulate)
+{
+#pragma unroll
+    for (int i = 0; i < 4; i++) {
+        if (col + i < numCols) {
+            out[col + i] = T(accumulate ? float(out[col + i]) + v[i] : v[i]);
+        }
+    }
+}
+
+// 16 rows by 64 columns of the result to a workgroup, whose waves take every fourth block and add up through LDS: for few
+// rows, where the weights' bytes are what takes time and every wave should be reading them.
+template <typename T, HcclAmdScaleType kScale>
+__global__ void __launch_bounds__(kThreads) FewRowsKernel(ProductArgs a)
+{
+    constexpr bool kPowers = kScale == HCCL_AMD_SCALE_E8M0;
+    typedef typename BlockScale<kScale>::Stored Stored;
+    __shared__ Float4 part[kWaves][4][64];
+    const int unit = int(blockIdx.x) / a.colTiles, col0 = int(blockIdx.x) % a.colTiles * 64;
+    const Unit u = FindUnit(a.offsets, a.groups, a.numRows, unit, 16);
+    if (u.group < 0) {
+        return;
+    }
+    const int expert = a.expertOfGroup == nullptr ? u.group : a.expertOfGroup[u.group];
+    if (expert < 0 || expert >= a.experts) {
+        return;
+    }
+    const int lane = int(threadIdx.x) % 64, wave = int(threadIdx.x) / 64, l16 = lane % 16, piece = lane / 16 * 16;
+    const int64_t row = min(u.first + l16, u.last - 1);
+    const uint8_t *rows = a.rows + row * a.rowPitch + piece;
+    const Stored *rowScales = static_cast<const Stored *>(a.rowScales) + row * a.rowScalePitch;
+    // (a tile of 64 columns lies within one block of 128 of the weights' scales)
+    const Stored *colScales = static_cast<const Stored *>(a.colScales) + (int64_t(expert) * ((a.numCols + 127) / 128) + col0 / 128) * a.blocks;
+    const uint8_t *cols[4];
+    Float4 sum[4];
+#pragma unroll
+    for (int f = 0; f < 4; f++) {
+        const int col = min(col0 + f * 16 + l16, a.numCols - 1);
+        cols[f] = a.cols + (int64_t(expert) * a.numCols + col) * a.colPitch + piece;
+        sum[f] = Zero4();
+    }
+    for (int b = wave; b < a.blocks; b += kWaves) {
+        const Int8 x = LoadLane(rows + int64_t(b) * 128);
+        Int8 w[4];
+#pragma unroll
+        for (int f = 0; f < 4; f++) {
+            w[f] = LoadLane(cols[f] + int64_t(b) * 128);
+        }
+        const Stored rs = rowScales[b], cs = colScales[b];
+        const Wide32 wide = Widen(x, Inside(rs));
+#pragma unroll
+        for (int f = 0; f < 4; f++) {
+            if constexpr (kPowers) {
+                sum[f] = MfmaWide(Widen(w[f], Inside(cs)), wide, sum[f]);
+            } else {
+                const Float4 p = MfmaWide(Widen(w[f], 1.0f), wide, Zero4());
+                const float s = rs * cs;
+#pragma unroll
+                for (int i = 0; i < 4; i++) {
+                    sum[f][i] = __builtin_fmaf(p[i], s, sum[f][i]);
+                }
+            }
+        }
+    }
+#pragma unroll
+    for (int f = 0; f < 4; f++) {
+        part[wave][f][lane] = sum[f];
+    }
+    __syncthreads();
+    // a wave adds up the 16 columns of its number
+    Float4 total = part[0][wave][lane];
+#pragma unroll
+    for (int w = 1; w < kWaves; w++) {
+        const Float4 other = part[w][wave][lane];
+#pragma unroll
+        for (int i = 0; i < 4; i++) {
+            total[i] += other[i];
+        }
+    }
+    if (u.first + l16 < u.last) {
+        const float v[4] = {total[0], total[1], total[2], total[3]};
+        StoreFour(static_cast<T *>(a.out) + int64_t(u.first + l16) * a.outPitch, v, col0 + wave * 16 + lane / 16 * 4, a.numCols, false);
+    }
+}
+
+// f(first block, number of blocks) for every group of the expert, ascending; blocks count over all groups.  Called by whole waves.
+template <typename F>
+__device__ __forceinline__ void ForGroupsOf(const ProductArgs &a, int expert, F f)
+{
+    if (a.offsets == nullptr) {
+        if ((a.expertOfGroup == nullptr ? 0 : a.expertOfGroup[0]) == expert) {
+            f(0, (a.groupedRows + 127) / 128);
+        }
+        return;
+    }
+    const int lane = int(__lane_id());
+    const int64_t most = int64_t(a.groupedRows) / 128 + a.groups;   // blocks there can be: none beyond is looked at
+    int64_t before = 0;
+    for (int g0 = 0; g0 < a.groups && before < most; g0 += 64) {
+        const int g = g0 + lane;
+        int n = 0;
+        bool is = false;
+        if (g < a.groups) {
+            const int lo = min(max(a.offsets[g], 0), a.groupedRows), hi = min(max(a.offsets[g + 1], lo), a.groupedRows);
+            n = (hi - lo + 127) / 128;
+            is = n > 0 && (a.expertOfGroup == nullptr ? g : a.expertOfGroup[g]) == expert;
+        }
+        int sum = n;
+#pragma unroll
+        for (int d = 1; d < 64; d <<= 1) {
+            const int other = __shfl_up(sum, d, 64);
+            sum += lane >= d ? other : 0;
+        }
+        unsigned long long left = __ballot(is);
+        while (left != 0) {
+            const int at = __ffsll(left) - 1;
+            left &= left - 1;
+            const int64_t first = before + __shfl(sum - n, at, 64);
+            const int64_t last = first + __shfl(n, at, 64);
+            if (first < most) {
+                f(int(first), int((last < most ? last : most) - first));
+            }
+        }
+        before += __shfl(sum, 63, 64);
+    }
+}
+
+// The weights' gradient, 64 x 64 to a workgroup, 16 rows to a wave.
+template <typename T, HcclAmdScaleType kScale>
+__global__ void __launch_bounds__(kThreads) GradSmallKernel(ProductArgs a)
+{
+    constexpr bool kPowers = kScale == HCCL_AMD_SCALE_E8M0;
+    typedef typename BlockScale<kScale>::Stored Stored;
+    const int rowTiles = (a.numRows + 63) / 64;
+    const int tile = int(blockIdx.x), col0 = tile % a.colTiles * 64, expert = tile / a.colTiles / rowTiles;
+    const int lane = int(threadIdx.x) % 64, wave = int(threadIdx.x) / 64, l16 = lane % 16, piece = lane / 16 * 16;
+    const int row0 = tile / a.colTiles % rowTiles * 64 + wave * 16;
+    const int row = min(row0 + l16, a.numRows - 1);
+    const uint8_t *rows = a.rows + int64_t(row) * a.rowPitch + piece;
+    const uint8_t *cols[4];
+    Float4 sum[4];
+#pragma unroll
+    for (int f = 0; f < 4; f++) {
+        cols[f] = a.cols + int64_t(min(col0 + f * 16 + l16, a.numCols - 1)) * a.colPitch + piece;
+        sum[f] = Zero4();
+    }
+    ForGroupsOf(a, expert, [&](int first, int count) {
+        for (int b = first; b < first + count; b++) {
+            const Int8 y = LoadLane(rows + int64_t(b) * 128);
+            const Stored rs = static_cast<const Stored *>(a.rowScales)[int64_t(b) * a.numRows + row];
+            const Stored *cs = static_cast<const Stored *>(a.colScales) + int64_t(b) * a.numCols;
+            const Wide32 wide = Widen(y, Inside(rs));
+#pragma unroll
+            for (int f = 0; f < 4; f++) {
+                const Int8 x = LoadLane(cols[f] + int64_t(b) * 128);
+                if constexpr (kPowers) {
+                    sum[f] = MfmaWide(Widen(x, Inside(cs[min(col0 + f * 16 + l16, a.numCols - 1)])), wide, sum[f]);
+                } else {
+                    const Float4 p = MfmaWide(Widen(x, 1.0f), wide, Zero4());
+#pragma unroll
+                    for (int i = 0; i < 4; i++) {
+                        sum[f][i] = __builtin_fmaf(p[i], rs * cs[min(col0 + f * 16 + lane / 16 * 4 + i, a.numCols - 1)], sum[f][i]);
+                    }
+                }
+            }
+        }
+    });
+    if (row0 + l16 < a.numRows) {
+        T *out = static_cast<T *>(a.out) + (int64_t(expert) * a.numRows + row0 + l16) * a.outPitch;
+#pragma unroll
+        for (int f = 0; f < 4; f++) {
+            const float v[4] = {sum[f][0], sum[f][1], sum[f][2], sum[f][3]};
+            StoreFour(out, v, col0 + f * 16 + lane / 16 * 4, a.numCols, a.accumulate);
+        }
+    }
+}
+
+// f(type, scale type) as constants
+template <typename F>
+void Choose(HcclDataType type, HcclAmdScaleType scaleType, F f)
+{
+    const auto byScale = [&](auto of) {
+        scaleType == HCCL_AMD_SCALE_FP32 ? f(of, std::integral_constant<HcclAmdScaleType, HCCL_AMD_SCALE_FP32>{})
+                                         : f(of, std::integral_constant<HcclAmdScaleType, HCCL_AMD_SCALE_E8M0>{});
+    };
+    switch (type) {
+        case HCCL_DATA_TYPE_FP32:
+            byScale(float{});
+            break;
+        case HCCL_DATA_TYPE_FP16:
+            byScale(_Float16{});
+            break;
+        default:
+            byScale(__bf16{});
+    }
+}
+
+constexpr uint64_t kMostTiles = uint64_t(1) << 23;   // workgroups of 256 below 2^32 threads (of 512 with 2^22)
+
+}  // namespace
+}  // namespace experts
+}  // namespace hcclamd
+
+using namespace hcclamd::experts;
+
+extern "C" {
+
+HcclResult HcclAmdBlockMatmul(const void *a, uint64_t aStride, const void *aScales, uint64_t aScaleStride, uint64_t rows,
+    uint32_t groups, const int32_t *offsets, const int32_t *expertOfGroup, const void *w, const void *wScales, uint32_t experts,
+    uint64_t n, uint64_t k, HcclAmdScaleType scaleType, void *y, HcclDataType yType, uint64_t yStride, void *stream)
+{
+    EXPERTS_CHK_PTR(stream);
+    EXPERTS_CHK_TYPE(Float(yType));
+    EXPERTS_CHK_TYPE(Scaled(scaleType));
+    EXPERTS_CHK(rows <= kMaxGroupedRows && n <= kMaxSize - 256 && k <= kMaxSize - 256);
+    EXPERTS_CHK(groups >= 1 && groups <= HCCL_AMD_MAX_GROUPS && experts >= 1 && experts <= HCCL_AMD_MAX_GROUPS);
+    EXPERTS_CHK(offsets != nullptr || groups == 1);
+    EXPERTS_CHK(expertOfGroup != nullptr || groups <= experts);
+    if (rows == 0 || n == 0) {
+        return HCCL_SUCCESS;
+    }
+    EXPERTS_CHK_PTR(y);
+    if (k != 0) {
+        EXPERTS_CHK_PTR(a);
+        EXPERTS_CHK_PTR(aScales);
+        EXPERTS_CHK_PTR(w);
+        EXPERTS_CHK_PTR(wScales);
+    }
+    ProductArgs p{};
+    p.rows = static_cast<const uint8_t *>(a);
+    p.cols = static_cast<const uint8_t *>(w);
+    p.rowScales = aScales;
+    p.colScales = wScales;
+    p.offsets = offsets;
+    p.expertOfGroup = expertOfGroup;
+    p.out = y;
+    p.rowPitch = int64_t(aStride == 0 ? Up128(k) : aStride);
+    p.colPitch = int64_t(Up128(k));
+    p.outPitch = int64_t(yStride == 0 ? n : yStride);
+    p.rowScalePitch = int64_t(aScaleStride == 0 ? Blocks(k) : aScaleStride);
+    p.numRows = int(rows);
+    p.numCols = int(n);
+    p.blocks = int(Blocks(k));
+    p.groups = int(groups);
+    p.experts = int(experts);
+    EXPERTS_CHK(uint64_t(p.rowPitch) >= Up128(k) && p.rowPitch % 16 == 0 && Aligned(a, 16) && Aligned(w, 16));
+    EXPERTS_CHK(uint64_t(p.rowScalePitch) >= Blocks(k) && ScaleAligned(scaleType, aScales) && ScaleAligned(scaleType, wScales));
+    EXPERTS_CHK(uint64_t(p.outPitch) >= n && AlignedTo(yType, y));
+    EXPERTS_CHK(Aligned(offsets, 4) && Aligned(expertOfGroup, 4));
+    p.colTiles = int((n + 63) / 64);
+    const uint64_t units = offsets == nullptr ? (rows + 15) / 16 : rows / 16 + groups;
+    EXPERTS_CHK(units * uint64_t(p.colTiles) <= kMostTiles);
+    Choose(yType, scaleType, [&](auto of, auto scale) {
+        hipLaunchKernelGGL((FewRowsKernel<decltype(of), decltype(scale)::value>), dim3(uint32_t(units * uint64_t(p.colTiles))), dim3(kThreads), 0,
+            static_cast<hipStream_t>(stream), p);
+    });
+    return Launched("HcclAmdBlockMatmul");
+}
+
+HcclResult HcclAmdBlockMatmulGradWeight(const void *yGradT, const void *yGradScales, const void *xT, const void *xScales,
+    uint64_t columns, uint64_t rows, uint64_t n, uint64_t k, HcclAmdScaleType scaleType, uint32_t groups, const int32_t *offsets,
+    const int32_t *expertOfGroup, uint32_t experts, void *wGrad, HcclDataType gradType, uint32_t accumulate, void *stream)
+{
+    EXPERTS_CHK_PTR(stream);
+    EXPERTS_CHK_TYPE(Float(gradType));
+    EXPERTS_CHK_TYPE(Scaled(scaleType));
+    EXPERTS_CHK(rows <= kMaxGroupedRows && n <= kMaxSize - 256 && k <= kMaxSize - 256);
+    EXPERTS_CHK(groups >= 1 && groups <= HCCL_AMD_MAX_GROUPS && experts >= 1 && experts <= HCCL_AMD_MAX_GROUPS);
+    EXPERTS_CHK(offsets != nullptr || groups == 1);
+    EXPERTS_CHK(columns % 128 == 0 && columns >= (rows / 128 + groups) * 128 && columns <= kMaxSize);
+    if (n == 0 || k == 0) {
+        return HCCL_SUCCESS;
+    }
+    EXPERTS_CHK_PTR(wGrad);
+    if (rows != 0) {
+        EXPERTS_CHK_PTR(yGradT);
+        EXPERTS_CHK_PTR(yGradScales);
+        EXPERTS_CHK_PTR(xT);
+        EXPERTS_CHK_PTR(xScales);
+    }
+    EXPERTS_CHK(Aligned(yGradT, 16) && Aligned(xT, 16) && ScaleAligned(scaleType, yGradScales) && ScaleAligned(scaleType, xScales));
+    EXPERTS_CHK(AlignedTo(gradType, wGrad) && Aligned(offsets, 4) && Aligned(expertOfGroup, 4));
+    ProductArgs p{};
+    p.rows = static_cast<const uint8_t *>(yGradT);
+    p.cols = static_cast<const uint8_t *>(xT);
+    p.rowScales = yGradScales;
+    p.colScales = xScales;
+    p.offsets = offsets;
+    p.expertOfGroup = expertOfGroup;
+    p.out = wGrad;
+    p.rowPitch = p.colPitch = int64_t(columns);
+    p.outPitch = int64_t(k);
+    p.numRows = int(n);
+    p.numCols = int(k);
+    p.groups = int(groups);
+    p.experts = int(experts);
+    p.groupedRows = int(rows);
+    p.accumulate = accumulate != 0;
+    p.colTiles = int((k + 63) / 64);
+    const uint64_t tiles = (n + 63) / 64 * uint64_t(p.colTiles) * experts;
+    EXPERTS_CHK(tiles <= kMostTiles);
+    Choose(gradType, scaleType, [&](auto of, auto scale) {
+        hipLaunchKernelGGL((GradSmallKernel<decltype(of), decltype(scale)::value>), dim3(uint32_t(tiles)), dim3(kThreads), 0,
+            static_cast<hipStream_t>(stream), p);
+    });
+    return Launched("HcclAmdBlockMatmulGradWeight");
+}
+
+}  // extern "C"
