@@ -127,8 +127,8 @@ struct BlockScale<HCCL_AMD_SCALE_FP32> {
     __device__ __forceinline__ explicit BlockScale(float top)
     {
         top = top > kLeastMax ? top : kLeastMax;
-        times = kLargest / top;
-        stored = top / kLargest;
+        times = 1.0f / top * kLargest;
+        stored = top * (1.0f / kLargest);
     }
 };
 

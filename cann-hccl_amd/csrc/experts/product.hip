@@ -32,6 +32,7 @@ struct ProductArgs {
     int groupedRows;                        // gradient: rows of all groups
     int colTiles;
     bool accumulate;
+    bool wideOut;                           // four neighbouring results can be stored at once
 };
 
 // The 8-bit matrix instructions keep fewer than 32 bits inside: on blocks of normally distributed values their results are
@@ -211,52 +212,211 @@ __device__ __forceinline__ void ForGroupsOf(const ProductArgs &a, int expert, F 
     }
 }
 
-// The weights' gradient, 64 x 64 to a workgroup, 16 rows to a wave.
-template <typename T, HcclAmdScaleType kScale>
-__global__ void __launch_bounds__(kThreads) GradSmallKernel(ProductArgs a)
+// ---- many rows -------------------------------------------------------------------------------------------
+
+typedef const __attribute__((address_space(1))) void *GlobalBytes;
+typedef __attribute__((address_space(3))) void *LdsBytes;
+
+// Loads that have been sent into LDS have arrived.
+__device__ __forceinline__ void LoadsDone() { asm volatile("s_waitcnt vmcnt(0)" ::: "memory"); }
+
+__device__ __forceinline__ uint32_t ScaleBits(float s) { return __float_as_uint(s); }
+__device__ __forceinline__ uint32_t ScaleBits(uint8_t s) { return s; }
+
+// kWR x kWC waves of 16 kRF rows by 64 columns each.  A step is one block of 128 values: its bytes go from memory into one
+// of two LDS buffers while the other one is multiplied, eight rows of 128 bytes to a wave's load, without passing through
+// registers.  The 16-byte pieces of a row lie in LDS in an order that depends on the row (piece p of row r at p ^ (r / 2 % 8)), so that the
+// 16 rows a lane group reads are in different banks; since such a load fills LDS in lane order, it is the lanes' addresses
+// in memory that are swapped.  Scales pass through a register of one thread each.
+// kPrecise: 16-bit matrix instructions on widened values, else 8-bit ones.  kGrad: the weights' gradient, scales by column too.
+template <typename T, HcclAmdScaleType kScale, bool kPrecise, bool kGrad, int kRF, int kWR, int kWC>
+__global__ void __launch_bounds__(64 * kWR * kWC) TileKernel(ProductArgs a)
 {
     constexpr bool kPowers = kScale == HCCL_AMD_SCALE_E8M0;
     typedef typename BlockScale<kScale>::Stored Stored;
-    const int rowTiles = (a.numRows + 63) / 64;
-    const int tile = int(blockIdx.x), col0 = tile % a.colTiles * 64, expert = tile / a.colTiles / rowTiles;
-    const int lane = int(threadIdx.x) % 64, wave = int(threadIdx.x) / 64, l16 = lane % 16, piece = lane / 16 * 16;
-    const int row0 = tile / a.colTiles % rowTiles * 64 + wave * 16;
-    const int row = min(row0 + l16, a.numRows - 1);
-    const uint8_t *rows = a.rows + int64_t(row) * a.rowPitch + piece;
-    const uint8_t *cols[4];
-    Float4 sum[4];
-#pragma unroll
-    for (int f = 0; f < 4; f++) {
-        cols[f] = a.cols + int64_t(min(col0 + f * 16 + l16, a.numCols - 1)) * a.colPitch + piece;
-        sum[f] = Zero4();
+    constexpr int kTileRows = 16 * kRF * kWR, kTileCols = 64 * kWC, kTileWaves = kWR * kWC, kTileThreads = 64 * kTileWaves;
+    constexpr int kLoads = (kTileRows + kTileCols) / 8 / kTileWaves, kRowLoads = kTileRows / 8 / kTileWaves;
+    constexpr int kScales = (kTileRows + kTileCols + kTileThreads - 1) / kTileThreads;
+    static_assert(kTileRows % (8 * kTileWaves) == 0 && kTileCols % (8 * kTileWaves) == 0, "whole loads");
+    __shared__ __align__(16) uint8_t tiles[2][(kTileRows + kTileCols) * 128];
+    __shared__ __align__(16) uint32_t scales[2][kTileRows + kTileCols];
+
+    const int lane = int(threadIdx.x) % 64, wave = __builtin_amdgcn_readfirstlane(int(threadIdx.x) / 64);
+    const int l16 = lane % 16, quarter = lane / 16;
+    int expert, row0, rowEnd, col0;
+    if constexpr (kGrad) {
+        const int rowTiles = (a.numRows + kTileRows - 1) / kTileRows, tile = int(blockIdx.x);
+        col0 = tile % a.colTiles * kTileCols;
+        row0 = tile / a.colTiles % rowTiles * kTileRows;
+        rowEnd = a.numRows;
+        expert = tile / a.colTiles / rowTiles;
+    } else {
+        const int unit = int(blockIdx.x) / a.colTiles;
+        col0 = int(blockIdx.x) % a.colTiles * kTileCols;
+        const Unit u = FindUnit(a.offsets, a.groups, a.numRows, unit, kTileRows);
+        if (u.group < 0) {
+            return;
+        }
+        expert = a.expertOfGroup == nullptr ? u.group : a.expertOfGroup[u.group];
+        if (expert < 0 || expert >= a.experts) {
+            return;
+        }
+        row0 = u.first;
+        rowEnd = u.last;
     }
-    ForGroupsOf(a, expert, [&](int first, int count) {
-        for (int b = first; b < first + count; b++) {
-            const Int8 y = LoadLane(rows + int64_t(b) * 128);
-            const Stored rs = static_cast<const Stored *>(a.rowScales)[int64_t(b) * a.numRows + row];
-            const Stored *cs = static_cast<const Stored *>(a.colScales) + int64_t(b) * a.numCols;
-            const Wide32 wide = Widen(y, Inside(rs));
+    const int64_t colBase = kGrad ? 0 : int64_t(expert) * a.numCols;
+
+    // what this lane loads: a 16-byte piece of a row, in every load
+    const uint8_t *from[kLoads];
 #pragma unroll
-            for (int f = 0; f < 4; f++) {
-                const Int8 x = LoadLane(cols[f] + int64_t(b) * 128);
-                if constexpr (kPowers) {
-                    sum[f] = MfmaWide(Widen(x, Inside(cs[min(col0 + f * 16 + l16, a.numCols - 1)])), wide, sum[f]);
+    for (int j = 0; j < kLoads; j++) {
+        const int oct = (j < kRowLoads ? j : j - kRowLoads) * kTileWaves + wave, piece = (lane % 8) ^ (lane / 16 + 4 * (oct % 2));
+        const int at = oct * 8 + lane / 8;
+        from[j] = (j < kRowLoads ? a.rows + int64_t(min(row0 + at, rowEnd - 1)) * a.rowPitch
+                                 : a.cols + (colBase + min(col0 + at, a.numCols - 1)) * a.colPitch) + piece * 16;
+    }
+    // and its scales
+    const Stored *scaleFrom[kScales];
+    int64_t scaleStep[kScales];
+#pragma unroll
+    for (int j = 0; j < kScales; j++) {
+        const int i = int(threadIdx.x) + j * kTileThreads;
+        if (i < kTileRows) {
+            const int64_t row = min(row0 + i, rowEnd - 1);
+            scaleFrom[j] = static_cast<const Stored *>(a.rowScales) + (kGrad ? row : row * a.rowScalePitch);
+            scaleStep[j] = kGrad ? a.numRows : 1;
+        } else {
+            const int64_t col = min(col0 + i - kTileRows, a.numCols - 1);
+            scaleFrom[j] = static_cast<const Stored *>(a.colScales) + (kGrad ? col : (int64_t(expert) * ((a.numCols + 127) / 128) + col / 128) * a.blocks);
+            scaleStep[j] = kGrad ? a.numCols : 1;
+        }
+    }
+    Stored coming[kScales];
+    const auto fetch = [&](int block, int to) {
+#pragma unroll
+        for (int j = 0; j < kLoads; j++) {
+            const int oct = (j < kRowLoads ? j : j - kRowLoads) * kTileWaves + wave;
+            uint8_t *lds = tiles[to] + ((j < kRowLoads ? 0 : kTileRows) + oct * 8) * 128;
+            __builtin_amdgcn_global_load_lds((GlobalBytes)(from[j] + int64_t(block) * 128), (LdsBytes)lds, 16, 0, 0);
+        }
+#pragma unroll
+        for (int j = 0; j < kScales; j++) {
+            if (int(threadIdx.x) + j * kTileThreads < kTileRows + kTileCols) {
+                coming[j] = scaleFrom[j][block * scaleStep[j]];
+            }
+        }
+    };
+
+    const int rowAt = wave / kWC * 16 * kRF, colAt = wave % kWC * 64;     // of this wave, in the tile
+    const int laneAt = l16 * 128 + ((quarter ^ (l16 / 2)) * 16);
+    const auto fragment = [&](const uint8_t *rows16) {
+        const Int4 lo = *reinterpret_cast<const Int4 *>(rows16 + laneAt), hi = *reinterpret_cast<const Int4 *>(rows16 + (laneAt ^ 64));
+        return Int8{lo.x, lo.y, lo.z, lo.w, hi.x, hi.y, hi.z, hi.w};
+    };
+    Float4 sum[kRF][4];
+#pragma unroll
+    for (int r = 0; r < kRF; r++) {
+#pragma unroll
+        for (int c = 0; c < 4; c++) {
+            sum[r][c] = Zero4();
+        }
+    }
+    const auto multiply = [&](int at) {
+        const uint8_t *rows = tiles[at] + rowAt * 128, *cols = tiles[at] + (kTileRows + colAt) * 128;
+        const uint32_t *rowScale = scales[at] + rowAt, *colScale = scales[at] + kTileRows + colAt;
+        Int8 w[4];
+        Wide32 wide[4];
+        float cs[4][4];
+#pragma unroll
+        for (int c = 0; c < 4; c++) {
+            w[c] = fragment(cols + c * 16 * 128);
+            if constexpr (kPrecise) {
+                wide[c] = Widen(w[c], kPowers ? PowerOf(uint8_t(colScale[c * 16 + l16])) : 1.0f);
+            }
+            if constexpr (!kPowers) {
+#pragma unroll
+                for (int i = 0; i < 4; i++) {
+                    cs[c][i] = __uint_as_float(colScale[kGrad ? c * 16 + quarter * 4 + i : 0]);
+                }
+            }
+        }
+#pragma unroll
+        for (int r = 0; r < kRF; r++) {
+            const Int8 x = fragment(rows + r * 16 * 128);
+            const uint32_t rs = rowScale[r * 16 + l16];
+            Wide32 wideRow;
+            if constexpr (kPrecise) {
+                wideRow = Widen(x, kPowers ? PowerOf(uint8_t(rs)) : 1.0f);
+            }
+#pragma unroll
+            for (int c = 0; c < 4; c++) {
+                if constexpr (kPowers && kPrecise) {
+                    sum[r][c] = MfmaWide(wide[c], wideRow, sum[r][c]);
+                } else if constexpr (kPowers) {
+                    sum[r][c] = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(w[c], x, sum[r][c], 0, 0, 0, int(colScale[0]), 0, int(rs));
                 } else {
-                    const Float4 p = MfmaWide(Widen(x, 1.0f), wide, Zero4());
+                    const Float4 p = kPrecise ? MfmaWide(wide[c], wideRow, Zero4())
+                                              : __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(w[c], x, Zero4(), 0, 0, 0, 0, 0, 0);
 #pragma unroll
                     for (int i = 0; i < 4; i++) {
-                        sum[f][i] = __builtin_fmaf(p[i], rs * cs[min(col0 + f * 16 + lane / 16 * 4 + i, a.numCols - 1)], sum[f][i]);
+                        sum[r][c][i] = __builtin_fmaf(p[i], __uint_as_float(rs) * cs[c][i], sum[r][c][i]);
                     }
                 }
             }
         }
-    });
-    if (row0 + l16 < a.numRows) {
-        T *out = static_cast<T *>(a.out) + (int64_t(expert) * a.numRows + row0 + l16) * a.outPitch;
+    };
+    const auto run = [&](int first, int count) {
+        __syncthreads();     // (the buffers are free: the blocks of another group may have been in them)
+        fetch(first, 0);
+        for (int i = 0; i < count; i++) {
+            const int at = i % 2;
 #pragma unroll
-        for (int f = 0; f < 4; f++) {
-            const float v[4] = {sum[f][0], sum[f][1], sum[f][2], sum[f][3]};
-            StoreFour(out, v, col0 + f * 16 + lane / 16 * 4, a.numCols, a.accumulate);
+            for (int j = 0; j < kScales; j++) {
+                if (int(threadIdx.x) + j * kTileThreads < kTileRows + kTileCols) {
+                    scales[at][int(threadIdx.x) + j * kTileThreads] = ScaleBits(coming[j]);
+                }
+            }
+            LoadsDone();
+            __syncthreads();   // this buffer is full, and nobody reads the other one any more
+            if (i + 1 < count) {
+                fetch(first + i + 1, 1 - at);
+            }
+            multiply(at);
+        }
+    };
+    if constexpr (kGrad) {
+        ForGroupsOf(a, expert, run);
+    } else {
+        if (a.blocks > 0) {
+            run(0, a.blocks);
+        }
+    }
+
+#pragma unroll
+    for (int r = 0; r < kRF; r++) {
+        const int row = row0 + rowAt + r * 16 + l16;
+        if (row < rowEnd) {
+            T *out = static_cast<T *>(a.out) + ((kGrad ? int64_t(expert) * a.numRows : 0) + row) * a.outPitch;
+#pragma unroll
+            for (int c = 0; c < 4; c++) {
+                const float v[4] = {sum[r][c][0], sum[r][c][1], sum[r][c][2], sum[r][c][3]};
+                const int col = col0 + colAt + c * 16 + quarter * 4;
+                if (a.wideOut) {
+                    if (col < a.numCols) {
+                        float w[4];
+                        if (kGrad && a.accumulate) {
+                            Load<true, 4>(out + col, w);
+                        }
+#pragma unroll
+                        for (int i = 0; i < 4; i++) {
+                            w[i] = kGrad && a.accumulate ? w[i] + v[i] : v[i];
+                        }
+                        Store<true, 4>(out + col, w);
+                    }
+                } else {
+                    StoreFour(out, v, col, a.numCols, kGrad && a.accumulate);
+                }
+            }
         }
     }
 }
@@ -281,7 +441,12 @@ void Choose(HcclDataType type, HcclAmdScaleType scaleType, F f)
     }
 }
 
-constexpr uint64_t kMostTiles = uint64_t(1) << 23;   // workgroups of 256 below 2^32 threads (of 512 with 2^22)
+constexpr uint64_t kMostTiles = uint64_t(1) << 22;   // workgroups of up to 512 below 2^32 threads
+
+bool WideOut(HcclDataType type, uint64_t width, const void *p, int64_t pitch)
+{
+    return width % 4 == 0 && pitch % 4 == 0 && Aligned(p, 4 * SizeOf(type));
+}
 
 }  // namespace
 }  // namespace experts
@@ -333,12 +498,36 @@ HcclResult HcclAmdBlockMatmul(const void *a, uint64_t aStride, const void *aScal
     EXPERTS_CHK(uint64_t(p.rowScalePitch) >= Blocks(k) && ScaleAligned(scaleType, aScales) && ScaleAligned(scaleType, wScales));
     EXPERTS_CHK(uint64_t(p.outPitch) >= n && AlignedTo(yType, y));
     EXPERTS_CHK(Aligned(offsets, 4) && Aligned(expertOfGroup, 4));
-    p.colTiles = int((n + 63) / 64);
-    const uint64_t units = offsets == nullptr ? (rows + 15) / 16 : rows / 16 + groups;
+    p.wideOut = WideOut(yType, n, y, p.outPitch);
+    const bool few = rows <= 32 * uint64_t(groups);
+    // sums of 16-bit results over more than two blocks: the 8-bit instruction's error is behind their own rounding
+    const bool fast = yType != HCCL_DATA_TYPE_FP32 && k > 256;
+    const bool large = fast && rows >= 256 * uint64_t(groups) && n >= 256;
+    const uint64_t tileRows = few ? 16 : large ? 256 : 128, tileCols = few ? 64 : large ? 256 : 128;
+    p.colTiles = int((n + tileCols - 1) / tileCols);
+    const uint64_t units = offsets == nullptr ? (rows + tileRows - 1) / tileRows : rows / tileRows + groups;
     EXPERTS_CHK(units * uint64_t(p.colTiles) <= kMostTiles);
     Choose(yType, scaleType, [&](auto of, auto scale) {
-        hipLaunchKernelGGL((FewRowsKernel<decltype(of), decltype(scale)::value>), dim3(uint32_t(units * uint64_t(p.colTiles))), dim3(kThreads), 0,
-            static_cast<hipStream_t>(stream), p);
+        typedef decltype(of) T;
+        constexpr HcclAmdScaleType kScale = decltype(scale)::value;
+        const auto go = [&](auto kernel, int threads) {
+            hipLaunchKernelGGL(kernel, dim3(uint32_t(units * uint64_t(p.colTiles))), dim3(threads), 0, static_cast<hipStream_t>(stream), p);
+        };
+        if (few) {
+            go(FewRowsKernel<T, kScale>, kThreads);
+            return;
+        }
+        if constexpr (sizeof(T) == 2) {
+            if (large) {
+                go(TileKernel<T, kScale, false, false, 8, 2, 4>, 512);
+                return;
+            }
+            if (fast) {
+                go(TileKernel<T, kScale, false, false, 4, 2, 2>, 256);
+                return;
+            }
+        }
+        go(TileKernel<T, kScale, true, false, 4, 2, 2>, 256);
     });
     return Launched("HcclAmdBlockMatmul");
 }
@@ -382,11 +571,12 @@ HcclResult HcclAmdBlockMatmulGradWeight(const void *yGradT, const void *yGradSca
     p.experts = int(experts);
     p.groupedRows = int(rows);
     p.accumulate = accumulate != 0;
-    p.colTiles = int((k + 63) / 64);
-    const uint64_t tiles = (n + 63) / 64 * uint64_t(p.colTiles) * experts;
+    p.wideOut = WideOut(gradType, k, wGrad, p.outPitch);
+    p.colTiles = int((k + 127) / 128);
+    const uint64_t tiles = (n + 127) / 128 * uint64_t(p.colTiles) * experts;
     EXPERTS_CHK(tiles <= kMostTiles);
     Choose(gradType, scaleType, [&](auto of, auto scale) {
-        hipLaunchKernelGGL((GradSmallKernel<decltype(of), decltype(scale)::value>), dim3(uint32_t(tiles)), dim3(kThreads), 0,
+        hipLaunchKernelGGL((TileKernel<decltype(of), decltype(scale)::value, true, true, 4, 2, 2>), dim3(uint32_t(tiles)), dim3(256), 0,
             static_cast<hipStream_t>(stream), p);
     });
     return Launched("HcclAmdBlockMatmulGradWeight");

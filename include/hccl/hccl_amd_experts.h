@@ -19,7 +19,7 @@
  * 8-bit rows.  HCCL_DATA_TYPE_FP8E4M3 values (largest 448) with one scale per 128 consecutive values: value = q * scale.
  * Every row is padded with zeros to a multiple of 128 values, starts on a 16-byte boundary, and its stride is a multiple
  * of 16.  Of a block, a = max(largest finite magnitude, 2^-96); the scale is
- *   HCCL_AMD_SCALE_FP32   float a / 448, q = round(v * (448 / a)), both quotients rounded to 32 bits
+ *   HCCL_AMD_SCALE_FP32   float a * (1 / 448), q = round(v * (1 / a * 448)), every quotient and product rounded to 32 bits
  *   HCCL_AMD_SCALE_E8M0   one byte b that stands for 2^(b - 127), the least power of two with a <= 448 * 2^(b - 127);
  *                         q = round(v / scale)
  * rounding to nearest, ties to even.  Infinities and NaN become the type's NaN and leave their block's scale alone. */

@@ -23,8 +23,8 @@ def block_scale(top, kind):
     """(what is stored, what values are multiplied by, the scale's value) of blocks with these maxima (numpy float32)."""
     top = np.maximum(top.astype(np.float32), np.float32(2.0 ** -96))
     if kind == FP32:
-        stored = top / np.float32(448)
-        return stored, np.float32(448) / top, stored.astype(np.float64)
+        stored = top * (np.float32(1) / np.float32(448))
+        return stored, np.float32(1) / top * np.float32(448), stored.astype(np.float64)
     m, p = np.frexp(top.astype(np.float64))               # m in [1/2, 1)
     power = p - 9 + (m > 0.875)
     return (power + 127).astype(np.uint8), np.exp2(-power.astype(np.float64)).astype(np.float32), np.exp2(power.astype(np.float64))
