@@ -238,8 +238,11 @@ __global__ void __launch_bounds__(64 * kWR * kWC) TileKernel(ProductArgs a)
     constexpr int kLoads = (kTileRows + kTileCols) / 8 / kTileWaves, kRowLoads = kTileRows / 8 / kTileWaves;
     constexpr int kScales = (kTileRows + kTileCols + kTileThreads - 1) / kTileThreads;
     static_assert(kTileRows % (8 * kTileWaves) == 0 && kTileCols % (8 * kTileWaves) == 0, "whole loads");
-    __shared__ __align__(16) uint8_t tiles[2][(kTileRows + kTileCols) * 128];
-    __shared__ __align__(16) uint32_t scales[2][kTileRows + kTileCols];
+    // (two variables, not halves of one: the compiler waits for all loads into LDS before it reads what they might write)
+    __shared__ __align__(16) uint8_t tile0[(kTileRows + kTileCols) * 128];
+    __shared__ __align__(16) uint8_t tile1[(kTileRows + kTileCols) * 128];
+    __shared__ __align__(16) uint32_t scales0[kTileRows + kTileCols];
+    __shared__ __align__(16) uint32_t scales1[kTileRows + kTileCols];
 
     const int lane = int(threadIdx.x) % 64, wave = __builtin_amdgcn_readfirstlane(int(threadIdx.x) / 64);
     const int l16 = lane % 16, quarter = lane / 16;
@@ -292,11 +295,11 @@ __global__ void __launch_bounds__(64 * kWR * kWC) TileKernel(ProductArgs a)
         }
     }
     Stored coming[kScales];
-    const auto fetch = [&](int block, int to) {
+    const auto fetch = [&](int block, uint8_t *tile) __attribute__((always_inline)) {
 #pragma unroll
         for (int j = 0; j < kLoads; j++) {
             const int oct = (j < kRowLoads ? j : j - kRowLoads) * kTileWaves + wave;
-            uint8_t *lds = tiles[to] + ((j < kRowLoads ? 0 : kTileRows) + oct * 8) * 128;
+            uint8_t *lds = tile + ((j < kRowLoads ? 0 : kTileRows) + oct * 8) * 128;
             __builtin_amdgcn_global_load_lds((GlobalBytes)(from[j] + int64_t(block) * 128), (LdsBytes)lds, 16, 0, 0);
         }
 #pragma unroll
@@ -321,9 +324,9 @@ __global__ void __launch_bounds__(64 * kWR * kWC) TileKernel(ProductArgs a)
             sum[r][c] = Zero4();
         }
     }
-    const auto multiply = [&](int at) {
-        const uint8_t *rows = tiles[at] + rowAt * 128, *cols = tiles[at] + (kTileRows + colAt) * 128;
-        const uint32_t *rowScale = scales[at] + rowAt, *colScale = scales[at] + kTileRows + colAt;
+    const auto multiply = [&](const uint8_t *tile, const uint32_t *scales) __attribute__((always_inline)) {
+        const uint8_t *rows = tile + rowAt * 128, *cols = tile + (kTileRows + colAt) * 128;
+        const uint32_t *rowScale = scales + rowAt, *colScale = scales + kTileRows + colAt;
         Int8 w[4];
         Wide32 wide[4];
         float cs[4][4];
@@ -365,23 +368,29 @@ __global__ void __launch_bounds__(64 * kWR * kWC) TileKernel(ProductArgs a)
             }
         }
     };
-    const auto run = [&](int first, int count) {
-        __syncthreads();     // (the buffers are free: the blocks of another group may have been in them)
-        fetch(first, 0);
-        for (int i = 0; i < count; i++) {
-            const int at = i % 2;
+    // One step: this buffer's loads are under way; those of the block after it go into the other one.
+    const auto step = [&](uint8_t *tile, uint32_t *scale, uint8_t *other, int next, bool more) __attribute__((always_inline)) {
 #pragma unroll
-            for (int j = 0; j < kScales; j++) {
-                if (int(threadIdx.x) + j * kTileThreads < kTileRows + kTileCols) {
-                    scales[at][int(threadIdx.x) + j * kTileThreads] = ScaleBits(coming[j]);
-                }
+        for (int j = 0; j < kScales; j++) {
+            if (int(threadIdx.x) + j * kTileThreads < kTileRows + kTileCols) {
+                scale[int(threadIdx.x) + j * kTileThreads] = ScaleBits(coming[j]);
             }
-            LoadsDone();
-            __syncthreads();   // this buffer is full, and nobody reads the other one any more
+        }
+        LoadsDone();
+        __syncthreads();   // this buffer is full, and nobody reads the other one any more
+        if (more) {
+            fetch(next, other);
+        }
+        multiply(tile, scale);
+    };
+    const auto run = [&](int first, int count) __attribute__((always_inline)) {
+        __syncthreads();     // (the buffers are free: the blocks of another group may have been in them)
+        fetch(first, tile0);
+        for (int i = 0; i < count; i += 2) {
+            step(tile0, scales0, tile1, first + i + 1, i + 1 < count);
             if (i + 1 < count) {
-                fetch(first + i + 1, 1 - at);
+                step(tile1, scales1, tile0, first + i + 2, i + 2 < count);
             }
-            multiply(at);
         }
     };
     if constexpr (kGrad) {
