@@ -203,17 +203,17 @@ __device__ __forceinline__ Unit FindUnit(const int32_t *__restrict__ offsets, in
         const int64_t start = before + sum - mine;
         const unsigned long long has = __ballot(unit >= start && unit < start + mine);
         if (has != 0) {
-            const int at = __ffsll(has) - 1;
-            Unit u;
+            const int at = __builtin_amdgcn_readfirstlane(__ffsll(has) - 1);
+            Unit u;                       // (readlane: the compiler sees that all lanes have the same)
             u.group = g0 + at;
-            u.groupFirst = __shfl(lo, at, 64);
-            u.groupLast = __shfl(hi, at, 64);
-            u.before = int(before) + __shfl(sum - mine, at, 64);
+            u.groupFirst = __builtin_amdgcn_readlane(lo, at);
+            u.groupLast = __builtin_amdgcn_readlane(hi, at);
+            u.before = int(before) + __builtin_amdgcn_readlane(sum - mine, at);
             u.first = u.groupFirst + (unit - u.before) * per;
             u.last = min(u.first + per, u.groupLast);
             return u;
         }
-        before += __shfl(sum, 63, 64);
+        before += __builtin_amdgcn_readlane(sum, 63);
     }
     return Unit{-1, 0, 0, 0, 0, 0};
 }

@@ -32,7 +32,7 @@ struct ProductArgs {
     int groupedRows;                        // gradient: rows of all groups
     int colTiles;
     bool accumulate;
-    bool wideOut;                           // four neighbouring results can be stored at once
+    bool wideOut;                           // results can be stored 16 bytes at once
 };
 
 // The 8-bit matrix instructions keep fewer than 32 bits inside: on blocks of normally distributed values their results are
@@ -85,12 +85,12 @@ __device__ __forceinline__ Int8 LoadLane(const uint8_t *p)
 __device__ __forceinline__ Float4 Zero4() { return Float4{0.0f, 0.0f, 0.0f, 0.0f}; }
 
 template <typename T>
-__device__ __forceinline__ void StoreFour(T *out, const float (&v)[4], int col, int numCols, bool accumulate)
+__device__ __forceinline__ void StoreFour(T *out, const float (&v)[4], int col, int numCols)
 {
 #pragma unroll
     for (int i = 0; i < 4; i++) {
         if (col + i < numCols) {
-            out[col + i] = T(accumulate ? float(out[col + i]) + v[i] : v[i]);
+            out[col + i] = T(v[i]);
         }
     }
 }
@@ -166,7 +166,7 @@ __global__ void __launch_bounds__(kThreads) FewRowsKernel(ProductArgs a)
     }
     if (u.first + l16 < u.last) {
         const float v[4] = {total[0], total[1], total[2], total[3]};
-        StoreFour(static_cast<T *>(a.out) + int64_t(u.first + l16) * a.outPitch, v, col0 + wave * 16 + lane / 16 * 4, a.numCols, false);
+        StoreFour(static_cast<T *>(a.out) + int64_t(u.first + l16) * a.outPitch, v, col0 + wave * 16 + lane / 16 * 4, a.numCols);
     }
 }
 
@@ -200,22 +200,70 @@ __device__ __forceinline__ void ForGroupsOf(const ProductArgs &a, int expert, F 
         }
         unsigned long long left = __ballot(is);
         while (left != 0) {
-            const int at = __ffsll(left) - 1;
+            const int at = __builtin_amdgcn_readfirstlane(__ffsll(left) - 1);
             left &= left - 1;
-            const int64_t first = before + __shfl(sum - n, at, 64);
-            const int64_t last = first + __shfl(n, at, 64);
+            const int64_t first = before + __builtin_amdgcn_readlane(sum - n, at);
+            const int64_t last = first + __builtin_amdgcn_readlane(n, at);
             if (first < most) {
                 f(int(first), int((last < most ? last : most) - first));
             }
         }
-        before += __shfl(sum, 63, 64);
+        before += __builtin_amdgcn_readlane(sum, 63);
     }
 }
 
 // ---- many rows -------------------------------------------------------------------------------------------
 
-typedef const __attribute__((address_space(1))) void *GlobalBytes;
+constexpr int kBufferFlags = 0x00027000;    // a raw buffer of 32-bit words
 typedef __attribute__((address_space(3))) void *LdsBytes;
+
+// How many units of `per` rows all groups make, `most` at most.  Called by all 64 lanes of a wave.
+__device__ __forceinline__ int CountUnits(const int32_t *__restrict__ offsets, int groups, int rows, int per, int most)
+{
+    if (offsets == nullptr) {
+        return min((rows + per - 1) / per, most);
+    }
+    int64_t sum = 0;
+    for (int g = int(__lane_id()); g < groups; g += 64) {
+        const int lo = min(max(offsets[g], 0), rows), hi = min(max(offsets[g + 1], lo), rows);
+        sum += (hi - lo + per - 1) / per;
+    }
+#pragma unroll
+    for (int d = 1; d < 64; d <<= 1) {
+        sum += __shfl_xor(sum, d, 64);
+    }
+    return __builtin_amdgcn_readfirstlane(int(sum < most ? sum : most));
+}
+
+// Workgroups go to the eight XCDs in turn, each of which has an L2 cache of its own: every XCD takes a run of neighbouring tiles.
+__device__ __forceinline__ int TileOf(int block, int tiles)
+{
+    const int xcd = block % 8, more = tiles % 8;
+    return xcd * (tiles / 8) + min(xcd, more) + block / 8;
+}
+
+struct Place {
+    int unit, col;
+};
+
+// A tile's place among units x colTiles: bands of eight columns of tiles,
+// unit by unit, so that the 32 tiles an XCD works on at a time share four units' rows and eight tiles' columns.
+__device__ __forceinline__ Place PlaceOf(int tile, int units, int colTiles)
+{
+    const int band = tile / (units * 8), width = min(8, colTiles - band * 8);
+    tile -= band * units * 8;
+    return Place{tile / width, band * 8 + tile % width};
+}
+
+// 16 bytes to a lane, from base + own + shared into LDS in lane order; what lies at `bytes` and beyond reads as zeros.  (The host's
+// pass over this file does not know buffers.)
+__device__ __forceinline__ void LoadToLds(const uint8_t *base, uint32_t bytes, uint8_t *lds, int own, int shared)
+{
+#if defined(__HIP_DEVICE_COMPILE__)
+    const auto buffer = __builtin_amdgcn_make_buffer_rsrc(const_cast<uint8_t *>(base), 0, int(bytes), kBufferFlags);
+    __builtin_amdgcn_raw_ptr_buffer_load_lds(buffer, (LdsBytes)lds, 16, own, shared, 0, 0);
+#endif
+}
 
 // Loads that have been sent into LDS have arrived.
 __device__ __forceinline__ void LoadsDone() { asm volatile("s_waitcnt vmcnt(0)" ::: "memory"); }
@@ -223,40 +271,49 @@ __device__ __forceinline__ void LoadsDone() { asm volatile("s_waitcnt vmcnt(0)" 
 __device__ __forceinline__ uint32_t ScaleBits(float s) { return __float_as_uint(s); }
 __device__ __forceinline__ uint32_t ScaleBits(uint8_t s) { return s; }
 
-// kWR x kWC waves of 16 kRF rows by 64 columns each.  A step is one block of 128 values: its bytes go from memory into one
+// kWR x kWC waves of 16 kRF rows by 16 kCF columns each.  A step is one block of 128 values: its bytes go from memory into one
 // of two LDS buffers while the other one is multiplied, eight rows of 128 bytes to a wave's load, without passing through
 // registers.  The 16-byte pieces of a row lie in LDS in an order that depends on the row (piece p of row r at p ^ (r / 2 % 8)), so that the
 // 16 rows a lane group reads are in different banks; since such a load fills LDS in lane order, it is the lanes' addresses
 // in memory that are swapped.  Scales pass through a register of one thread each.
 // kPrecise: 16-bit matrix instructions on widened values, else 8-bit ones.  kGrad: the weights' gradient, scales by column too.
-template <typename T, HcclAmdScaleType kScale, bool kPrecise, bool kGrad, int kRF, int kWR, int kWC>
+template <typename T, HcclAmdScaleType kScale, bool kPrecise, bool kGrad, int kRF, int kCF, int kWR, int kWC>
 __global__ void __launch_bounds__(64 * kWR * kWC) TileKernel(ProductArgs a)
 {
     constexpr bool kPowers = kScale == HCCL_AMD_SCALE_E8M0;
     typedef typename BlockScale<kScale>::Stored Stored;
-    constexpr int kTileRows = 16 * kRF * kWR, kTileCols = 64 * kWC, kTileWaves = kWR * kWC, kTileThreads = 64 * kTileWaves;
+    constexpr int kTileRows = 16 * kRF * kWR, kTileCols = 16 * kCF * kWC, kTileWaves = kWR * kWC, kTileThreads = 64 * kTileWaves;
     constexpr int kLoads = (kTileRows + kTileCols) / 8 / kTileWaves, kRowLoads = kTileRows / 8 / kTileWaves;
-    constexpr int kScales = (kTileRows + kTileCols + kTileThreads - 1) / kTileThreads;
+    constexpr int kScales = (kTileRows + kTileCols + kTileThreads - 1) / kTileThreads;   // to a thread (past the last column's: that again)
     static_assert(kTileRows % (8 * kTileWaves) == 0 && kTileCols % (8 * kTileWaves) == 0, "whole loads");
     // (two variables, not halves of one: the compiler waits for all loads into LDS before it reads what they might write)
     __shared__ __align__(16) uint8_t tile0[(kTileRows + kTileCols) * 128];
     __shared__ __align__(16) uint8_t tile1[(kTileRows + kTileCols) * 128];
-    __shared__ __align__(16) uint32_t scales0[kTileRows + kTileCols];
-    __shared__ __align__(16) uint32_t scales1[kTileRows + kTileCols];
+    __shared__ __align__(16) uint32_t scales0[kScales * kTileThreads];
+    __shared__ __align__(16) uint32_t scales1[kScales * kTileThreads];
 
     const int lane = int(threadIdx.x) % 64, wave = __builtin_amdgcn_readfirstlane(int(threadIdx.x) / 64);
     const int l16 = lane % 16, quarter = lane / 16;
     int expert, row0, rowEnd, col0;
     if constexpr (kGrad) {
-        const int rowTiles = (a.numRows + kTileRows - 1) / kTileRows, tile = int(blockIdx.x);
-        col0 = tile % a.colTiles * kTileCols;
-        row0 = tile / a.colTiles % rowTiles * kTileRows;
+        const int rowTiles = (a.numRows + kTileRows - 1) / kTileRows;
+        // (experts one after the other, each cut among the XCDs: their rows, and with them their tiles' costs, differ)
+        const int each = rowTiles * a.colTiles, more = each % 8, block = int(blockIdx.x) % (8 * (each / 8 + (more != 0)));
+        expert = int(blockIdx.x) / (8 * (each / 8 + (more != 0)));
+        if (block / 8 >= each / 8 + (block % 8 < more)) {
+            return;
+        }
+        const Place at = PlaceOf(TileOf(block, each), rowTiles, a.colTiles);
+        row0 = at.unit * kTileRows;
         rowEnd = a.numRows;
-        expert = tile / a.colTiles / rowTiles;
+        col0 = at.col * kTileCols;
     } else {
-        const int unit = int(blockIdx.x) / a.colTiles;
-        col0 = int(blockIdx.x) % a.colTiles * kTileCols;
-        const Unit u = FindUnit(a.offsets, a.groups, a.numRows, unit, kTileRows);
+        const int units = CountUnits(a.offsets, a.groups, a.numRows, kTileRows, int(gridDim.x) / a.colTiles);
+        if (int(blockIdx.x) >= units * a.colTiles) {
+            return;
+        }
+        const Place at = PlaceOf(TileOf(int(blockIdx.x), units * a.colTiles), units, a.colTiles);
+        const Unit u = FindUnit(a.offsets, a.groups, a.numRows, at.unit, kTileRows);
         if (u.group < 0) {
             return;
         }
@@ -266,17 +323,19 @@ __global__ void __launch_bounds__(64 * kWR * kWC) TileKernel(ProductArgs a)
         }
         row0 = u.first;
         rowEnd = u.last;
+        col0 = at.col * kTileCols;
     }
     const int64_t colBase = kGrad ? 0 : int64_t(expert) * a.numCols;
 
-    // what this lane loads: a 16-byte piece of a row, in every load
-    const uint8_t *from[kLoads];
+    // what this lane loads: a 16-byte piece of a row, in every load (rows behind the last one are beyond the buffer and read as zeros)
+    const uint8_t *rowsFrom = a.rows + int64_t(row0) * a.rowPitch, *colsFrom = a.cols + (colBase + col0) * a.colPitch;
+    const uint32_t rowBytes = uint32_t(min(rowEnd - row0, kTileRows)) * uint32_t(a.rowPitch);
+    const uint32_t colBytes = uint32_t(min(a.numCols - col0, kTileCols)) * uint32_t(a.colPitch);
+    int from[kLoads];
 #pragma unroll
     for (int j = 0; j < kLoads; j++) {
         const int oct = (j < kRowLoads ? j : j - kRowLoads) * kTileWaves + wave, piece = (lane % 8) ^ (lane / 16 + 4 * (oct % 2));
-        const int at = oct * 8 + lane / 8;
-        from[j] = (j < kRowLoads ? a.rows + int64_t(min(row0 + at, rowEnd - 1)) * a.rowPitch
-                                 : a.cols + (colBase + min(col0 + at, a.numCols - 1)) * a.colPitch) + piece * 16;
+        from[j] = int(uint32_t(oct * 8 + lane / 8) * uint32_t(j < kRowLoads ? a.rowPitch : a.colPitch) + uint32_t(piece * 16));
     }
     // and its scales
     const Stored *scaleFrom[kScales];
@@ -294,48 +353,56 @@ __global__ void __launch_bounds__(64 * kWR * kWC) TileKernel(ProductArgs a)
             scaleStep[j] = kGrad ? a.numCols : 1;
         }
     }
-    Stored coming[kScales];
-    const auto fetch = [&](int block, uint8_t *tile) __attribute__((always_inline)) {
+    uint32_t coming[kScales];
+    // Sends for a block; with `any` false for none: everything lies beyond an empty buffer, which costs no traffic, and the code of
+    // a step has no branch the scheduler could not look past.
+    const auto fetch = [&](int block, bool any, uint8_t *tile) __attribute__((always_inline)) {
 #pragma unroll
         for (int j = 0; j < kLoads; j++) {
             const int oct = (j < kRowLoads ? j : j - kRowLoads) * kTileWaves + wave;
             uint8_t *lds = tile + ((j < kRowLoads ? 0 : kTileRows) + oct * 8) * 128;
-            __builtin_amdgcn_global_load_lds((GlobalBytes)(from[j] + int64_t(block) * 128), (LdsBytes)lds, 16, 0, 0);
+            LoadToLds(j < kRowLoads ? rowsFrom : colsFrom, !any ? 0 : j < kRowLoads ? rowBytes : colBytes, lds, from[j], block * 128);
         }
 #pragma unroll
         for (int j = 0; j < kScales; j++) {
-            if (int(threadIdx.x) + j * kTileThreads < kTileRows + kTileCols) {
-                coming[j] = scaleFrom[j][block * scaleStep[j]];
-            }
+            coming[j] = ScaleBits(scaleFrom[j][block * scaleStep[j]]);
         }
     };
 
-    const int rowAt = wave / kWC * 16 * kRF, colAt = wave % kWC * 64;     // of this wave, in the tile
+    const int rowAt = wave / kWC * 16 * kRF, colAt = wave % kWC * 16 * kCF;     // of this wave, in the tile
     const int laneAt = l16 * 128 + ((quarter ^ (l16 / 2)) * 16);
     const auto fragment = [&](const uint8_t *rows16) {
         const Int4 lo = *reinterpret_cast<const Int4 *>(rows16 + laneAt), hi = *reinterpret_cast<const Int4 *>(rows16 + (laneAt ^ 64));
         return Int8{lo.x, lo.y, lo.z, lo.w, hi.x, hi.y, hi.z, hi.w};
     };
-    Float4 sum[kRF][4];
+    Float4 sum[kRF][kCF];
 #pragma unroll
     for (int r = 0; r < kRF; r++) {
 #pragma unroll
-        for (int c = 0; c < 4; c++) {
+        for (int c = 0; c < kCF; c++) {
             sum[r][c] = Zero4();
         }
     }
-    const auto multiply = [&](const uint8_t *tile, const uint32_t *scales) __attribute__((always_inline)) {
-        const uint8_t *rows = tile + rowAt * 128, *cols = tile + (kTileRows + colAt) * 128;
-        const uint32_t *rowScale = scales + rowAt, *colScale = scales + kTileRows + colAt;
-        Int8 w[4];
-        Wide32 wide[4];
-        float cs[4][4];
+    const auto keepScales = [&](uint32_t *scale) __attribute__((always_inline)) {
 #pragma unroll
-        for (int c = 0; c < 4; c++) {
-            w[c] = fragment(cols + c * 16 * 128);
-            if constexpr (kPrecise) {
-                wide[c] = Widen(w[c], kPowers ? PowerOf(uint8_t(colScale[c * 16 + l16])) : 1.0f);
-            }
+        for (int j = 0; j < kScales; j++) {
+            scale[int(threadIdx.x) + j * kTileThreads] = coming[j];
+        }
+    };
+    // The widened operands' form of a step: the block after it is sent for first, then this one is read and multiplied, in the order the
+    // compiler likes (widening between the products).
+    const auto wideStep = [&](uint8_t *tile, uint32_t *scale, uint8_t *other, int next, int last) __attribute__((always_inline)) {
+        keepScales(scale);
+        LoadsDone();
+        __syncthreads();     // this block is there, and nobody reads the other buffer any more
+        fetch(min(next, last), next <= last, other);
+        const uint8_t *rows = tile + rowAt * 128, *cols = tile + (kTileRows + colAt) * 128;
+        const uint32_t *rowScale = scale + rowAt, *colScale = scale + kTileRows + colAt;
+        Wide32 wide[kCF];
+        float cs[kCF][4];
+#pragma unroll
+        for (int c = 0; c < kCF; c++) {
+            wide[c] = Widen(fragment(cols + c * 16 * 128), kPowers ? PowerOf(uint8_t(colScale[c * 16 + l16])) : 1.0f);
             if constexpr (!kPowers) {
 #pragma unroll
                 for (int i = 0; i < 4; i++) {
@@ -345,51 +412,123 @@ __global__ void __launch_bounds__(64 * kWR * kWC) TileKernel(ProductArgs a)
         }
 #pragma unroll
         for (int r = 0; r < kRF; r++) {
-            const Int8 x = fragment(rows + r * 16 * 128);
-            const uint32_t rs = rowScale[r * 16 + l16];
-            Wide32 wideRow;
-            if constexpr (kPrecise) {
-                wideRow = Widen(x, kPowers ? PowerOf(uint8_t(rs)) : 1.0f);
-            }
+            const uint32_t power = rowScale[r * 16 + l16];
+            const Wide32 wideRow = Widen(fragment(rows + r * 16 * 128), kPowers ? PowerOf(uint8_t(power)) : 1.0f);
 #pragma unroll
-            for (int c = 0; c < 4; c++) {
-                if constexpr (kPowers && kPrecise) {
+            for (int c = 0; c < kCF; c++) {
+                if constexpr (kPowers) {
                     sum[r][c] = MfmaWide(wide[c], wideRow, sum[r][c]);
-                } else if constexpr (kPowers) {
-                    sum[r][c] = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(w[c], x, sum[r][c], 0, 0, 0, int(colScale[0]), 0, int(rs));
                 } else {
-                    const Float4 p = kPrecise ? MfmaWide(wide[c], wideRow, Zero4())
-                                              : __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(w[c], x, Zero4(), 0, 0, 0, 0, 0, 0);
+                    const Float4 p = MfmaWide(wide[c], wideRow, Zero4());
 #pragma unroll
                     for (int i = 0; i < 4; i++) {
-                        sum[r][c][i] = __builtin_fmaf(p[i], __uint_as_float(rs) * cs[c][i], sum[r][c][i]);
+                        sum[r][c][i] = __builtin_fmaf(p[i], __uint_as_float(power) * cs[c][i], sum[r][c][i]);
                     }
                 }
             }
         }
     };
-    // One step: this buffer's loads are under way; those of the block after it go into the other one.
-    const auto step = [&](uint8_t *tile, uint32_t *scale, uint8_t *other, int next, bool more) __attribute__((always_inline)) {
+    // What a step multiplies first has been read by the step before: its columns and its first sixteen rows.
+    Int8 w[kCF], x;
+    uint32_t rs = 0;
+    // One step.  Before its last sixteen rows are multiplied all of its block has been read: there the waves meet, the block after
+    // next is sent for into this step's buffer, and behind a column's last product the next step's take its place.
+    // (Behind the last block nothing is sent for, and what is read of the other buffer is not used.)
+    const auto step = [&](uint8_t *tile, const uint32_t *scale, uint8_t *other, uint32_t *otherScale, int afterNext, int last) __attribute__((always_inline)) {
+        const uint8_t *rows = tile + rowAt * 128;
+        const uint32_t *rowScale = scale + rowAt, *colScale = scale + kTileRows + colAt;
+        Wide32 wide[kCF];
+        float cs[kCF][4];
+        int csPower = 0;
 #pragma unroll
-        for (int j = 0; j < kScales; j++) {
-            if (int(threadIdx.x) + j * kTileThreads < kTileRows + kTileCols) {
-                scale[int(threadIdx.x) + j * kTileThreads] = ScaleBits(coming[j]);
+        for (int c = 0; c < kCF; c++) {
+            if constexpr (kPrecise) {
+                wide[c] = Widen(w[c], kPowers ? PowerOf(uint8_t(colScale[c * 16 + l16])) : 1.0f);
+            }
+            if constexpr (!kPowers) {
+#pragma unroll
+                for (int i = 0; i < 4; i++) {
+                    cs[c][i] = __uint_as_float(colScale[kGrad ? c * 16 + quarter * 4 + i : 0]);
+                }
+            } else {
+                csPower = int(colScale[0]);
             }
         }
-        LoadsDone();
-        __syncthreads();   // this buffer is full, and nobody reads the other one any more
-        if (more) {
-            fetch(next, other);
+#pragma unroll
+        for (int r = 0; r < kRF; r++) {
+            Int8 after;
+            uint32_t afterScale = 0;
+            if (r + 1 < kRF) {
+                after = fragment(rows + (r + 1) * 16 * 128);
+                afterScale = rowScale[(r + 1) * 16 + l16];
+            } else {
+                keepScales(otherScale);
+                LoadsDone();
+                __syncthreads();   // the next block is there, and nobody reads this one any more
+                fetch(min(afterNext, last), afterNext <= last, tile);
+                after = fragment(other + rowAt * 128);
+                afterScale = otherScale[rowAt + l16];
+            }
+            Wide32 wideRow;
+            if constexpr (kPrecise) {
+                wideRow = Widen(x, kPowers ? PowerOf(uint8_t(rs)) : 1.0f);
+            }
+            Float4 p[kCF];
+#pragma unroll
+            for (int c = 0; c < kCF; c++) {
+                if constexpr (kPowers && kPrecise) {
+                    sum[r][c] = MfmaWide(wide[c], wideRow, sum[r][c]);
+                } else if constexpr (kPowers) {
+                    sum[r][c] = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(w[c], x, sum[r][c], 0, 0, 0, csPower, 0, int(rs));
+                } else {
+                    p[c] = kPrecise ? MfmaWide(wide[c], wideRow, Zero4()) : __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(w[c], x, Zero4(), 0, 0, 0, 0, 0, 0);
+                }
+                if (r + 1 == kRF) {
+                    w[c] = fragment(other + (kTileRows + colAt + c * 16) * 128);
+                }
+            }
+            if constexpr (!kPowers) {
+#pragma unroll
+                for (int c = 0; c < kCF; c++) {
+#pragma unroll
+                    for (int i = 0; i < 4; i++) {
+                        sum[r][c][i] = __builtin_fmaf(p[c][i], __uint_as_float(rs) * cs[c][i], sum[r][c][i]);
+                    }
+                }
+            }
+            x = after;
+            rs = afterScale;
+            __builtin_amdgcn_sched_barrier(0);   // (the scheduler would read all rows first and run out of registers)
         }
-        multiply(tile, scale);
     };
     const auto run = [&](int first, int count) __attribute__((always_inline)) {
+        const int last = first + count - 1;
+        LoadsDone();
         __syncthreads();     // (the buffers are free: the blocks of another group may have been in them)
-        fetch(first, tile0);
+        fetch(first, true, tile0);
+        if constexpr (kPrecise) {
+            for (int i = 0; i < count; i += 2) {
+                wideStep(tile0, scales0, tile1, first + i + 1, last);
+                if (i + 1 < count) {
+                    wideStep(tile1, scales1, tile0, first + i + 2, last);
+                }
+            }
+            return;
+        }
+        keepScales(scales0);
+        LoadsDone();
+        __syncthreads();
+        fetch(min(first + 1, last), count > 1, tile1);
+        x = fragment(tile0 + rowAt * 128);
+        rs = scales0[rowAt + l16];
+#pragma unroll
+        for (int c = 0; c < kCF; c++) {
+            w[c] = fragment(tile0 + (kTileRows + colAt + c * 16) * 128);
+        }
         for (int i = 0; i < count; i += 2) {
-            step(tile0, scales0, tile1, first + i + 1, i + 1 < count);
+            step(tile0, scales0, tile1, scales1, first + i + 2, last);
             if (i + 1 < count) {
-                step(tile1, scales1, tile0, first + i + 2, i + 2 < count);
+                step(tile1, scales1, tile0, scales0, first + i + 3, last);
             }
         }
     };
@@ -401,29 +540,50 @@ __global__ void __launch_bounds__(64 * kWR * kWC) TileKernel(ProductArgs a)
         }
     }
 
+    // Out through LDS: a lane holds four neighbours of a row, the lanes of an instruction 16 rows; what leaves is whole rows of the
+    // wave's part, 16 bytes to a lane.  Pieces of a row lie in an order that depends on the row here too.
+    constexpr int kRowBytes = 16 * kCF * int(sizeof(T)), kPieces = kRowBytes / 16, kPer = 16 / int(sizeof(T));
+    constexpr int kWaveBytes = 16 * kRF * kRowBytes, kHalf = kTileWaves / 2;
+    static_assert(kWaveBytes * kHalf <= int(sizeof(tile0)), "the results fit the buffers");
+    LoadsDone();
+    __syncthreads();
+    uint8_t *mine = wave < kHalf ? tile0 + wave * kWaveBytes : tile1 + (wave - kHalf) * kWaveBytes;
+    const int64_t base = kGrad ? int64_t(expert) * a.numRows : 0;
+    const auto key = [](int row) { return sizeof(T) == 4 ? row % kPieces : row / 2 % kPieces; };
 #pragma unroll
     for (int r = 0; r < kRF; r++) {
-        const int row = row0 + rowAt + r * 16 + l16;
-        if (row < rowEnd) {
-            T *out = static_cast<T *>(a.out) + ((kGrad ? int64_t(expert) * a.numRows : 0) + row) * a.outPitch;
 #pragma unroll
-            for (int c = 0; c < 4; c++) {
-                const float v[4] = {sum[r][c][0], sum[r][c][1], sum[r][c][2], sum[r][c][3]};
-                const int col = col0 + colAt + c * 16 + quarter * 4;
-                if (a.wideOut) {
-                    if (col < a.numCols) {
-                        float w[4];
-                        if (kGrad && a.accumulate) {
-                            Load<true, 4>(out + col, w);
-                        }
+        for (int c = 0; c < kCF; c++) {
+            const int row = r * 16 + l16, byte = (c * 16 + quarter * 4) * int(sizeof(T));
+            float v[4] = {sum[r][c][0], sum[r][c][1], sum[r][c][2], sum[r][c][3]};
+            if (kGrad && a.accumulate) {
 #pragma unroll
-                        for (int i = 0; i < 4; i++) {
-                            w[i] = kGrad && a.accumulate ? w[i] + v[i] : v[i];
-                        }
-                        Store<true, 4>(out + col, w);
+                for (int i = 0; i < 4; i++) {
+                    const int to = row0 + rowAt + row, col = col0 + colAt + c * 16 + quarter * 4 + i;
+                    if (to < rowEnd && col < a.numCols) {
+                        v[i] += float(static_cast<const T *>(a.out)[(base + to) * a.outPitch + col]);
                     }
-                } else {
-                    StoreFour(out, v, col, a.numCols, kGrad && a.accumulate);
+                }
+            }
+            Store<true, 4>(reinterpret_cast<T *>(mine + row * kRowBytes + ((byte / 16 ^ key(row)) * 16 + byte % 16)), v);
+        }
+    }
+#pragma unroll
+    for (int i = 0; i < 16 * kRF * kPieces / 64; i++) {
+        const int at = i * 64 + lane, rowHere = at / kPieces, row = row0 + rowAt + rowHere, col = col0 + colAt + at % kPieces * kPer;
+        typedef T Vec __attribute__((ext_vector_type(kPer), aligned(16)));
+        const Vec v = *reinterpret_cast<const Vec *>(mine + rowHere * kRowBytes + ((at % kPieces) ^ key(rowHere)) * 16);
+        if (row >= rowEnd) {
+            continue;
+        }
+        T *out = static_cast<T *>(a.out) + (base + row) * a.outPitch + col;
+        if (a.wideOut && col < a.numCols) {
+            __builtin_nontemporal_store(v, reinterpret_cast<Vec *>(out));
+        } else if (!a.wideOut) {
+#pragma unroll
+            for (int j = 0; j < kPer; j++) {
+                if (col + j < a.numCols) {
+                    out[j] = v[j];
                 }
             }
         }
@@ -452,9 +612,11 @@ void Choose(HcclDataType type, HcclAmdScaleType scaleType, F f)
 
 constexpr uint64_t kMostTiles = uint64_t(1) << 22;   // workgroups of up to 512 below 2^32 threads
 
+constexpr int64_t kMostPitch = int64_t(1) << 23;     // bytes of a row: those of a tile's 256 rows are within 2^31
+
 bool WideOut(HcclDataType type, uint64_t width, const void *p, int64_t pitch)
 {
-    return width % 4 == 0 && pitch % 4 == 0 && Aligned(p, 4 * SizeOf(type));
+    return width * SizeOf(type) % 16 == 0 && uint64_t(pitch) * SizeOf(type) % 16 == 0 && Aligned(p, 16);
 }
 
 }  // namespace
@@ -516,6 +678,7 @@ HcclResult HcclAmdBlockMatmul(const void *a, uint64_t aStride, const void *aScal
     p.colTiles = int((n + tileCols - 1) / tileCols);
     const uint64_t units = offsets == nullptr ? (rows + tileRows - 1) / tileRows : rows / tileRows + groups;
     EXPERTS_CHK(units * uint64_t(p.colTiles) <= kMostTiles);
+    EXPERTS_CHK(p.rowPitch < kMostPitch && p.colPitch < kMostPitch);
     Choose(yType, scaleType, [&](auto of, auto scale) {
         typedef decltype(of) T;
         constexpr HcclAmdScaleType kScale = decltype(scale)::value;
@@ -528,15 +691,15 @@ HcclResult HcclAmdBlockMatmul(const void *a, uint64_t aStride, const void *aScal
         }
         if constexpr (sizeof(T) == 2) {
             if (large) {
-                go(TileKernel<T, kScale, false, false, 8, 2, 4>, 512);
+                go(TileKernel<T, kScale, false, false, 8, 4, 2, 4>, 512);
                 return;
             }
             if (fast) {
-                go(TileKernel<T, kScale, false, false, 4, 2, 2>, 256);
+                go(TileKernel<T, kScale, false, false, 4, 4, 2, 2>, 256);
                 return;
             }
         }
-        go(TileKernel<T, kScale, true, false, 4, 2, 2>, 256);
+        go(TileKernel<T, kScale, true, false, 4, 4, 2, 2>, 256);
     });
     return Launched("HcclAmdBlockMatmul");
 }
@@ -580,12 +743,13 @@ HcclResult HcclAmdBlockMatmulGradWeight(const void *yGradT, const void *yGradSca
     p.experts = int(experts);
     p.groupedRows = int(rows);
     p.accumulate = accumulate != 0;
+    EXPERTS_CHK(p.rowPitch < kMostPitch);
     p.wideOut = WideOut(gradType, k, wGrad, p.outPitch);
     p.colTiles = int((k + 127) / 128);
-    const uint64_t tiles = (n + 127) / 128 * uint64_t(p.colTiles) * experts;
+    const uint64_t tiles = ((n + 127) / 128 * uint64_t(p.colTiles) + 7) / 8 * 8 * experts;
     EXPERTS_CHK(tiles <= kMostTiles);
     Choose(gradType, scaleType, [&](auto of, auto scale) {
-        hipLaunchKernelGGL((TileKernel<decltype(of), decltype(scale)::value, true, true, 4, 2, 2>), dim3(uint32_t(tiles)), dim3(256), 0,
+        hipLaunchKernelGGL((TileKernel<decltype(of), decltype(scale)::value, true, true, 4, 4, 2, 2>), dim3(uint32_t(tiles)), dim3(256), 0,
             static_cast<hipStream_t>(stream), p);
     });
     return Launched("HcclAmdBlockMatmulGradWeight");
