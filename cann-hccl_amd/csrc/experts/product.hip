@@ -428,78 +428,82 @@ __global__ void __launch_bounds__(64 * kWR * kWC) TileKernel(ProductArgs a)
             }
         }
     };
-    // What a step multiplies first has been read by the step before: its columns and its first sixteen rows.
-    Int8 w[kCF], x;
-    uint32_t rs = 0;
-    // One step.  Before its last sixteen rows are multiplied all of its block has been read: there the waves meet, the block after
-    // next is sent for into this step's buffer, and behind a column's last product the next step's take its place.
+    // What a step multiplies first has been read by the step before: its columns and its first 32 rows.
+    Int8 w[kCF], x0, x1;
+    uint32_t rs0 = 0, rs1 = 0;
+    // One step.  Rows are read two sixteens ahead.  Before the last 32 are multiplied all of the block has been read: there the waves
+    // meet, the block after next is sent for into this step's buffer, and behind a column's last product the next step's take its place.
     // (Behind the last block nothing is sent for, and what is read of the other buffer is not used.)
     const auto step = [&](uint8_t *tile, const uint32_t *scale, uint8_t *other, uint32_t *otherScale, int afterNext, int last) __attribute__((always_inline)) {
         const uint8_t *rows = tile + rowAt * 128;
         const uint32_t *rowScale = scale + rowAt, *colScale = scale + kTileRows + colAt;
-        Wide32 wide[kCF];
-        float cs[kCF][4];
-        int csPower = 0;
-#pragma unroll
-        for (int c = 0; c < kCF; c++) {
-            if constexpr (kPrecise) {
-                wide[c] = Widen(w[c], kPowers ? PowerOf(uint8_t(colScale[c * 16 + l16])) : 1.0f);
-            }
-            if constexpr (!kPowers) {
-#pragma unroll
-                for (int i = 0; i < 4; i++) {
-                    cs[c][i] = __uint_as_float(colScale[kGrad ? c * 16 + quarter * 4 + i : 0]);
-                }
+        const float cs = kPowers ? 0.0f : __uint_as_float(colScale[0]);
+        const int csPower = kPowers ? int(colScale[0]) : 0;
+        const auto product = [&](Float4 &to, int c, const Int8 &x, uint32_t rs) __attribute__((always_inline)) {
+            if constexpr (kPowers) {
+                to = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(w[c], x, to, 0, 0, 0, csPower, 0, int(rs));
             } else {
-                csPower = int(colScale[0]);
+                to = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(w[c], x, Zero4(), 0, 0, 0, 0, 0, 0);
             }
-        }
+        };
+        const auto add = [&](Float4 &to, const Float4 &p, uint32_t rs) __attribute__((always_inline)) {
+            const float by = __uint_as_float(rs) * cs;
 #pragma unroll
-        for (int r = 0; r < kRF; r++) {
-            Int8 after;
-            uint32_t afterScale = 0;
-            if (r + 1 < kRF) {
-                after = fragment(rows + (r + 1) * 16 * 128);
-                afterScale = rowScale[(r + 1) * 16 + l16];
-            } else {
-                keepScales(otherScale);
-                LoadsDone();
-                __syncthreads();   // the next block is there, and nobody reads this one any more
-                fetch(min(afterNext, last), afterNext <= last, tile);
-                after = fragment(other + rowAt * 128);
-                afterScale = otherScale[rowAt + l16];
+            for (int i = 0; i < 4; i++) {
+                to[i] = __builtin_fmaf(p[i], by, to[i]);
             }
-            Wide32 wideRow;
-            if constexpr (kPrecise) {
-                wideRow = Widen(x, kPowers ? PowerOf(uint8_t(rs)) : 1.0f);
-            }
+        };
+#pragma unroll
+        for (int r = 0; r < kRF - 2; r++) {
+            const Int8 after = fragment(rows + (r + 2) * 16 * 128);
+            const uint32_t afterScale = rowScale[(r + 2) * 16 + l16];
             Float4 p[kCF];
 #pragma unroll
             for (int c = 0; c < kCF; c++) {
-                if constexpr (kPowers && kPrecise) {
-                    sum[r][c] = MfmaWide(wide[c], wideRow, sum[r][c]);
-                } else if constexpr (kPowers) {
-                    sum[r][c] = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(w[c], x, sum[r][c], 0, 0, 0, csPower, 0, int(rs));
-                } else {
-                    p[c] = kPrecise ? MfmaWide(wide[c], wideRow, Zero4()) : __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(w[c], x, Zero4(), 0, 0, 0, 0, 0, 0);
-                }
-                if (r + 1 == kRF) {
-                    w[c] = fragment(other + (kTileRows + colAt + c * 16) * 128);
-                }
+                product(kPowers ? sum[r][c] : p[c], c, x0, rs0);
             }
             if constexpr (!kPowers) {
 #pragma unroll
                 for (int c = 0; c < kCF; c++) {
-#pragma unroll
-                    for (int i = 0; i < 4; i++) {
-                        sum[r][c][i] = __builtin_fmaf(p[c][i], __uint_as_float(rs) * cs[c][i], sum[r][c][i]);
-                    }
+                    add(sum[r][c], p[c], rs0);
                 }
             }
-            x = after;
-            rs = afterScale;
+            x0 = x1;
+            rs0 = rs1;
+            x1 = after;
+            rs1 = afterScale;
             __builtin_amdgcn_sched_barrier(0);   // (the scheduler would read all rows first and run out of registers)
         }
+        keepScales(otherScale);
+        LoadsDone();
+        __syncthreads();   // the next block is there, and nobody reads this one any more
+        fetch(min(afterNext, last), afterNext <= last, tile);
+        const Int8 next0 = fragment(other + rowAt * 128), next1 = fragment(other + (rowAt + 16) * 128);
+        const uint32_t nextScale0 = otherScale[rowAt + l16], nextScale1 = otherScale[rowAt + 16 + l16];
+#pragma unroll
+        for (int c = 0; c < kCF; c++) {
+            Float4 p, q;
+            product(kPowers ? sum[kRF - 2][c] : p, c, x0, rs0);
+            product(kPowers ? sum[kRF - 1][c] : q, c, x1, rs1);
+            w[c] = fragment(other + (kTileRows + colAt + c * 16) * 128);
+            if constexpr (!kPowers) {
+                add(sum[kRF - 2][c], p, rs0);
+                add(sum[kRF - 1][c], q, rs1);
+            }
+        }
+        __builtin_amdgcn_sched_barrier(0);
+        x0 = next0;
+        x1 = next1;
+        rs0 = nextScale0;
+        rs1 = nextScale1;
+    };
+    // A wave all of whose rows lie behind the group's last one only loads.
+    const bool idle = !kGrad && row0 + rowAt >= rowEnd;
+    const auto idleStep = [&](uint8_t *to, uint32_t *scale, int next, int last) __attribute__((always_inline)) {
+        keepScales(scale);
+        LoadsDone();
+        __syncthreads();
+        fetch(min(next, last), next <= last, to);
     };
     const auto run = [&](int first, int count) __attribute__((always_inline)) {
         const int last = first + count - 1;
@@ -507,7 +511,10 @@ __global__ void __launch_bounds__(64 * kWR * kWC) TileKernel(ProductArgs a)
         __syncthreads();     // (the buffers are free: the blocks of another group may have been in them)
         fetch(first, true, tile0);
         if constexpr (kPrecise) {
-            for (int i = 0; i < count; i += 2) {
+            for (int i = 0; idle && i < count; i++) {
+                idleStep(i % 2 == 0 ? tile1 : tile0, i % 2 == 0 ? scales0 : scales1, first + i + 1, last);
+            }
+            for (int i = 0; !idle && i < count; i += 2) {
                 wideStep(tile0, scales0, tile1, first + i + 1, last);
                 if (i + 1 < count) {
                     wideStep(tile1, scales1, tile0, first + i + 2, last);
@@ -519,13 +526,18 @@ __global__ void __launch_bounds__(64 * kWR * kWC) TileKernel(ProductArgs a)
         LoadsDone();
         __syncthreads();
         fetch(min(first + 1, last), count > 1, tile1);
-        x = fragment(tile0 + rowAt * 128);
-        rs = scales0[rowAt + l16];
+        x0 = fragment(tile0 + rowAt * 128);
+        x1 = fragment(tile0 + (rowAt + 16) * 128);
+        rs0 = scales0[rowAt + l16];
+        rs1 = scales0[rowAt + 16 + l16];
 #pragma unroll
         for (int c = 0; c < kCF; c++) {
             w[c] = fragment(tile0 + (kTileRows + colAt + c * 16) * 128);
         }
-        for (int i = 0; i < count; i += 2) {
+        for (int i = 0; idle && i < count; i++) {
+            idleStep(i % 2 == 0 ? tile0 : tile1, i % 2 == 0 ? scales1 : scales0, first + i + 2, last);
+        }
+        for (int i = 0; !idle && i < count; i += 2) {
             step(tile0, scales0, tile1, scales1, first + i + 2, last);
             if (i + 1 < count) {
                 step(tile1, scales1, tile0, scales0, first + i + 3, last);
