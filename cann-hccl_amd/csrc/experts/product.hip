@@ -14,9 +14,6 @@ namespace hcclamd {
 namespace experts {
 namespace {
 
-constexpr int kThreads = 256;
-constexpr int kWaves = kThreads / 64;
-
 struct ProductArgs {
     const uint8_t *rows, *cols;
     const void *rowScales, *colScales;
@@ -95,15 +92,16 @@ __device__ __forceinline__ void StoreFour(T *out, const float (&v)[4], int col, 
     }
 }
 
-// 16 rows by 64 columns of the result to a workgroup, whose waves take every fourth block and add up through LDS: for few
-// rows, where the weights' bytes are what takes time and every wave should be reading them.
-template <typename T, HcclAmdScaleType kScale>
-__global__ void __launch_bounds__(kThreads) FewRowsKernel(ProductArgs a)
+// 16 rows by 16 kCF columns of the result to a workgroup, whose kWaves waves share the blocks out among them, kAhead at a time, and
+// add up through LDS: for few rows, where the weights' bytes are what takes time and as many waves as possible should be reading
+// them, all they need next at once.
+template <typename T, HcclAmdScaleType kScale, int kCF, int kWaves, int kAhead>
+__global__ void __launch_bounds__(64 * kWaves) FewRowsKernel(ProductArgs a)
 {
     constexpr bool kPowers = kScale == HCCL_AMD_SCALE_E8M0;
     typedef typename BlockScale<kScale>::Stored Stored;
-    __shared__ Float4 part[kWaves][4][64];
-    const int unit = int(blockIdx.x) / a.colTiles, col0 = int(blockIdx.x) % a.colTiles * 64;
+    __shared__ Float4 part[kWaves][kCF][64];
+    const int unit = int(blockIdx.x) / a.colTiles, col0 = int(blockIdx.x) % a.colTiles * 16 * kCF;
     const Unit u = FindUnit(a.offsets, a.groups, a.numRows, unit, 16);
     if (u.group < 0) {
         return;
@@ -112,48 +110,62 @@ __global__ void __launch_bounds__(kThreads) FewRowsKernel(ProductArgs a)
     if (expert < 0 || expert >= a.experts) {
         return;
     }
-    const int lane = int(threadIdx.x) % 64, wave = int(threadIdx.x) / 64, l16 = lane % 16, piece = lane / 16 * 16;
+    const int lane = int(threadIdx.x) % 64, wave = __builtin_amdgcn_readfirstlane(int(threadIdx.x) / 64), l16 = lane % 16, piece = lane / 16 * 16;
     const int64_t row = min(u.first + l16, u.last - 1);
     const uint8_t *rows = a.rows + row * a.rowPitch + piece;
     const Stored *rowScales = static_cast<const Stored *>(a.rowScales) + row * a.rowScalePitch;
-    // (a tile of 64 columns lies within one block of 128 of the weights' scales)
+    // (a workgroup's columns lie within one block of 128 of the weights' scales)
     const Stored *colScales = static_cast<const Stored *>(a.colScales) + (int64_t(expert) * ((a.numCols + 127) / 128) + col0 / 128) * a.blocks;
-    const uint8_t *cols[4];
-    Float4 sum[4];
+    const uint8_t *cols[kCF];
+    Float4 sum[kCF];
 #pragma unroll
-    for (int f = 0; f < 4; f++) {
+    for (int f = 0; f < kCF; f++) {
         const int col = min(col0 + f * 16 + l16, a.numCols - 1);
         cols[f] = a.cols + (int64_t(expert) * a.numCols + col) * a.colPitch + piece;
         sum[f] = Zero4();
     }
-    for (int b = wave; b < a.blocks; b += kWaves) {
-        const Int8 x = LoadLane(rows + int64_t(b) * 128);
-        Int8 w[4];
+    for (int b0 = wave; b0 < a.blocks; b0 += kWaves * kAhead) {
+        Int8 x[kAhead], w[kAhead][kCF];
+        Stored rs[kAhead], cs[kAhead];
 #pragma unroll
-        for (int f = 0; f < 4; f++) {
-            w[f] = LoadLane(cols[f] + int64_t(b) * 128);
+        for (int j = 0; j < kAhead; j++) {
+            const int b = min(b0 + j * kWaves, a.blocks - 1);       // (past the end the last one again, not used)
+            x[j] = LoadLane(rows + int64_t(b) * 128);
+#pragma unroll
+            for (int f = 0; f < kCF; f++) {
+                w[j][f] = LoadLane(cols[f] + int64_t(b) * 128);
+            }
+            rs[j] = rowScales[b];
+            cs[j] = colScales[b];
         }
-        const Stored rs = rowScales[b], cs = colScales[b];
-        const Wide32 wide = Widen(x, Inside(rs));
 #pragma unroll
-        for (int f = 0; f < 4; f++) {
-            if constexpr (kPowers) {
-                sum[f] = MfmaWide(Widen(w[f], Inside(cs)), wide, sum[f]);
-            } else {
-                const Float4 p = MfmaWide(Widen(w[f], 1.0f), wide, Zero4());
-                const float s = rs * cs;
+        for (int j = 0; j < kAhead; j++) {
+            if (b0 + j * kWaves < a.blocks) {
+                const Wide32 wide = Widen(x[j], Inside(rs[j]));
 #pragma unroll
-                for (int i = 0; i < 4; i++) {
-                    sum[f][i] = __builtin_fmaf(p[i], s, sum[f][i]);
+                for (int f = 0; f < kCF; f++) {
+                    if constexpr (kPowers) {
+                        sum[f] = MfmaWide(Widen(w[j][f], Inside(cs[j])), wide, sum[f]);
+                    } else {
+                        const Float4 p = MfmaWide(Widen(w[j][f], 1.0f), wide, Zero4());
+                        const float s = rs[j] * cs[j];
+#pragma unroll
+                        for (int i = 0; i < 4; i++) {
+                            sum[f][i] = __builtin_fmaf(p[i], s, sum[f][i]);
+                        }
+                    }
                 }
             }
         }
     }
 #pragma unroll
-    for (int f = 0; f < 4; f++) {
+    for (int f = 0; f < kCF; f++) {
         part[wave][f][lane] = sum[f];
     }
     __syncthreads();
+    if (wave >= kCF) {
+        return;
+    }
     // a wave adds up the 16 columns of its number
     Float4 total = part[0][wave][lane];
 #pragma unroll
@@ -214,7 +226,7 @@ __device__ __forceinline__ void ForGroupsOf(const ProductArgs &a, int expert, F 
 
 // ---- many rows -------------------------------------------------------------------------------------------
 
-constexpr int kBufferFlags = 0x00027000;    // a raw buffer of 32-bit words
+[[maybe_unused]] constexpr int kBufferFlags = 0x00027000;    // a raw buffer of 32-bit words
 typedef __attribute__((address_space(3))) void *LdsBytes;
 
 // How many units of `per` rows all groups make, `most` at most.  Called by all 64 lanes of a wave.
@@ -624,6 +636,15 @@ void Choose(HcclDataType type, HcclAmdScaleType scaleType, F f)
 
 constexpr uint64_t kMostTiles = uint64_t(1) << 22;   // workgroups of up to 512 below 2^32 threads
 
+// Tiles of 256 x 256 or of 128 x 128, from how many there are of each.  Of a product with 8192 values to a sum, a step takes 1.72 us where a
+// compute unit has a tile of 256, 1.25 us where it has two of 128 and 0.82 us where it has one; 256 and 512 are under way at once.
+// (2048 rows by 4096: 115 us with 256, 82 with 128; 4096 rows: 133 and 160.)
+bool LargeTiles(uint64_t tiles256, uint64_t tiles128)
+{
+    const uint64_t rest = tiles128 % 512;
+    return (tiles256 + 255) / 256 * 172 < tiles128 / 512 * 125 + (rest == 0 ? 0 : rest <= 256 ? 82 : 125);
+}
+
 constexpr int64_t kMostPitch = int64_t(1) << 23;     // bytes of a row: those of a tile's 256 rows are within 2^31
 
 bool WideOut(HcclDataType type, uint64_t width, const void *p, int64_t pitch)
@@ -682,13 +703,21 @@ HcclResult HcclAmdBlockMatmul(const void *a, uint64_t aStride, const void *aScal
     EXPERTS_CHK(uint64_t(p.outPitch) >= n && AlignedTo(yType, y));
     EXPERTS_CHK(Aligned(offsets, 4) && Aligned(expertOfGroup, 4));
     p.wideOut = WideOut(yType, n, y, p.outPitch);
-    const bool few = rows <= 32 * uint64_t(groups);
+    // Which kernel, 64 groups by 4096 x 2048 and one by 4096 x 8192, 32-bit scales: few rows against tiles of 128 takes 13 us against 17
+    // (8 rows, 64 groups), 88 against 100 (256 rows), 126 against 103 (512 rows); 8 against 49 (1 row, one group), 43 against 52 (128 rows), 83
+    // against 52 (256 rows).  16 columns to a workgroup instead of 64: 8 against 21 (1 row), 12 against 24 (16 rows), 39 against 24 (64 rows).
+    // Units there can be: every group that has rows ends with a shorter one.
+    const auto unitsOf = [&](uint64_t per) { return offsets == nullptr ? (rows + per - 1) / per : rows / per + (rows < groups ? rows : groups); };
+    const uint64_t few64 = unitsOf(16) * ((n + 63) / 64);
+    const bool few = rows <= 4 * uint64_t(groups) || few64 <= 640, narrow = few64 < 192;
     // sums of 16-bit results over more than two blocks: the 8-bit instruction's error is behind their own rounding
     const bool fast = yType != HCCL_DATA_TYPE_FP32 && k > 256;
-    const bool large = fast && rows >= 256 * uint64_t(groups) && n >= 256;
-    const uint64_t tileRows = few ? 16 : large ? 256 : 128, tileCols = few ? 64 : large ? 256 : 128;
+    // half of the groups' last units are counted: the others' rows fill up one that is counted already
+    const auto tilesOf = [&](uint64_t per) { return ((rows + per - 1) / per + (rows < groups ? rows : groups) / 2) * ((n + per - 1) / per); };
+    const bool large = !few && fast && LargeTiles(tilesOf(256), tilesOf(128));
+    const uint64_t tileRows = few ? 16 : large ? 256 : 128, tileCols = few ? (narrow ? 16 : 64) : large ? 256 : 128;
     p.colTiles = int((n + tileCols - 1) / tileCols);
-    const uint64_t units = offsets == nullptr ? (rows + tileRows - 1) / tileRows : rows / tileRows + groups;
+    const uint64_t units = unitsOf(tileRows);
     EXPERTS_CHK(units * uint64_t(p.colTiles) <= kMostTiles);
     EXPERTS_CHK(p.rowPitch < kMostPitch && p.colPitch < kMostPitch);
     Choose(yType, scaleType, [&](auto of, auto scale) {
@@ -698,7 +727,7 @@ HcclResult HcclAmdBlockMatmul(const void *a, uint64_t aStride, const void *aScal
             hipLaunchKernelGGL(kernel, dim3(uint32_t(units * uint64_t(p.colTiles))), dim3(threads), 0, static_cast<hipStream_t>(stream), p);
         };
         if (few) {
-            go(FewRowsKernel<T, kScale>, kThreads);
+            narrow ? go(FewRowsKernel<T, kScale, 1, 8, 4>, 512) : go(FewRowsKernel<T, kScale, 4, 4, 2>, 256);
             return;
         }
         if constexpr (sizeof(T) == 2) {

@@ -479,6 +479,14 @@ def test_matmul_large(stream, kind, rows, n, k):
     check_matmul(stream, rng, rows, 8, 8, n // 2, k, kind, "fp32", strides=True)
 
 
+@pytest.mark.parametrize("kind", ["fp32", "e8m0"])
+@pytest.mark.parametrize("rows,groups,n,k,dtype", [(4100, 1, 4100, 300, "bf16"), (4100, 1, 4104, 1000, "fp16"), (6000, 3, 2600, 513, "bf16")])
+def test_matmul_many_tiles(stream, kind, rows, groups, n, k, dtype):
+    """Enough for tiles of 256 x 256; groups whose last tile is nearly empty, odd and even numbers of blocks."""
+    rng = np.random.default_rng(rows + k)
+    check_matmul(stream, rng, rows, groups, groups, n, k, kind, dtype, strides=n % 8 != 0)
+
+
 def test_matmul_offsets_and_owners_that_point_outside(stream):
     """Whatever the device's offsets and owners hold, no row outside is written and no weights outside are read."""
     rng = np.random.default_rng(8)
