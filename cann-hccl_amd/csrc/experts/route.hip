@@ -5,13 +5,16 @@
 //   loss = c E sum_e (n_e / A) (sum_t p_te / T)       d loss / d p_te = c E n_e / (A T)
 //   w_j = p_j, or p_j / sum of the chosen p           dx = p (g - sum p g), and for the quotient w_j (dw_j - sum_i w_i dw_i)
 //
-// The logits are read once.  A workgroup holds a tile of tokens in LDS; several lanes share a token.  Every lane keeps the
-// topK largest of its experts in registers as a sorted list -- inserting costs five instructions per entry and no exchange
-// between lanes, whereas finding one maximum after the other over a whole wave costs six exchanges for each -- and the lists of a
-// token's lanes are merged at the end.  Which tokens of the tile chose an expert is a mask of one bit per token: set with
-// LDS atomics whose order cannot matter, its bits counted in front of a token give the token's place, and counts and rows are the
-// same in every run.  Tiles leave counts and probability sums in the workspace, a second launch sums them expert by expert in
-// tile order, a third adds up the rows' places.  Up to one tile (single tokens of a decoding step, small batches) one launch does it all.
+// The logits are read once, into registers, a token's by several lanes.  Every lane keeps the topK largest of its experts as a
+// sorted list: a new one is put in without exchanges between lanes -- for 16-bit logits value and expert share a word, and one
+// median of three per entry does it -- and the lists of a token's lanes are merged at the end.  Which tokens of a tile of 64 chose an
+// expert is a mask of one bit per token: set with LDS atomics whose order cannot matter, its bits counted in front of a token give the
+// token's place, so that counts and rows are the same in every run.  A workgroup goes through several tiles and leaves its counts and
+// probability sums in the workspace; a second launch adds up what lies in front of every workgroup's, a third adds that to the
+// rows.  Up to 64 tokens (a decoding
+// step) one launch does it all.
+#include <type_traits>
+
 #include "common.h"
 
 namespace hcclamd {
@@ -20,7 +23,7 @@ namespace {
 
 constexpr int kThreads = 256;
 constexpr uint32_t kNone = 0xffffffffu;
-constexpr uint64_t kMaxTokens = uint64_t(1) << 25;   // 64 lanes each stay below the 2^32 threads of a grid
+constexpr uint64_t kMaxTokens = uint64_t(1) << 25;
 
 struct RouteArgs {
     const void *logits;
@@ -31,65 +34,194 @@ struct RouteArgs {
     int32_t *counts;
     int32_t *offsets;
     float *loss;
-    int32_t *tileCounts;   // [tiles][experts + 1]: rows per expert, then first row per expert within the expert's; last column: tokens that chose
-    float *tileSums;       // [tiles][experts]: sum of probabilities
+    int32_t *blockCounts;  // [blocks][experts + 1]: rows per expert; last column: tokens that chose
+    float *blockSums;      // [blocks][experts]: sum of probabilities
     float *sums;           // [experts]
     int64_t stride;
-    int tokens, experts, topK, tiles;
-    int rowWords;          // LDS words from one token to the next
+    int tokens, experts, topK;
+    int blocks, tiles;     // workgroups; tiles of each
     float lossScale;
     bool renormalise;
 };
 
-// (value, expert) pairs ordered by value, then by lower expert.  Lists are sorted, largest first; an empty place is
-// (-inf, kNone), which every logit that may be chosen precedes.
-struct Entry {
-    float v;
-    uint32_t e;
-};
+// exp of a difference to the row's maximum.  Its argument, at most 0, is rounded twice, which moves a probability by 2^-24 of
+// the difference; the hardware's power of two is good to one unit.
+__device__ __forceinline__ float Exp(float d) { return __builtin_amdgcn_exp2f(d * 1.44269504088896340736f); }
 
-__device__ __forceinline__ bool Before(const Entry &a, const Entry &b) { return a.v > b.v || (a.v == b.v && a.e < b.e); }
+// ---- sorted lists of the K largest ------------------------------------------------------------------------
+// Ordered by value, then by lower expert.  An empty place precedes nothing; -inf and NaN are never put in.
 
-// No instruction.  Without it the compiler reasons about chains of dozens of selects as one, for hours.
-__device__ __forceinline__ void Settle(Entry &x) { asm("" : "+v"(x.v), "+v"(x.e)); }
-
-// The larger half of two sorted lists: element by element against the other one backwards, which leaves a sequence that
-// rises and falls once, then sorted by halving.
+// 16-bit logits: a word of the value, mapped to an unsigned number of the same order, and the expert, complemented.  0: empty.
 template <int K>
-__device__ __forceinline__ void Merge(Entry (&a)[K], int lanes)
-{
-    Entry b[K];
-#pragma unroll
-    for (int i = 0; i < K; i++) {
-        b[i].v = __shfl_xor(a[i].v, lanes, 64);
-        b[i].e = __shfl_xor(a[i].e, lanes, 64);
-    }
-#pragma unroll
-    for (int i = 0; i < K; i++) {
-        const bool take = Before(b[K - 1 - i], a[i]);
-        a[i].v = take ? b[K - 1 - i].v : a[i].v;
-        a[i].e = take ? b[K - 1 - i].e : a[i].e;
-        Settle(a[i]);
-    }
-#pragma unroll
-    for (int d = K / 2; d > 0; d >>= 1) {
+struct WordList {
+    uint32_t best[K];
+
+    __device__ __forceinline__ WordList()
+    {
 #pragma unroll
         for (int i = 0; i < K; i++) {
-            if ((i & d) == 0) {
-                const bool swap = Before(a[i + d], a[i]);
-                const Entry lo = a[i], hi = a[i + d];
-                a[i].v = swap ? hi.v : lo.v;
-                a[i].e = swap ? hi.e : lo.e;
-                a[i + d].v = swap ? lo.v : hi.v;
-                a[i + d].e = swap ? lo.e : hi.e;
-                Settle(a[i]);
-                Settle(a[i + d]);
+            best[i] = 0;
+        }
+    }
+    template <typename T>
+    __device__ __forceinline__ void Put(float v, uint32_t expert)
+    {
+        // (v + 0: both zeros are one value)
+        uint32_t bits;     // of the logit, in the upper half
+        if constexpr (std::is_same_v<T, __bf16>) {
+            bits = __float_as_uint(v + 0.0f);
+        } else {
+            bits = uint32_t(__builtin_bit_cast(uint16_t, T(v + 0.0f))) << 16;
+        }
+        const uint32_t order = bits ^ (uint32_t(int32_t(bits) >> 31) | 0x80000000u);
+        const uint32_t word = v > -__builtin_inff() ? (order & 0xffff0000u) | (0xffffu - expert) : 0;
+        // of a sorted list and a new word the i-th is the median of the (i - 1)-th, the i-th and the new one
+#pragma unroll
+        for (int i = K - 1; i > 0; i--) {
+            const uint32_t low = best[i - 1] < word ? best[i - 1] : word;
+            best[i] = best[i] > low ? best[i] : low;
+        }
+        best[0] = best[0] > word ? best[0] : word;
+    }
+    // The larger half of two lists: element by element against the other one backwards, which leaves a sequence that rises and falls
+    // once, then sorted by halving.
+    __device__ __forceinline__ void Merge(int lanes)
+    {
+        uint32_t other[K];
+#pragma unroll
+        for (int i = 0; i < K; i++) {
+            other[i] = __shfl_xor(best[i], lanes, 64);
+        }
+#pragma unroll
+        for (int i = 0; i < K; i++) {
+            best[i] = best[i] > other[K - 1 - i] ? best[i] : other[K - 1 - i];
+        }
+#pragma unroll
+        for (int d = K / 2; d > 0; d >>= 1) {
+#pragma unroll
+            for (int i = 0; i < K; i++) {
+                if ((i & d) == 0) {
+                    const uint32_t hi = best[i] > best[i + d] ? best[i] : best[i + d], lo = best[i] > best[i + d] ? best[i + d] : best[i];
+                    best[i] = hi;
+                    best[i + d] = lo;
+                }
             }
         }
     }
+    template <typename T>
+    __device__ __forceinline__ float Value(int i) const
+    {
+        const uint32_t order = best[i] >> 16;
+        return float(__builtin_bit_cast(T, uint16_t(order ^ ((order & 0x8000u) != 0 ? 0x8000u : 0xffffu))));
+    }
+    __device__ __forceinline__ uint32_t Expert(int i) const { return best[i] == 0 ? kNone : 0xffffu - (best[i] & 0xffffu); }
+};
+
+// 32-bit logits: value and expert apart.
+template <int K>
+struct PairList {
+    float v[K];
+    uint32_t e[K];
+
+    __device__ __forceinline__ PairList()
+    {
+#pragma unroll
+        for (int i = 0; i < K; i++) {
+            v[i] = -__builtin_inff();
+            e[i] = kNone;
+        }
+    }
+    // No instruction.  Without it the compiler reasons about chains of dozens of selects as one, for hours.
+    __device__ __forceinline__ void Settle(int i) { asm("" : "+v"(v[i]), "+v"(e[i])); }
+
+    // x goes behind the last entry that is not less, those after it move on.  A lane's experts come in ascending order: of
+    // equal values the one that is there stays in front (and NaN, greater than nothing, is never put in).
+    template <typename T>
+    __device__ __forceinline__ void Put(float x, uint32_t expert)
+    {
+        bool ahead = x > v[K - 1];
+#pragma unroll
+        for (int i = K - 1; i > 0; i--) {
+            const bool further = x > v[i - 1];
+            v[i] = further ? v[i - 1] : ahead ? x : v[i];
+            e[i] = further ? e[i - 1] : ahead ? expert : e[i];
+            ahead = further;
+        }
+        v[0] = ahead ? x : v[0];
+        e[0] = ahead ? expert : e[0];
+    }
+    __device__ __forceinline__ void Merge(int lanes)
+    {
+        float ov[K];
+        uint32_t oe[K];
+#pragma unroll
+        for (int i = 0; i < K; i++) {
+            ov[i] = __shfl_xor(v[i], lanes, 64);
+            oe[i] = __shfl_xor(e[i], lanes, 64);
+        }
+#pragma unroll
+        for (int i = 0; i < K; i++) {
+            const int j = K - 1 - i;
+            const bool take = ov[j] > v[i] || (ov[j] == v[i] && oe[j] < e[i]);
+            v[i] = take ? ov[j] : v[i];
+            e[i] = take ? oe[j] : e[i];
+            Settle(i);
+        }
+#pragma unroll
+        for (int d = K / 2; d > 0; d >>= 1) {
+#pragma unroll
+            for (int i = 0; i < K; i++) {
+                if ((i & d) == 0) {
+                    const bool swap = v[i + d] > v[i] || (v[i + d] == v[i] && e[i + d] < e[i]);
+                    const float hv = swap ? v[i + d] : v[i], lv = swap ? v[i] : v[i + d];
+                    const uint32_t he = swap ? e[i + d] : e[i], le = swap ? e[i] : e[i + d];
+                    v[i] = hv;
+                    e[i] = he;
+                    v[i + d] = lv;
+                    e[i + d] = le;
+                    Settle(i);
+                    Settle(i + d);
+                }
+            }
+        }
+    }
+    template <typename T>
+    __device__ __forceinline__ float Value(int i) const { return v[i]; }
+    __device__ __forceinline__ uint32_t Expert(int i) const { return e[i]; }
+};
+
+template <typename T, int K>
+using List = std::conditional_t<sizeof(T) == 2, WordList<K>, PairList<K>>;
+
+// ---- sums ------------------------------------------------------------------------------------------------
+
+// Adds up over the lanes whose numbers agree above the lowest bits: kLanes neighbouring lanes, a power of two up to 64.
+template <int kLanes>
+__device__ __forceinline__ float AddNeighbours(float x)
+{
+#pragma unroll
+    for (int d = 1; d < kLanes; d <<= 1) {
+        x += __shfl_xor(x, d, 64);
+    }
+    return x;
 }
 
-// Exclusive prefix sums of n <= 1024 values in LDS by one workgroup, and the total; `part`: kThreads words.
+// The same over 16 lanes without a pass through LDS.
+template <>
+__device__ __forceinline__ float AddNeighbours<16>(float x)
+{
+    const auto turned = [&](auto by) {
+        return __int_as_float(__builtin_amdgcn_update_dpp(0, __float_as_int(x), 0x120 + decltype(by)::value, 0xf, 0xf, true));   // row_ror
+    };
+    x += turned(std::integral_constant<int, 8>{});
+    x += turned(std::integral_constant<int, 4>{});
+    x += turned(std::integral_constant<int, 2>{});
+    x += turned(std::integral_constant<int, 1>{});
+    return x;
+}
+
+// Exclusive prefix sums of n <= 1024 values in LDS, in place, by kThreads threads; returns the total.  `part`: a word per wave.
+template <int kThreads>
 __device__ __forceinline__ int Scan(int *values, int n, int *part)
 {
     const int per = (n + kThreads - 1) / kThreads, from = min(n, int(threadIdx.x) * per), to = min(n, from + per);
@@ -97,16 +229,22 @@ __device__ __forceinline__ int Scan(int *values, int n, int *part)
     for (int i = from; i < to; i++) {
         mine += values[i];
     }
-    part[threadIdx.x] = mine;
-    __syncthreads();
-    for (int d = 1; d < kThreads; d <<= 1) {
-        const int other = int(threadIdx.x) >= d ? part[threadIdx.x - d] : 0;
-        __syncthreads();
-        part[threadIdx.x] += other;
-        __syncthreads();
+    const int lane = int(threadIdx.x) % 64;
+    int sum = mine;
+#pragma unroll
+    for (int d = 1; d < 64; d <<= 1) {
+        const int other = __shfl_up(sum, d, 64);
+        sum += lane >= d ? other : 0;
     }
-    int at = part[threadIdx.x] - mine;
-    const int total = part[kThreads - 1];
+    if (lane == 63) {
+        part[threadIdx.x / 64] = sum;
+    }
+    __syncthreads();
+    int at = sum - mine, total = 0;
+    for (int w = 0; w < kThreads / 64; w++) {
+        at += w < int(threadIdx.x) / 64 ? part[w] : 0;
+        total += part[w];
+    }
     for (int i = from; i < to; i++) {
         const int v = values[i];
         values[i] = at;
@@ -116,220 +254,253 @@ __device__ __forceinline__ int Scan(int *values, int n, int *part)
     return total;
 }
 
-// counts[experts + 1], offsets and the loss from per-expert counts and sums in LDS; afterwards `count` holds the offsets.
+// counts[experts + 1], offsets and the loss (`write`) from per-expert counts and sums in LDS; afterwards `count` holds the offsets.
+template <int kThreads>
 __device__ __forceinline__ void Finish(const RouteArgs &a, int *count, const float *sum, int tokens, int *part, float *partSum, bool write)
 {
     float load = 0.0f;
-    for (int e = threadIdx.x; e < a.experts; e += kThreads) {
+    for (int e = threadIdx.x; e < a.experts && write; e += kThreads) {
         load += float(count[e]) * sum[e];
-        if (write) {
-            a.counts[e] = count[e];
-        }
+        a.counts[e] = count[e];
+    }
+    load = AddNeighbours<64>(load);
+    if (threadIdx.x % 64 == 0) {
+        partSum[threadIdx.x / 64] = load;
     }
     __syncthreads();
-    const int rows = Scan(count, a.experts, part);
+    const int rows = Scan<kThreads>(count, a.experts, part);
     if (!write) {
         return;
     }
     for (int e = threadIdx.x; e < a.experts; e += kThreads) {
         a.offsets[e] = count[e];
     }
-    partSum[threadIdx.x] = load;
-    for (int d = kThreads / 2; d > 0; d >>= 1) {
-        __syncthreads();
-        if (int(threadIdx.x) < d) {
-            partSum[threadIdx.x] += partSum[threadIdx.x + d];
-        }
-    }
     if (threadIdx.x == 0) {
+        float all = 0.0f;
+        for (int w = 0; w < kThreads / 64; w++) {
+            all += partSum[w];
+        }
         a.counts[a.experts] = tokens;
         a.offsets[a.experts] = rows;
-        a.loss[0] = rows == 0 ? 0.0f : a.lossScale * float(a.experts) * (partSum[0] / float(rows) / float(tokens));
+        a.loss[0] = rows == 0 ? 0.0f : a.lossScale * float(a.experts) * (all / float(rows) / float(tokens));
+    }
+}
+
+// The waves' parts of the sums of probabilities: over a wave's tokens in registers, over the waves in LDS, into sum[0 .. experts).
+template <int kWaveTokens, int kLanes, int kEach>
+__device__ __forceinline__ void Columns(const float (&column)[kEach], float *sum, int experts, int lane, int wave, int l)
+{
+#pragma unroll
+    for (int i = 0; i < kEach; i++) {
+        const float s = AddNeighbours<kWaveTokens>(column[i]);
+        const int e = (i / 8 * kLanes + l) * 8 + i % 8;
+        if (lane % kWaveTokens == 0 && e < experts) {
+            sum[wave * experts + e] = s;
+        }
+    }
+    __syncthreads();
+    for (int e = threadIdx.x; e < experts; e += kThreads) {
+        float s = sum[e];
+        for (int w = 1; w < kThreads / 64; w++) {
+            s += sum[w * experts + e];
+        }
+        sum[e] = s;
     }
     __syncthreads();
 }
 
-// kLanes lanes to a token, kThreads / kLanes tokens to a tile; lists of K.
-template <typename T, int K, int kLanes>
+// kLanes lanes to a token, each with kChunks times eight neighbouring experts; lists of K.  Token t of a wave's 64 / kLanes is in
+// the lanes whose number leaves t.
+template <typename T, int K, int kLanes, int kChunks, bool kWide>
 __global__ void __launch_bounds__(kThreads) RouteKernel(RouteArgs a)
 {
-    constexpr int kTile = kThreads / kLanes;
-    extern __shared__ float lds[];
-    float *tile = lds;                                                               // [kTile][rowWords]
-    float *share = tile + kTile * a.rowWords;                                        // [kTile]: 1 / sum of a token's exponentials, 0 without
-    uint32_t *chose = reinterpret_cast<uint32_t *>(share + kTile);                   // [experts][2]: one bit per token
-    int *count = reinterpret_cast<int *>(chose + 2 * a.experts);                     // [experts]
-    float *sum = reinterpret_cast<float *>(count + a.experts);                       // [experts]
-    int *part = reinterpret_cast<int *>(sum + a.experts);                            // [kThreads]
-    float *partSum = reinterpret_cast<float *>(part + kThreads);                     // [kThreads]
-    uint32_t *routed = reinterpret_cast<uint32_t *>(partSum + kThreads);             // [1]
-
-    const int first = int(blockIdx.x) * kTile, here = min(kTile, a.tokens - first);
+    constexpr int kWaveTokens = 64 / kLanes, kTile = kWaveTokens * kThreads / 64, kEach = 8 * kChunks;
+    extern __shared__ uint32_t lds[];
     const int E = a.experts;
-    for (int e = threadIdx.x; e < 2 * E; e += kThreads) {
-        chose[e] = 0;
+    uint32_t *chose = lds;                                                // [experts][2]: one bit per token of the tile
+    int *count = reinterpret_cast<int *>(chose + 2 * E);                  // [experts]: rows of the tiles so far
+    float *sum = reinterpret_cast<float *>(count + E);                    // [waves][experts]
+    int *part = reinterpret_cast<int *>(sum + kThreads / 64 * E);         // [waves]
+    float *partSum = reinterpret_cast<float *>(part + kThreads / 64);     // [waves]
+    int *routed = reinterpret_cast<int *>(partSum + kThreads / 64);       // [1]
+
+    const int lane = int(threadIdx.x) % 64, wave = int(threadIdx.x) / 64, l = lane / kWaveTokens, r = wave * kWaveTokens + lane % kWaveTokens;
+    for (int e = threadIdx.x; e < E; e += kThreads) {
+        chose[2 * e] = chose[2 * e + 1] = 0;
+        count[e] = 0;
     }
     if (threadIdx.x == 0) {
         *routed = 0;
     }
-    const T *logits = static_cast<const T *>(a.logits) + int64_t(first) * a.stride;
-    for (int r = threadIdx.x / kLanes, l = threadIdx.x % kLanes; r < here; r += kTile) {
-        const bool in = a.mask == nullptr || a.mask[first + r] != 0;
-        for (int e = l; e < E; e += kLanes) {
-            tile[r * a.rowWords + e] = in ? float(logits[int64_t(r) * a.stride + e]) : -__builtin_inff();
-        }
-    }
     __syncthreads();
-
-    const int r = threadIdx.x / kLanes, l = threadIdx.x % kLanes;
-    float *row = tile + r * a.rowWords;
-    Entry best[K];
+    float column[kEach];          // this lane's part of the sums of probabilities
 #pragma unroll
-    for (int i = 0; i < K; i++) {
-        best[i] = Entry{-__builtin_inff(), kNone};
+    for (int i = 0; i < kEach; i++) {
+        column[i] = 0.0f;
     }
-    if (r < here) {
-        for (int e = l; e < E; e += kLanes) {
-            const float x = row[e];
-            // x goes behind the last entry that is not less, those after it move on.  Experts come in ascending order: of
-            // equal values the one that is there stays in front (and NaN, greater than nothing, is never put in)
-            bool ahead = x > best[K - 1].v;
+    for (int tile = 0; tile < a.tiles; tile++) {
+        const int token = (int(blockIdx.x) * a.tiles + tile) * kTile + r;
+        const bool in = token < a.tokens && (a.mask == nullptr || a.mask[token] != 0);
+        const T *row = static_cast<const T *>(a.logits) + int64_t(in ? token : 0) * a.stride;
+        float x[kEach];
+        List<T, K> best;
 #pragma unroll
-            for (int i = K - 1; i > 0; i--) {
-                const bool further = x > best[i - 1].v;
-                best[i].v = further ? best[i - 1].v : ahead ? x : best[i].v;
-                best[i].e = further ? best[i - 1].e : ahead ? uint32_t(e) : best[i].e;
-                ahead = further;
+        for (int c = 0; c < kChunks; c++) {
+            const int e = (c * kLanes + l) * 8;
+            if (kWide) {
+                float v[8];
+                if (in && e < E) {
+                    Load<true, 8>(row + e, v);
+                }
+#pragma unroll
+                for (int i = 0; i < 8; i++) {
+                    x[c * 8 + i] = in && e < E ? v[i] : -__builtin_inff();
+                }
+            } else {
+#pragma unroll
+                for (int i = 0; i < 8; i++) {
+                    x[c * 8 + i] = in && e + i < E ? float(row[e + i]) : -__builtin_inff();
+                }
             }
-            best[0].v = ahead ? x : best[0].v;
-            best[0].e = ahead ? uint32_t(e) : best[0].e;
         }
-    }
+#pragma unroll
+        for (int c = 0; c < kChunks; c++) {
+#pragma unroll
+            for (int i = 0; i < 8; i++) {
+                best.template Put<T>(x[c * 8 + i], uint32_t((c * kLanes + l) * 8 + i));
+            }
+        }
 #pragma unroll 1
-    for (int d = 1; d < kLanes; d <<= 1) {
-        Merge<K>(best, d);
-    }
-    const float top = best[0].v;
-    const bool any = best[0].e != kNone;
-    float total = 0.0f;
-    if (r < here && any) {
-        for (int e = l; e < E; e += kLanes) {
-            const float x = expf(row[e] - top);
-            row[e] = x;
-            total += x;
+        for (int d = kWaveTokens; d < 64; d <<= 1) {
+            best.Merge(d);
         }
-    }
+        const bool any = best.Expert(0) != kNone;
+        const float top = any ? best.template Value<T>(0) : 0.0f;
+        float total = 0.0f;
 #pragma unroll
-    for (int d = 1; d < kLanes; d <<= 1) {
-        total += __shfl_xor(total, d, 64);
-    }
-    // (a row that chose nothing adds nothing to the sums, whatever it holds)
-    const float times = any ? 1.0f / total : 0.0f;
-    if (r < here && l == 0) {
-        share[r] = times;
-        if (any) {
-            atomicAdd(routed, 1u);   // a whole number: the order does not matter
+        for (int i = 0; i < kEach; i++) {
+            x[i] = Exp(x[i] - top);
+            total += x[i];
         }
-    }
-    float inside = 0.0f, weight[K];
 #pragma unroll
-    for (int i = 0; i < K; i++) {
-        weight[i] = i < a.topK && best[i].e != kNone ? expf(best[i].v - top) : 0.0f;
-        inside += weight[i];
-    }
-    const bool bad = any && !(total < __builtin_inff());   // a NaN or +inf in the row: its weights are NaN, chosen or not by these
-    const float by = bad ? __builtin_nanf("") : a.renormalise ? (any ? 1.0f / inside : 0.0f) : times;
-    if (r < here) {
+        for (int d = kWaveTokens; d < 64; d <<= 1) {
+            total += __shfl_xor(total, d, 64);
+        }
+        // (a token that chose nothing adds nothing to the sums, whatever its row holds)
+        const float times = 1.0f / total;
+#pragma unroll
+        for (int i = 0; i < kEach; i++) {
+            column[i] += any ? x[i] * times : 0.0f;
+        }
+        float inside = 0.0f, weight[K];
 #pragma unroll
         for (int i = 0; i < K; i++) {
-            if (i < a.topK && i % kLanes == l) {
-                const int64_t at = int64_t(first + r) * a.topK + i;
-                const bool is = best[i].e != kNone;
-                a.expertOf[at] = is ? int32_t(best[i].e) : -1;
-                a.weights[at] = is ? weight[i] * by : 0.0f;
-                if (is) {
-                    atomicOr(&chose[2 * best[i].e + (r >> 5)], 1u << (r & 31));
+            weight[i] = i < a.topK && best.Expert(i) != kNone ? Exp(best.template Value<T>(i) - top) : 0.0f;
+            inside += weight[i];
+        }
+        const bool bad = !(total < __builtin_inff());   // a NaN or +inf in the row: its weights are NaN, chosen or not by these
+        const float by = bad ? __builtin_nanf("") : a.renormalise ? 1.0f / inside : times;
+        if (any && l == 0) {
+            atomicAdd(routed, 1);   // a whole number: the order does not matter
+        }
+        if (token < a.tokens) {
+#pragma unroll
+            for (int i = 0; i < K; i++) {
+                if (i < a.topK && i % kLanes == l) {
+                    const int64_t at = int64_t(token) * a.topK + i;
+                    const uint32_t e = best.Expert(i);
+                    a.expertOf[at] = int32_t(e);      // (kNone is -1)
+                    a.weights[at] = e != kNone ? weight[i] * by : 0.0f;
+                    if (e != kNone) {
+                        atomicOr(&chose[2 * e + (r >> 5)], 1u << (r & 31));
+                    }
                 }
             }
         }
-    }
-    __syncthreads();
-    // sums of probabilities: the experts over the threads, the tile's tokens cut among the threads of one expert
-    const int perExpert = E >= kThreads ? 1 : kThreads / E;
-    for (int e0 = 0; e0 < E; e0 += kThreads) {
-        const int e = e0 + int(threadIdx.x) % (E >= kThreads ? kThreads : E), piece = E >= kThreads ? 0 : int(threadIdx.x) / E;
-        const int step = (here + perExpert - 1) / perExpert;
-        float s = 0.0f;
-        if (e < E && piece < perExpert) {
-            for (int t = piece * step; t < min(here, piece * step + step); t++) {
-                if (share[t] != 0.0f) {
-                    s += tile[t * a.rowWords + e] * share[t];
-                }
+        __syncthreads();
+        // a choice's place among the workgroup's rows of its expert
+        int32_t place[K];
+#pragma unroll
+        for (int i = 0; i < K; i++) {
+            place[i] = -1;
+            const uint32_t e = best.Expert(i);
+            if (i < a.topK && i % kLanes == l && e != kNone && token < a.tokens) {
+                const uint32_t low = chose[2 * e], high = chose[2 * e + 1];
+                place[i] = count[e] + (r < 32 ? __popc(low & ((1u << r) - 1)) : __popc(low) + __popc(high & ((1u << (r - 32)) - 1)));
             }
         }
-        partSum[threadIdx.x] = s;
         __syncthreads();
-        if (e < E && piece == 0) {
-            for (int i = 1; i < perExpert; i++) {
-                s += partSum[int(threadIdx.x) + i * E];
-            }
-            sum[e] = s;
-            count[e] = __popc(chose[2 * e]) + __popc(chose[2 * e + 1]);
-        }
-        __syncthreads();
-    }
-    const bool alone = a.tiles == 1;
-    if (!alone) {
         for (int e = threadIdx.x; e < E; e += kThreads) {
-            a.tileCounts[int64_t(blockIdx.x) * (E + 1) + e] = count[e];
-            a.tileSums[int64_t(blockIdx.x) * E + e] = sum[e];
+            count[e] += __popc(chose[2 * e]) + __popc(chose[2 * e + 1]);
+            chose[2 * e] = chose[2 * e + 1] = 0;
         }
-        if (threadIdx.x == 0) {
-            a.tileCounts[int64_t(blockIdx.x) * (E + 1) + E] = int(*routed);
+        __syncthreads();
+        if (a.blocks == 1 && tile + 1 == a.tiles) {
+            // a single workgroup: its places become rows at once
+            Columns<kWaveTokens, kLanes>(column, sum, E, lane, wave, l);
+            Finish<kThreads>(a, count, sum, *routed, part, partSum, true);
         }
-    } else {
-        Finish(a, count, sum, int(*routed), part, partSum, true);
-    }
-    // a token's place among the tile's rows of its expert; with a single tile that is all
-    if (r < here) {
+        if (token < a.tokens) {
 #pragma unroll
-        for (int i = 0; i < K; i++) {
-            if (i < a.topK && i % kLanes == l) {
-                int32_t place = -1;
-                if (best[i].e != kNone) {
-                    const uint32_t low = chose[2 * best[i].e], high = chose[2 * best[i].e + 1];
-                    place = r < 32 ? __popc(low & ((1u << r) - 1)) : __popc(low) + __popc(high & ((1u << (r - 32)) - 1));
-                    place += alone ? count[best[i].e] : 0;
+            for (int i = 0; i < K; i++) {
+                if (i < a.topK && i % kLanes == l) {
+                    const bool last = a.blocks == 1 && tile + 1 == a.tiles;
+                    a.rowOf[int64_t(token) * a.topK + i] = place[i] < 0 ? -1 : place[i] + (last ? count[best.Expert(i)] : 0);
                 }
-                a.rowOf[int64_t(first + r) * a.topK + i] = place;
             }
         }
+    }
+    if (a.blocks == 1) {
+        for (int i = threadIdx.x; i < (a.tiles - 1) * kTile * a.topK; i += kThreads) {   // the tiles before the last one
+            const int e = a.expertOf[i];
+            if (e >= 0) {
+                a.rowOf[i] += count[e];
+            }
+        }
+        return;
+    }
+    Columns<kWaveTokens, kLanes>(column, sum, E, lane, wave, l);
+    for (int e = threadIdx.x; e < E; e += kThreads) {
+        a.blockCounts[int64_t(blockIdx.x) * (E + 1) + e] = count[e];
+        a.blockSums[int64_t(blockIdx.x) * E + e] = sum[e];
+    }
+    if (threadIdx.x == 0) {
+        a.blockCounts[int64_t(blockIdx.x) * (E + 1) + E] = *routed;
     }
 }
 
-// Sums the tiles' counts and probabilities, 16 experts (columns) to a workgroup and 16 runs of tiles to an expert, and leaves in
-// tileCounts what lies in front of every tile.  Column `experts` holds the tokens that chose.
-__global__ void __launch_bounds__(kThreads) TileScanKernel(RouteArgs a)
+constexpr int kMostBlocks = 1024, kScanCols = 8, kScanRuns = kThreads / kScanCols, kScanEach = kMostBlocks / kScanRuns;
+
+// Adds up the workgroups' counts and probabilities, eight experts (columns) to a workgroup and 32 runs of rows to an expert, all of a run
+// on its way at once, and leaves in blockCounts what lies in front of every workgroup.  Column `experts` holds the tokens that chose.
+__global__ void __launch_bounds__(kThreads) ScanKernel(RouteArgs a)
 {
-    __shared__ int parts[16][17];
-    __shared__ float partSums[16][17];
-    const int c = threadIdx.x % 16, run = threadIdx.x / 16, e = int(blockIdx.x) * 16 + c;
-    const int per = (a.tiles + 15) / 16, from = min(a.tiles, run * per), to = min(a.tiles, from + per);
+    __shared__ int parts[kScanRuns][kScanCols + 1];
+    __shared__ float partSums[kScanRuns][kScanCols + 1];
+    const int c = int(threadIdx.x) % kScanCols, run = int(threadIdx.x) / kScanCols, e = int(blockIdx.x) * kScanCols + c;
     const int64_t width = a.experts + 1;
-    int n = 0;
-    float s = 0.0f;
-    if (e <= a.experts) {
-        for (int t = from; t < to; t++) {
-            n += a.tileCounts[t * width + e];
-            s += e < a.experts ? a.tileSums[int64_t(t) * a.experts + e] : 0.0f;
-        }
+    const int per = (a.blocks + kScanRuns - 1) / kScanRuns, from = run * per;
+    int n[kScanEach], all = 0;
+    float p[kScanEach], sum = 0.0f;
+#pragma unroll
+    for (int i = 0; i < kScanEach; i++) {
+        const bool in = i < per && from + i < a.blocks;
+        n[i] = in && e <= a.experts ? a.blockCounts[(from + i) * width + e] : 0;
+        p[i] = in && e < a.experts ? a.blockSums[int64_t(from + i) * a.experts + e] : 0.0f;
     }
-    parts[run][c] = n;
-    partSums[run][c] = s;
+#pragma unroll
+    for (int i = 0; i < kScanEach; i++) {
+        all += n[i];
+        sum += p[i];
+    }
+    parts[run][c] = all;
+    partSums[run][c] = sum;
     __syncthreads();
-    int before = 0, all = 0;
-    float sum = 0.0f;
-    for (int i = 0; i < 16; i++) {
+    int before = 0;
+    all = 0;
+    sum = 0.0f;
+#pragma unroll
+    for (int i = 0; i < kScanRuns; i++) {
         before += i < run ? parts[i][c] : 0;
         all += parts[i][c];
         sum += partSums[i][c];
@@ -337,10 +508,12 @@ __global__ void __launch_bounds__(kThreads) TileScanKernel(RouteArgs a)
     if (e > a.experts) {
         return;
     }
-    for (int t = from; t < to; t++) {
-        const int here = a.tileCounts[t * width + e];
-        a.tileCounts[t * width + e] = before;
-        before += here;
+#pragma unroll
+    for (int i = 0; i < kScanEach; i++) {
+        if (i < per && from + i < a.blocks) {
+            a.blockCounts[(from + i) * width + e] = before;
+            before += n[i];
+        }
     }
     if (run == 0) {
         a.counts[e] = all;
@@ -350,27 +523,30 @@ __global__ void __launch_bounds__(kThreads) TileScanKernel(RouteArgs a)
     }
 }
 
-// Every choice's row: its expert's first row, the rows of the tiles before its own, its place in its tile.
-__global__ void __launch_bounds__(kThreads) RowsKernel(RouteArgs a, int tile)
+// Every choice's row: its expert's first row, the rows of the workgroups before its own, its place in its own.
+__global__ void __launch_bounds__(kThreads) RowsKernel(RouteArgs a, int tokensEach)
 {
-    extern __shared__ float lds[];
-    int *count = reinterpret_cast<int *>(lds);                       // [experts]
-    float *sum = reinterpret_cast<float *>(count + a.experts);       // [experts]
-    int *part = reinterpret_cast<int *>(sum + a.experts);            // [kThreads]
-    float *partSum = reinterpret_cast<float *>(part + kThreads);     // [kThreads]
-    for (int e = threadIdx.x; e < a.experts; e += kThreads) {
+    extern __shared__ uint32_t lds[];
+    const int E = a.experts, block = int(blockIdx.x);
+    int *count = reinterpret_cast<int *>(lds);                           // [experts]
+    float *sum = reinterpret_cast<float *>(count + E);                   // [experts]
+    int *before = reinterpret_cast<int *>(sum + E);                      // [experts]
+    int *part = before + E;                                              // [waves]
+    float *partSum = reinterpret_cast<float *>(part + kThreads / 64);    // [waves]
+    for (int e = threadIdx.x; e < E; e += kThreads) {
         count[e] = a.counts[e];
-        sum[e] = a.sums[e];
+        sum[e] = block == 0 ? a.sums[e] : 0.0f;
+        before[e] = a.blockCounts[int64_t(block) * (E + 1) + e];
     }
-    const int tokens = a.counts[a.experts];
+    const int tokens = a.counts[E];
     __syncthreads();
-    Finish(a, count, sum, tokens, part, partSum, blockIdx.x == 0);
-    const int64_t all = int64_t(a.tokens) * a.topK;
-    for (int64_t i = int64_t(blockIdx.x) * kThreads + threadIdx.x; i < all; i += int64_t(gridDim.x) * kThreads) {
+    Finish<kThreads>(a, count, sum, tokens, part, partSum, block == 0);
+    const int64_t first = int64_t(block) * tokensEach * a.topK;
+    const int64_t last = min(first + int64_t(tokensEach) * a.topK, int64_t(a.tokens) * a.topK);
+    for (int64_t i = first + threadIdx.x; i < last; i += kThreads) {
         const int e = a.expertOf[i];
         if (e >= 0) {
-            const int64_t t = i / a.topK / tile;
-            a.rowOf[i] += count[e] + a.tileCounts[t * (a.experts + 1) + e];
+            a.rowOf[i] += count[e] + before[e];
         }
     }
 }
@@ -389,45 +565,59 @@ struct RouteGradArgs {
     bool renormalise;
 };
 
-// kLanes lanes to a token, kEach experts to a lane, in vectors of four that the lanes of a token take in turn.
+// kLanes lanes to a token (at least as many as it has choices), kEach experts to a lane, in vectors of four that the lanes of a token
+// take in turn.  A workgroup goes through tokens, what it knows of the experts stays in registers.  What the weights' gradients add at
+// the chosen experts is worked out by one lane for each and put in on the way out through LDS.
 template <typename T, int kLanes, int kEach, bool kWide>
 __global__ void __launch_bounds__(kThreads) RouteGradKernel(RouteGradArgs a)
 {
-    const int l = threadIdx.x % kLanes;
-    const int64_t t = (int64_t(blockIdx.x) * kThreads + threadIdx.x) / kLanes;
-    const int E = a.experts;
-    __shared__ int total;
-    if (a.lossGrad != nullptr) {   // rows in all
-        if (threadIdx.x == 0) {
-            total = 0;
-        }
-        __syncthreads();
+    constexpr int kTokens = kThreads / kLanes;
+    __shared__ __align__(16) float rows[kTokens][kLanes * kEach];
+    __shared__ int parts[kThreads / 64];
+    const int l = int(threadIdx.x) % kLanes, slot = int(threadIdx.x) / kLanes, E = a.experts;
+    // the balance loss's gradient of p_te is c E n_e / (A T) * lossGrad
+    float load[kEach];
+#pragma unroll
+    for (int i = 0; i < kEach; i++) {
+        load[i] = 0.0f;
+    }
+    if (a.lossGrad != nullptr) {
         int n = 0;
         for (int e = threadIdx.x; e < E; e += kThreads) {
             n += a.counts[e];
         }
-        atomicAdd(&total, n);      // whole numbers: the order does not matter
+#pragma unroll
+        for (int d = 1; d < 64; d <<= 1) {
+            n += __shfl_xor(n, d, 64);
+        }
+        if (threadIdx.x % 64 == 0) {
+            parts[threadIdx.x / 64] = n;
+        }
         __syncthreads();
-    }
-    if (t >= a.tokens) {
-        return;
-    }
-    const int32_t *chosen = a.expertOf + t * a.topK;
-    T *out = static_cast<T *>(a.logitGrad) + t * a.gradStride;
-    const T *in = static_cast<const T *>(a.logits) + t * a.stride;
-    float x[kEach];
-    if ((a.mask != nullptr && a.mask[t] == 0) || chosen[0] < 0) {
+        int all = 0;
+#pragma unroll
+        for (int w = 0; w < kThreads / 64; w++) {
+            all += parts[w];
+        }
+        const float by = all > 0 ? a.lossGrad[0] * a.lossScale * float(E) / float(all) / float(a.counts[E]) : 0.0f;
 #pragma unroll
         for (int i = 0; i < kEach; i++) {
-            x[i] = 0.0f;
+            const int e = (i / 4 * kLanes + l) * 4 + i % 4;
+            load[i] = e < E ? by * float(a.counts[e]) : 0.0f;
         }
-    } else {
-        float top = -__builtin_inff();
+    }
+    for (int64_t t = int64_t(blockIdx.x) * kTokens + slot; t < a.tokens; t += int64_t(gridDim.x) * kTokens) {
+        T *out = static_cast<T *>(a.logitGrad) + t * a.gradStride;
+        const T *in = static_cast<const T *>(a.logits) + t * a.stride;
+        const int chosen = l < a.topK ? a.expertOf[t * a.topK + l] : -1;
+        const float dw = chosen >= 0 && a.weightGrad != nullptr ? a.weightGrad[t * a.topK + l] : 0.0f;
+        const bool none = (a.mask != nullptr && a.mask[t] == 0) || a.expertOf[t * a.topK] < 0;
+        float x[kEach];
 #pragma unroll
         for (int i = 0; i < kEach; i += 4) {
             const int e = (i / 4 * kLanes + l) * 4;
-            float v[4];
             if (kWide) {
+                float v[4];
                 if (e < E) {
                     Load<true, 4>(in + e, v);
                 }
@@ -442,6 +632,8 @@ __global__ void __launch_bounds__(kThreads) RouteGradKernel(RouteGradArgs a)
                 }
             }
         }
+        const float logit = chosen >= 0 && chosen < E ? float(in[chosen]) : -__builtin_inff();
+        float top = -__builtin_inff();
 #pragma unroll
         for (int i = 0; i < kEach; i++) {
             top = x[i] > top ? x[i] : top;
@@ -451,125 +643,107 @@ __global__ void __launch_bounds__(kThreads) RouteGradKernel(RouteGradArgs a)
             const float other = __shfl_xor(top, d, 64);
             top = other > top ? other : top;
         }
-        // the balance loss's gradient of p_te is c E n_e / (A T) * lossGrad
-        float load = 0.0f;
-        if (a.lossGrad != nullptr && total > 0) {
-            load = a.lossGrad[0] * a.lossScale * float(E) / float(total) / float(a.counts[E]);
-        }
-        float sum = 0.0f, dot = 0.0f, g[kEach];
+        float sum = 0.0f, dot = 0.0f;
 #pragma unroll
         for (int i = 0; i < kEach; i++) {
-            const int e = (i / 4 * kLanes + l) * 4 + i % 4;
-            x[i] = expf(x[i] - top);
+            x[i] = Exp(x[i] - top);
             sum += x[i];
-            g[i] = a.lossGrad != nullptr && e < E ? load * float(a.counts[e]) : 0.0f;
+            dot = __builtin_fmaf(x[i], load[i], dot);
         }
-        // what the weights' gradients add: to g at the chosen, or with the quotient at the end
-        float inside = 0.0f, mean = 0.0f;
-        if (a.weightGrad != nullptr) {
-            for (int j = 0; j < a.topK; j++) {
-                const int c = chosen[j];
-                if (c < 0) {
-                    break;
-                }
-                const float dw = a.weightGrad[t * a.topK + j];
-                if (a.renormalise) {
-                    const float w = expf(float(in[c]) - top);
-                    inside += w;
-                    mean += w * dw;
-                } else {
+        const float w = chosen >= 0 ? Exp(logit - top) : 0.0f;
+        sum = AddNeighbours<kLanes>(sum);
+        const float by = 1.0f / sum;
+        float more;     // what this lane's choice adds
+        if (a.renormalise) {
+            const float inside = AddNeighbours<kLanes>(w), mean = AddNeighbours<kLanes>(w * dw) / inside;
+            more = w / inside * (dw - mean);
+        } else {
+            dot = __builtin_fmaf(w, dw, dot);
+            more = w * by * dw;
+        }
+        dot = AddNeighbours<kLanes>(dot) * by;
 #pragma unroll
-                    for (int i = 0; i < kEach; i++) {
-                        g[i] += (i / 4 * kLanes + l) * 4 + i % 4 == c ? dw : 0.0f;
+        for (int i = 0; i < kEach; i += 4) {
+            Float4 v;
+#pragma unroll
+            for (int j = 0; j < 4; j++) {
+                v[j] = none ? 0.0f : x[i + j] * by * (load[i + j] - dot);
+            }
+            *reinterpret_cast<Float4 *>(&rows[slot][(i / 4 * kLanes + l) * 4]) = v;
+        }
+        // (a token's lanes are in one wave, whose LDS operations keep their order)
+        __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+        __builtin_amdgcn_wave_barrier();
+        if (a.weightGrad != nullptr && chosen >= 0 && chosen < E && !none) {
+            rows[slot][chosen] += more;
+        }
+        __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+        __builtin_amdgcn_wave_barrier();
+#pragma unroll
+        for (int i = 0; i < kEach; i += 4) {
+            const int e = (i / 4 * kLanes + l) * 4;
+            const Float4 f = *reinterpret_cast<const Float4 *>(&rows[slot][e]);
+            const float v[4] = {f[0], f[1], f[2], f[3]};
+            if (kWide) {
+                if (e < E) {
+                    Store<true, 4>(out + e, v);
+                }
+            } else {
+#pragma unroll
+                for (int j = 0; j < 4; j++) {
+                    if (e + j < E) {
+                        out[e + j] = T(v[j]);
                     }
                 }
             }
         }
-#pragma unroll
-        for (int i = 0; i < kEach; i++) {
-            dot += x[i] * g[i];
-        }
-#pragma unroll
-        for (int d = 1; d < kLanes; d <<= 1) {
-            sum += __shfl_xor(sum, d, 64);
-            dot += __shfl_xor(dot, d, 64);
-        }
-        const float by = 1.0f / sum;
-        dot *= by;
-#pragma unroll
-        for (int i = 0; i < kEach; i++) {
-            x[i] = x[i] * by * (g[i] - dot);
-        }
-        if (a.weightGrad != nullptr && a.renormalise) {
-            mean /= inside;
-            for (int j = 0; j < a.topK; j++) {
-                const int c = chosen[j];
-                if (c < 0) {
-                    break;
-                }
-                const float more = expf(float(in[c]) - top) / inside * (a.weightGrad[t * a.topK + j] - mean);
-#pragma unroll
-                for (int i = 0; i < kEach; i++) {
-                    x[i] += (i / 4 * kLanes + l) * 4 + i % 4 == c ? more : 0.0f;
-                }
-            }
-        }
-    }
-#pragma unroll
-    for (int i = 0; i < kEach; i += 4) {
-        const int e = (i / 4 * kLanes + l) * 4;
-        const float v[4] = {x[i], x[i + 1], x[i + 2], x[i + 3]};
-        if (kWide) {
-            if (e < E) {
-                Store<true, 4>(out + e, v);
-            }
-        } else {
-#pragma unroll
-            for (int j = 0; j < 4; j++) {
-                if (e + j < E) {
-                    out[e + j] = T(v[j]);
-                }
-            }
-        }
+        __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+        __builtin_amdgcn_wave_barrier();
     }
 }
 
-// Tokens to a tile.  Up to 64 tokens one tile of 64 makes it a single launch; beyond, as many as leave a tile for each of the
-// 256 compute units, and no more LDS than two workgroups can share.
-int TileOf(uint64_t tokens, uint32_t experts)
+// Tokens of a tile: 64 with four lanes to a token, 16 with sixteen.  Sixteen lanes where a lane would have more than 64 experts,
+// and for few tokens, where the time is one lane's.
+int TileOf(uint64_t tokens, uint32_t experts) { return experts > 256 || tokens <= 64 * 256 / 4 ? 16 : 64; }
+
+// Workgroups: at most 1024, four to a compute unit, each with as many tiles as that takes.
+int TilesOf(uint64_t tokens, int tile)
 {
-    if (experts > 256) {
-        return 16;
-    }
-    return tokens <= 64 || tokens >= 64 * 256 ? 64 : 16;
+    const uint64_t tiles = (tokens + uint64_t(tile) - 1) / uint64_t(tile);
+    return tiles == 0 ? 1 : tiles <= 4 ? int(tiles) : int((tiles + kMostBlocks - 1) / kMostBlocks);
 }
 
-// LDS words from one token to the next: as many beyond a multiple of the 64 banks as lanes share a token, so that the
-// lanes of a wave find their words in different banks.
-int RowWords(uint32_t experts, int lanes) { return int((experts + 63 - uint32_t(lanes)) / 64 * 64) + lanes; }
-
-template <typename T, int K, int kLanes>
-void LaunchRoute(const RouteArgs &a, hipStream_t stream)
+int BlocksOf(uint64_t tokens, int tile)
 {
-    constexpr int kTile = kThreads / kLanes;
-    const size_t lds = 4 * (size_t(kTile) * a.rowWords + kTile + 4 * size_t(a.experts) + 2 * kThreads + 1);
-    hipLaunchKernelGGL((RouteKernel<T, K, kLanes>), dim3(a.tiles), dim3(kThreads), lds, stream, a);
+    const uint64_t each = uint64_t(tile) * uint64_t(TilesOf(tokens, tile));
+    return tokens == 0 ? 1 : int((tokens + each - 1) / each);
+}
+
+template <typename T, int K, int kLanes, int kChunks>
+void LaunchRoute(const RouteArgs &a, bool wide, hipStream_t stream)
+{
+    const size_t lds = 4 * ((3 + kThreads / 64) * size_t(a.experts) + 2 * (kThreads / 64) + 1);
+    const auto go = [&](auto kernel) { hipLaunchKernelGGL(kernel, dim3(a.blocks), dim3(kThreads), lds, stream, a); };
+    wide ? go(RouteKernel<T, K, kLanes, kChunks, true>) : go(RouteKernel<T, K, kLanes, kChunks, false>);
 }
 
 template <typename T, int K>
-void LaunchRouteTile(const RouteArgs &a, int tile, hipStream_t stream)
+void LaunchRouteShape(const RouteArgs &a, int tile, bool wide, hipStream_t stream)
 {
-    tile == 64 ? LaunchRoute<T, K, 4>(a, stream) : LaunchRoute<T, K, 16>(a, stream);
+    if (tile == 64) {
+        a.experts <= 64 ? LaunchRoute<T, K, 4, 2>(a, wide, stream) : LaunchRoute<T, K, 4, 8>(a, wide, stream);
+    } else {
+        a.experts <= 256 ? LaunchRoute<T, K, 16, 2>(a, wide, stream) : LaunchRoute<T, K, 16, 8>(a, wide, stream);
+    }
 }
 
 template <typename T>
-void LaunchRouteType(const RouteArgs &a, int tile, hipStream_t stream)
+void LaunchRouteType(const RouteArgs &a, int tile, bool wide, hipStream_t stream)
 {
-    a.topK == 1   ? LaunchRouteTile<T, 1>(a, tile, stream)
-    : a.topK == 2 ? LaunchRouteTile<T, 2>(a, tile, stream)
-    : a.topK <= 4 ? LaunchRouteTile<T, 4>(a, tile, stream)
-    : a.topK <= 8 ? LaunchRouteTile<T, 8>(a, tile, stream)
-                  : LaunchRouteTile<T, 16>(a, tile, stream);
+    a.topK <= 2   ? LaunchRouteShape<T, 2>(a, tile, wide, stream)
+    : a.topK <= 4 ? LaunchRouteShape<T, 4>(a, tile, wide, stream)
+    : a.topK <= 8 ? LaunchRouteShape<T, 8>(a, tile, wide, stream)
+                  : LaunchRouteShape<T, 16>(a, tile, wide, stream);
 }
 
 template <typename T, bool kWide>
@@ -577,7 +751,7 @@ void LaunchRouteGrad(const RouteGradArgs &a, hipStream_t stream)
 {
     const auto go = [&](auto kernel, int lanes) {
         const int64_t blocks = (int64_t(a.tokens) * lanes + kThreads - 1) / kThreads;
-        hipLaunchKernelGGL(kernel, dim3(uint32_t(blocks)), dim3(kThreads), 0, stream, a);
+        hipLaunchKernelGGL(kernel, dim3(uint32_t(blocks < 1024 ? blocks : 1024)), dim3(kThreads), 0, stream, a);
     };
     if (a.experts <= 64) {
         go(RouteGradKernel<T, 16, 4, kWide>, 16);
@@ -603,8 +777,8 @@ HcclResult HcclAmdExpertRouteWorkspace(uint64_t tokens, uint32_t experts, uint64
     EXPERTS_CHK_PTR(bytes);
     EXPERTS_CHK(experts >= 1 && experts <= HCCL_AMD_MAX_EXPERTS);
     EXPERTS_CHK(tokens <= kMaxTokens);
-    const uint64_t tile = uint64_t(TileOf(tokens, experts)), tiles = (tokens + tile - 1) / tile;
-    *bytes = tiles <= 1 ? 0 : 4 * (tiles * (2 * uint64_t(experts) + 1) + experts);
+    const uint64_t blocks = uint64_t(BlocksOf(tokens, TileOf(tokens, experts)));
+    *bytes = blocks == 1 ? 0 : 4 * (blocks * (2 * uint64_t(experts) + 1) + experts);
     return HCCL_SUCCESS;
 }
 
@@ -650,28 +824,28 @@ HcclResult HcclAmdExpertRoute(const void *logits, HcclDataType logitType, uint64
     a.tokens = int(tokens);
     a.experts = int(experts);
     a.topK = int(topK);
-    a.tiles = tokens == 0 ? 1 : int((tokens + uint64_t(tile) - 1) / uint64_t(tile));   // no token: the one tile writes the zeros
-    a.tileCounts = static_cast<int32_t *>(workspace);
-    a.tileSums = reinterpret_cast<float *>(a.tileCounts + int64_t(a.tiles) * (a.experts + 1));
-    a.sums = a.tileSums + int64_t(a.tiles) * a.experts;
-    a.rowWords = RowWords(experts, kThreads / tile);
+    a.tiles = TilesOf(tokens, tile);
+    a.blocks = BlocksOf(tokens, tile);       // no token: the one workgroup writes the zeros
+    a.blockCounts = static_cast<int32_t *>(workspace);
+    a.blockSums = reinterpret_cast<float *>(a.blockCounts + int64_t(a.blocks) * (a.experts + 1));
     a.lossScale = lossScale;
     a.renormalise = renormalise != 0;
     const hipStream_t on = static_cast<hipStream_t>(stream);
-    logitType == HCCL_DATA_TYPE_FP32   ? LaunchRouteType<float>(a, tile, on)
-    : logitType == HCCL_DATA_TYPE_FP16 ? LaunchRouteType<_Float16>(a, tile, on)
-                                       : LaunchRouteType<__bf16>(a, tile, on);
+    a.sums = a.blockSums + int64_t(a.blocks) * a.experts;
+    const bool wide = experts % 8 == 0 && Aligned(logits, 16) && uint64_t(a.stride) * SizeOf(logitType) % 16 == 0;
+    logitType == HCCL_DATA_TYPE_FP32   ? LaunchRouteType<float>(a, tile, wide, on)
+    : logitType == HCCL_DATA_TYPE_FP16 ? LaunchRouteType<_Float16>(a, tile, wide, on)
+                                       : LaunchRouteType<__bf16>(a, tile, wide, on);
     HcclResult r = Launched("HcclAmdExpertRoute");
-    if (r != HCCL_SUCCESS || a.tiles == 1) {
+    if (r != HCCL_SUCCESS || a.blocks == 1) {
         return r;
     }
-    hipLaunchKernelGGL(TileScanKernel, dim3(experts / 16 + 1), dim3(kThreads), 0, on, a);
+    hipLaunchKernelGGL(ScanKernel, dim3(experts / kScanCols + 1), dim3(kThreads), 0, on, a);
     r = Launched("HcclAmdExpertRoute");
     if (r != HCCL_SUCCESS) {
         return r;
     }
-    const uint64_t blocks = (tokens * topK + kThreads - 1) / kThreads;
-    hipLaunchKernelGGL(RowsKernel, dim3(uint32_t(blocks < 512 ? blocks : 512)), dim3(kThreads), 4 * (2 * size_t(experts) + 2 * kThreads), on, a, tile);
+    hipLaunchKernelGGL(RowsKernel, dim3(a.blocks), dim3(kThreads), 4 * (3 * size_t(experts) + 2 * (kThreads / 64)), on, a, tile * a.tiles);
     return Launched("HcclAmdExpertRoute");
 }
 

@@ -120,7 +120,7 @@ def check_route(logits, topk, renorm, mask, got, grad, dw, dl, loss_scale=0.01):
 
 @pytest.mark.parametrize("dtype", ["fp32", "bf16", "fp16"])
 @pytest.mark.parametrize("tokens,experts,topk", [(1, 1, 1), (1, 64, 6), (3, 5, 5), (64, 8, 2), (65, 8, 2), (63, 60, 4), (200, 127, 7), (257, 256, 8),
-                                                 (100, 257, 3), (33, 1000, 16), (17, 1024, 9), (1000, 16, 16), (4099, 64, 1)])
+                                                 (100, 257, 3), (33, 1000, 16), (17, 1024, 9), (1000, 16, 16), (4099, 64, 1), (48, 200, 8), (5003, 60, 4)])
 def test_route(stream, dtype, tokens, experts, topk):
     rng = np.random.default_rng(tokens * 7 + experts)
     for renorm in (False, True):
@@ -183,6 +183,16 @@ def test_route_masked_places(stream, dtype, renorm):
     # nobody takes part: zeros
     got, grad = run_route(stream, logits, 4, renorm, np.zeros(80, np.uint8), dw=dw, dl=dl)
     assert not got["counts"].any() and not got["offsets"].any() and not got["loss"].any() and not grad.any() and (got["row_of"] == -1).all()
+
+
+@pytest.mark.parametrize("dtype", ["fp32", "bf16", "fp16"])
+def test_route_zeros_of_both_signs_are_ties(stream, dtype):
+    logits = torch.tensor([[-0.0, 0.0, -1.0, 0.0, -0.0, -2.0]] * 3).to(TYPE[dtype])
+    logits[1] *= -1
+    dw = np.ones((3, 4), np.float32)
+    got, grad = run_route(stream, logits, 4, True, dw=dw, dl=1.0)
+    check_route(logits, 4, True, None, got, grad, dw, 1.0)
+    assert got["expert"][0].tolist() == [0, 1, 3, 4] and got["expert"][1].tolist() == [5, 2, 0, 1]
 
 
 def test_route_nan_of_a_token_that_takes_part(stream):
