@@ -78,10 +78,16 @@ struct WordList {
         // of a sorted list and a new word the i-th is the median of the (i - 1)-th, the i-th and the new one
 #pragma unroll
         for (int i = K - 1; i > 0; i--) {
-            const uint32_t low = best[i - 1] < word ? best[i - 1] : word;
-            best[i] = best[i] > low ? best[i] : low;
+            asm("v_med3_u32 %0, %1, %2, %3" : "=v"(best[i]) : "v"(best[i - 1]), "v"(best[i]), "v"(word));
         }
         best[0] = best[0] > word ? best[0] : word;
+    }
+    __device__ __forceinline__ void Clear()
+    {
+#pragma unroll
+        for (int i = 0; i < K; i++) {
+            best[i] = 0;
+        }
     }
     // The larger half of two lists: element by element against the other one backwards, which leaves a sequence that rises and falls
     // once, then sorted by halving.
@@ -131,6 +137,7 @@ struct PairList {
             e[i] = kNone;
         }
     }
+    __device__ __forceinline__ void Clear() { *this = PairList(); }
     // No instruction.  Without it the compiler reasons about chains of dozens of selects as one, for hours.
     __device__ __forceinline__ void Settle(int i) { asm("" : "+v"(v[i]), "+v"(e[i])); }
 
@@ -206,7 +213,7 @@ __device__ __forceinline__ float AddNeighbours(float x)
     return x;
 }
 
-// The same over 16 lanes without a pass through LDS.
+// The same over 16 lanes without LDS.
 template <>
 __device__ __forceinline__ float AddNeighbours<16>(float x)
 {
@@ -286,16 +293,37 @@ __device__ __forceinline__ void Finish(const RouteArgs &a, int *count, const flo
     }
 }
 
-// The waves' parts of the sums of probabilities: over a wave's tokens in registers, over the waves in LDS, into sum[0 .. experts).
-template <int kWaveTokens, int kLanes, int kEach>
-__device__ __forceinline__ void Columns(const float (&column)[kEach], float *sum, int experts, int lane, int wave, int l)
+// One step of adding up over lanes and sharing out the sums: of 2 kHalf values a lane keeps the half that its bit names, and adds what
+// its partner, whose bit is the other one, has of it.  kDpp: how lanes are exchanged.
+template <int kDpp, int kHalf, int kEach>
+__device__ __forceinline__ void AddAndShare(float (&v)[kEach], bool upper)
 {
 #pragma unroll
-    for (int i = 0; i < kEach; i++) {
-        const float s = AddNeighbours<kWaveTokens>(column[i]);
-        const int e = (i / 8 * kLanes + l) * 8 + i % 8;
-        if (lane % kWaveTokens == 0 && e < experts) {
-            sum[wave * experts + e] = s;
+    for (int i = 0; i < kHalf; i++) {
+        const float keep = upper ? v[i + kHalf] : v[i], give = upper ? v[i] : v[i + kHalf];
+        v[i] = keep + __int_as_float(__builtin_amdgcn_update_dpp(0, __float_as_int(give), kDpp, 0xf, 0xf, true));
+    }
+}
+
+// The waves' parts of the sums of probabilities: over a wave's tokens in registers, over the waves in LDS, into sum[0 .. experts).
+// Partners' numbers differ in the bits 15, 7, 3 and 1 (mirrored rows and halves of rows, quads turned round), which reach all 16 lanes.
+template <int kWaveTokens, int kLanes, int kEach>
+__device__ __forceinline__ void Columns(float (&column)[kEach], float *sum, int experts, int lane, int wave, int l)
+{
+    constexpr int kQuarter = kWaveTokens == 16 ? kEach / 4 : kEach, kMine = kEach / kWaveTokens;
+    static_assert(kMine >= 1, "a sum to a lane at least");
+    if constexpr (kWaveTokens == 16) {
+        AddAndShare<0x140, kEach / 2>(column, (lane & 8) != 0);
+        AddAndShare<0x141, kEach / 4>(column, (lane & 4) != 0);
+    }
+    AddAndShare<0x1b, kQuarter / 2>(column, (lane & 2) != 0);
+    AddAndShare<0xb1, kQuarter / 4>(column, (lane & 1) != 0);
+    const int first = lane % kWaveTokens * kMine;     // (the highest bit has chosen between the halves of all)
+#pragma unroll
+    for (int i = 0; i < kMine; i++) {
+        const int at = first + i, e = (at / 8 * kLanes + l) * 8 + at % 8;
+        if (e < experts) {
+            sum[wave * experts + e] = column[i];
         }
     }
     __syncthreads();
@@ -341,7 +369,8 @@ __global__ void __launch_bounds__(kThreads) RouteKernel(RouteArgs a)
     for (int tile = 0; tile < a.tiles; tile++) {
         const int token = (int(blockIdx.x) * a.tiles + tile) * kTile + r;
         const bool in = token < a.tokens && (a.mask == nullptr || a.mask[token] != 0);
-        const T *row = static_cast<const T *>(a.logits) + int64_t(in ? token : 0) * a.stride;
+        // (the row of a token that takes no part is read and forgotten)
+        const T *row = static_cast<const T *>(a.logits) + int64_t(min(token, max(a.tokens - 1, 0))) * a.stride;
         float x[kEach];
         List<T, K> best;
 #pragma unroll
@@ -349,17 +378,17 @@ __global__ void __launch_bounds__(kThreads) RouteKernel(RouteArgs a)
             const int e = (c * kLanes + l) * 8;
             if (kWide) {
                 float v[8];
-                if (in && e < E) {
+                if (e < E && a.tokens > 0) {
                     Load<true, 8>(row + e, v);
                 }
 #pragma unroll
                 for (int i = 0; i < 8; i++) {
-                    x[c * 8 + i] = in && e < E ? v[i] : -__builtin_inff();
+                    x[c * 8 + i] = e < E ? v[i] : -__builtin_inff();
                 }
             } else {
 #pragma unroll
                 for (int i = 0; i < 8; i++) {
-                    x[c * 8 + i] = in && e + i < E ? float(row[e + i]) : -__builtin_inff();
+                    x[c * 8 + i] = e + i < E && a.tokens > 0 ? float(row[e + i]) : -__builtin_inff();
                 }
             }
         }
@@ -373,6 +402,9 @@ __global__ void __launch_bounds__(kThreads) RouteKernel(RouteArgs a)
 #pragma unroll 1
         for (int d = kWaveTokens; d < 64; d <<= 1) {
             best.Merge(d);
+        }
+        if (!in) {
+            best.Clear();
         }
         const bool any = best.Expert(0) != kNone;
         const float top = any ? best.template Value<T>(0) : 0.0f;
