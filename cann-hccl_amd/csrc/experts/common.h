@@ -65,40 +65,62 @@ typedef int32_t Int8 __attribute__((ext_vector_type(8)));
 typedef uint32_t Word2 __attribute__((ext_vector_type(2)));
 typedef uint32_t Word4 __attribute__((ext_vector_type(4)));
 
-// N consecutive elements from p; kWide: p is aligned to 16 bytes (or to all of them, if they are fewer).
+// N consecutive elements from p, in loads of 16 bytes (or one of all of them, if they are fewer).  kWide: p is aligned to that; else to
+// an element, which the hardware takes too (a lane's load then touches one line more).
 template <bool kWide, int N, typename T>
 __device__ __forceinline__ void Load(const T *p, float (&v)[N])
 {
-    if constexpr (kWide) {
-        typedef T Vec __attribute__((ext_vector_type(N), aligned(N * sizeof(T) < 16 ? N * sizeof(T) : 16)));
-        const Vec x = *reinterpret_cast<const Vec *>(p);
+    constexpr int kAlign = !kWide ? sizeof(T) : N * sizeof(T) < 16 ? N * sizeof(T) : 16;
+    typedef T Vec __attribute__((ext_vector_type(N), aligned(kAlign)));
+    const Vec x = *reinterpret_cast<const Vec *>(p);
 #pragma unroll
-        for (int i = 0; i < N; i++) {
-            v[i] = float(x[i]);
-        }
-    } else {
-#pragma unroll
-        for (int i = 0; i < N; i++) {
-            v[i] = float(p[i]);
-        }
+    for (int i = 0; i < N; i++) {
+        v[i] = float(x[i]);
     }
 }
 
 template <bool kWide, int N, typename T>
 __device__ __forceinline__ void Store(T *p, const float (&v)[N])
 {
-    if constexpr (kWide) {
-        typedef T Vec __attribute__((ext_vector_type(N), aligned(N * sizeof(T) < 16 ? N * sizeof(T) : 16)));
-        Vec x;
+    constexpr int kAlign = !kWide ? sizeof(T) : N * sizeof(T) < 16 ? N * sizeof(T) : 16;
+    typedef T Vec __attribute__((ext_vector_type(N), aligned(kAlign)));
+    Vec x;
 #pragma unroll
+    for (int i = 0; i < N; i++) {
+        x[i] = T(v[i]);
+    }
+    *reinterpret_cast<Vec *>(p) = x;
+}
+
+// N elements from column `at` of a row of `width`, `fill` beyond it.  kWide: the row is aligned and its width a multiple of N.
+template <bool kWide, int N, typename T>
+__device__ __forceinline__ void LoadPart(const T *row, int at, int width, float (&v)[N], float fill = 0.0f)
+{
+#pragma unroll
+    for (int i = 0; i < N; i++) {
+        v[i] = fill;
+    }
+    if (kWide ? at < width : at + N <= width) {
+        Load<kWide, N>(row + at, v);
+    } else if (!kWide && at < width) {
         for (int i = 0; i < N; i++) {
-            x[i] = T(v[i]);
+            if (at + i < width) {
+                v[i] = float(row[at + i]);
+            }
         }
-        *reinterpret_cast<Vec *>(p) = x;
-    } else {
-#pragma unroll
+    }
+}
+
+template <bool kWide, int N, typename T>
+__device__ __forceinline__ void StorePart(T *row, int at, int width, const float (&v)[N])
+{
+    if (kWide ? at < width : at + N <= width) {
+        Store<kWide, N>(row + at, v);
+    } else if (!kWide && at < width) {
         for (int i = 0; i < N; i++) {
-            p[i] = T(v[i]);
+            if (at + i < width) {
+                row[at + i] = T(v[i]);
+            }
         }
     }
 }

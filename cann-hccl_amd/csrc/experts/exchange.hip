@@ -31,43 +31,6 @@ struct PackArgs {
     int width, padded, topK, pieces;
 };
 
-// kEach values of a row from column `at` on; zeros beyond the width.
-template <bool kWide, typename T>
-__device__ __forceinline__ void LoadRow(const T *row, int at, int width, float (&v)[kEach])
-{
-    if (kWide) {
-        if (at < width) {
-            Load<true, kEach>(row + at, v);
-        }
-#pragma unroll
-        for (int i = 0; i < kEach; i++) {
-            v[i] = at < width ? v[i] : 0.0f;
-        }
-    } else {
-#pragma unroll
-        for (int i = 0; i < kEach; i++) {
-            v[i] = at + i < width ? float(row[at + i]) : 0.0f;
-        }
-    }
-}
-
-template <bool kWide, typename T>
-__device__ __forceinline__ void StoreRow(T *row, int at, int width, const float (&v)[kEach])
-{
-    if (kWide) {
-        if (at < width) {
-            Store<true, kEach>(row + at, v);
-        }
-    } else {
-#pragma unroll
-        for (int i = 0; i < kEach; i++) {
-            if (at + i < width) {
-                row[at + i] = T(v[i]);
-            }
-        }
-    }
-}
-
 // A wave to a token and a piece of its width: read once, written to all of the token's rows.
 template <typename T, bool kWide>
 __global__ void __launch_bounds__(kThreads) CopyKernel(PackArgs a)
@@ -76,11 +39,11 @@ __global__ void __launch_bounds__(kThreads) CopyKernel(PackArgs a)
         const int64_t t = w / a.pieces;
         const int at = int(w % a.pieces) * kPiece + int(threadIdx.x % 64) * kEach;
         float v[kEach];
-        LoadRow<kWide>(static_cast<const T *>(a.x) + t * a.xStride, at, a.width, v);
+        LoadPart<kWide, kEach>(static_cast<const T *>(a.x) + t * a.xStride, at, a.width, v);
         for (int j = 0; j < a.topK; j++) {
             const int64_t r = a.rowOf == nullptr ? t : a.rowOf[t * a.topK + j];
             if (r >= 0 && r < a.rows) {
-                StoreRow<kWide>(static_cast<T *>(a.out) + r * a.outStride, at, a.width, v);
+                StorePart<kWide, kEach>(static_cast<T *>(a.out) + r * a.outStride, at, a.width, v);
             }
         }
     }
@@ -94,7 +57,7 @@ __global__ void __launch_bounds__(kThreads) QuantKernel(PackArgs a)
         const int64_t t = w / a.pieces;
         const int at = int(w % a.pieces) * kPiece + int(threadIdx.x % 64) * kEach;
         float v[kEach];
-        LoadRow<kWide>(static_cast<const T *>(a.x) + t * a.xStride, at, a.width, v);
+        LoadPart<kWide, kEach>(static_cast<const T *>(a.x) + t * a.xStride, at, a.width, v);
         float top = 0.0f;
 #pragma unroll
         for (int i = 0; i < kEach; i++) {
@@ -159,7 +122,7 @@ __global__ void __launch_bounds__(kThreads) CombineKernel(CombineArgs a)
                 is[j] = r >= 0 && r < a.rows;
                 by[j] = !is[j] || a.weights == nullptr ? 1.0f : a.weights[t * a.topK + j0 + j];
                 if (is[j]) {
-                    LoadRow<kWide>(static_cast<const T *>(a.x) + r * a.xStride, at, a.width, v[j]);
+                    LoadPart<kWide, kEach>(static_cast<const T *>(a.x) + r * a.xStride, at, a.width, v[j]);
                 }
             }
 #pragma unroll
@@ -172,7 +135,7 @@ __global__ void __launch_bounds__(kThreads) CombineKernel(CombineArgs a)
                 }
             }
         }
-        StoreRow<kWide>(static_cast<T *>(a.y) + t * a.yStride, at, a.width, sum);
+        StorePart<kWide, kEach>(static_cast<T *>(a.y) + t * a.yStride, at, a.width, sum);
     }
 }
 
@@ -200,13 +163,13 @@ __global__ void __launch_bounds__(kThreads) CombineGradKernel(CombineArgs a)
         }
         for (int at = int(threadIdx.x) * kEach; at < a.width; at += kThreads * kEach) {
             float d[kEach];
-            LoadRow<kWide>(dy, at, a.width, d);
+            LoadPart<kWide, kEach>(dy, at, a.width, d);
 #pragma unroll
             for (int j = 0; j < kRows; j++) {
                 if (r[j] >= 0) {
                     if (a.weightGrad != nullptr) {
                         float v[kEach];
-                        LoadRow<kWide>(static_cast<const T *>(a.x) + r[j] * a.xStride, at, a.width, v);
+                        LoadPart<kWide, kEach>(static_cast<const T *>(a.x) + r[j] * a.xStride, at, a.width, v);
 #pragma unroll
                         for (int i = 0; i < kEach; i++) {
                             dot[j] = __builtin_fmaf(d[i], v[i], dot[j]);
@@ -218,7 +181,7 @@ __global__ void __launch_bounds__(kThreads) CombineGradKernel(CombineArgs a)
                         for (int i = 0; i < kEach; i++) {
                             g[i] = by[j] * d[i];
                         }
-                        StoreRow<kWide>(static_cast<T *>(a.xGrad) + r[j] * a.xGradStride, at, a.width, g);
+                        StorePart<kWide, kEach>(static_cast<T *>(a.xGrad) + r[j] * a.xGradStride, at, a.width, g);
                     }
                 }
             }

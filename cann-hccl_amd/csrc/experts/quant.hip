@@ -31,23 +31,8 @@ __device__ __forceinline__ void LoadTile(const T *x, int64_t stride, int first, 
     const int r0 = first + 8 * (int(threadIdx.x) / 16), c = column + 8 * (int(threadIdx.x) % 16);
 #pragma unroll
     for (int p = 0; p < 8; p++) {
-        const bool in = r0 + p < last;
-        const T *row = x + int64_t(r0 + p) * stride;
-        if (kWide) {
-            if (in && c < width) {
-                Load<true, 8>(row + c, v[p]);
-            } else {
-#pragma unroll
-                for (int i = 0; i < 8; i++) {
-                    v[p][i] = 0.0f;
-                }
-            }
-        } else {
-#pragma unroll
-            for (int i = 0; i < 8; i++) {
-                v[p][i] = in && c + i < width ? float(row[c + i]) : 0.0f;
-            }
-        }
+        // (rows behind the last one: no column is within their width)
+        LoadPart<kWide, 8>(x + int64_t(r0 + p) * stride, c, r0 + p < last ? width : 0, v[p]);
     }
 }
 

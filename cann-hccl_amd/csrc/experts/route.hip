@@ -375,21 +375,11 @@ __global__ void __launch_bounds__(kThreads) RouteKernel(RouteArgs a)
         List<T, K> best;
 #pragma unroll
         for (int c = 0; c < kChunks; c++) {
-            const int e = (c * kLanes + l) * 8;
-            if (kWide) {
-                float v[8];
-                if (e < E && a.tokens > 0) {
-                    Load<true, 8>(row + e, v);
-                }
+            float v[8];
+            LoadPart<kWide, 8>(row, (c * kLanes + l) * 8, a.tokens > 0 ? E : 0, v, -__builtin_inff());
 #pragma unroll
-                for (int i = 0; i < 8; i++) {
-                    x[c * 8 + i] = e < E ? v[i] : -__builtin_inff();
-                }
-            } else {
-#pragma unroll
-                for (int i = 0; i < 8; i++) {
-                    x[c * 8 + i] = e + i < E && a.tokens > 0 ? float(row[e + i]) : -__builtin_inff();
-                }
+            for (int i = 0; i < 8; i++) {
+                x[c * 8 + i] = v[i];
             }
         }
 #pragma unroll
@@ -647,21 +637,11 @@ __global__ void __launch_bounds__(kThreads) RouteGradKernel(RouteGradArgs a)
         float x[kEach];
 #pragma unroll
         for (int i = 0; i < kEach; i += 4) {
-            const int e = (i / 4 * kLanes + l) * 4;
-            if (kWide) {
-                float v[4];
-                if (e < E) {
-                    Load<true, 4>(in + e, v);
-                }
+            float v[4];
+            LoadPart<kWide, 4>(in, (i / 4 * kLanes + l) * 4, E, v, -__builtin_inff());
 #pragma unroll
-                for (int j = 0; j < 4; j++) {
-                    x[i + j] = e < E ? v[j] : -__builtin_inff();
-                }
-            } else {
-#pragma unroll
-                for (int j = 0; j < 4; j++) {
-                    x[i + j] = e + j < E ? float(in[e + j]) : -__builtin_inff();
-                }
+            for (int j = 0; j < 4; j++) {
+                x[i + j] = v[j];
             }
         }
         const float logit = chosen >= 0 && chosen < E ? float(in[chosen]) : -__builtin_inff();
@@ -716,18 +696,7 @@ __global__ void __launch_bounds__(kThreads) RouteGradKernel(RouteGradArgs a)
             const int e = (i / 4 * kLanes + l) * 4;
             const Float4 f = *reinterpret_cast<const Float4 *>(&rows[slot][e]);
             const float v[4] = {f[0], f[1], f[2], f[3]};
-            if (kWide) {
-                if (e < E) {
-                    Store<true, 4>(out + e, v);
-                }
-            } else {
-#pragma unroll
-                for (int j = 0; j < 4; j++) {
-                    if (e + j < E) {
-                        out[e + j] = T(v[j]);
-                    }
-                }
-            }
+            StorePart<kWide, 4>(out, e, E, v);
         }
         __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
         __builtin_amdgcn_wave_barrier();
