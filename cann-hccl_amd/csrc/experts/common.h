@@ -92,17 +92,25 @@ __device__ __forceinline__ void Store(T *p, const float (&v)[N])
     *reinterpret_cast<Vec *>(p) = x;
 }
 
-// N elements from column `at` of a row of `width`, `fill` beyond it.  kWide: the row is aligned and its width a multiple of N.
-template <bool kWide, int N, typename T>
+// How a row can be taken, N elements at a time: anyhow, aligned and of a multiple of N elements, or such that the caller's lanes cover
+// it exactly and no lane has to look.
+constexpr int kAnyhow = 0, kAligned = 1, kExactly = 2;
+
+// N elements from column `at` of a row of `width`, `fill` beyond it.
+template <int kHow, int N, typename T>
 __device__ __forceinline__ void LoadPart(const T *row, int at, int width, float (&v)[N], float fill = 0.0f)
 {
+    if constexpr (kHow == kExactly) {
+        Load<true, N>(row + at, v);
+        return;
+    }
 #pragma unroll
     for (int i = 0; i < N; i++) {
         v[i] = fill;
     }
-    if (kWide ? at < width : at + N <= width) {
-        Load<kWide, N>(row + at, v);
-    } else if (!kWide && at < width) {
+    if (kHow == kAligned ? at < width : at + N <= width) {
+        Load<kHow == kAligned, N>(row + at, v);
+    } else if (kHow == kAnyhow && at < width) {
         for (int i = 0; i < N; i++) {
             if (at + i < width) {
                 v[i] = float(row[at + i]);
@@ -111,12 +119,14 @@ __device__ __forceinline__ void LoadPart(const T *row, int at, int width, float 
     }
 }
 
-template <bool kWide, int N, typename T>
+template <int kHow, int N, typename T>
 __device__ __forceinline__ void StorePart(T *row, int at, int width, const float (&v)[N])
 {
-    if (kWide ? at < width : at + N <= width) {
-        Store<kWide, N>(row + at, v);
-    } else if (!kWide && at < width) {
+    if (kHow == kExactly) {
+        Store<true, N>(row + at, v);
+    } else if (kHow == kAligned ? at < width : at + N <= width) {
+        Store<kHow == kAligned, N>(row + at, v);
+    } else if (kHow == kAnyhow && at < width) {
         for (int i = 0; i < N; i++) {
             if (at + i < width) {
                 row[at + i] = T(v[i]);

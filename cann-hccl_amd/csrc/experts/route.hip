@@ -305,27 +305,32 @@ __device__ __forceinline__ void AddAndShare(float (&v)[kEach], bool upper)
     }
 }
 
-// The waves' parts of the sums of probabilities: over a wave's tokens in registers, over the waves in LDS, into sum[0 .. experts).
-// Partners' numbers differ in the bits 15, 7, 3 and 1 (mirrored rows and halves of rows, quads turned round), which reach all 16 lanes.
+// A tile's probabilities, added up over a wave's tokens, into the wave's own sums in LDS.  Partners' numbers differ in the bits 15, 7, 3
+// and 1 (mirrored rows and halves of rows, quads turned round), which reach all 16 lanes.
 template <int kWaveTokens, int kLanes, int kEach>
-__device__ __forceinline__ void Columns(float (&column)[kEach], float *sum, int experts, int lane, int wave, int l)
+__device__ __forceinline__ void Columns(float (&p)[kEach], float *sum, int experts, int lane, int wave, int l)
 {
     constexpr int kQuarter = kWaveTokens == 16 ? kEach / 4 : kEach, kMine = kEach / kWaveTokens;
     static_assert(kMine >= 1, "a sum to a lane at least");
     if constexpr (kWaveTokens == 16) {
-        AddAndShare<0x140, kEach / 2>(column, (lane & 8) != 0);
-        AddAndShare<0x141, kEach / 4>(column, (lane & 4) != 0);
+        AddAndShare<0x140, kEach / 2>(p, (lane & 8) != 0);
+        AddAndShare<0x141, kEach / 4>(p, (lane & 4) != 0);
     }
-    AddAndShare<0x1b, kQuarter / 2>(column, (lane & 2) != 0);
-    AddAndShare<0xb1, kQuarter / 4>(column, (lane & 1) != 0);
+    AddAndShare<0x1b, kQuarter / 2>(p, (lane & 2) != 0);
+    AddAndShare<0xb1, kQuarter / 4>(p, (lane & 1) != 0);
     const int first = lane % kWaveTokens * kMine;     // (the highest bit has chosen between the halves of all)
 #pragma unroll
     for (int i = 0; i < kMine; i++) {
         const int at = first + i, e = (at / 8 * kLanes + l) * 8 + at % 8;
         if (e < experts) {
-            sum[wave * experts + e] = column[i];
+            sum[wave * experts + e] += p[i];
         }
     }
+}
+
+// The waves' sums into the first one's.
+__device__ __forceinline__ void AddWaves(float *sum, int experts)
+{
     __syncthreads();
     for (int e = threadIdx.x; e < experts; e += kThreads) {
         float s = sum[e];
@@ -339,7 +344,7 @@ __device__ __forceinline__ void Columns(float (&column)[kEach], float *sum, int 
 
 // kLanes lanes to a token, each with kChunks times eight neighbouring experts; lists of K.  Token t of a wave's 64 / kLanes is in
 // the lanes whose number leaves t.
-template <typename T, int K, int kLanes, int kChunks, bool kWide>
+template <typename T, int K, int kLanes, int kChunks, int kHow>
 __global__ void __launch_bounds__(kThreads) RouteKernel(RouteArgs a)
 {
     constexpr int kWaveTokens = 64 / kLanes, kTile = kWaveTokens * kThreads / 64, kEach = 8 * kChunks;
@@ -356,16 +361,14 @@ __global__ void __launch_bounds__(kThreads) RouteKernel(RouteArgs a)
     for (int e = threadIdx.x; e < E; e += kThreads) {
         chose[2 * e] = chose[2 * e + 1] = 0;
         count[e] = 0;
+        for (int w = 0; w < kThreads / 64; w++) {
+            sum[w * E + e] = 0.0f;
+        }
     }
     if (threadIdx.x == 0) {
         *routed = 0;
     }
     __syncthreads();
-    float column[kEach];          // this lane's part of the sums of probabilities
-#pragma unroll
-    for (int i = 0; i < kEach; i++) {
-        column[i] = 0.0f;
-    }
     for (int tile = 0; tile < a.tiles; tile++) {
         const int token = (int(blockIdx.x) * a.tiles + tile) * kTile + r;
         const bool in = token < a.tokens && (a.mask == nullptr || a.mask[token] != 0);
@@ -376,7 +379,7 @@ __global__ void __launch_bounds__(kThreads) RouteKernel(RouteArgs a)
 #pragma unroll
         for (int c = 0; c < kChunks; c++) {
             float v[8];
-            LoadPart<kWide, 8>(row, (c * kLanes + l) * 8, a.tokens > 0 ? E : 0, v, -__builtin_inff());
+            LoadPart<kHow, 8>(row, (c * kLanes + l) * 8, a.tokens > 0 ? E : 0, v, -__builtin_inff());
 #pragma unroll
             for (int i = 0; i < 8; i++) {
                 x[c * 8 + i] = v[i];
@@ -412,8 +415,9 @@ __global__ void __launch_bounds__(kThreads) RouteKernel(RouteArgs a)
         const float times = 1.0f / total;
 #pragma unroll
         for (int i = 0; i < kEach; i++) {
-            column[i] += any ? x[i] * times : 0.0f;
+            x[i] = any ? x[i] * times : 0.0f;
         }
+        Columns<kWaveTokens, kLanes>(x, sum, E, lane, wave, l);
         float inside = 0.0f, weight[K];
 #pragma unroll
         for (int i = 0; i < K; i++) {
@@ -459,7 +463,7 @@ __global__ void __launch_bounds__(kThreads) RouteKernel(RouteArgs a)
         __syncthreads();
         if (a.blocks == 1 && tile + 1 == a.tiles) {
             // a single workgroup: its places become rows at once
-            Columns<kWaveTokens, kLanes>(column, sum, E, lane, wave, l);
+            AddWaves(sum, E);
             Finish<kThreads>(a, count, sum, *routed, part, partSum, true);
         }
         if (token < a.tokens) {
@@ -481,7 +485,7 @@ __global__ void __launch_bounds__(kThreads) RouteKernel(RouteArgs a)
         }
         return;
     }
-    Columns<kWaveTokens, kLanes>(column, sum, E, lane, wave, l);
+    AddWaves(sum, E);
     for (int e = threadIdx.x; e < E; e += kThreads) {
         a.blockCounts[int64_t(blockIdx.x) * (E + 1) + e] = count[e];
         a.blockSums[int64_t(blockIdx.x) * E + e] = sum[e];
@@ -590,7 +594,7 @@ struct RouteGradArgs {
 // kLanes lanes to a token (at least as many as it has choices), kEach experts to a lane, in vectors of four that the lanes of a token
 // take in turn.  A workgroup goes through tokens, what it knows of the experts stays in registers.  What the weights' gradients add at
 // the chosen experts is worked out by one lane for each and put in on the way out through LDS.
-template <typename T, int kLanes, int kEach, bool kWide>
+template <typename T, int kLanes, int kEach, int kHow>
 __global__ void __launch_bounds__(kThreads) RouteGradKernel(RouteGradArgs a)
 {
     constexpr int kTokens = kThreads / kLanes;
@@ -638,7 +642,7 @@ __global__ void __launch_bounds__(kThreads) RouteGradKernel(RouteGradArgs a)
 #pragma unroll
         for (int i = 0; i < kEach; i += 4) {
             float v[4];
-            LoadPart<kWide, 4>(in, (i / 4 * kLanes + l) * 4, E, v, -__builtin_inff());
+            LoadPart<kHow, 4>(in, (i / 4 * kLanes + l) * 4, E, v, -__builtin_inff());
 #pragma unroll
             for (int j = 0; j < 4; j++) {
                 x[i + j] = v[j];
@@ -696,7 +700,7 @@ __global__ void __launch_bounds__(kThreads) RouteGradKernel(RouteGradArgs a)
             const int e = (i / 4 * kLanes + l) * 4;
             const Float4 f = *reinterpret_cast<const Float4 *>(&rows[slot][e]);
             const float v[4] = {f[0], f[1], f[2], f[3]};
-            StorePart<kWide, 4>(out, e, E, v);
+            StorePart<kHow, 4>(out, e, E, v);
         }
         __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
         __builtin_amdgcn_wave_barrier();
@@ -705,7 +709,7 @@ __global__ void __launch_bounds__(kThreads) RouteGradKernel(RouteGradArgs a)
 
 // Tokens of a tile: 64 with four lanes to a token, 16 with sixteen.  Sixteen lanes where a lane would have more than 64 experts,
 // and for few tokens, where the time is one lane's.
-int TileOf(uint64_t tokens, uint32_t experts) { return experts > 256 || tokens <= 64 * 256 / 4 ? 16 : 64; }
+int TileOf(uint64_t tokens, uint32_t experts) { return experts > 256 || tokens <= 64 * 64 ? 16 : 64; }
 
 // Workgroups: at most 1024, four to a compute unit, each with as many tiles as that takes.
 int TilesOf(uint64_t tokens, int tile)
@@ -725,7 +729,9 @@ void LaunchRoute(const RouteArgs &a, bool wide, hipStream_t stream)
 {
     const size_t lds = 4 * ((3 + kThreads / 64) * size_t(a.experts) + 2 * (kThreads / 64) + 1);
     const auto go = [&](auto kernel) { hipLaunchKernelGGL(kernel, dim3(a.blocks), dim3(kThreads), lds, stream, a); };
-    wide ? go(RouteKernel<T, K, kLanes, kChunks, true>) : go(RouteKernel<T, K, kLanes, kChunks, false>);
+    wide && a.experts == 8 * kLanes * kChunks && a.tokens > 0 ? go(RouteKernel<T, K, kLanes, kChunks, kExactly>)
+    : wide                                                    ? go(RouteKernel<T, K, kLanes, kChunks, kAligned>)
+                                                              : go(RouteKernel<T, K, kLanes, kChunks, kAnyhow>);
 }
 
 template <typename T, int K>
@@ -747,7 +753,7 @@ void LaunchRouteType(const RouteArgs &a, int tile, bool wide, hipStream_t stream
                   : LaunchRouteShape<T, 16>(a, tile, wide, stream);
 }
 
-template <typename T, bool kWide>
+template <typename T, int kHow>
 void LaunchRouteGrad(const RouteGradArgs &a, hipStream_t stream)
 {
     const auto go = [&](auto kernel, int lanes) {
@@ -755,13 +761,13 @@ void LaunchRouteGrad(const RouteGradArgs &a, hipStream_t stream)
         hipLaunchKernelGGL(kernel, dim3(uint32_t(blocks < 1024 ? blocks : 1024)), dim3(kThreads), 0, stream, a);
     };
     if (a.experts <= 64) {
-        go(RouteGradKernel<T, 16, 4, kWide>, 16);
+        go(RouteGradKernel<T, 16, 4, kHow>, 16);
     } else if (a.experts <= 128) {
-        go(RouteGradKernel<T, 16, 8, kWide>, 16);
+        go(RouteGradKernel<T, 16, 8, kHow>, 16);
     } else if (a.experts <= 256) {
-        go(RouteGradKernel<T, 16, 16, kWide>, 16);
+        go(RouteGradKernel<T, 16, 16, kHow>, 16);
     } else {
-        go(RouteGradKernel<T, 64, 16, kWide>, 64);
+        go(RouteGradKernel<T, 64, 16, kHow>, 64);
     }
 }
 
@@ -888,16 +894,12 @@ HcclResult HcclAmdExpertRouteGrad(const void *logits, HcclDataType logitType, ui
     const uint64_t four = 4 * SizeOf(logitType);
     const bool wide = experts % 4 == 0 && a.stride % 4 == 0 && a.gradStride % 4 == 0 && Aligned(logits, four) && Aligned(logitGrad, four);
     const hipStream_t on = static_cast<hipStream_t>(stream);
-    switch (logitType) {
-        case HCCL_DATA_TYPE_FP32:
-            wide ? LaunchRouteGrad<float, true>(a, on) : LaunchRouteGrad<float, false>(a, on);
-            break;
-        case HCCL_DATA_TYPE_FP16:
-            wide ? LaunchRouteGrad<_Float16, true>(a, on) : LaunchRouteGrad<_Float16, false>(a, on);
-            break;
-        default:
-            wide ? LaunchRouteGrad<__bf16, true>(a, on) : LaunchRouteGrad<__bf16, false>(a, on);
-    }
+    const bool exactly = wide && (experts == 64 || experts == 128 || experts == 256 || experts == 1024);
+    const auto go = [&](auto of) {
+        typedef decltype(of) T;
+        exactly ? LaunchRouteGrad<T, kExactly>(a, on) : wide ? LaunchRouteGrad<T, kAligned>(a, on) : LaunchRouteGrad<T, kAnyhow>(a, on);
+    };
+    logitType == HCCL_DATA_TYPE_FP32 ? go(float{}) : logitType == HCCL_DATA_TYPE_FP16 ? go(_Float16{}) : go(__bf16{});
     return Launched("HcclAmdExpertRouteGrad");
 }
 
