@@ -137,7 +137,7 @@ _lib = None
 
 def lib():
     """Loads lib/libhccl.so; raises if it has not been built (there is no fallback path)."""
-    global _lib, _call
+    global _lib, _call, _expert
     if _lib is not None:
         return _lib
     if not os.path.exists(LIB_PATH):
@@ -212,7 +212,8 @@ def lib():
     L.HcclAmdBlockQuantColumns.argtypes = [vp, i32, u64, u64, u64, u32, vp, i32, vp, u64, vp, vp]
     L.HcclAmdBlockMatmul.argtypes = [vp, u64, vp, u64, u64, u32, vp, vp, vp, vp, u32, u64, u64, i32, vp, i32, u64, vp]
     L.HcclAmdBlockMatmulGradWeight.argtypes = [vp, vp, vp, vp, u64, u64, u64, u64, i32, u32, vp, vp, u32, vp, i32, u32, vp]
-    _call = _native_call(L) or _through_ctypes
+    ranks = _native_ranks(L)
+    _call, _expert = (ranks.call, ranks.expert) if ranks else (_through_ctypes, _through_ctypes)
     _lib = L
     return L
 
@@ -225,8 +226,8 @@ _KINDS = ("HcclAllReduce", "HcclReduceScatter", "HcclAmdReduceScatterNoAlloc", "
  _ALL_TO_ALL_V) = range(9)
 
 
-def _native_call(L):
-    """The native loop over L's functions; None where the extension is not there for this interpreter."""
+def _native_ranks(L):
+    """The native calls of L's functions; None where the extension is not there for this interpreter."""
     if not os.path.exists(RANKS_PATH):
         return None
     loader = importlib.machinery.ExtensionFileLoader("_hccl_ranks", RANKS_PATH)
@@ -236,7 +237,8 @@ def _native_call(L):
     except ImportError:
         return None
     ranks.bind(tuple(ctypes.cast(getattr(L, name), ctypes.c_void_p).value for name in _KINDS))
-    return ranks.call
+    ranks.bind_experts(tuple(ctypes.cast(getattr(L, name), ctypes.c_void_p).value for name in EXPERT_EXPORTS[1:]))
+    return ranks
 
 
 def _through_ctypes(*args):
@@ -249,6 +251,23 @@ def _load_and_call(*args):
 
 
 _call = _load_and_call
+
+
+def _load_and_expert(*args):
+    lib()
+    return _expert(*args)
+
+
+_expert = _load_and_expert
+
+
+def _expert_call(kind, *args):
+    """One experts' operator, EXPERT_EXPORTS[kind + 1]."""
+    code = _expert(kind, *args)
+    if code == -1:
+        code = getattr(lib(), EXPERT_EXPORTS[kind + 1])(*args)
+    if code != HCCL_SUCCESS:
+        raise HcclError(EXPERT_EXPORTS[kind + 1], code)
 
 
 class HcclError(RuntimeError):
@@ -487,37 +506,36 @@ def expert_route_workspace(tokens, experts):
 def expert_route(logits, dtype, tokens, experts, topk, expert_of, weights, row_of, counts, offsets, loss, workspace, workspace_bytes, stream,
                  renorm=False, mask=None, loss_scale=1.0, stride=0):
     """The topk experts of every token, their weights, rows in expert order, per-expert counts and the balance loss."""
-    _check("HcclAmdExpertRoute", lib().HcclAmdExpertRoute(logits, dtype, tokens, experts, stride, topk, 1 if renorm else 0, mask, loss_scale, expert_of,
-                                                          weights, row_of, counts, offsets, loss, workspace, workspace_bytes, stream))
+    _expert_call(0, logits, dtype, tokens, experts, stride, topk, 1 if renorm else 0, mask, loss_scale, expert_of, weights, row_of, counts,
+                 offsets, loss, workspace, workspace_bytes, stream)
 
 
 def expert_route_grad(logits, dtype, tokens, experts, topk, expert_of, counts, weight_grad, loss_grad, logit_grad, stream, renorm=False, mask=None,
                       loss_scale=1.0, stride=0, grad_stride=0):
-    _check("HcclAmdExpertRouteGrad", lib().HcclAmdExpertRouteGrad(logits, dtype, tokens, experts, stride, topk, 1 if renorm else 0, mask, loss_scale,
-                                                                  expert_of, counts, weight_grad, loss_grad, logit_grad, grad_stride, stream))
+    _expert_call(1, logits, dtype, tokens, experts, stride, topk, 1 if renorm else 0, mask, loss_scale, expert_of, counts, weight_grad,
+                 loss_grad, logit_grad, grad_stride, stream)
 
 
 def expert_pack(x, dtype, tokens, width, topk, row_of, out, rows, stream, scales=None, scale_type=HCCL_AMD_SCALE_NONE, x_stride=0, out_stride=0,
                 scale_stride=0):
     """Tokens into expert order: copied, or (scale_type) as 8-bit rows with a scale per 128 values."""
-    _check("HcclAmdExpertPack", lib().HcclAmdExpertPack(x, dtype, tokens, width, x_stride, topk, row_of, scale_type, out, rows, out_stride, scales,
-                                                        scale_stride, stream))
+    _expert_call(2, x, dtype, tokens, width, x_stride, topk, row_of, scale_type, out, rows, out_stride, scales, scale_stride, stream)
 
 
 def expert_combine(x, dtype, rows, width, tokens, topk, row_of, weights, y, stream, x_stride=0, y_stride=0):
     """Rows back to their tokens, weighted and summed (weights None: the gradient of expert_pack)."""
-    _check("HcclAmdExpertCombine", lib().HcclAmdExpertCombine(x, dtype, rows, width, x_stride, tokens, topk, row_of, weights, y, y_stride, stream))
+    _expert_call(3, x, dtype, rows, width, x_stride, tokens, topk, row_of, weights, y, y_stride, stream)
 
 
 def expert_combine_grad(y_grad, x, dtype, rows, width, tokens, topk, row_of, weights, x_grad, weight_grad, stream, y_grad_stride=0, x_stride=0,
                         x_grad_stride=0):
-    _check("HcclAmdExpertCombineGrad", lib().HcclAmdExpertCombineGrad(y_grad, y_grad_stride, x, dtype, rows, width, x_stride, tokens, topk, row_of,
-                                                                      weights, x_grad, x_grad_stride, weight_grad, stream))
+    _expert_call(4, y_grad, y_grad_stride, x, dtype, rows, width, x_stride, tokens, topk, row_of, weights, x_grad, x_grad_stride, weight_grad,
+                 stream)
 
 
 def block_quant_weights(w, dtype, experts, n, k, scale_type, q, scales, q_t, scales_t, stream, stride=0):
     """Weights in 8 bits with a scale per 128 x 128, as they are and / or transposed."""
-    _check("HcclAmdBlockQuantWeights", lib().HcclAmdBlockQuantWeights(w, dtype, experts, n, k, stride, scale_type, q, scales, q_t, scales_t, stream))
+    _expert_call(5, w, dtype, experts, n, k, stride, scale_type, q, scales, q_t, scales_t, stream)
 
 
 def block_columns(rows, groups):
@@ -526,19 +544,17 @@ def block_columns(rows, groups):
 
 
 def block_quant_columns(x, dtype, rows, width, groups, offsets, scale_type, q_t, columns, scales, stream, stride=0):
-    _check("HcclAmdBlockQuantColumns", lib().HcclAmdBlockQuantColumns(x, dtype, rows, width, stride, groups, offsets, scale_type, q_t, columns, scales,
-                                                                      stream))
+    _expert_call(6, x, dtype, rows, width, stride, groups, offsets, scale_type, q_t, columns, scales, stream)
 
 
 def block_matmul(a, a_scales, rows, w, w_scales, experts, n, k, scale_type, y, y_dtype, stream, groups=1, offsets=None, expert_of_group=None,
                  a_stride=0, a_scale_stride=0, y_stride=0):
     """8-bit rows, group by group, times their experts' 8-bit weights."""
-    _check("HcclAmdBlockMatmul", lib().HcclAmdBlockMatmul(a, a_stride, a_scales, a_scale_stride, rows, groups, offsets, expert_of_group, w, w_scales,
-                                                          experts, n, k, scale_type, y, y_dtype, y_stride, stream))
+    _expert_call(7, a, a_stride, a_scales, a_scale_stride, rows, groups, offsets, expert_of_group, w, w_scales, experts, n, k, scale_type, y,
+                 y_dtype, y_stride, stream)
 
 
 def block_matmul_grad_weight(y_grad_t, y_grad_scales, x_t, x_scales, columns, rows, n, k, scale_type, groups, offsets, experts, w_grad, grad_dtype,
                              stream, expert_of_group=None, accumulate=False):
-    _check("HcclAmdBlockMatmulGradWeight", lib().HcclAmdBlockMatmulGradWeight(y_grad_t, y_grad_scales, x_t, x_scales, columns, rows, n, k, scale_type,
-                                                                              groups, offsets, expert_of_group, experts, w_grad, grad_dtype,
-                                                                              1 if accumulate else 0, stream))
+    _expert_call(8, y_grad_t, y_grad_scales, x_t, x_scales, columns, rows, n, k, scale_type, groups, offsets, expert_of_group, experts, w_grad,
+                 grad_dtype, 1 if accumulate else 0, stream)

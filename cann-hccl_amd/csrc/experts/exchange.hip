@@ -20,6 +20,17 @@ __device__ __forceinline__ int64_t FirstWave()
     return int64_t(blockIdx.x) * kWaves + __builtin_amdgcn_readfirstlane(int(threadIdx.x) / 64);
 }
 
+// The rows of a token's choices, all loaded at once: choice j's is in lane j, -1 where there is none within [0, rows).
+__device__ __forceinline__ int RowsOf(const int32_t *rowOf, int64_t token, int topK, int64_t rows)
+{
+    const int j = int(__lane_id());
+    if (rowOf == nullptr) {
+        return j == 0 && token < rows ? int(token) : -1;
+    }
+    const int r = j < topK ? rowOf[token * topK + j] : -1;
+    return r >= 0 && r < rows ? r : -1;
+}
+
 struct PackArgs {
     const void *x;
     const int32_t *rowOf;
@@ -38,11 +49,12 @@ __global__ void __launch_bounds__(kThreads) CopyKernel(PackArgs a)
     for (int64_t w = FirstWave(); w < a.waves; w += int64_t(gridDim.x) * kWaves) {
         const int64_t t = w / a.pieces;
         const int at = int(w % a.pieces) * kPiece + int(threadIdx.x % 64) * kEach;
+        const int rows = RowsOf(a.rowOf, t, a.topK, a.rows);
         float v[kEach];
         LoadPart<kWide, kEach>(static_cast<const T *>(a.x) + t * a.xStride, at, a.width, v);
         for (int j = 0; j < a.topK; j++) {
-            const int64_t r = a.rowOf == nullptr ? t : a.rowOf[t * a.topK + j];
-            if (r >= 0 && r < a.rows) {
+            const int64_t r = __builtin_amdgcn_readlane(rows, j);
+            if (r >= 0) {
                 StorePart<kWide, kEach>(static_cast<T *>(a.out) + r * a.outStride, at, a.width, v);
             }
         }
@@ -56,6 +68,7 @@ __global__ void __launch_bounds__(kThreads) QuantKernel(PackArgs a)
     for (int64_t w = FirstWave(); w < a.waves; w += int64_t(gridDim.x) * kWaves) {
         const int64_t t = w / a.pieces;
         const int at = int(w % a.pieces) * kPiece + int(threadIdx.x % 64) * kEach;
+        const int rows = RowsOf(a.rowOf, t, a.topK, a.rows);
         float v[kEach];
         LoadPart<kWide, kEach>(static_cast<const T *>(a.x) + t * a.xStride, at, a.width, v);
         float top = 0.0f;
@@ -77,8 +90,8 @@ __global__ void __launch_bounds__(kThreads) QuantKernel(PackArgs a)
         q.x = Quantise4(s[0], s[1], s[2], s[3]);
         q.y = Quantise4(s[4], s[5], s[6], s[7]);
         for (int j = 0; j < a.topK; j++) {
-            const int64_t r = a.rowOf == nullptr ? t : a.rowOf[t * a.topK + j];
-            if (r >= 0 && r < a.rows && at < a.padded) {
+            const int64_t r = __builtin_amdgcn_readlane(rows, j);
+            if (r >= 0 && at < a.padded) {
                 *reinterpret_cast<Word2 *>(static_cast<uint8_t *>(a.out) + r * a.outStride + at) = q;
                 if (threadIdx.x % 16 == 0) {
                     static_cast<typename BlockScale<kScale>::Stored *>(a.scales)[r * a.scaleStride + at / 128] = scale.stored;
@@ -109,28 +122,25 @@ __global__ void __launch_bounds__(kThreads) CombineKernel(CombineArgs a)
     for (int64_t w = FirstWave(); w < a.waves; w += int64_t(gridDim.x) * kWaves) {
         const int64_t t = w / a.pieces;
         const int at = int(w % a.pieces) * kPiece + int(threadIdx.x % 64) * kEach;
+        const int rows = RowsOf(a.rowOf, t, a.topK, a.rows), lane = int(__lane_id());
+        const float weight = rows >= 0 && a.weights != nullptr ? a.weights[t * a.topK + lane] : 1.0f;
         float sum[kEach] = {};
         for (int j0 = 0; j0 < a.topK; j0 += 4) {
-            float v[4][kEach], by[4];
-            bool is[4];
+            float v[4][kEach];
 #pragma unroll
             for (int j = 0; j < 4; j++) {
-                int64_t r = -1;
-                if (j0 + j < a.topK) {
-                    r = a.rowOf == nullptr ? t : a.rowOf[t * a.topK + j0 + j];
-                }
-                is[j] = r >= 0 && r < a.rows;
-                by[j] = !is[j] || a.weights == nullptr ? 1.0f : a.weights[t * a.topK + j0 + j];
-                if (is[j]) {
+                const int64_t r = __builtin_amdgcn_readlane(rows, j0 + j);     // (-1 from lanes beyond topK)
+                if (r >= 0) {
                     LoadPart<kWide, kEach>(static_cast<const T *>(a.x) + r * a.xStride, at, a.width, v[j]);
                 }
             }
 #pragma unroll
             for (int j = 0; j < 4; j++) {
-                if (is[j]) {
+                if (__builtin_amdgcn_readlane(rows, j0 + j) >= 0) {
+                    const float by = __int_as_float(__builtin_amdgcn_readlane(__float_as_int(weight), j0 + j));
 #pragma unroll
                     for (int i = 0; i < kEach; i++) {
-                        sum[i] = __builtin_fmaf(by[j], v[j][i], sum[i]);
+                        sum[i] = __builtin_fmaf(by, v[j][i], sum[i]);
                     }
                 }
             }
@@ -146,20 +156,15 @@ __global__ void __launch_bounds__(kThreads) CombineGradKernel(CombineArgs a)
     __shared__ float part[kWaves][kRows];
     for (int64_t t = blockIdx.x; t < a.tokens; t += gridDim.x) {
         const T *dy = static_cast<const T *>(a.yGrad) + t * a.yStride;
+        const int rows = RowsOf(a.rowOf, t, a.topK, a.rows), lane = int(__lane_id());
+        const float weight = rows >= 0 && a.weights != nullptr ? a.weights[t * a.topK + lane] : 1.0f;
         int64_t r[kRows];
         float by[kRows], dot[kRows];
 #pragma unroll
         for (int j = 0; j < kRows; j++) {
-            r[j] = -1;
+            r[j] = __builtin_amdgcn_readlane(rows, j);
+            by[j] = __int_as_float(__builtin_amdgcn_readlane(__float_as_int(weight), j));
             dot[j] = 0.0f;
-            by[j] = 0.0f;
-            if (j < a.topK) {
-                r[j] = a.rowOf == nullptr ? t : a.rowOf[t * a.topK + j];
-                if (r[j] >= a.rows) {
-                    r[j] = -1;
-                }
-                by[j] = a.weights == nullptr ? 1.0f : a.weights[t * a.topK + j];
-            }
         }
         for (int at = int(threadIdx.x) * kEach; at < a.width; at += kThreads * kEach) {
             float d[kEach];

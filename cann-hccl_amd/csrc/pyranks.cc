@@ -6,6 +6,9 @@
 // per collective: 8-rank all-reduce of 8 KiB 7.6 us through ctypes, 4.4 us here; 64-rank all-to-all-v of short blocks,
 // tables as numpy arrays, 80 us and 29 us.
 //
+// The experts' operators (hccl_amd_experts.h) are single calls of up to 18 arguments, whose conversion by ctypes costs more than
+// the launch: expert() makes them in the same way.  Packing 64 tokens, call to call: 7.4 us through ctypes, 6.9 us here.
+//
 // Whatever this loop does not recognise (other sequence or pointer types than lists or tuples of integers, None and
 // c_void_p) it leaves alone: call() then returns -1 before any call was made and the caller goes through ctypes.
 //
@@ -16,8 +19,12 @@
 
 #include <cstdint>
 #include <cstring>
+#include <tuple>
+#include <type_traits>
+#include <utility>
 
 #include "hccl/hccl.h"
+#include "hccl/hccl_amd_experts.h"
 #include "hccl/hccl_amd_ext.h"
 
 namespace {
@@ -41,6 +48,21 @@ struct Functions {
 };
 static_assert(sizeof(Functions) == KIND_COUNT * sizeof(void *), "one function per kind");
 Functions g_fn = {};
+
+// the experts' operators, in the order of the mirror's EXPERT_EXPORTS without its first (a query)
+struct ExpertFunctions {
+    decltype(&HcclAmdExpertRoute) route;
+    decltype(&HcclAmdExpertRouteGrad) routeGrad;
+    decltype(&HcclAmdExpertPack) pack;
+    decltype(&HcclAmdExpertCombine) combine;
+    decltype(&HcclAmdExpertCombineGrad) combineGrad;
+    decltype(&HcclAmdBlockQuantWeights) quantWeights;
+    decltype(&HcclAmdBlockQuantColumns) quantColumns;
+    decltype(&HcclAmdBlockMatmul) matmul;
+    decltype(&HcclAmdBlockMatmulGradWeight) matmulGradWeight;
+};
+constexpr long kExpertKinds = sizeof(ExpertFunctions) / sizeof(void *);
+ExpertFunctions g_expert = {};
 
 constexpr Py_ssize_t kMostRanks = 64;
 PyObject *g_valueName = nullptr;      // "value"
@@ -85,6 +107,49 @@ int AsNumber(PyObject *o, uint64_t *out)
         return 0;
     }
     return 1;
+}
+
+// An argument of the C API from a Python one: pointers, whole numbers and enumerations, floats.
+template <typename T>
+bool AsArgument(PyObject *o, T *out)
+{
+    if constexpr (std::is_pointer_v<T>) {
+        void *p = nullptr;
+        const bool ok = AsPointer(o, &p) == 1;
+        *out = static_cast<T>(p);
+        return ok;
+    } else if constexpr (std::is_floating_point_v<T>) {
+        if (!PyFloat_CheckExact(o)) {
+            return false;
+        }
+        *out = static_cast<T>(PyFloat_AS_DOUBLE(o));
+        return true;
+    } else {
+        uint64_t n = 0;
+        const bool ok = AsNumber(o, &n) == 1;
+        *out = static_cast<T>(n);
+        return ok;
+    }
+}
+
+template <typename... A, size_t... I>
+long Forward(HcclResult (*fn)(A...), PyObject *const *args, std::index_sequence<I...>)
+{
+    std::tuple<A...> value;
+    if (!(AsArgument(args[I], &std::get<I>(value)) && ...)) {
+        return -1;
+    }
+    HcclResult res = HCCL_SUCCESS;
+    Py_BEGIN_ALLOW_THREADS
+    res = fn(std::get<I>(value)...);
+    Py_END_ALLOW_THREADS
+    return static_cast<long>(res);
+}
+
+template <typename... A>
+long Forward(HcclResult (*fn)(A...), PyObject *const *args, Py_ssize_t n)
+{
+    return fn == nullptr || n != Py_ssize_t(sizeof...(A)) ? -1 : Forward(fn, args, std::index_sequence_for<A...>{});
 }
 
 bool Plain(PyObject *o) { return PyList_CheckExact(o) || PyTuple_CheckExact(o); }
@@ -205,7 +270,54 @@ PyObject *Bind(PyObject *, PyObject *addresses)
     Py_RETURN_NONE;
 }
 
+// expert(kind, the C function's arguments ...) -> HcclResult, or -1 (not recognised, nothing called).
+PyObject *Expert(PyObject *, PyObject *const *args, Py_ssize_t nargs)
+{
+    uint64_t kind = 0;
+    long res = -1;
+    if (nargs >= 1 && AsNumber(args[0], &kind) == 1) {
+        const Py_ssize_t n = nargs - 1;
+        PyObject *const *a = args + 1;
+        switch (kind) {
+            case 0: res = Forward(g_expert.route, a, n); break;
+            case 1: res = Forward(g_expert.routeGrad, a, n); break;
+            case 2: res = Forward(g_expert.pack, a, n); break;
+            case 3: res = Forward(g_expert.combine, a, n); break;
+            case 4: res = Forward(g_expert.combineGrad, a, n); break;
+            case 5: res = Forward(g_expert.quantWeights, a, n); break;
+            case 6: res = Forward(g_expert.quantColumns, a, n); break;
+            case 7: res = Forward(g_expert.matmul, a, n); break;
+            case 8: res = Forward(g_expert.matmulGradWeight, a, n); break;
+            default: break;
+        }
+    }
+    return PyLong_FromLong(res);
+}
+
+// bind_experts(addresses): the experts' functions, in the order of ExpertFunctions, as integers.
+PyObject *BindExperts(PyObject *, PyObject *addresses)
+{
+    if (!PyTuple_CheckExact(addresses) || PyTuple_GET_SIZE(addresses) != kExpertKinds) {
+        PyErr_SetString(PyExc_TypeError, "bind_experts: a tuple of one address per operator");
+        return nullptr;
+    }
+    void *address[kExpertKinds];
+    for (long k = 0; k < kExpertKinds; k++) {
+        address[k] = PyLong_AsVoidPtr(PyTuple_GET_ITEM(addresses, k));
+        if (address[k] == nullptr) {
+            if (!PyErr_Occurred()) {
+                PyErr_SetString(PyExc_ValueError, "bind_experts: null address");
+            }
+            return nullptr;
+        }
+    }
+    std::memcpy(&g_expert, address, sizeof(g_expert));
+    Py_RETURN_NONE;
+}
+
 PyMethodDef g_methods[] = {
+    {"expert", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(Expert)), METH_FASTCALL, "one call of an experts' operator"},
+    {"bind_experts", BindExperts, METH_O, "the functions that expert() calls"},
     {"call", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(Call)), METH_FASTCALL, "one collective, called for every rank"},
     {"bind", Bind, METH_O, "the functions that call() calls"},
     {nullptr, nullptr, 0, nullptr},

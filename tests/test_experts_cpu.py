@@ -193,3 +193,24 @@ def test_reference_scales():
     assert (tops.astype(np.float64) <= 448 * value).all() and (tops.astype(np.float64) > 224 * value).all()
     assert np.array_equal(times.astype(np.float64) * value, np.ones(len(tops)))
     assert ref.block_scale(np.float32([0]), ref.E8M0)[0][0] == 127 - 96 - 8
+
+
+def test_native_calls_and_ctypes_refuse_alike():
+    """The mirror's two ways to a call give the same answers; what the native one does not recognise it leaves alone."""
+    L = H.lib()
+    pack = (P, BF16, 10, 300, 0, 2, P, 1, P, 20, 0, P, 0, N)
+    for at, value in ((13, None), (0, None), (1, INT8), (5, 0), (6, None), (10, 392), (11, P + 2)):
+        args = pack[:at] + (value,) + pack[at + 1:]
+        code = L.HcclAmdExpertPack(*args)
+        assert code in (PARA, PTR, NOT_SUPPORT)
+        assert H._expert(2, *args) in ((code,) if H._expert is not H._through_ctypes else (-1,))
+        with pytest.raises(H.HcclError) as e:
+            H._expert_call(2, *args)
+        assert e.value.code == code
+    if H._expert is not H._through_ctypes:
+        refused = (P, BF16, 0, 64, 0, 8, 0, None, 0.01, None, None, None, None, None, None, None, 0, N)
+        assert H._expert(0, *refused) == PTR
+        for args in (refused[:-1], refused + (1,), refused[:8] + (1,) + refused[9:], ("1",) + refused[1:], refused[:2] + (1.0,) + refused[3:]):
+            assert H._expert(0, *args) == -1
+        assert H._expert(9) == -1 and H._expert() == -1 and H._expert("0") == -1
+        assert H._expert(0, ctypes.c_void_p(P), *refused[1:]) == PTR
