@@ -288,9 +288,10 @@ __device__ __forceinline__ uint32_t ScaleBits(uint8_t s) { return s; }
 // registers.  The 16-byte pieces of a row lie in LDS in an order that depends on the row (piece p of row r at p ^ (r / 2 % 8)), so that the
 // 16 rows a lane group reads are in different banks; since such a load fills LDS in lane order, it is the lanes' addresses
 // in memory that are swapped.  Scales pass through a register of one thread each.
+// (Two waves to a SIMD are asked for: with the registers of one the compiler keeps products apart from what it computes with.)
 // kPrecise: 16-bit matrix instructions on widened values, else 8-bit ones.  kGrad: the weights' gradient, scales by column too.
 template <typename T, HcclAmdScaleType kScale, bool kPrecise, bool kGrad, int kRF, int kCF, int kWR, int kWC>
-__global__ void __launch_bounds__(64 * kWR * kWC) TileKernel(ProductArgs a)
+__global__ void __launch_bounds__(64 * kWR * kWC, 2) TileKernel(ProductArgs a)
 {
     constexpr bool kPowers = kScale == HCCL_AMD_SCALE_E8M0;
     typedef typename BlockScale<kScale>::Stored Stored;

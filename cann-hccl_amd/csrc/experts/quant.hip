@@ -14,6 +14,10 @@ constexpr int kThreads = 256;
 constexpr int kTile = 128;
 constexpr int kPitch = kTile + 16;    // LDS bytes from one transposed row to the next
 
+// Where the eight bytes of rows 8 * group + [0, 8) of column c lie in the transposed tile.  16-byte pieces change places by column / 16: with the
+// pitch, which moves every other eight columns by half the banks, the 64 writes of a wave are spread over all banks evenly.
+__device__ __forceinline__ int TransposedAt(int c, int group) { return c * kPitch + (group ^ c / 16 * 2) * 8; }
+
 struct TileArgs {
     const void *x;
     const int32_t *offsets;
@@ -43,7 +47,7 @@ __device__ __forceinline__ void StoreTransposed(const uint8_t *tile, uint8_t *to
     for (int i = 0; i < 4; i++) {
         const int piece = int(threadIdx.x) + i * kThreads, c = piece / 8, b = piece % 8 * 16;
         if (column + c < width) {
-            *reinterpret_cast<Word4 *>(to + int64_t(column + c) * pitch + at + b) = *reinterpret_cast<const Word4 *>(tile + c * kPitch + b);
+            *reinterpret_cast<Word4 *>(to + int64_t(column + c) * pitch + at + b) = *reinterpret_cast<const Word4 *>(tile + TransposedAt(c, b / 8));
         }
     }
 }
@@ -53,7 +57,7 @@ template <typename T, HcclAmdScaleType kScale, bool kWide>
 __global__ void __launch_bounds__(kThreads) ColumnsKernel(TileArgs a)
 {
     __shared__ __align__(16) uint8_t tile[kTile * kPitch];
-    __shared__ float tops[16][kTile];
+    __shared__ float tops[16][kTile + 1];
     const int tiles = (a.width + kTile - 1) / kTile;
     const int unit = int(blockIdx.x) / tiles, column = int(blockIdx.x) % tiles * kTile;   // the tiles of a unit's rows lie next to each other
     const Unit u = FindUnit(a.offsets, a.groups, a.rows, unit, kTile);
@@ -95,7 +99,7 @@ __global__ void __launch_bounds__(kThreads) ColumnsKernel(TileArgs a)
         for (int p = 0; p < 8; p++) {
             s[p] = Scaled8(v[p][i], times);
         }
-        *reinterpret_cast<Word2 *>(tile + (cg + i) * kPitch + rg * 8) = Word2{Quantise4(s[0], s[1], s[2], s[3]), Quantise4(s[4], s[5], s[6], s[7])};
+        *reinterpret_cast<Word2 *>(tile + TransposedAt(cg + i, rg)) = Word2{Quantise4(s[0], s[1], s[2], s[3]), Quantise4(s[4], s[5], s[6], s[7])};
     }
     __syncthreads();
     StoreTransposed(tile, static_cast<uint8_t *>(a.qT), a.pitchT, int64_t(unit) * kTile, column, a.width);
@@ -161,7 +165,7 @@ __global__ void __launch_bounds__(kThreads) WeightsKernel(TileArgs a)
     }
 #pragma unroll
     for (int i = 0; i < 8; i++) {
-        *reinterpret_cast<Word2 *>(tile + (cg + i) * kPitch + rg * 8) =
+        *reinterpret_cast<Word2 *>(tile + TransposedAt(cg + i, rg)) =
             Word2{Quantise4(v[0][i], v[1][i], v[2][i], v[3][i]), Quantise4(v[4][i], v[5][i], v[6][i], v[7][i])};
     }
     __syncthreads();
