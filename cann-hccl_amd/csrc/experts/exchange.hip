@@ -1,6 +1,12 @@
 // Rows into expert order and back: HcclAmdExpertPack, HcclAmdExpertCombine and its gradient.  No arithmetic to speak of: bytes
 // moved bound all three, so every row is read once and written once, 16 bytes to a lane, 512 values to a wave and step, and what
-// a step needs is loaded before any of it is used.
+// a step needs is loaded before any of it is used, the token's row numbers and weights first.  A copy to all of a token's rows needs
+// one reading of the token; a wave to a token and 512 values gives 131072 waves for 16384 x 4096, each with no more than it can
+// hold in registers.
+//
+// Measured, where a large copy reaches 5.15 TB/s: 16384 tokens of 4096 values to eight rows each in 8 bits (0.68 GB) 122 us, 5.5 TB/s;
+// back and weighted (1.2 GB) 246 us, 4.9 TB/s; the gradients of that (2.2 GB) 424 us, 5.2 TB/s.  2001 values to a row, off every
+// boundary (8191 tokens, four rows each): 41 and 74 us, 4.0 TB/s.  64 tokens of 8192: 4 us.
 #include "common.h"
 
 namespace hcclamd {

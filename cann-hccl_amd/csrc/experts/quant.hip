@@ -1,7 +1,8 @@
 // 8-bit operands of the experts' products that are not rows: columns (HcclAmdBlockQuantColumns, for the weights' gradient, whose
 // sum runs over rows) and weights (HcclAmdBlockQuantWeights).  Both take tiles of 128 x 128, read once, 16 bytes to a lane; a
 // thread holds eight values of each of eight rows that follow each other, so its part of a transposed row is eight bytes in one
-// piece.  The transposed tile passes through LDS and leaves it in whole lines of 128 bytes.  Bytes moved bound it.
+// piece.  The transposed tile passes through LDS and leaves it in whole lines of 128 bytes.  Bytes moved bound it: 16411 rows of
+// 4096 values (0.2 GB) take 48 us, 4.2 TB/s, where a large copy reaches 5.15.
 #include <type_traits>
 
 #include "common.h"
