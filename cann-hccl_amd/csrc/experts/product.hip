@@ -94,7 +94,8 @@ __device__ __forceinline__ void StoreFour(T *out, const float (&v)[4], int col, 
 
 // 16 rows by 16 kCF columns of the result to a workgroup, whose kWaves waves share the blocks out among them, kAhead at a time, and
 // add up through LDS: for few rows, where the weights' bytes are what takes time and as many waves as possible should be reading
-// them, all they need next at once.
+// them, all they need next at once.  8 rows at 8 of 64 experts by 4096 x 2048 (67 MB of weights): 13.3 us, 5.0 TB/s, what a copy
+// reaches; one row by 4096 x 8192 (34 MB): 9 us.
 template <typename T, HcclAmdScaleType kScale, int kCF, int kWaves, int kAhead>
 __global__ void __launch_bounds__(64 * kWaves) FewRowsKernel(ProductArgs a)
 {
@@ -288,6 +289,12 @@ __device__ __forceinline__ uint32_t ScaleBits(uint8_t s) { return s; }
 // registers.  The 16-byte pieces of a row lie in LDS in an order that depends on the row (piece p of row r at p ^ (r / 2 % 8)), so that the
 // 16 rows a lane group reads are in different banks; since such a load fills LDS in lane order, it is the lanes' addresses
 // in memory that are swapped.  Scales pass through a register of one thread each.
+// 256 x 256 to a workgroup of eight waves needs 128 KiB of LDS and 128 sums to a lane, all there is; reading it takes 1536 cycles of LDS a step
+// and filling it 512, its products 2048 of the matrix unit, so that neither can wait long for the other.  Measured: 8192 x 4096 x 8192, scales
+// of powers of two, 217 to 237 us (2.3 to 2.5 PFLOP/s; the matrix unit alone reaches 4.4, a library's product with one scale for all 2.7);
+// 32768 rows of 64 experts by 4096 x 2048, 32-bit scales, 385 us (1.43), a fifth of it tiles that are not full; the weights'
+// gradient of 16 experts, 16411 rows, 2048 x 4096, 335 us (0.82), of which its 0.5 GB of results take 100: widening and scaling are as many
+// cycles as its products.
 // (Two waves to a SIMD are asked for: with the registers of one the compiler keeps products apart from what it computes with.)
 // kPrecise: 16-bit matrix instructions on widened values, else 8-bit ones.  kGrad: the weights' gradient, scales by column too.
 template <typename T, HcclAmdScaleType kScale, bool kPrecise, bool kGrad, int kRF, int kCF, int kWR, int kWC>
@@ -637,13 +644,13 @@ void Choose(HcclDataType type, HcclAmdScaleType scaleType, F f)
 
 constexpr uint64_t kMostTiles = uint64_t(1) << 22;   // workgroups of up to 512 below 2^32 threads
 
-// Tiles of 256 x 256 or of 128 x 128, from how many there are of each.  Of a product with 8192 values to a sum, a step takes 1.72 us where a
-// compute unit has a tile of 256, 1.25 us where it has two of 128 and 0.82 us where it has one; 256 and 512 are under way at once.
-// (2048 rows by 4096: 115 us with 256, 82 with 128; 4096 rows: 133 and 160.)
+// Tiles of 256 x 256 or of 128 x 128, from how many there are of each.  Of a product with 8192 values to a sum, a step takes 1.75 us where a
+// compute unit has a tile of 256, 1.18 us where it has two of 128 and 0.70 us where it has one; 256 and 512 are under way at once.
+// (2048 rows by 4096: 119 us with 256, 76 with 128; 4096 rows: 134 and 159.)
 bool LargeTiles(uint64_t tiles256, uint64_t tiles128)
 {
     const uint64_t rest = tiles128 % 512;
-    return (tiles256 + 255) / 256 * 172 < tiles128 / 512 * 125 + (rest == 0 ? 0 : rest <= 256 ? 82 : 125);
+    return (tiles256 + 255) / 256 * 175 < tiles128 / 512 * 118 + (rest == 0 ? 0 : rest <= 256 ? 70 : 118);
 }
 
 constexpr int64_t kMostPitch = int64_t(1) << 23;     // bytes of a row: those of a tile's 256 rows are within 2^31
@@ -704,9 +711,9 @@ HcclResult HcclAmdBlockMatmul(const void *a, uint64_t aStride, const void *aScal
     EXPERTS_CHK(uint64_t(p.outPitch) >= n && AlignedTo(yType, y));
     EXPERTS_CHK(Aligned(offsets, 4) && Aligned(expertOfGroup, 4));
     p.wideOut = WideOut(yType, n, y, p.outPitch);
-    // Which kernel, 64 groups by 4096 x 2048 and one by 4096 x 8192, 32-bit scales: few rows against tiles of 128 takes 13 us against 17
-    // (8 rows, 64 groups), 88 against 100 (256 rows), 126 against 103 (512 rows); 8 against 49 (1 row, one group), 43 against 52 (128 rows), 83
-    // against 52 (256 rows).  16 columns to a workgroup instead of 64: 8 against 21 (1 row), 12 against 24 (16 rows), 39 against 24 (64 rows).
+    // Which kernel, 64 groups by 4096 x 2048 and one by 4096 x 8192, 32-bit scales: few rows against tiles of 128 takes 13 us against 16
+    // (8 rows, 64 groups), 90 against 100 (256 rows), 108 against 103 (512 rows); 9 against 45 (1 row, one group), 44 against 49 (128 rows), 85
+    // against 49 (256 rows).  16 columns to a workgroup instead of 64: 9 against 21 (1 row), 13 against 24 (16 rows), 40 against 25 (64 rows).
     // Units there can be: every group that has rows ends with a shorter one.
     const auto unitsOf = [&](uint64_t per) { return offsets == nullptr ? (rows + per - 1) / per : rows / per + (rows < groups ? rows : groups); };
     const uint64_t few64 = unitsOf(16) * ((n + 63) / 64);

@@ -18,7 +18,7 @@
  *
  * 8-bit rows.  HCCL_DATA_TYPE_FP8E4M3 values (largest 448) with one scale per 128 consecutive values: value = q * scale.
  * Every row is padded with zeros to a multiple of 128 values, starts on a 16-byte boundary, and its stride is a multiple
- * of 16.  Of a block, a = max(largest finite magnitude, 2^-96); the scale is
+ * of 16 below 2^23.  Of a block, a = max(largest finite magnitude, 2^-96); the scale is
  *   HCCL_AMD_SCALE_FP32   float a * (1 / 448), q = round(v * (1 / a * 448)), every quotient and product rounded to 32 bits
  *   HCCL_AMD_SCALE_E8M0   one byte b that stands for 2^(b - 127), the least power of two with a <= 448 * 2^(b - 127);
  *                         q = round(v / scale)
@@ -108,14 +108,16 @@ extern HcclResult HcclAmdBlockQuantColumns(const void *x, HcclDataType type, uin
  *   expertOfGroup[groups]        the weights a group uses; NULL: group g uses weights g
  *   w[experts][n][ceil128(k)]    8-bit weights, wScales[experts][ceil(n/128)][ceil(k/128)], as HcclAmdBlockQuantWeights leaves them
  *   y[rows][yStride]             yType FP32, FP16 or BFP16, n to a row
- * Rows outside all groups are left as they are.  The gradient of the rows is the same call with the transposed weights. */
+ * Rows outside all groups are left as they are.  The gradient of the rows is the same call with the transposed weights.
+ * Sums: products are exact, 32-bit results and sums over up to 256 values are added in 32 bits; 16-bit results over more values come from the
+ * 8-bit matrix instruction, which is 1.3e-5 off (2-norm), two orders below their own rounding. */
 extern HcclResult HcclAmdBlockMatmul(const void *a, uint64_t aStride, const void *aScales, uint64_t aScaleStride, uint64_t rows,
     uint32_t groups, const int32_t *offsets, const int32_t *expertOfGroup, const void *w, const void *wScales, uint32_t experts,
     uint64_t n, uint64_t k, HcclAmdScaleType scaleType, void *y, HcclDataType yType, uint64_t yStride, void *stream);
 
 /* wGrad[e][n][k] = sum over the rows r of e's groups of yGrad[r][n] * x[r][k] (added to what is there with `accumulate`), from
- * both sides' 8-bit columns (HcclAmdBlockQuantColumns of the same rows, groups, offsets and columns).  Experts without rows get
- * zeros.  wGrad: FP32, FP16 or BFP16. */
+ * both sides' 8-bit columns (HcclAmdBlockQuantColumns of the same rows, groups, offsets and columns, below 2^23).  Experts without
+ * rows get zeros; all sums are in 32 bits.  wGrad: FP32, FP16 or BFP16. */
 extern HcclResult HcclAmdBlockMatmulGradWeight(const void *yGradT, const void *yGradScales, const void *xT, const void *xScales,
     uint64_t columns, uint64_t rows, uint64_t n, uint64_t k, HcclAmdScaleType scaleType, uint32_t groups, const int32_t *offsets,
     const int32_t *expertOfGroup, uint32_t experts, void *wGrad, HcclDataType gradType, uint32_t accumulate, void *stream);

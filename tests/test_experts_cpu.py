@@ -133,6 +133,7 @@ def test_quant_columns_refuses(want, kw):
     (PARA, dict(groups=0)), (PARA, dict(experts=0)), (PARA, dict(groups=4097, owner=P)), (PARA, dict(offsets=None)), (PARA, dict(groups=5)),
     (PARA, dict(stride=299)), (PARA, dict(stride=392)), (PARA, dict(a=P + 8)), (PARA, dict(w=P + 8)), (PARA, dict(s_stride=2)), (PARA, dict(sa=P + 1)),
     (PARA, dict(y_stride=99)), (PARA, dict(y=P + 1)), (PARA, dict(offsets=P + 1)), (PARA, dict(rows=(1 << 28) + 1)),
+    (PARA, dict(stride=1 << 23)), (PARA, dict(k=1 << 23)),
     (OK, dict(rows=0, a=None)), (OK, dict(n=0, w=None)),
 ])
 def test_matmul_refuses(want, kw):
@@ -145,7 +146,7 @@ def test_matmul_refuses(want, kw):
 @pytest.mark.parametrize("want,kw", [
     (PTR, dict(stream=None)), (PTR, dict(dy=None)), (PTR, dict(sdy=None)), (PTR, dict(x=None)), (PTR, dict(sx=None)), (PTR, dict(dw=None)),
     (NOT_SUPPORT, dict(type=INT8)), (NOT_SUPPORT, dict(kind=0)), (PARA, dict(groups=0)), (PARA, dict(experts=4097)), (PARA, dict(offsets=None)),
-    (PARA, dict(columns=384)), (PARA, dict(columns=513)), (PARA, dict(dy=P + 8)), (PARA, dict(dw=P + 1)), (OK, dict(n=0)), (OK, dict(k=0)),
+    (PARA, dict(columns=384)), (PARA, dict(columns=513)), (PARA, dict(columns=1 << 23)), (PARA, dict(dy=P + 8)), (PARA, dict(dw=P + 1)), (OK, dict(n=0)), (OK, dict(k=0)),
 ])
 def test_grad_weight_refuses(want, kw):
     a = dict(dy=P, sdy=P, x=P, sx=P, columns=512, rows=50, n=100, k=300, kind=1, groups=4, offsets=P, owner=None, experts=4, dw=P, type=BF16, add=0, stream=N)
