@@ -492,7 +492,9 @@ __global__ void __launch_bounds__(64 * kWR * kWC, 2) TileKernel(ProductArgs a)
             rs0 = rs1;
             x1 = after;
             rs1 = afterScale;
-            __builtin_amdgcn_sched_barrier(0);   // (the scheduler would read all rows first and run out of registers)
+            if (r % 2 == 1) {
+                __builtin_amdgcn_sched_barrier(0);   // (the scheduler would read all rows first and run out of registers)
+            }
         }
         keepScales(otherScale);
         LoadsDone();

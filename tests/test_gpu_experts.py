@@ -602,3 +602,59 @@ def test_products_in_a_graph(stream):
         step(stream.cuda_stream)
         done(stream)
         assert torch.equal(got, out) and torch.equal(got_loss, loss) and bool(out.any())
+
+
+# ---- addresses beyond 2^32 bytes ------------------------------------------------------------------------------------------------------
+
+def test_exchange_beyond_32_bits(stream):
+    """Rows 3 GB apart, tokens likewise."""
+    W, far = 264, 1_600_000_000
+    big = torch.empty(far * 2 + W, dtype=torch.bfloat16, device="cuda")
+    x = torch.randn(3, W, device="cuda").bfloat16()
+    row = torch.tensor([[2], [0], [1]], dtype=torch.int32, device="cuda")
+    y, dw = torch.empty(3, W, dtype=torch.bfloat16, device="cuda"), torch.empty(3, 1, device="cuda")
+    w = torch.tensor([[1.0], [2.0], [4.0]], device="cuda")
+    q, s = torch.empty(3, up128(W), dtype=torch.uint8, device="cuda"), torch.empty(3, 3, device="cuda")
+    ready()
+    S = stream.cuda_stream
+    BF = H.HCCL_DATA_TYPE_BFP16
+    H.expert_pack(x.data_ptr(), BF, 3, W, 1, row.data_ptr(), big.data_ptr(), 3, S, out_stride=far)
+    H.expert_combine(big.data_ptr(), BF, 3, W, 3, 1, row.data_ptr(), w.data_ptr(), y.data_ptr(), S, x_stride=far)
+    H.expert_pack(big.data_ptr(), BF, 3, W, 1, None, q.data_ptr(), 3, S, scales=s.data_ptr(), scale_type=ref.FP32, x_stride=far)
+    H.expert_combine_grad(x.data_ptr(), big.data_ptr(), BF, 3, W, 3, 1, row.data_ptr(), w.data_ptr(), None, dw.data_ptr(), S, x_stride=far)
+    done(stream)
+    for t in range(3):
+        assert torch.equal(big[int(row[t]) * far:int(row[t]) * far + W], x[t])
+    assert torch.equal(y, (x.float() * w).bfloat16())
+    codes, stored, _ = ref.quant_rows(x[[1, 2, 0]].float().cpu().numpy(), ref.FP32)
+    assert np.array_equal(q.cpu().numpy(), codes) and np.array_equal(s.cpu().numpy(), stored)
+    X = x.double().cpu().numpy()
+    assert close(dw.cpu().numpy()[:, 0], (X * X).sum(1), (W + 1) * U * (X * X).sum(1))
+    del big
+    torch.cuda.empty_cache()
+
+
+@pytest.mark.parametrize("rows,experts,n", [(300, 3, 200_064), (600_000, 2, 64)])
+def test_matmul_beyond_32_bits(stream, rows, experts, n):
+    """Weights, or rows, of more than 4 GiB; the last expert's and the last rows' results."""
+    k = 8192
+    g = torch.Generator(device="cuda").manual_seed(6)
+    a = torch.randint(0, 120, (rows, k), generator=g, device="cuda", dtype=torch.uint8)
+    w = torch.randint(0, 120, (experts, n, k), generator=g, device="cuda", dtype=torch.uint8)
+    nb = (n + 127) // 128
+    sa, sw = torch.rand((rows, k // 128), generator=g, device="cuda"), torch.rand((experts, nb, k // 128), generator=g, device="cuda")
+    cut = rows - rows // 3
+    off = torch.tensor([0] + [cut] * (experts - 1) + [rows], dtype=torch.int32, device="cuda")
+    y = torch.empty(rows, n, device="cuda", dtype=torch.bfloat16)
+    ready()
+    H.block_matmul(a.data_ptr(), sa.data_ptr(), rows, w.data_ptr(), sw.data_ptr(), experts, n, k, ref.FP32, y.data_ptr(), H.HCCL_DATA_TYPE_BFP16,
+                   stream.cuda_stream, groups=experts, offsets=off.data_ptr())
+    done(stream)
+    value = lambda q, s: q.view(torch.float8_e4m3fn).double() * s.double().repeat_interleave(128, -1)  # noqa: E731
+    for lo, e in ((cut - 20, 0), (rows - 20, experts - 1)):
+        x = value(a[lo:lo + 20], sa[lo:lo + 20])
+        m = value(w[e, n - 64:], sw[e, torch.arange(n - 64, n, device="cuda") // 128])
+        want = x @ m.T                                     # (all values positive: the sum of the magnitudes is the sum)
+        assert close(y[lo:lo + 20, n - 64:].double().cpu().numpy(), want.cpu().numpy(), 2 * (k + 3 * k // 128 + 2) * U * want.cpu().numpy(), torch.bfloat16)
+    del a, w, y
+    torch.cuda.empty_cache()
