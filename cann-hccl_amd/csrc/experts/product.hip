@@ -92,18 +92,18 @@ __device__ __forceinline__ void StoreFour(T *out, const float (&v)[4], int col, 
     }
 }
 
-// 16 rows by 16 kCF columns of the result to a workgroup, whose kWaves waves share the blocks out among them, kAhead at a time, and
+// 16 kRF rows by 16 kCF columns of the result to a workgroup, whose kWaves waves share the blocks out among them, kAhead at a time, and
 // add up through LDS: for few rows, where the weights' bytes are what takes time and as many waves as possible should be reading
 // them, all they need next at once.  8 rows at 8 of 64 experts by 4096 x 2048 (67 MB of weights): 13.3 us, 5.0 TB/s, what a copy
 // reaches; one row by 4096 x 8192 (34 MB): 9 us.
-template <typename T, HcclAmdScaleType kScale, int kCF, int kWaves, int kAhead>
+template <typename T, HcclAmdScaleType kScale, int kRF, int kCF, int kWaves, int kAhead>
 __global__ void __launch_bounds__(64 * kWaves) FewRowsKernel(ProductArgs a)
 {
     constexpr bool kPowers = kScale == HCCL_AMD_SCALE_E8M0;
     typedef typename BlockScale<kScale>::Stored Stored;
-    __shared__ Float4 part[kWaves][kCF][64];
+    __shared__ Float4 part[kWaves][kRF * kCF][64];
     const int unit = int(blockIdx.x) / a.colTiles, col0 = int(blockIdx.x) % a.colTiles * 16 * kCF;
-    const Unit u = FindUnit(a.offsets, a.groups, a.numRows, unit, 16);
+    const Unit u = FindUnit(a.offsets, a.groups, a.numRows, unit, 16 * kRF);
     if (u.group < 0) {
         return;
     }
@@ -112,47 +112,65 @@ __global__ void __launch_bounds__(64 * kWaves) FewRowsKernel(ProductArgs a)
         return;
     }
     const int lane = int(threadIdx.x) % 64, wave = __builtin_amdgcn_readfirstlane(int(threadIdx.x) / 64), l16 = lane % 16, piece = lane / 16 * 16;
-    const int64_t row = min(u.first + l16, u.last - 1);
-    const uint8_t *rows = a.rows + row * a.rowPitch + piece;
-    const Stored *rowScales = static_cast<const Stored *>(a.rowScales) + row * a.rowScalePitch;
+    const uint8_t *rows[kRF], *cols[kCF];
+    const Stored *rowScales[kRF];
+    Float4 sum[kRF][kCF];
+#pragma unroll
+    for (int r = 0; r < kRF; r++) {
+        const int64_t row = min(u.first + r * 16 + l16, u.last - 1);
+        rows[r] = a.rows + row * a.rowPitch + piece;
+        rowScales[r] = static_cast<const Stored *>(a.rowScales) + row * a.rowScalePitch;
+    }
     // (a workgroup's columns lie within one block of 128 of the weights' scales)
     const Stored *colScales = static_cast<const Stored *>(a.colScales) + (int64_t(expert) * ((a.numCols + 127) / 128) + col0 / 128) * a.blocks;
-    const uint8_t *cols[kCF];
-    Float4 sum[kCF];
 #pragma unroll
     for (int f = 0; f < kCF; f++) {
         const int col = min(col0 + f * 16 + l16, a.numCols - 1);
         cols[f] = a.cols + (int64_t(expert) * a.numCols + col) * a.colPitch + piece;
-        sum[f] = Zero4();
+#pragma unroll
+        for (int r = 0; r < kRF; r++) {
+            sum[r][f] = Zero4();
+        }
     }
     for (int b0 = wave; b0 < a.blocks; b0 += kWaves * kAhead) {
-        Int8 x[kAhead], w[kAhead][kCF];
-        Stored rs[kAhead], cs[kAhead];
+        Int8 x[kAhead][kRF], w[kAhead][kCF];
+        Stored rs[kAhead][kRF], cs[kAhead];
 #pragma unroll
         for (int j = 0; j < kAhead; j++) {
             const int b = min(b0 + j * kWaves, a.blocks - 1);       // (past the end the last one again, not used)
-            x[j] = LoadLane(rows + int64_t(b) * 128);
 #pragma unroll
             for (int f = 0; f < kCF; f++) {
                 w[j][f] = LoadLane(cols[f] + int64_t(b) * 128);
             }
-            rs[j] = rowScales[b];
+#pragma unroll
+            for (int r = 0; r < kRF; r++) {
+                x[j][r] = LoadLane(rows[r] + int64_t(b) * 128);
+                rs[j][r] = rowScales[r][b];
+            }
             cs[j] = colScales[b];
         }
 #pragma unroll
         for (int j = 0; j < kAhead; j++) {
             if (b0 + j * kWaves < a.blocks) {
-                const Wide32 wide = Widen(x[j], Inside(rs[j]));
+                Wide32 wide[kRF];
+#pragma unroll
+                for (int r = 0; r < kRF; r++) {
+                    wide[r] = Widen(x[j][r], Inside(rs[j][r]));
+                }
 #pragma unroll
                 for (int f = 0; f < kCF; f++) {
-                    if constexpr (kPowers) {
-                        sum[f] = MfmaWide(Widen(w[j][f], Inside(cs[j])), wide, sum[f]);
-                    } else {
-                        const Float4 p = MfmaWide(Widen(w[j][f], 1.0f), wide, Zero4());
-                        const float s = rs[j] * cs[j];
+                    const Wide32 wideCol = Widen(w[j][f], Inside(cs[j]));
 #pragma unroll
-                        for (int i = 0; i < 4; i++) {
-                            sum[f][i] = __builtin_fmaf(p[i], s, sum[f][i]);
+                    for (int r = 0; r < kRF; r++) {
+                        if constexpr (kPowers) {
+                            sum[r][f] = MfmaWide(wideCol, wide[r], sum[r][f]);
+                        } else {
+                            const Float4 p = MfmaWide(wideCol, wide[r], Zero4());
+                            const float s = rs[j][r] * cs[j];
+#pragma unroll
+                            for (int i = 0; i < 4; i++) {
+                                sum[r][f][i] = __builtin_fmaf(p[i], s, sum[r][f][i]);
+                            }
                         }
                     }
                 }
@@ -160,26 +178,29 @@ __global__ void __launch_bounds__(64 * kWaves) FewRowsKernel(ProductArgs a)
         }
     }
 #pragma unroll
-    for (int f = 0; f < kCF; f++) {
-        part[wave][f][lane] = sum[f];
-    }
-    __syncthreads();
-    if (wave >= kCF) {
-        return;
-    }
-    // a wave adds up the 16 columns of its number
-    Float4 total = part[0][wave][lane];
+    for (int r = 0; r < kRF; r++) {
 #pragma unroll
-    for (int w = 1; w < kWaves; w++) {
-        const Float4 other = part[w][wave][lane];
-#pragma unroll
-        for (int i = 0; i < 4; i++) {
-            total[i] += other[i];
+        for (int f = 0; f < kCF; f++) {
+            part[wave][r * kCF + f][lane] = sum[r][f];
         }
     }
-    if (u.first + l16 < u.last) {
-        const float v[4] = {total[0], total[1], total[2], total[3]};
-        StoreFour(static_cast<T *>(a.out) + int64_t(u.first + l16) * a.outPitch, v, col0 + wave * 16 + lane / 16 * 4, a.numCols);
+    __syncthreads();
+    // the waves take the 16 x 16 parts in turn
+    for (int at = wave; at < kRF * kCF; at += kWaves) {
+        Float4 total = part[0][at][lane];
+#pragma unroll
+        for (int w = 1; w < kWaves; w++) {
+            const Float4 other = part[w][at][lane];
+#pragma unroll
+            for (int i = 0; i < 4; i++) {
+                total[i] += other[i];
+            }
+        }
+        const int row = u.first + at / kCF * 16 + l16;
+        if (row < u.last) {
+            const float v[4] = {total[0], total[1], total[2], total[3]};
+            StoreFour(static_cast<T *>(a.out) + int64_t(row) * a.outPitch, v, col0 + at % kCF * 16 + lane / 16 * 4, a.numCols);
+        }
     }
 }
 
@@ -715,17 +736,19 @@ HcclResult HcclAmdBlockMatmul(const void *a, uint64_t aStride, const void *aScal
     p.wideOut = WideOut(yType, n, y, p.outPitch);
     // Which kernel, 64 groups by 4096 x 2048 and one by 4096 x 8192, 32-bit scales: few rows against tiles of 128 takes 13 us against 16
     // (8 rows, 64 groups), 90 against 100 (256 rows), 108 against 103 (512 rows); 9 against 45 (1 row, one group), 44 against 49 (128 rows), 85
-    // against 49 (256 rows).  16 columns to a workgroup instead of 64: 9 against 21 (1 row), 13 against 24 (16 rows), 40 against 25 (64 rows).
+    // against 49 (256 rows).  16 columns to a workgroup instead of 64: 9 against 21 (1 row), 13 against 24 (16 rows), 40 against 25 (64 rows).  32 rows
+    // instead of 16: 18 against 21 (32 rows, 16 columns), 31 against 24 (64 rows, 64 columns), 32 against 43 (128 rows).
     // Units there can be: every group that has rows ends with a shorter one.
     const auto unitsOf = [&](uint64_t per) { return offsets == nullptr ? (rows + per - 1) / per : rows / per + (rows < groups ? rows : groups); };
-    const uint64_t few64 = unitsOf(16) * ((n + 63) / 64);
-    const bool few = rows <= 4 * uint64_t(groups) || few64 <= 640, narrow = few64 < 192;
+    const uint64_t few64 = unitsOf(16) * ((n + 63) / 64), hit = rows < groups ? rows : groups;
+    const bool few = rows <= 4 * uint64_t(groups) || few64 <= 640, several = rows > 16 * hit;
+    const bool narrow = few64 < (several ? 256 : 192), twice = several && (narrow ? few64 >= 128 : few64 > 512);
     // sums of 16-bit results over more than two blocks: the 8-bit instruction's error is behind their own rounding
     const bool fast = yType != HCCL_DATA_TYPE_FP32 && k > 256;
     // half of the groups' last units are counted: the others' rows fill up one that is counted already
     const auto tilesOf = [&](uint64_t per) { return ((rows + per - 1) / per + (rows < groups ? rows : groups) / 2) * ((n + per - 1) / per); };
     const bool large = !few && fast && LargeTiles(tilesOf(256), tilesOf(128));
-    const uint64_t tileRows = few ? 16 : large ? 256 : 128, tileCols = few ? (narrow ? 16 : 64) : large ? 256 : 128;
+    const uint64_t tileRows = few ? (twice ? 32 : 16) : large ? 256 : 128, tileCols = few ? (narrow ? 16 : 64) : large ? 256 : 128;
     p.colTiles = int((n + tileCols - 1) / tileCols);
     const uint64_t units = unitsOf(tileRows);
     EXPERTS_CHK(units * uint64_t(p.colTiles) <= kMostTiles);
@@ -737,7 +760,8 @@ HcclResult HcclAmdBlockMatmul(const void *a, uint64_t aStride, const void *aScal
             hipLaunchKernelGGL(kernel, dim3(uint32_t(units * uint64_t(p.colTiles))), dim3(threads), 0, static_cast<hipStream_t>(stream), p);
         };
         if (few) {
-            narrow ? go(FewRowsKernel<T, kScale, 1, 8, 4>, 512) : go(FewRowsKernel<T, kScale, 4, 4, 2>, 256);
+            narrow ? (twice ? go(FewRowsKernel<T, kScale, 2, 1, 8, 4>, 512) : go(FewRowsKernel<T, kScale, 1, 1, 8, 4>, 512))
+                   : (twice ? go(FewRowsKernel<T, kScale, 2, 4, 4, 2>, 256) : go(FewRowsKernel<T, kScale, 1, 4, 4, 2>, 256));
             return;
         }
         if constexpr (sizeof(T) == 2) {

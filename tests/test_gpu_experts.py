@@ -463,7 +463,7 @@ def rows_ok(v):
 @pytest.mark.parametrize("kind", ["fp32", "e8m0"])
 @pytest.mark.parametrize("rows,groups,experts,n,k", [
     (1, 1, 1, 1, 1), (1, 1, 1, 64, 128), (7, 1, 1, 65, 200), (16, 1, 1, 128, 384), (17, 3, 3, 100, 129), (8, 64, 64, 96, 256), (40, 200, 200, 33, 64),
-    (64, 2, 2, 256, 1000), (130, 5, 5, 130, 640), (300, 1, 1, 300, 512), (513, 4, 4, 257, 300), (1000, 9, 9, 520, 1100)])
+    (64, 2, 2, 256, 1000), (130, 5, 5, 130, 640), (300, 1, 1, 300, 512), (33, 1, 1, 4000, 257), (130, 1, 1, 4100, 384), (70, 2, 2, 3900, 130), (513, 4, 4, 257, 300), (1000, 9, 9, 520, 1100)])
 def test_matmul(stream, kind, rows, groups, experts, n, k):
     rng = np.random.default_rng(rows + n + k)
     for dtype in ("bf16", "fp16", "fp32"):
