@@ -204,12 +204,13 @@ __global__ void __launch_bounds__(64 * kWaves) FewRowsKernel(ProductArgs a)
     }
 }
 
-// f(first block, number of blocks) for every group of the expert, ascending; blocks count over all groups.  Called by whole waves.
+// f(first block, number of blocks, one at least) for every group of the expert that has rows, ascending; blocks count over all
+// groups.  Called by whole waves.
 template <typename F>
 __device__ __forceinline__ void ForGroupsOf(const ProductArgs &a, int expert, F f)
 {
     if (a.offsets == nullptr) {
-        if ((a.expertOfGroup == nullptr ? 0 : a.expertOfGroup[0]) == expert) {
+        if (a.groupedRows > 0 && (a.expertOfGroup == nullptr ? 0 : a.expertOfGroup[0]) == expert) {
             f(0, (a.groupedRows + 127) / 128);
         }
         return;

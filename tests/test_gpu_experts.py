@@ -560,6 +560,24 @@ def test_grad_weight(stream, kind, rows, groups, experts, n, k, dtype):
     assert close(more.numpy().reshape(want.shape), want + f, room + U * (np.abs(f) + np.abs(want)), t)
 
 
+@pytest.mark.parametrize("kind", ["fp32", "e8m0"])
+@pytest.mark.parametrize("dtype", ["fp32", "bf16"])
+@pytest.mark.parametrize("groups", [0, 3])
+def test_grad_weight_without_rows(stream, kind, dtype, groups):
+    """No row at all, the operands absent: zeros, or with accumulate what was there.  groups 0: no offsets, one group of all rows."""
+    print("grad weight without rows", kind, dtype, groups, flush=True)
+    experts, n, k, t = max(1, groups), 130, 200, TYPE[dtype]
+    first = torch.randn(experts * n, k, device="cuda").to(t)
+    dw, more = Out(experts * n, k, t), Out(experts * n, k, t).fill(first)
+    off = torch.zeros(groups + 1, dtype=torch.int32, device="cuda")
+    ready()
+    for out, add in ((dw, False), (more, True)):
+        H.block_matmul_grad_weight(None, None, None, None, H.block_columns(0, experts), 0, n, k, KIND[kind], experts, off.data_ptr() if groups else None,
+                                   experts, out.ptr, dt(t), stream.cuda_stream, accumulate=add)
+    done(stream)
+    assert not dw.get().any() and torch.equal(more.get(), first)
+
+
 def test_products_in_a_graph(stream):
     """Captured calls, replayed with the program's own work between: every replay is the eager result."""
     torch.manual_seed(4)
