@@ -47,12 +47,16 @@ inline bool Aligned(const void *p, uint64_t to) { return reinterpret_cast<uintpt
 inline bool AlignedTo(HcclDataType t, const void *p) { return Aligned(p, SizeOf(t)); }
 inline bool ScaleAligned(HcclAmdScaleType s, const void *p) { return s != HCCL_AMD_SCALE_FP32 || Aligned(p, 4); }
 
-inline HcclResult Launched(const char *fn)
+// The launch's own answer decides: the thread's last error may be of another call, which its caller has dealt with or has yet to see.
+template <typename... P>
+HcclResult Launch(const char *fn, void (*kernel)(P...), uint32_t blocks, int threads, size_t lds, hipStream_t stream, P... args)
 {
-    const hipError_t e = hipGetLastError();
+    void *argv[] = {&args...};
+    const hipError_t e = hipLaunchKernel(reinterpret_cast<const void *>(kernel), dim3(blocks), dim3(uint32_t(threads)), argv, lds, stream);
     if (e == hipSuccess) {
         return HCCL_SUCCESS;
     }
+    (void)hipGetLastError();   // reported here, not once more by whoever asks next
     HCCL_LOG_ERROR("%s: %s", fn, hipGetErrorString(e));
     return HCCL_E_RUNTIME;
 }

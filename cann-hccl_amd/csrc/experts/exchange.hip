@@ -223,17 +223,15 @@ __global__ void __launch_bounds__(kThreads) CombineGradKernel(CombineArgs a)
 }
 
 template <typename F>
-void ByType(HcclDataType type, F f)
+HcclResult ByType(HcclDataType type, F f)
 {
     switch (type) {
         case HCCL_DATA_TYPE_FP32:
-            f(float{});
-            break;
+            return f(float{});
         case HCCL_DATA_TYPE_FP16:
-            f(_Float16{});
-            break;
+            return f(_Float16{});
         default:
-            f(__bf16{});
+            return f(__bf16{});
     }
 }
 
@@ -291,12 +289,10 @@ HcclResult HcclAmdExpertPack(const void *x, HcclDataType type, uint64_t tokens, 
         a.pieces = int((width + kPiece - 1) / kPiece);
         a.waves = int64_t(tokens) * a.pieces;
         const bool wide = Wide(type, width, x, a.xStride) && Wide(type, width, out, a.outStride);
-        ByType(type, [&](auto of) {
+        return ByType(type, [&](auto of) {
             typedef decltype(of) T;
-            const auto go = [&](auto kernel) { hipLaunchKernelGGL(kernel, dim3(BlocksOf(a.waves)), dim3(kThreads), 0, on, a); };
-            wide ? go(CopyKernel<T, true>) : go(CopyKernel<T, false>);
+            return Launch("HcclAmdExpertPack", wide ? CopyKernel<T, true> : CopyKernel<T, false>, BlocksOf(a.waves), kThreads, 0, on, a);
         });
-        return Launched("HcclAmdExpertPack");
     }
     EXPERTS_CHK_PTR(scales);
     EXPERTS_CHK(ScaleAligned(scaleType, scales));
@@ -308,16 +304,14 @@ HcclResult HcclAmdExpertPack(const void *x, HcclDataType type, uint64_t tokens, 
     a.pieces = (a.padded + kPiece - 1) / kPiece;
     a.waves = int64_t(tokens) * a.pieces;
     const bool wide = Wide(type, width, x, a.xStride);
-    ByType(type, [&](auto of) {
+    return ByType(type, [&](auto of) {
         typedef decltype(of) T;
-        const auto go = [&](auto kernel) { hipLaunchKernelGGL(kernel, dim3(BlocksOf(a.waves)), dim3(kThreads), 0, on, a); };
+        const auto go = [&](auto kernel) { return Launch("HcclAmdExpertPack", kernel, BlocksOf(a.waves), kThreads, 0, on, a); };
         if (scaleType == HCCL_AMD_SCALE_FP32) {
-            wide ? go(QuantKernel<T, HCCL_AMD_SCALE_FP32, true>) : go(QuantKernel<T, HCCL_AMD_SCALE_FP32, false>);
-        } else {
-            wide ? go(QuantKernel<T, HCCL_AMD_SCALE_E8M0, true>) : go(QuantKernel<T, HCCL_AMD_SCALE_E8M0, false>);
+            return wide ? go(QuantKernel<T, HCCL_AMD_SCALE_FP32, true>) : go(QuantKernel<T, HCCL_AMD_SCALE_FP32, false>);
         }
+        return wide ? go(QuantKernel<T, HCCL_AMD_SCALE_E8M0, true>) : go(QuantKernel<T, HCCL_AMD_SCALE_E8M0, false>);
     });
-    return Launched("HcclAmdExpertPack");
 }
 
 HcclResult HcclAmdExpertCombine(const void *x, HcclDataType type, uint64_t rows, uint64_t width, uint64_t xStride, uint64_t tokens,
@@ -353,12 +347,10 @@ HcclResult HcclAmdExpertCombine(const void *x, HcclDataType type, uint64_t rows,
     a.waves = int64_t(tokens) * a.pieces;
     const bool wide = Wide(type, width, x, a.xStride) && Wide(type, width, y, a.yStride);
     const hipStream_t on = static_cast<hipStream_t>(stream);
-    ByType(type, [&](auto of) {
+    return ByType(type, [&](auto of) {
         typedef decltype(of) T;
-        const auto go = [&](auto kernel) { hipLaunchKernelGGL(kernel, dim3(BlocksOf(a.waves)), dim3(kThreads), 0, on, a); };
-        wide ? go(CombineKernel<T, true>) : go(CombineKernel<T, false>);
+        return Launch("HcclAmdExpertCombine", wide ? CombineKernel<T, true> : CombineKernel<T, false>, BlocksOf(a.waves), kThreads, 0, on, a);
     });
-    return Launched("HcclAmdExpertCombine");
 }
 
 HcclResult HcclAmdExpertCombineGrad(const void *yGrad, uint64_t yGradStride, const void *x, HcclDataType type, uint64_t rows,
@@ -400,18 +392,17 @@ HcclResult HcclAmdExpertCombineGrad(const void *yGrad, uint64_t yGradStride, con
     a.topK = int(topK);
     const bool wide = Wide(type, width, x, a.xStride) && Wide(type, width, yGrad, a.yStride) && Wide(type, width, xGrad, a.xGradStride);
     const hipStream_t on = static_cast<hipStream_t>(stream);
-    ByType(type, [&](auto of) {
+    return ByType(type, [&](auto of) {
         typedef decltype(of) T;
-        const auto go = [&](auto kernel) { hipLaunchKernelGGL(kernel, dim3(BlocksOf(int64_t(tokens) * kWaves)), dim3(kThreads), 0, on, a); };
+        const auto go = [&](auto kernel) { return Launch("HcclAmdExpertCombineGrad", kernel, BlocksOf(int64_t(tokens) * kWaves), kThreads, 0, on, a); };
         if (topK <= 2) {
-            wide ? go(CombineGradKernel<T, 2, true>) : go(CombineGradKernel<T, 2, false>);
-        } else if (topK <= 8) {
-            wide ? go(CombineGradKernel<T, 8, true>) : go(CombineGradKernel<T, 8, false>);
-        } else {
-            wide ? go(CombineGradKernel<T, 16, true>) : go(CombineGradKernel<T, 16, false>);
+            return wide ? go(CombineGradKernel<T, 2, true>) : go(CombineGradKernel<T, 2, false>);
         }
+        if (topK <= 8) {
+            return wide ? go(CombineGradKernel<T, 8, true>) : go(CombineGradKernel<T, 8, false>);
+        }
+        return wide ? go(CombineGradKernel<T, 16, true>) : go(CombineGradKernel<T, 16, false>);
     });
-    return Launched("HcclAmdExpertCombineGrad");
 }
 
 }  // extern "C"

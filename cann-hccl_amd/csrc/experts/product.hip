@@ -648,21 +648,19 @@ __global__ void __launch_bounds__(64 * kWR * kWC, 2) TileKernel(ProductArgs a)
 
 // f(type, scale type) as constants
 template <typename F>
-void Choose(HcclDataType type, HcclAmdScaleType scaleType, F f)
+HcclResult Choose(HcclDataType type, HcclAmdScaleType scaleType, F f)
 {
     const auto byScale = [&](auto of) {
-        scaleType == HCCL_AMD_SCALE_FP32 ? f(of, std::integral_constant<HcclAmdScaleType, HCCL_AMD_SCALE_FP32>{})
-                                         : f(of, std::integral_constant<HcclAmdScaleType, HCCL_AMD_SCALE_E8M0>{});
+        return scaleType == HCCL_AMD_SCALE_FP32 ? f(of, std::integral_constant<HcclAmdScaleType, HCCL_AMD_SCALE_FP32>{})
+                                                : f(of, std::integral_constant<HcclAmdScaleType, HCCL_AMD_SCALE_E8M0>{});
     };
     switch (type) {
         case HCCL_DATA_TYPE_FP32:
-            byScale(float{});
-            break;
+            return byScale(float{});
         case HCCL_DATA_TYPE_FP16:
-            byScale(_Float16{});
-            break;
+            return byScale(_Float16{});
         default:
-            byScale(__bf16{});
+            return byScale(__bf16{});
     }
 }
 
@@ -754,30 +752,26 @@ HcclResult HcclAmdBlockMatmul(const void *a, uint64_t aStride, const void *aScal
     const uint64_t units = unitsOf(tileRows);
     EXPERTS_CHK(units * uint64_t(p.colTiles) <= kMostTiles);
     EXPERTS_CHK(p.rowPitch < kMostPitch && p.colPitch < kMostPitch);
-    Choose(yType, scaleType, [&](auto of, auto scale) {
+    return Choose(yType, scaleType, [&](auto of, auto scale) {
         typedef decltype(of) T;
         constexpr HcclAmdScaleType kScale = decltype(scale)::value;
         const auto go = [&](auto kernel, int threads) {
-            hipLaunchKernelGGL(kernel, dim3(uint32_t(units * uint64_t(p.colTiles))), dim3(threads), 0, static_cast<hipStream_t>(stream), p);
+            return Launch("HcclAmdBlockMatmul", kernel, uint32_t(units * uint64_t(p.colTiles)), threads, 0, static_cast<hipStream_t>(stream), p);
         };
         if (few) {
-            narrow ? (twice ? go(FewRowsKernel<T, kScale, 2, 1, 8, 4>, 512) : go(FewRowsKernel<T, kScale, 1, 1, 8, 4>, 512))
-                   : (twice ? go(FewRowsKernel<T, kScale, 2, 4, 4, 2>, 256) : go(FewRowsKernel<T, kScale, 1, 4, 4, 2>, 256));
-            return;
+            return narrow ? (twice ? go(FewRowsKernel<T, kScale, 2, 1, 8, 4>, 512) : go(FewRowsKernel<T, kScale, 1, 1, 8, 4>, 512))
+                          : (twice ? go(FewRowsKernel<T, kScale, 2, 4, 4, 2>, 256) : go(FewRowsKernel<T, kScale, 1, 4, 4, 2>, 256));
         }
         if constexpr (sizeof(T) == 2) {
             if (large) {
-                go(TileKernel<T, kScale, false, false, 8, 4, 2, 4>, 512);
-                return;
+                return go(TileKernel<T, kScale, false, false, 8, 4, 2, 4>, 512);
             }
             if (fast) {
-                go(TileKernel<T, kScale, false, false, 4, 4, 2, 2>, 256);
-                return;
+                return go(TileKernel<T, kScale, false, false, 4, 4, 2, 2>, 256);
             }
         }
-        go(TileKernel<T, kScale, true, false, 4, 4, 2, 2>, 256);
+        return go(TileKernel<T, kScale, true, false, 4, 4, 2, 2>, 256);
     });
-    return Launched("HcclAmdBlockMatmul");
 }
 
 HcclResult HcclAmdBlockMatmulGradWeight(const void *yGradT, const void *yGradScales, const void *xT, const void *xScales,
@@ -824,11 +818,10 @@ HcclResult HcclAmdBlockMatmulGradWeight(const void *yGradT, const void *yGradSca
     p.colTiles = int((k + 127) / 128);
     const uint64_t tiles = ((n + 127) / 128 * uint64_t(p.colTiles) + 7) / 8 * 8 * experts;
     EXPERTS_CHK(tiles <= kMostTiles);
-    Choose(gradType, scaleType, [&](auto of, auto scale) {
-        hipLaunchKernelGGL((TileKernel<decltype(of), decltype(scale)::value, true, true, 4, 4, 2, 2>), dim3(uint32_t(tiles)), dim3(256), 0,
+    return Choose(gradType, scaleType, [&](auto of, auto scale) {
+        return Launch("HcclAmdBlockMatmulGradWeight", TileKernel<decltype(of), decltype(scale)::value, true, true, 4, 4, 2, 2>, uint32_t(tiles), 256, 0,
             static_cast<hipStream_t>(stream), p);
     });
-    return Launched("HcclAmdBlockMatmulGradWeight");
 }
 
 }  // extern "C"

@@ -175,24 +175,22 @@ __global__ void __launch_bounds__(kThreads) WeightsKernel(TileArgs a)
 
 // f(type, scale type, whether 16 bytes can be loaded at once), as constants
 template <typename F>
-void Choose(HcclDataType type, HcclAmdScaleType scaleType, bool wide, F f)
+HcclResult Choose(HcclDataType type, HcclAmdScaleType scaleType, bool wide, F f)
 {
     const auto byWide = [&](auto of, auto scale) {
-        wide ? f(of, scale, std::true_type{}) : f(of, scale, std::false_type{});
+        return wide ? f(of, scale, std::true_type{}) : f(of, scale, std::false_type{});
     };
     const auto byScale = [&](auto of) {
-        scaleType == HCCL_AMD_SCALE_FP32 ? byWide(of, std::integral_constant<HcclAmdScaleType, HCCL_AMD_SCALE_FP32>{})
-                                         : byWide(of, std::integral_constant<HcclAmdScaleType, HCCL_AMD_SCALE_E8M0>{});
+        return scaleType == HCCL_AMD_SCALE_FP32 ? byWide(of, std::integral_constant<HcclAmdScaleType, HCCL_AMD_SCALE_FP32>{})
+                                                : byWide(of, std::integral_constant<HcclAmdScaleType, HCCL_AMD_SCALE_E8M0>{});
     };
     switch (type) {
         case HCCL_DATA_TYPE_FP32:
-            byScale(float{});
-            break;
+            return byScale(float{});
         case HCCL_DATA_TYPE_FP16:
-            byScale(_Float16{});
-            break;
+            return byScale(_Float16{});
         default:
-            byScale(__bf16{});
+            return byScale(__bf16{});
     }
 }
 
@@ -235,11 +233,10 @@ HcclResult HcclAmdBlockQuantWeights(const void *w, HcclDataType type, uint32_t e
     a.rows = int(n);
     a.width = int(k);
     const bool wide = k % 8 == 0 && Aligned(w, 16) && uint64_t(a.stride) * SizeOf(type) % 16 == 0;
-    Choose(type, scaleType, wide, [&](auto of, auto scale, auto is) {
-        hipLaunchKernelGGL((WeightsKernel<decltype(of), decltype(scale)::value, decltype(is)::value>),
-            dim3(uint32_t(Blocks(n) * Blocks(k) * experts)), dim3(kThreads), 0, static_cast<hipStream_t>(stream), a);
+    return Choose(type, scaleType, wide, [&](auto of, auto scale, auto is) {
+        return Launch("HcclAmdBlockQuantWeights", WeightsKernel<decltype(of), decltype(scale)::value, decltype(is)::value>,
+            uint32_t(Blocks(n) * Blocks(k) * experts), kThreads, 0, static_cast<hipStream_t>(stream), a);
     });
-    return Launched("HcclAmdBlockQuantWeights");
 }
 
 HcclResult HcclAmdBlockQuantColumns(const void *x, HcclDataType type, uint64_t rows, uint64_t width, uint64_t xStride,
@@ -273,11 +270,10 @@ HcclResult HcclAmdBlockQuantColumns(const void *x, HcclDataType type, uint64_t r
     a.width = int(width);
     a.groups = int(groups);
     const bool wide = width % 8 == 0 && Aligned(x, 16) && uint64_t(a.stride) * SizeOf(type) % 16 == 0;
-    Choose(type, scaleType, wide, [&](auto of, auto scale, auto is) {
-        hipLaunchKernelGGL((ColumnsKernel<decltype(of), decltype(scale)::value, decltype(is)::value>),
-            dim3(uint32_t(Blocks(width) * units)), dim3(kThreads), 0, static_cast<hipStream_t>(stream), a);
+    return Choose(type, scaleType, wide, [&](auto of, auto scale, auto is) {
+        return Launch("HcclAmdBlockQuantColumns", ColumnsKernel<decltype(of), decltype(scale)::value, decltype(is)::value>,
+            uint32_t(Blocks(width) * units), kThreads, 0, static_cast<hipStream_t>(stream), a);
     });
-    return Launched("HcclAmdBlockQuantColumns");
 }
 
 }  // extern "C"

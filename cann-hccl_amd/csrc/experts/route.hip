@@ -788,50 +788,50 @@ int BlocksOf(uint64_t tokens, int tile)
 }
 
 template <typename T, int K, int kLanes, int kChunks>
-void LaunchRoute(const RouteArgs &a, bool wide, hipStream_t stream)
+HcclResult LaunchRoute(const RouteArgs &a, bool wide, hipStream_t stream)
 {
     const size_t lds = 4 * ((3 + kThreads / 64) * size_t(a.experts) + 2 * (kThreads / 64) + 1);
-    const auto go = [&](auto kernel) { hipLaunchKernelGGL(kernel, dim3(a.blocks), dim3(kThreads), lds, stream, a); };
-    wide && a.experts == 8 * kLanes * kChunks && a.tokens > 0 ? go(RouteKernel<T, K, kLanes, kChunks, kExactly>)
-    : wide                                                    ? go(RouteKernel<T, K, kLanes, kChunks, kAligned>)
-                                                              : go(RouteKernel<T, K, kLanes, kChunks, kAnyhow>);
+    const auto go = [&](auto kernel) { return Launch("HcclAmdExpertRoute", kernel, uint32_t(a.blocks), kThreads, lds, stream, a); };
+    return wide && a.experts == 8 * kLanes * kChunks && a.tokens > 0 ? go(RouteKernel<T, K, kLanes, kChunks, kExactly>)
+           : wide                                                    ? go(RouteKernel<T, K, kLanes, kChunks, kAligned>)
+                                                                     : go(RouteKernel<T, K, kLanes, kChunks, kAnyhow>);
 }
 
 template <typename T, int K>
-void LaunchRouteShape(const RouteArgs &a, int tile, bool wide, hipStream_t stream)
+HcclResult LaunchRouteShape(const RouteArgs &a, int tile, bool wide, hipStream_t stream)
 {
     if (tile == 64) {
-        a.experts <= 64 ? LaunchRoute<T, K, 4, 2>(a, wide, stream) : LaunchRoute<T, K, 4, 8>(a, wide, stream);
-    } else {
-        a.experts <= 256 ? LaunchRoute<T, K, 16, 2>(a, wide, stream) : LaunchRoute<T, K, 16, 8>(a, wide, stream);
+        return a.experts <= 64 ? LaunchRoute<T, K, 4, 2>(a, wide, stream) : LaunchRoute<T, K, 4, 8>(a, wide, stream);
     }
+    return a.experts <= 256 ? LaunchRoute<T, K, 16, 2>(a, wide, stream) : LaunchRoute<T, K, 16, 8>(a, wide, stream);
 }
 
 template <typename T>
-void LaunchRouteType(const RouteArgs &a, int tile, bool wide, hipStream_t stream)
+HcclResult LaunchRouteType(const RouteArgs &a, int tile, bool wide, hipStream_t stream)
 {
-    a.topK <= 2   ? LaunchRouteShape<T, 2>(a, tile, wide, stream)
-    : a.topK <= 4 ? LaunchRouteShape<T, 4>(a, tile, wide, stream)
-    : a.topK <= 8 ? LaunchRouteShape<T, 8>(a, tile, wide, stream)
-                  : LaunchRouteShape<T, 16>(a, tile, wide, stream);
+    return a.topK <= 2   ? LaunchRouteShape<T, 2>(a, tile, wide, stream)
+           : a.topK <= 4 ? LaunchRouteShape<T, 4>(a, tile, wide, stream)
+           : a.topK <= 8 ? LaunchRouteShape<T, 8>(a, tile, wide, stream)
+                         : LaunchRouteShape<T, 16>(a, tile, wide, stream);
 }
 
 template <typename T, int kHow>
-void LaunchRouteGrad(const RouteGradArgs &a, hipStream_t stream)
+HcclResult LaunchRouteGrad(const RouteGradArgs &a, hipStream_t stream)
 {
     const auto go = [&](auto kernel, int lanes) {
         const int64_t blocks = (int64_t(a.tokens) * lanes + kThreads - 1) / kThreads;
-        hipLaunchKernelGGL(kernel, dim3(uint32_t(blocks < 1024 ? blocks : 1024)), dim3(kThreads), 0, stream, a);
+        return Launch("HcclAmdExpertRouteGrad", kernel, uint32_t(blocks < 1024 ? blocks : 1024), kThreads, 0, stream, a);
     };
     if (a.experts <= 64) {
-        go(RouteGradKernel<T, 16, 4, kHow>, 16);
-    } else if (a.experts <= 128) {
-        go(RouteGradKernel<T, 16, 8, kHow>, 16);
-    } else if (a.experts <= 256) {
-        go(RouteGradKernel<T, 16, 16, kHow>, 16);
-    } else {
-        go(RouteGradKernel<T, 64, 16, kHow>, 64);
+        return go(RouteGradKernel<T, 16, 4, kHow>, 16);
     }
+    if (a.experts <= 128) {
+        return go(RouteGradKernel<T, 16, 8, kHow>, 16);
+    }
+    if (a.experts <= 256) {
+        return go(RouteGradKernel<T, 16, 16, kHow>, 16);
+    }
+    return go(RouteGradKernel<T, 64, 16, kHow>, 64);
 }
 
 }  // namespace
@@ -903,10 +903,9 @@ HcclResult HcclAmdExpertRoute(const void *logits, HcclDataType logitType, uint64
     const hipStream_t on = static_cast<hipStream_t>(stream);
     a.sums = a.blockSums + int64_t(a.blocks) * a.experts;
     const bool wide = experts % 8 == 0 && Aligned(logits, 16) && uint64_t(a.stride) * SizeOf(logitType) % 16 == 0;
-    logitType == HCCL_DATA_TYPE_FP32   ? LaunchRouteType<float>(a, tile, wide, on)
-    : logitType == HCCL_DATA_TYPE_FP16 ? LaunchRouteType<_Float16>(a, tile, wide, on)
-                                       : LaunchRouteType<__bf16>(a, tile, wide, on);
-    HcclResult r = Launched("HcclAmdExpertRoute");
+    HcclResult r = logitType == HCCL_DATA_TYPE_FP32   ? LaunchRouteType<float>(a, tile, wide, on)
+                   : logitType == HCCL_DATA_TYPE_FP16 ? LaunchRouteType<_Float16>(a, tile, wide, on)
+                                                      : LaunchRouteType<__bf16>(a, tile, wide, on);
     if (r != HCCL_SUCCESS || a.blocks == 1) {
         return r;
     }
@@ -914,17 +913,13 @@ HcclResult HcclAmdExpertRoute(const void *logits, HcclDataType logitType, uint64
     // 256 experts 13 instead of 15; with more of them that reading takes as long as a launch of its own.
     const bool few = a.blocks <= 32;
     if (!few) {
-        hipLaunchKernelGGL(ScanKernel, dim3(experts / kScanCols + 1), dim3(kThreads), 0, on, a);
-        r = Launched("HcclAmdExpertRoute");
+        r = Launch("HcclAmdExpertRoute", ScanKernel, experts / kScanCols + 1, kThreads, 0, on, a);
         if (r != HCCL_SUCCESS) {
             return r;
         }
     }
-    const auto rows = [&](auto kernel) {
-        hipLaunchKernelGGL(kernel, dim3(a.blocks), dim3(kThreads), 4 * (3 * size_t(experts) + 1 + 2 * (kThreads / 64)), on, a, tile * a.tiles);
-    };
-    few ? rows(RowsKernel<true>) : rows(RowsKernel<false>);
-    return Launched("HcclAmdExpertRoute");
+    return Launch("HcclAmdExpertRoute", few ? RowsKernel<true> : RowsKernel<false>, uint32_t(a.blocks), kThreads,
+        4 * (3 * size_t(experts) + 1 + 2 * (kThreads / 64)), on, a, tile * a.tiles);
 }
 
 HcclResult HcclAmdExpertRouteGrad(const void *logits, HcclDataType logitType, uint64_t tokens, uint32_t experts, uint64_t logitStride,
@@ -968,10 +963,9 @@ HcclResult HcclAmdExpertRouteGrad(const void *logits, HcclDataType logitType, ui
     const bool exactly = wide && (experts == 64 || experts == 128 || experts == 256 || experts == 1024);
     const auto go = [&](auto of) {
         typedef decltype(of) T;
-        exactly ? LaunchRouteGrad<T, kExactly>(a, on) : wide ? LaunchRouteGrad<T, kAligned>(a, on) : LaunchRouteGrad<T, kAnyhow>(a, on);
+        return exactly ? LaunchRouteGrad<T, kExactly>(a, on) : wide ? LaunchRouteGrad<T, kAligned>(a, on) : LaunchRouteGrad<T, kAnyhow>(a, on);
     };
-    logitType == HCCL_DATA_TYPE_FP32 ? go(float{}) : logitType == HCCL_DATA_TYPE_FP16 ? go(_Float16{}) : go(__bf16{});
-    return Launched("HcclAmdExpertRouteGrad");
+    return logitType == HCCL_DATA_TYPE_FP32 ? go(float{}) : logitType == HCCL_DATA_TYPE_FP16 ? go(_Float16{}) : go(__bf16{});
 }
 
 }  // extern "C"

@@ -622,6 +622,60 @@ def test_products_in_a_graph(stream):
         assert torch.equal(got, out) and torch.equal(got_loss, loss) and bool(out.any())
 
 
+def test_an_error_of_another_hip_call_is_none_of_theirs(stream):
+    """A HIP call that failed before, on the host and without harm: every operator succeeds, does all of its work, and leaves that error to
+    whoever asks for it."""
+    torch.manual_seed(5)
+    T, E, k, W, N = 900, 16, 2, 256, 192                      # (a router's call of three launches)
+    x, logits, w = torch.randn(T, W, device="cuda").bfloat16(), torch.randn(T, E, device="cuda"), torch.randn(E, N, W, device="cuda").bfloat16()
+    need = H.expert_route_workspace(T, E)
+    columns = H.block_columns(T * k, E)
+    dw_in, dl_in = torch.randn(T, k, device="cuda"), torch.ones(1, device="cuda")
+    BF, F, K, P = H.HCCL_DATA_TYPE_BFP16, H.HCCL_DATA_TYPE_FP32, ref.FP32, lambda v: v.data_ptr()  # noqa: E731
+    u8, i32, f32, bf = torch.uint8, torch.int32, torch.float32, torch.bfloat16
+    shapes = {"expert": (T, k, i32), "weights": (T, k, f32), "row": (T, k, i32), "counts": (1, E + 1, i32), "offsets": (1, E + 1, i32), "loss": (1, 1, f32),
+              "d_logits": (T, E, f32), "q": (T * k, W, u8), "s": (T * k, 2, f32), "wq": (E * N, W, u8), "ws": (E * 2, 2, f32), "y": (T * k, N, bf),
+              "out": (T, N, bf), "dx": (T * k, N, bf), "dweights": (T, k, f32), "yt": (N, columns, u8), "yts": (columns // 128, N, f32), "xt": (N, columns, u8),
+              "xts": (columns // 128, N, f32), "grad": (E * N, N, f32)}
+
+    def run():
+        o = {n: torch.zeros(a, b, dtype=t, device="cuda") for n, (a, b, t) in shapes.items()}
+        work = torch.zeros(need, dtype=u8, device="cuda")
+        ready()
+        S = stream.cuda_stream
+        calls = (
+            lambda: H.expert_route(P(logits), F, T, E, k, P(o["expert"]), P(o["weights"]), P(o["row"]), P(o["counts"]), P(o["offsets"]), P(o["loss"]), P(work),
+                                   need, S),
+            lambda: H.expert_route_grad(P(logits), F, T, E, k, P(o["expert"]), P(o["counts"]), P(dw_in), P(dl_in), P(o["d_logits"]), S),
+            lambda: H.expert_pack(P(x), BF, T, W, k, P(o["row"]), P(o["q"]), T * k, S, scales=P(o["s"]), scale_type=K),
+            lambda: H.block_quant_weights(P(w), BF, E, N, W, K, P(o["wq"]), P(o["ws"]), None, None, S),
+            lambda: H.block_matmul(P(o["q"]), P(o["s"]), T * k, P(o["wq"]), P(o["ws"]), E, N, W, K, P(o["y"]), BF, S, groups=E, offsets=P(o["offsets"])),
+            lambda: H.expert_combine(P(o["y"]), BF, T * k, N, T, k, P(o["row"]), P(o["weights"]), P(o["out"]), S),
+            lambda: H.expert_combine_grad(P(o["out"]), P(o["y"]), BF, T * k, N, T, k, P(o["row"]), P(o["weights"]), P(o["dx"]), P(o["dweights"]), S),
+            lambda: H.block_quant_columns(P(o["dx"]), BF, T * k, N, E, P(o["offsets"]), K, P(o["yt"]), columns, P(o["yts"]), S),
+            lambda: H.block_quant_columns(P(o["y"]), BF, T * k, N, E, P(o["offsets"]), K, P(o["xt"]), columns, P(o["xts"]), S),
+            lambda: H.block_matmul_grad_weight(P(o["yt"]), P(o["yts"]), P(o["xt"]), P(o["xts"]), columns, T * k, N, N, K, E, P(o["offsets"]), E, P(o["grad"]), F, S))
+        return o, calls
+
+    hip = H.lib()                                             # (the runtime that the library has loaded)
+    want, calls = run()
+    for call in calls:
+        call()
+    done(stream)
+    got, calls = run()
+    for call in calls:
+        try:
+            failed = hip.hipSetDevice(9999)                   # no such device
+            assert failed != 0
+            call()
+            assert hip.hipPeekAtLastError() == failed
+        finally:
+            hip.hipGetLastError()
+    done(stream)
+    for name in shapes:
+        assert torch.equal(got[name].view(u8), want[name].view(u8)) and bool(want[name].any()), name
+
+
 # ---- addresses beyond 2^32 bytes ------------------------------------------------------------------------------------------------------
 
 def test_exchange_beyond_32_bits(stream):
