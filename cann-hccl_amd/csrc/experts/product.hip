@@ -2,10 +2,10 @@
 //
 //   y[r][c] = sum over blocks b of ra[r][b] * ca[c][b] * sum over the 128 values of b of rows[r][.] * cols[c][.]
 //
-// rows: a group's rows, or the output gradient's columns; cols: an expert's weights, or the columns of the experts' inputs.  The
-// matrix instruction takes 16 x 16 x 128: one block of 128 to an instruction.  Its first operand is `cols`, so that a lane
-// holds four neighbouring values of one row of the result.  Scales that are powers of two go into the instruction itself;
-// 32-bit ones multiply its result, which is then added in 32 bits.
+// rows: a group's rows, or the output gradient's columns; cols: an expert's weights, or the columns of the experts' inputs.  Both
+// are widened to 16 bits on their way from LDS into the matrix instruction, 16 x 16 x 32, four of which take a block of 128.  Its first
+// operand is `cols`, so that a lane holds four neighbouring values of one row of the result.  Scales that are powers of two go into the
+// widened values; 32-bit ones multiply a block's sum, which is then added in 32 bits.
 #include <type_traits>
 
 #include "common.h"
@@ -32,9 +32,11 @@ struct ProductArgs {
     bool wideOut;                           // results can be stored 16 bytes at once
 };
 
-// The 8-bit matrix instructions keep fewer than 32 bits inside: on blocks of normally distributed values their results are
-// 1.3e-5 off (2-norm), those of the 16-bit ones 1.5e-8.  8-bit values fit 16-bit ones exactly, and so does their product with a
-// power of two; converting costs an instruction per two values and halves the rate (2.2 for 4.4 PFLOP/s).
+// Why not the 8-bit matrix instructions, whose rate is twice as high (4.4 for 2.2 PFLOP/s): inside a block of 128 they drop what is small
+// next to the block's largest product.  Measured, off by (2-norm): normally distributed values 1.5e-5; values of one sign over the type's
+// whole range 7e-5, always downwards, and up to 2.2e-4 at one result; two large products that cancel, all other values around 2 instead
+// of 448: 0.15.  A sum in 32 bits is 3.5e-5 off there and 1e-8 to 1e-7 elsewhere; so are those of the 16-bit instruction: 8-bit values fit
+// 16-bit ones exactly, and so does their product with a power of two.  Widening costs an instruction per two values.
 typedef __bf16 Half8 __attribute__((ext_vector_type(8)));
 
 struct Wide32 {     // a lane's 32 values of a block
@@ -311,15 +313,15 @@ __device__ __forceinline__ uint32_t ScaleBits(uint8_t s) { return s; }
 // registers.  The 16-byte pieces of a row lie in LDS in an order that depends on the row (piece p of row r at p ^ (r / 2 % 8)), so that the
 // 16 rows a lane group reads are in different banks; since such a load fills LDS in lane order, it is the lanes' addresses
 // in memory that are swapped.  Scales pass through a register of one thread each.
-// 256 x 256 to a workgroup of eight waves needs 128 KiB of LDS and 128 sums to a lane, all there is; reading it takes 1536 cycles of LDS a step
-// and filling it 512, its products 2048 of the matrix unit, so that neither can wait long for the other.  Measured: 8192 x 4096 x 8192, scales
-// of powers of two, 217 to 237 us (2.3 to 2.5 PFLOP/s; the matrix unit alone reaches 4.4, a library's product with one scale for all 2.7);
-// 32768 rows of 64 experts by 4096 x 2048, 32-bit scales, 385 us (1.43), a fifth of it tiles that are not full; the weights'
-// gradient of 16 experts, 16411 rows, 2048 x 4096, 335 us (0.82), of which its 0.5 GB of results take 100: widening and scaling are as many
-// cycles as its products.
+// Bound by the matrix unit together with the vector unit: 128 x 128 to a workgroup of four waves takes 128 conversions and, with 32-bit
+// scales, 80 multiplications and sums a wave and step, for 64 products.  256 x 256 to eight waves takes 192 for 128 and all there is of LDS and
+// registers.  Measured: 8192 x 4096 x 8192, scales of powers of two, 256 x 256: 380 us (1.45 PFLOP/s; a library's 16-bit product reaches 1.44),
+// 128 x 128: 443; 32-bit scales 456 (1.2), where 256 x 256 takes 480.  32768 rows of 64 experts by 4096 x 2048, 32-bit scales: 566 us (0.97), a
+// fifth of it tiles that are not full.  The weights' gradient of 16 experts, 16411 rows, 2048 x 4096: 335 us (0.82), of which its 0.5 GB of
+// results take 100.
 // (Two waves to a SIMD are asked for: with the registers of one the compiler keeps products apart from what it computes with.)
-// kPrecise: 16-bit matrix instructions on widened values, else 8-bit ones.  kGrad: the weights' gradient, scales by column too.
-template <typename T, HcclAmdScaleType kScale, bool kPrecise, bool kGrad, int kRF, int kCF, int kWR, int kWC>
+// kGrad: the weights' gradient, scales by column too.
+template <typename T, HcclAmdScaleType kScale, bool kGrad, int kRF, int kCF, int kWR, int kWC>
 __global__ void __launch_bounds__(64 * kWR * kWC, 2) TileKernel(ProductArgs a)
 {
     constexpr bool kPowers = kScale == HCCL_AMD_SCALE_E8M0;
@@ -431,9 +433,9 @@ __global__ void __launch_bounds__(64 * kWR * kWC, 2) TileKernel(ProductArgs a)
             scale[int(threadIdx.x) + j * kTileThreads] = coming[j];
         }
     };
-    // The widened operands' form of a step: the block after it is sent for first, then this one is read and multiplied, in the order the
-    // compiler likes (widening between the products).
-    const auto wideStep = [&](uint8_t *tile, uint32_t *scale, uint8_t *other, int next, int last) __attribute__((always_inline)) {
+    // One step: the block after it is sent for first, then this one is read, widened and multiplied, in the order the compiler likes
+    // (widening between the products).
+    const auto step = [&](uint8_t *tile, uint32_t *scale, uint8_t *other, int next, int last) __attribute__((always_inline)) {
         keepScales(scale);
         LoadsDone();
         __syncthreads();     // this block is there, and nobody reads the other buffer any more
@@ -470,77 +472,6 @@ __global__ void __launch_bounds__(64 * kWR * kWC, 2) TileKernel(ProductArgs a)
             }
         }
     };
-    // What a step multiplies first has been read by the step before: its columns and its first 32 rows.
-    Int8 w[kCF], x0, x1;
-    uint32_t rs0 = 0, rs1 = 0;
-    // One step.  Rows are read two sixteens ahead.  Before the last 32 are multiplied all of the block has been read: there the waves
-    // meet, the block after next is sent for into this step's buffer, and behind a column's last product the next step's take its place.
-    // (Behind the last block nothing is sent for, and what is read of the other buffer is not used.)
-    const auto step = [&](uint8_t *tile, const uint32_t *scale, uint8_t *other, uint32_t *otherScale, int afterNext, int last) __attribute__((always_inline)) {
-        const uint8_t *rows = tile + rowAt * 128;
-        const uint32_t *rowScale = scale + rowAt, *colScale = scale + kTileRows + colAt;
-        const float cs = kPowers ? 0.0f : __uint_as_float(colScale[0]);
-        const int csPower = kPowers ? int(colScale[0]) : 0;
-        const auto product = [&](Float4 &to, int c, const Int8 &x, uint32_t rs) __attribute__((always_inline)) {
-            if constexpr (kPowers) {
-                to = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(w[c], x, to, 0, 0, 0, csPower, 0, int(rs));
-            } else {
-                to = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(w[c], x, Zero4(), 0, 0, 0, 0, 0, 0);
-            }
-        };
-        const auto add = [&](Float4 &to, const Float4 &p, uint32_t rs) __attribute__((always_inline)) {
-            const float by = __uint_as_float(rs) * cs;
-#pragma unroll
-            for (int i = 0; i < 4; i++) {
-                to[i] = __builtin_fmaf(p[i], by, to[i]);
-            }
-        };
-#pragma unroll
-        for (int r = 0; r < kRF - 2; r++) {
-            const Int8 after = fragment(rows + (r + 2) * 16 * 128);
-            const uint32_t afterScale = rowScale[(r + 2) * 16 + l16];
-            Float4 p[kCF];
-#pragma unroll
-            for (int c = 0; c < kCF; c++) {
-                product(kPowers ? sum[r][c] : p[c], c, x0, rs0);
-            }
-            if constexpr (!kPowers) {
-#pragma unroll
-                for (int c = 0; c < kCF; c++) {
-                    add(sum[r][c], p[c], rs0);
-                }
-            }
-            x0 = x1;
-            rs0 = rs1;
-            x1 = after;
-            rs1 = afterScale;
-            if (r % 2 == 1) {
-                __builtin_amdgcn_sched_barrier(0);   // (the scheduler would read all rows first and run out of registers)
-            }
-        }
-        keepScales(otherScale);
-        LoadsDone();
-        __syncthreads();   // the next block is there, and nobody reads this one any more
-        fetch(min(afterNext, last), afterNext <= last, tile);
-        const Int8 next0 = fragment(other + rowAt * 128), next1 = fragment(other + (rowAt + 16) * 128);
-        const uint32_t nextScale0 = otherScale[rowAt + l16], nextScale1 = otherScale[rowAt + 16 + l16];
-#pragma unroll
-        for (int c = 0; c < kCF; c++) {
-            Float4 p, q;
-            product(kPowers ? sum[kRF - 2][c] : p, c, x0, rs0);
-            product(kPowers ? sum[kRF - 1][c] : q, c, x1, rs1);
-            w[c] = fragment(other + (kTileRows + colAt + c * 16) * 128);
-            if constexpr (!kPowers) {
-                add(sum[kRF - 2][c], p, rs0);
-                add(sum[kRF - 1][c], q, rs1);
-            }
-        }
-        __builtin_amdgcn_sched_barrier(0);
-        x0 = next0;
-        x1 = next1;
-        rs0 = nextScale0;
-        rs1 = nextScale1;
-    };
     // A wave all of whose rows lie behind the group's last one only loads.
     const bool idle = !kGrad && row0 + rowAt >= rowEnd;
     const auto idleStep = [&](uint8_t *to, uint32_t *scale, int next, int last) __attribute__((always_inline)) {
@@ -554,37 +485,13 @@ __global__ void __launch_bounds__(64 * kWR * kWC, 2) TileKernel(ProductArgs a)
         LoadsDone();
         __syncthreads();     // (the buffers are free: the blocks of another group may have been in them)
         fetch(first, true, tile0);
-        if constexpr (kPrecise) {
-            for (int i = 0; idle && i < count; i++) {
-                idleStep(i % 2 == 0 ? tile1 : tile0, i % 2 == 0 ? scales0 : scales1, first + i + 1, last);
-            }
-            for (int i = 0; !idle && i < count; i += 2) {
-                wideStep(tile0, scales0, tile1, first + i + 1, last);
-                if (i + 1 < count) {
-                    wideStep(tile1, scales1, tile0, first + i + 2, last);
-                }
-            }
-            return;
-        }
-        keepScales(scales0);
-        LoadsDone();
-        __syncthreads();
-        fetch(min(first + 1, last), count > 1, tile1);
-        x0 = fragment(tile0 + rowAt * 128);
-        x1 = fragment(tile0 + (rowAt + 16) * 128);
-        rs0 = scales0[rowAt + l16];
-        rs1 = scales0[rowAt + 16 + l16];
-#pragma unroll
-        for (int c = 0; c < kCF; c++) {
-            w[c] = fragment(tile0 + (kTileRows + colAt + c * 16) * 128);
-        }
         for (int i = 0; idle && i < count; i++) {
-            idleStep(i % 2 == 0 ? tile0 : tile1, i % 2 == 0 ? scales1 : scales0, first + i + 2, last);
+            idleStep(i % 2 == 0 ? tile1 : tile0, i % 2 == 0 ? scales0 : scales1, first + i + 1, last);
         }
         for (int i = 0; !idle && i < count; i += 2) {
-            step(tile0, scales0, tile1, scales1, first + i + 2, last);
+            step(tile0, scales0, tile1, first + i + 1, last);
             if (i + 1 < count) {
-                step(tile1, scales1, tile0, scales0, first + i + 3, last);
+                step(tile1, scales1, tile0, first + i + 2, last);
             }
         }
     };
@@ -666,13 +573,13 @@ HcclResult Choose(HcclDataType type, HcclAmdScaleType scaleType, F f)
 
 constexpr uint64_t kMostTiles = uint64_t(1) << 22;   // workgroups of up to 512 below 2^32 threads
 
-// Tiles of 256 x 256 or of 128 x 128, from how many there are of each.  Of a product with 8192 values to a sum, a step takes 1.75 us where a
-// compute unit has a tile of 256, 1.18 us where it has two of 128 and 0.70 us where it has one; 256 and 512 are under way at once.
-// (2048 rows by 4096: 119 us with 256, 76 with 128; 4096 rows: 134 and 159.)
-bool LargeTiles(uint64_t tiles256, uint64_t tiles128)
+// Tiles of 256 x 256 or of 128 x 128, from how many there are of each, for scales of powers of two (with 32-bit ones the smaller are never
+// slower).  256 of them are under way at once, or twice as many small ones: a round takes 4 us and 2.85 for every block against 0.95 a block.
+// (By 4096 columns: 2048 rows of 8192 values 177 us with 256, 119 with 128; 4096 rows 190 and 228; 8192 rows of 1024 values 59 and 63, of 512
+// values 36 and 35.)
+bool LargeTiles(uint64_t tiles256, uint64_t tiles128, uint64_t blocks)
 {
-    const uint64_t rest = tiles128 % 512;
-    return (tiles256 + 255) / 256 * 175 < tiles128 / 512 * 118 + (rest == 0 ? 0 : rest <= 256 ? 70 : 118);
+    return (tiles256 + 255) / 256 * (400 + 285 * blocks) < (tiles128 + 255) / 256 * 95 * blocks;
 }
 
 constexpr int64_t kMostPitch = int64_t(1) << 23;     // bytes of a row: those of a tile's 256 rows are within 2^31
@@ -742,11 +649,9 @@ HcclResult HcclAmdBlockMatmul(const void *a, uint64_t aStride, const void *aScal
     const uint64_t few64 = unitsOf(16) * ((n + 63) / 64), hit = rows < groups ? rows : groups;
     const bool few = rows <= 4 * uint64_t(groups) || few64 <= 640, several = rows > 16 * hit;
     const bool narrow = few64 < (several ? 256 : 192), twice = several && (narrow ? few64 >= 128 : few64 > 512);
-    // sums of 16-bit results over more than two blocks: the 8-bit instruction's error is behind their own rounding
-    const bool fast = yType != HCCL_DATA_TYPE_FP32 && k > 256;
     // half of the groups' last units are counted: the others' rows fill up one that is counted already
     const auto tilesOf = [&](uint64_t per) { return ((rows + per - 1) / per + (rows < groups ? rows : groups) / 2) * ((n + per - 1) / per); };
-    const bool large = !few && fast && LargeTiles(tilesOf(256), tilesOf(128));
+    const bool large = !few && yType != HCCL_DATA_TYPE_FP32 && scaleType == HCCL_AMD_SCALE_E8M0 && LargeTiles(tilesOf(256), tilesOf(128), Blocks(k));
     const uint64_t tileRows = few ? (twice ? 32 : 16) : large ? 256 : 128, tileCols = few ? (narrow ? 16 : 64) : large ? 256 : 128;
     p.colTiles = int((n + tileCols - 1) / tileCols);
     const uint64_t units = unitsOf(tileRows);
@@ -762,15 +667,12 @@ HcclResult HcclAmdBlockMatmul(const void *a, uint64_t aStride, const void *aScal
             return narrow ? (twice ? go(FewRowsKernel<T, kScale, 2, 1, 8, 4>, 512) : go(FewRowsKernel<T, kScale, 1, 1, 8, 4>, 512))
                           : (twice ? go(FewRowsKernel<T, kScale, 2, 4, 4, 2>, 256) : go(FewRowsKernel<T, kScale, 1, 4, 4, 2>, 256));
         }
-        if constexpr (sizeof(T) == 2) {
+        if constexpr (sizeof(T) == 2 && kScale == HCCL_AMD_SCALE_E8M0) {
             if (large) {
-                return go(TileKernel<T, kScale, false, false, 8, 4, 2, 4>, 512);
-            }
-            if (fast) {
-                return go(TileKernel<T, kScale, false, false, 4, 4, 2, 2>, 256);
+                return go(TileKernel<T, kScale, false, 8, 4, 2, 4>, 512);
             }
         }
-        return go(TileKernel<T, kScale, true, false, 4, 4, 2, 2>, 256);
+        return go(TileKernel<T, kScale, false, 4, 4, 2, 2>, 256);
     });
 }
 
@@ -819,7 +721,7 @@ HcclResult HcclAmdBlockMatmulGradWeight(const void *yGradT, const void *yGradSca
     const uint64_t tiles = ((n + 127) / 128 * uint64_t(p.colTiles) + 7) / 8 * 8 * experts;
     EXPERTS_CHK(tiles <= kMostTiles);
     return Choose(gradType, scaleType, [&](auto of, auto scale) {
-        return Launch("HcclAmdBlockMatmulGradWeight", TileKernel<decltype(of), decltype(scale)::value, true, true, 4, 4, 2, 2>, uint32_t(tiles), 256, 0,
+        return Launch("HcclAmdBlockMatmulGradWeight", TileKernel<decltype(of), decltype(scale)::value, true, 4, 4, 2, 2>, uint32_t(tiles), 256, 0,
             static_cast<hipStream_t>(stream), p);
     });
 }

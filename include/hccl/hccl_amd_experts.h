@@ -109,8 +109,7 @@ extern HcclResult HcclAmdBlockQuantColumns(const void *x, HcclDataType type, uin
  *   w[experts][n][ceil128(k)]    8-bit weights, wScales[experts][ceil(n/128)][ceil(k/128)], as HcclAmdBlockQuantWeights leaves them
  *   y[rows][yStride]             yType FP32, FP16 or BFP16, n to a row
  * Rows outside all groups are left as they are.  The gradient of the rows is the same call with the transposed weights.
- * Sums: products are exact, 32-bit results and sums over up to 256 values are added in 32 bits; 16-bit results over more values come from the
- * 8-bit matrix instruction, which is 1.3e-5 off (2-norm), two orders below their own rounding. */
+ * Sums: products are exact and added in 32 bits, whatever the type of the results. */
 extern HcclResult HcclAmdBlockMatmul(const void *a, uint64_t aStride, const void *aScales, uint64_t aScaleStride, uint64_t rows,
     uint32_t groups, const int32_t *offsets, const int32_t *expertOfGroup, const void *w, const void *wScales, uint32_t experts,
     uint64_t n, uint64_t k, HcclAmdScaleType scaleType, void *y, HcclDataType yType, uint64_t yStride, void *stream);

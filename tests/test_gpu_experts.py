@@ -497,6 +497,71 @@ def test_matmul_many_tiles(stream, kind, rows, groups, n, k, dtype):
     check_matmul(stream, rng, rows, groups, groups, n, k, kind, dtype, strides=n % 8 != 0)
 
 
+def run_matmul(stream, qa, sa, qw, sw, n, k, kind, dtype):
+    """All rows in one group without offsets."""
+    rows, t = qa.shape[0], TYPE[dtype]
+    A, SA, W, SW = (torch.from_numpy(v).cuda() for v in (qa, sa, qw, sw))
+    y = Out(rows, n, t)
+    ready()
+    H.block_matmul(A.data_ptr(), SA.data_ptr(), rows, W.data_ptr(), SW.data_ptr(), 1, n, k, KIND[kind], y.ptr, dt(t), stream.cuda_stream)
+    done(stream)
+    return y.numpy()
+
+
+@pytest.mark.parametrize("kind", ["fp32", "e8m0"])
+@pytest.mark.parametrize("dtype", ["bf16", "fp16", "fp32"])
+@pytest.mark.parametrize("rows,n,k", [(40, 200, 1024), (16, 64, 384), (1000, 1100, 1024), (4100, 4100, 384)])
+def test_matmul_sums_are_in_32_bits(stream, kind, dtype, rows, n, k):
+    """Two large products of every block cancel, what is left is 10^5 times smaller: sums of fewer bits lose it."""
+    print("matmul, cancelling", kind, dtype, rows, n, k, flush=True)
+    rng = np.random.default_rng(rows + k)
+    a, w = (2 * rng.standard_normal((m, k)).astype(np.float32) for m in (rows, n))
+    a[:, 0::128] = a[:, 1::128] = w[:, 0::128] = 448
+    w[:, 1::128] = -448
+    qa, sa, va = ref.quant_rows(a, KIND[kind])
+    qw, sw, vw = ref.quant_weights(w[None], KIND[kind])
+    got = run_matmul(stream, qa, sa, qw, sw, n, k, kind, dtype)
+    want = ref.rows_values(qa, va) @ ref.weights_values(qw, vw)[0].T
+    # the results' own rounding, and k roundings of partial sums up to 448^2, independent of each other: their 2-norm per result, four times
+    room = HALF[TYPE[dtype]] * np.linalg.norm(want) + 4 * k ** 0.5 * U * 448 ** 2 * want.size ** 0.5
+    assert np.linalg.norm(got - want) < room, (np.linalg.norm(got - want) / room)
+    assert room < 0.04 * np.linalg.norm(want)
+
+
+@pytest.mark.parametrize("kind", ["fp32", "e8m0"])
+@pytest.mark.parametrize("rows,n,k", [(24, 100, 1000), (700, 500, 1000), (4100, 4100, 260)])
+def test_products_of_32_bits_as_a_whole(stream, kind, rows, n, k):
+    """The 2-norm of all errors, which leaves no room for sums of fewer bits as the bounds for single results do: results and weights' gradient."""
+    print("products of 32 bits", kind, rows, n, k, flush=True)
+    rng = np.random.default_rng(rows + n)
+    a, w = (rng.standard_normal((m, k)).astype(np.float32) for m in (rows, n))
+    qa, sa, va = ref.quant_rows(a, KIND[kind])
+    qw, sw, vw = ref.quant_weights(w[None], KIND[kind])
+    got = run_matmul(stream, qa, sa, qw, sw, n, k, kind, "fp32")
+    want = ref.rows_values(qa, va) @ ref.weights_values(qw, vw)[0].T
+
+    def room(terms):
+        # independent roundings, cut off at worst (2 U), of partial sums that grow as the root of their terms: 2 U sqrt(terms / 2) of the result
+        return 2 * U * (terms / 2) ** 0.5 + 4 * U
+
+    assert np.linalg.norm(got - want) < room(k) * np.linalg.norm(want)
+    if rows * n > 1 << 20:
+        return
+    dy, x = (torch.from_numpy(rng.standard_normal((rows, c))).bfloat16() for c in (n, k))
+    columns, sdt = H.block_columns(rows, 1), torch.float32 if kind == "fp32" else torch.uint8
+    (qy, sy), (qx, sx) = ((Out(c, columns, torch.uint8), Out(columns // 128, c, sdt)) for c in (n, k))
+    dw, ins = Out(n, k, torch.float32), [v.cuda() for v in (dy, x)]
+    ready()
+    S = stream.cuda_stream
+    for v, q, s, c in ((ins[0], qy, sy, n), (ins[1], qx, sx, k)):
+        H.block_quant_columns(v.data_ptr(), H.HCCL_DATA_TYPE_BFP16, rows, c, 1, None, KIND[kind], q.ptr, columns, s.ptr, S)
+    H.block_matmul_grad_weight(qy.ptr, sy.ptr, qx.ptr, sx.ptr, columns, rows, n, k, KIND[kind], 1, None, 1, dw.ptr, H.HCCL_DATA_TYPE_FP32, S)
+    done(stream)
+    y64, x64 = (ref.from_fp8(q) * np.repeat(v.T, 128, 1) for q, _, v in (ref.quant_columns(t.float().numpy(), [0, rows], KIND[kind]) for t in (dy, x)))
+    want = y64 @ x64.T
+    assert np.linalg.norm(dw.numpy() - want) < room(rows) * np.linalg.norm(want)
+
+
 def test_matmul_offsets_and_owners_that_point_outside(stream):
     """Whatever the device's offsets and owners hold, no row outside is written and no weights outside are read."""
     rng = np.random.default_rng(8)
