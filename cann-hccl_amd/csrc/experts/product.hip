@@ -6,6 +6,8 @@
 // are widened to 16 bits on their way from LDS into the matrix instruction, 16 x 16 x 32, four of which take a block of 128.  Its first
 // operand is `cols`, so that a lane holds four neighbouring values of one row of the result.  Scales that are powers of two go into the
 // widened values; 32-bit ones multiply a block's sum, which is then added in 32 bits.
+#include <algorithm>
+#include <cmath>
 #include <type_traits>
 
 #include "common.h"
@@ -573,13 +575,33 @@ HcclResult Choose(HcclDataType type, HcclAmdScaleType scaleType, F f)
 
 constexpr uint64_t kMostTiles = uint64_t(1) << 22;   // workgroups of up to 512 below 2^32 threads
 
-// Tiles of 256 x 256 or of 128 x 128, from how many there are of each, for scales of powers of two (with 32-bit ones the smaller are never
-// slower).  256 of them are under way at once, or twice as many small ones: a round takes 4 us and 2.85 for every block against 0.95 a block.
-// (By 4096 columns: 2048 rows of 8192 values 177 us with 256, 119 with 128; 4096 rows 190 and 228; 8192 rows of 1024 values 59 and 63, of 512
-// values 36 and 35.)
-bool LargeTiles(uint64_t tiles256, uint64_t tiles128, uint64_t blocks)
+// What a product takes in each form, in microseconds: `call`, and for every 256 workgroups, one to a compute unit, `round` and `block` times the
+// blocks of 128 along its sums.  The form that should take least is taken.  The figures are least squares of relative errors over 616 products:
+// 1, 4, 16, 60, 128 groups, 4 to 12000 rows, 300 to 7168 columns, sums of 300 to 8192, and 260 of 1, 8 and 64 groups by 512 to 14336.  What is taken so is
+// 1.4 % slower than the fastest of all on average, in 9 of 876 by more than a quarter.  For instance, columns x sum, us in the order below:
+//   one group     4096 x 8192:    1 row    8   20   22   58;   64 rows  38   24   31   60;   256 rows 142   81   54   68;   2048 rows  -   -   -  126
+//                 1408 x 2048:    4 rows   6    7    7   17;   96 rows  16    9   10   19;   800 rows  82   30   24   20
+//   64 groups     4096 x 2048:    8 rows  21   13   14   19;   60 groups, 1408 x 2048: 800 rows 105 42 37 41, 1500 rows 177 64 49 41
+//   256 x 256 against 128 x 128, scales of powers of two, 4096 columns: 2048 rows x 8192 177 and 119, 4096 rows x 8192 190 and 228, 8192 rows x 1024 59
+//                 and 63, x 512 36 and 35.  With 32-bit scales the larger is never faster (8192 x 4096 x 8192: 480 and 444).
+struct Form {
+    uint32_t rows, cols;
+    double call, round, block;
+};
+constexpr Form kNarrow = {16, 16, 2.4, 1.4, 0.1}, kFew = {16, 64, 3.0, 0.45, 0.3}, kTwice = {32, 64, 2.7, 0.75, 0.355};
+constexpr Form kTile = {128, 128, 3.1, 1.0, 0.9}, kLargeTile = {256, 256, 3.0, 4.0, 2.85};
+
+// How many groups have rows, and how many units their rows make, is known on the device only.  If rows fall to groups at random, `hit` of them have
+// some; half of the last unit of each is counted, since the others' rows fill up one that is counted already.
+double TimeOf(const Form &form, uint64_t rows, uint64_t groups, uint64_t n, uint64_t blocks)
 {
-    return (tiles256 + 255) / 256 * (400 + 285 * blocks) < (tiles128 + 255) / 256 * 95 * blocks;
+    const uint64_t colTiles = (n + form.cols - 1) / form.cols;
+    double units = double((rows + form.rows - 1) / form.rows);
+    if (groups > 1) {
+        const double hit = double(rows) * double(groups) / double(rows + groups);
+        units = std::max(double(rows) / form.rows + hit / 2, hit);
+    }
+    return form.call + std::ceil(units * double(colTiles) / 256) * (form.round + form.block * double(blocks));
 }
 
 constexpr int64_t kMostPitch = int64_t(1) << 23;     // bytes of a row: those of a tile's 256 rows are within 2^31
@@ -640,21 +662,16 @@ HcclResult HcclAmdBlockMatmul(const void *a, uint64_t aStride, const void *aScal
     EXPERTS_CHK(uint64_t(p.outPitch) >= n && AlignedTo(yType, y));
     EXPERTS_CHK(Aligned(offsets, 4) && Aligned(expertOfGroup, 4));
     p.wideOut = WideOut(yType, n, y, p.outPitch);
-    // Which kernel, 64 groups by 4096 x 2048 and one by 4096 x 8192, 32-bit scales: few rows against tiles of 128 takes 13 us against 16
-    // (8 rows, 64 groups), 90 against 100 (256 rows), 108 against 103 (512 rows); 9 against 45 (1 row, one group), 44 against 49 (128 rows), 85
-    // against 49 (256 rows).  16 columns to a workgroup instead of 64: 9 against 21 (1 row), 13 against 24 (16 rows), 40 against 25 (64 rows).  32 rows
-    // instead of 16: 18 against 21 (32 rows, 16 columns), 31 against 24 (64 rows, 64 columns), 32 against 43 (128 rows).
-    // Units there can be: every group that has rows ends with a shorter one.
-    const auto unitsOf = [&](uint64_t per) { return offsets == nullptr ? (rows + per - 1) / per : rows / per + (rows < groups ? rows : groups); };
-    const uint64_t few64 = unitsOf(16) * ((n + 63) / 64), hit = rows < groups ? rows : groups;
-    const bool few = rows <= 4 * uint64_t(groups) || few64 <= 640, several = rows > 16 * hit;
-    const bool narrow = few64 < (several ? 256 : 192), twice = several && (narrow ? few64 >= 128 : few64 > 512);
-    // half of the groups' last units are counted: the others' rows fill up one that is counted already
-    const auto tilesOf = [&](uint64_t per) { return ((rows + per - 1) / per + (rows < groups ? rows : groups) / 2) * ((n + per - 1) / per); };
-    const bool large = !few && yType != HCCL_DATA_TYPE_FP32 && scaleType == HCCL_AMD_SCALE_E8M0 && LargeTiles(tilesOf(256), tilesOf(128), Blocks(k));
-    const uint64_t tileRows = few ? (twice ? 32 : 16) : large ? 256 : 128, tileCols = few ? (narrow ? 16 : 64) : large ? 256 : 128;
-    p.colTiles = int((n + tileCols - 1) / tileCols);
-    const uint64_t units = unitsOf(tileRows);
+    const Form *form = &kNarrow;
+    for (const Form *other : {&kFew, &kTwice, &kTile, &kLargeTile}) {
+        const bool can = other != &kLargeTile || (scaleType == HCCL_AMD_SCALE_E8M0 && yType != HCCL_DATA_TYPE_FP32);
+        if (can && TimeOf(*other, rows, groups, n, Blocks(k)) < TimeOf(*form, rows, groups, n, Blocks(k))) {
+            form = other;
+        }
+    }
+    p.colTiles = int((n + form->cols - 1) / form->cols);
+    // units there can be: every group that has rows ends with a shorter one
+    const uint64_t units = offsets == nullptr ? (rows + form->rows - 1) / form->rows : rows / form->rows + std::min<uint64_t>(rows, groups);
     EXPERTS_CHK(units * uint64_t(p.colTiles) <= kMostTiles);
     EXPERTS_CHK(p.rowPitch < kMostPitch && p.colPitch < kMostPitch);
     return Choose(yType, scaleType, [&](auto of, auto scale) {
@@ -663,12 +680,17 @@ HcclResult HcclAmdBlockMatmul(const void *a, uint64_t aStride, const void *aScal
         const auto go = [&](auto kernel, int threads) {
             return Launch("HcclAmdBlockMatmul", kernel, uint32_t(units * uint64_t(p.colTiles)), threads, 0, static_cast<hipStream_t>(stream), p);
         };
-        if (few) {
-            return narrow ? (twice ? go(FewRowsKernel<T, kScale, 2, 1, 8, 4>, 512) : go(FewRowsKernel<T, kScale, 1, 1, 8, 4>, 512))
-                          : (twice ? go(FewRowsKernel<T, kScale, 2, 4, 4, 2>, 256) : go(FewRowsKernel<T, kScale, 1, 4, 4, 2>, 256));
+        if (form == &kNarrow) {
+            return go(FewRowsKernel<T, kScale, 1, 1, 8, 4>, 512);
+        }
+        if (form == &kFew) {
+            return go(FewRowsKernel<T, kScale, 1, 4, 4, 2>, 256);
+        }
+        if (form == &kTwice) {
+            return go(FewRowsKernel<T, kScale, 2, 4, 4, 2>, 256);
         }
         if constexpr (sizeof(T) == 2 && kScale == HCCL_AMD_SCALE_E8M0) {
-            if (large) {
+            if (form == &kLargeTile) {
                 return go(TileKernel<T, kScale, false, 8, 4, 2, 4>, 512);
             }
         }

@@ -510,7 +510,7 @@ def run_matmul(stream, qa, sa, qw, sw, n, k, kind, dtype):
 
 @pytest.mark.parametrize("kind", ["fp32", "e8m0"])
 @pytest.mark.parametrize("dtype", ["bf16", "fp16", "fp32"])
-@pytest.mark.parametrize("rows,n,k", [(40, 200, 1024), (16, 64, 384), (1000, 1100, 1024), (4100, 4100, 384)])
+@pytest.mark.parametrize("rows,n,k", [(40, 200, 1024), (16, 64, 384), (1000, 1100, 1024), (4100, 4100, 384), (4000, 4000, 640)])
 def test_matmul_sums_are_in_32_bits(stream, kind, dtype, rows, n, k):
     """Two large products of every block cancel, what is left is 10^5 times smaller: sums of fewer bits lose it."""
     print("matmul, cancelling", kind, dtype, rows, n, k, flush=True)
@@ -560,6 +560,16 @@ def test_products_of_32_bits_as_a_whole(stream, kind, rows, n, k):
     y64, x64 = (ref.from_fp8(q) * np.repeat(v.T, 128, 1) for q, _, v in (ref.quant_columns(t.float().numpy(), [0, rows], KIND[kind]) for t in (dy, x)))
     want = y64 @ x64.T
     assert np.linalg.norm(dw.numpy() - want) < room(rows) * np.linalg.norm(want)
+
+
+@pytest.mark.parametrize("dtype", ["bf16", "fp16"])
+@pytest.mark.parametrize("rows,groups,n,k", [(4000, 1, 4000, 640), (3999, 1, 4001, 700), (7600, 3, 4000, 1500)])
+def test_matmul_large_tiles(stream, dtype, rows, groups, n, k):
+    """Scales of powers of two and as many tiles of 256 x 256 as compute units: the form with those; odd and even numbers of blocks, rows and
+    columns that end inside a tile, also on odd addresses."""
+    print("matmul, large tiles", dtype, rows, groups, n, k, flush=True)
+    rng = np.random.default_rng(rows + k)
+    check_matmul(stream, rng, rows, groups, groups, n, k, "e8m0", dtype, strides=n % 8 != 0)
 
 
 def test_matmul_offsets_and_owners_that_point_outside(stream):
