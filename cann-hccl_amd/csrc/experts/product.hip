@@ -662,17 +662,22 @@ HcclResult HcclAmdBlockMatmul(const void *a, uint64_t aStride, const void *aScal
     EXPERTS_CHK(uint64_t(p.outPitch) >= n && AlignedTo(yType, y));
     EXPERTS_CHK(Aligned(offsets, 4) && Aligned(expertOfGroup, 4));
     p.wideOut = WideOut(yType, n, y, p.outPitch);
-    const Form *form = &kNarrow;
-    for (const Form *other : {&kFew, &kTwice, &kTile, &kLargeTile}) {
+    const auto columnsOf = [&](const Form &form) { return (n + form.cols - 1) / form.cols; };
+    // units there can be: every group that has rows ends with a shorter one
+    const auto unitsOf = [&](const Form &form) {
+        return offsets == nullptr ? (rows + form.rows - 1) / form.rows : rows / form.rows + std::min<uint64_t>(rows, groups);
+    };
+    EXPERTS_CHK(unitsOf(kTile) * columnsOf(kTile) <= kMostTiles);
+    const Form *form = &kTile;
+    for (const Form *other : {&kNarrow, &kFew, &kTwice, &kLargeTile}) {
         const bool can = other != &kLargeTile || (scaleType == HCCL_AMD_SCALE_E8M0 && yType != HCCL_DATA_TYPE_FP32);
-        if (can && TimeOf(*other, rows, groups, n, Blocks(k)) < TimeOf(*form, rows, groups, n, Blocks(k))) {
+        if (can && unitsOf(*other) * columnsOf(*other) <= kMostTiles &&
+            TimeOf(*other, rows, groups, n, Blocks(k)) < TimeOf(*form, rows, groups, n, Blocks(k))) {
             form = other;
         }
     }
-    p.colTiles = int((n + form->cols - 1) / form->cols);
-    // units there can be: every group that has rows ends with a shorter one
-    const uint64_t units = offsets == nullptr ? (rows + form->rows - 1) / form->rows : rows / form->rows + std::min<uint64_t>(rows, groups);
-    EXPERTS_CHK(units * uint64_t(p.colTiles) <= kMostTiles);
+    p.colTiles = int(columnsOf(*form));
+    const uint64_t units = unitsOf(*form);
     EXPERTS_CHK(p.rowPitch < kMostPitch && p.colPitch < kMostPitch);
     return Choose(yType, scaleType, [&](auto of, auto scale) {
         typedef decltype(of) T;

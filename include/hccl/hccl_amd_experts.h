@@ -91,14 +91,15 @@ extern HcclResult HcclAmdExpertCombineGrad(const void *yGrad, uint64_t yGradStri
  *   w[experts][n][wStride]               FP32, FP16 or BFP16
  *   q[experts][n][ceil128(k)]            scales[experts][ceil(n/128)][ceil(k/128)]
  *   qT[experts][k][ceil128(n)]           the same values transposed, scalesT[experts][ceil(k/128)][ceil(n/128)]
- * Either pair may be NULL. */
+ * Either pair may be NULL.  Limit: experts * ceil(n/128) * ceil(k/128) <= 2^23. */
 extern HcclResult HcclAmdBlockQuantWeights(const void *w, HcclDataType type, uint32_t experts, uint64_t n, uint64_t k, uint64_t wStride,
     HcclAmdScaleType scaleType, void *q, void *scales, void *qT, void *scalesT, void *stream);
 
 /* 8-bit columns: x[rows][xStride] of `width` columns, transposed, with one scale per column and 128 rows of a group.
  * offsets[groups + 1] are the groups' first rows, ascending.  In qT[width][columns] every group starts at a multiple of 128 and is
  * padded with zeros to one; group g starts at sum over h < g of ceil128(rows of h).  scales[columns / 128][width].
- * columns: a multiple of 128, at least (rows / 128 + groups) * 128 (rows / 128 rounded down) so that any offsets fit. */
+ * columns: a multiple of 128, at least (rows / 128 + groups) * 128 (rows / 128 rounded down) so that any offsets fit.
+ * Limits: rows <= 2^28, (rows / 128 + groups) * ceil(width / 128) <= 2^23. */
 extern HcclResult HcclAmdBlockQuantColumns(const void *x, HcclDataType type, uint64_t rows, uint64_t width, uint64_t xStride,
     uint32_t groups, const int32_t *offsets, HcclAmdScaleType scaleType, void *qT, uint64_t columns, void *scales, void *stream);
 
@@ -109,14 +110,16 @@ extern HcclResult HcclAmdBlockQuantColumns(const void *x, HcclDataType type, uin
  *   w[experts][n][ceil128(k)]    8-bit weights, wScales[experts][ceil(n/128)][ceil(k/128)], as HcclAmdBlockQuantWeights leaves them
  *   y[rows][yStride]             yType FP32, FP16 or BFP16, n to a row
  * Rows outside all groups are left as they are.  The gradient of the rows is the same call with the transposed weights.
- * Sums: products are exact and added in 32 bits, whatever the type of the results. */
+ * Sums: products are exact and added in 32 bits, whatever the type of the results.
+ * Limits: rows <= 2^28, and (rows / 128 + the lesser of rows and groups) * ceil(n / 128) <= 2^22. */
 extern HcclResult HcclAmdBlockMatmul(const void *a, uint64_t aStride, const void *aScales, uint64_t aScaleStride, uint64_t rows,
     uint32_t groups, const int32_t *offsets, const int32_t *expertOfGroup, const void *w, const void *wScales, uint32_t experts,
     uint64_t n, uint64_t k, HcclAmdScaleType scaleType, void *y, HcclDataType yType, uint64_t yStride, void *stream);
 
 /* wGrad[e][n][k] = sum over the rows r of e's groups of yGrad[r][n] * x[r][k] (added to what is there with `accumulate`), from
  * both sides' 8-bit columns (HcclAmdBlockQuantColumns of the same rows, groups, offsets and columns, below 2^23).  Experts without
- * rows get zeros; all sums are in 32 bits.  wGrad: FP32, FP16 or BFP16. */
+ * rows get zeros; all sums are in 32 bits.  wGrad: FP32, FP16 or BFP16.  Limits: ceil(n / 128) * ceil(k / 128), rounded up to a multiple
+ * of 8, times experts <= 2^22. */
 extern HcclResult HcclAmdBlockMatmulGradWeight(const void *yGradT, const void *yGradScales, const void *xT, const void *xScales,
     uint64_t columns, uint64_t rows, uint64_t n, uint64_t k, HcclAmdScaleType scaleType, uint32_t groups, const int32_t *offsets,
     const int32_t *expertOfGroup, uint32_t experts, void *wGrad, HcclDataType gradType, uint32_t accumulate, void *stream);

@@ -196,6 +196,12 @@ def test_reference_scales():
     assert ref.block_scale(np.float32([0]), ref.E8M0)[0][0] == 127 - 96 - 8
 
 
+@pytest.mark.parametrize("rows,groups,n", [(1 << 28, 1, 257), ((1 << 28) - 1, 4096, 200), (1 << 16, 4096, 128 * 1100)])
+def test_matmul_refuses_more_tiles_than_a_launch_holds(rows, groups, n):
+    assert (rows // 128 + min(rows, groups)) * -(-n // 128) > 1 << 22
+    assert H.lib().HcclAmdBlockMatmul(P, 0, P, 0, rows, groups, P, None if groups == 1 else P, P, P, 4, n, 128, 1, P, BF16, 0, N) == PARA
+
+
 def test_native_calls_and_ctypes_refuse_alike():
     """The mirror's two ways to a call give the same answers; what the native one does not recognise it leaves alone."""
     L = H.lib()

@@ -572,6 +572,33 @@ def test_matmul_large_tiles(stream, dtype, rows, groups, n, k):
     check_matmul(stream, rng, rows, groups, groups, n, k, "e8m0", dtype, strides=n % 8 != 0)
 
 
+def test_matmul_of_many_small_groups_by_many_columns(stream):
+    """So many groups and columns that a launch cannot hold a workgroup for every 16 of a group's rows: a form with larger tiles takes it."""
+    print("matmul, 4096 groups by 65536 columns", flush=True)
+    rng = np.random.default_rng(12)
+    rows, groups, experts, n, k = 16384, 4096, 2, 65536, 128
+    offsets = some_groups(rng, rows, groups, skew=False)
+    own = rng.integers(0, experts, groups).astype(np.int32)
+    qa, sa, va = ref.quant_rows(rng.standard_normal((rows, k)).astype(np.float32), ref.FP32)
+    qw, sw, vw = ref.quant_weights(rng.standard_normal((experts, n, k)).astype(np.float32), ref.FP32)
+    A, SA, W, SW, off, og = (torch.from_numpy(v).cuda() for v in (qa, sa, qw, sw, offsets, own))
+    y = torch.full((rows, n), float("nan"), dtype=torch.bfloat16, device="cuda")
+    ready()
+    H.block_matmul(A.data_ptr(), SA.data_ptr(), rows, W.data_ptr(), SW.data_ptr(), experts, n, k, ref.FP32, y.data_ptr(), H.HCCL_DATA_TYPE_BFP16,
+                   stream.cuda_stream, groups=groups, offsets=off.data_ptr(), expert_of_group=og.data_ptr())
+    done(stream)
+    assert bool(torch.isfinite(y).all())
+    group = np.searchsorted(offsets, np.arange(rows), side="right") - 1
+    for r in [0, rows - 1] + rng.integers(0, rows, 30).tolist():
+        e = own[group[r]]
+        m = ref.from_fp8(qw[e]) * np.repeat(vw[e], 128, 0)
+        x = ref.rows_values(qa[r:r + 1], va[r:r + 1])
+        want, size = x @ m.T, np.abs(x) @ np.abs(m).T
+        assert close(y[r:r + 1].double().cpu().numpy(), want, 2 * (k + 5) * U * size, torch.bfloat16), r
+    del y
+    torch.cuda.empty_cache()
+
+
 def test_matmul_offsets_and_owners_that_point_outside(stream):
     """Whatever the device's offsets and owners hold, no row outside is written and no weights outside are read."""
     rng = np.random.default_rng(8)
