@@ -70,21 +70,21 @@ typedef uint32_t Word2 __attribute__((ext_vector_type(2)));
 typedef uint32_t Word4 __attribute__((ext_vector_type(4)));
 
 // N consecutive elements from p, in loads of 16 bytes (or one of all of them, if they are fewer).  kWide: p is aligned to that; else to
-// an element, which the hardware takes too (a lane's load then touches one line more).
-template <bool kWide, int N, typename T>
-__device__ __forceinline__ void Load(const T *p, float (&v)[N])
+// an element, which the hardware takes too (a lane's load then touches one line more).  V: float, or T itself for bits as they are.
+template <bool kWide, int N, typename T, typename V>
+__device__ __forceinline__ void Load(const T *p, V (&v)[N])
 {
     constexpr int kAlign = !kWide ? sizeof(T) : N * sizeof(T) < 16 ? N * sizeof(T) : 16;
     typedef T Vec __attribute__((ext_vector_type(N), aligned(kAlign)));
     const Vec x = *reinterpret_cast<const Vec *>(p);
 #pragma unroll
     for (int i = 0; i < N; i++) {
-        v[i] = float(x[i]);
+        v[i] = V(x[i]);
     }
 }
 
-template <bool kWide, int N, typename T>
-__device__ __forceinline__ void Store(T *p, const float (&v)[N])
+template <bool kWide, int N, typename T, typename V>
+__device__ __forceinline__ void Store(T *p, const V (&v)[N])
 {
     constexpr int kAlign = !kWide ? sizeof(T) : N * sizeof(T) < 16 ? N * sizeof(T) : 16;
     typedef T Vec __attribute__((ext_vector_type(N), aligned(kAlign)));
@@ -101,8 +101,8 @@ __device__ __forceinline__ void Store(T *p, const float (&v)[N])
 constexpr int kAnyhow = 0, kAligned = 1, kExactly = 2;
 
 // N elements from column `at` of a row of `width`, `fill` beyond it.
-template <int kHow, int N, typename T>
-__device__ __forceinline__ void LoadPart(const T *row, int at, int width, float (&v)[N], float fill = 0.0f)
+template <int kHow, int N, typename T, typename V>
+__device__ __forceinline__ void LoadPart(const T *row, int at, int width, V (&v)[N], V fill = V(0))
 {
     if constexpr (kHow == kExactly) {
         Load<true, N>(row + at, v);
@@ -117,14 +117,14 @@ __device__ __forceinline__ void LoadPart(const T *row, int at, int width, float 
     } else if (kHow == kAnyhow && at < width) {
         for (int i = 0; i < N; i++) {
             if (at + i < width) {
-                v[i] = float(row[at + i]);
+                v[i] = V(row[at + i]);
             }
         }
     }
 }
 
-template <int kHow, int N, typename T>
-__device__ __forceinline__ void StorePart(T *row, int at, int width, const float (&v)[N])
+template <int kHow, int N, typename T, typename V>
+__device__ __forceinline__ void StorePart(T *row, int at, int width, const V (&v)[N])
 {
     if (kHow == kExactly) {
         Store<true, N>(row + at, v);

@@ -7,6 +7,8 @@
 // Measured, where a large copy reaches 5.15 TB/s: 16384 tokens of 4096 values to eight rows each in 8 bits (0.68 GB) 122 us, 5.5 TB/s;
 // back and weighted (1.2 GB) 246 us, 4.9 TB/s; the gradients of that (2.2 GB) 424 us, 5.2 TB/s.  2001 values to a row, off every
 // boundary (8191 tokens, four rows each): 41 and 74 us, 4.0 TB/s.  64 tokens of 8192: 4 us.
+#include <type_traits>
+
 #include "common.h"
 
 namespace hcclamd {
@@ -48,7 +50,8 @@ struct PackArgs {
     int width, padded, topK, pieces;
 };
 
-// A wave to a token and a piece of its width: read once, written to all of the token's rows.
+// A wave to a token and a piece of its width: read once, written to all of the token's rows.  T: words of the elements' size (as numbers, some
+// NaN would come out with other bits).
 template <typename T, bool kWide>
 __global__ void __launch_bounds__(kThreads) CopyKernel(PackArgs a)
 {
@@ -56,7 +59,7 @@ __global__ void __launch_bounds__(kThreads) CopyKernel(PackArgs a)
         const int64_t t = w / a.pieces;
         const int at = int(w % a.pieces) * kPiece + int(threadIdx.x % 64) * kEach;
         const int rows = RowsOf(a.rowOf, t, a.topK, a.rows);
-        float v[kEach];
+        T v[kEach];
         LoadPart<kWide, kEach>(static_cast<const T *>(a.x) + t * a.xStride, at, a.width, v);
         for (int j = 0; j < a.topK; j++) {
             const int64_t r = __builtin_amdgcn_readlane(rows, j);
@@ -290,7 +293,7 @@ HcclResult HcclAmdExpertPack(const void *x, HcclDataType type, uint64_t tokens, 
         a.waves = int64_t(tokens) * a.pieces;
         const bool wide = Wide(type, width, x, a.xStride) && Wide(type, width, out, a.outStride);
         return ByType(type, [&](auto of) {
-            typedef decltype(of) T;
+            typedef std::conditional_t<sizeof(of) == 4, uint32_t, uint16_t> T;
             return Launch("HcclAmdExpertPack", wide ? CopyKernel<T, true> : CopyKernel<T, false>, BlocksOf(a.waves), kThreads, 0, on, a);
         });
     }

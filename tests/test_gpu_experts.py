@@ -340,6 +340,24 @@ def test_pack_copies_and_combine(stream, dtype, tokens, width, topk):
         assert close(dwt.numpy(), dots.sum(2), (width + 1) * U * np.abs(dots).sum(2))
 
 
+@pytest.mark.parametrize("dtype", ["bf16", "fp16", "fp32"])
+@pytest.mark.parametrize("shift", [0, 1])
+def test_pack_copies_bits(stream, dtype, shift):
+    """Every pattern of 16 bits, the NaN that signal among them, and of 32 bits those and random ones; aligned and off every boundary."""
+    t = TYPE[dtype]
+    if dtype == "fp32":
+        high = np.arange(1 << 16, dtype=np.uint32) << 16
+        bits = torch.from_numpy((high | np.random.default_rng(9).integers(0, 1 << 16, 1 << 16, dtype=np.uint32)).view(np.int32)).reshape(64, 1024)
+    else:
+        bits = torch.arange(1 << 16, dtype=torch.int32).to(torch.int16).reshape(64, 1024)
+    row = torch.randperm(64, generator=torch.Generator().manual_seed(1)).int().reshape(64, 1)
+    x, out, r = Out(64, 1024, bits.dtype, 1024 + shift, shift).fill(bits.cuda()), Out(64, 1024, bits.dtype, 1024 + shift, shift), row.cuda()
+    ready()
+    H.expert_pack(x.ptr, dt(t), 64, 1024, 1, r.data_ptr(), out.ptr, 64, stream.cuda_stream, x_stride=x.stride, out_stride=out.stride)
+    done(stream)
+    assert torch.equal(out.get().cpu()[row[:, 0].long()], bits)
+
+
 def test_rows_without_a_map_and_rows_that_are_not_there(stream):
     """rowOf None: row t is token t.  Rows outside [0, rows) are skipped."""
     x = torch.randn(5, 256, device="cuda")
