@@ -713,6 +713,7 @@ HcclResult HcclAmdBlockMatmulGradWeight(const void *yGradT, const void *yGradSca
     EXPERTS_CHK(rows <= kMaxGroupedRows && n <= kMaxSize - 256 && k <= kMaxSize - 256);
     EXPERTS_CHK(groups >= 1 && groups <= HCCL_AMD_MAX_GROUPS && experts >= 1 && experts <= HCCL_AMD_MAX_GROUPS);
     EXPERTS_CHK(offsets != nullptr || groups == 1);
+    EXPERTS_CHK(expertOfGroup != nullptr || groups <= experts);
     EXPERTS_CHK(columns % 128 == 0 && columns >= (rows / 128 + groups) * 128 && columns <= kMaxSize);
     if (n == 0 || k == 0) {
         return HCCL_SUCCESS;

@@ -106,7 +106,7 @@ extern HcclResult HcclAmdBlockQuantColumns(const void *x, HcclDataType type, uin
 /* y[r] = a[r] * w[e]^T for the rows r of every group, e the group's expert.
  *   a[rows][aStride]             8-bit rows of k values, aScales[rows][aScaleStride]
  *   offsets[groups + 1]          first row of every group, ascending; NULL: one group of all rows
- *   expertOfGroup[groups]        the weights a group uses; NULL: group g uses weights g
+ *   expertOfGroup[groups]        the weights a group uses; NULL: group g uses weights g, groups <= experts
  *   w[experts][n][ceil128(k)]    8-bit weights, wScales[experts][ceil(n/128)][ceil(k/128)], as HcclAmdBlockQuantWeights leaves them
  *   y[rows][yStride]             yType FP32, FP16 or BFP16, n to a row
  * Rows outside all groups are left as they are.  The gradient of the rows is the same call with the transposed weights.
@@ -117,9 +117,9 @@ extern HcclResult HcclAmdBlockMatmul(const void *a, uint64_t aStride, const void
     uint64_t n, uint64_t k, HcclAmdScaleType scaleType, void *y, HcclDataType yType, uint64_t yStride, void *stream);
 
 /* wGrad[e][n][k] = sum over the rows r of e's groups of yGrad[r][n] * x[r][k] (added to what is there with `accumulate`), from
- * both sides' 8-bit columns (HcclAmdBlockQuantColumns of the same rows, groups, offsets and columns, below 2^23).  Experts without
- * rows get zeros; all sums are in 32 bits.  wGrad: FP32, FP16 or BFP16.  Limits: ceil(n / 128) * ceil(k / 128), rounded up to a multiple
- * of 8, times experts <= 2^22. */
+ * both sides' 8-bit columns (HcclAmdBlockQuantColumns of the same rows, groups, offsets and columns, below 2^23).  offsets and
+ * expertOfGroup as in HcclAmdBlockMatmul.  Experts without rows get zeros; all sums are in 32 bits.  wGrad: FP32, FP16 or BFP16.
+ * Limit: ceil(n / 128) * ceil(k / 128), rounded up to a multiple of 8, times experts <= 2^22. */
 extern HcclResult HcclAmdBlockMatmulGradWeight(const void *yGradT, const void *yGradScales, const void *xT, const void *xScales,
     uint64_t columns, uint64_t rows, uint64_t n, uint64_t k, HcclAmdScaleType scaleType, uint32_t groups, const int32_t *offsets,
     const int32_t *expertOfGroup, uint32_t experts, void *wGrad, HcclDataType gradType, uint32_t accumulate, void *stream);

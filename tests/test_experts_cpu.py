@@ -196,6 +196,13 @@ def test_reference_scales():
     assert ref.block_scale(np.float32([0]), ref.E8M0)[0][0] == 127 - 96 - 8
 
 
+def test_grad_weight_refuses_groups_without_weights():
+    """Group g uses weights g: more groups than weights are refused, as the product refuses them."""
+    for fn, args in (("HcclAmdBlockMatmulGradWeight", (P, P, P, P, 1024, 50, 100, 300, 1, 5, P, None, 4, P, BF16, 0, N)),
+                     ("HcclAmdBlockMatmul", (P, 0, P, 0, 50, 5, P, None, P, P, 4, 100, 300, 1, P, BF16, 0, N))):
+        assert getattr(H.lib(), fn)(*args) == PARA
+
+
 @pytest.mark.parametrize("rows,groups,n", [(1 << 28, 1, 257), ((1 << 28) - 1, 4096, 200), (1 << 16, 4096, 128 * 1100)])
 def test_matmul_refuses_more_tiles_than_a_launch_holds(rows, groups, n):
     assert (rows // 128 + min(rows, groups)) * -(-n // 128) > 1 << 22
