@@ -42,6 +42,8 @@ inline uint64_t Up128(uint64_t n) { return (n + 127) / 128 * 128; }
 inline uint64_t Blocks(uint64_t n) { return (n + 127) / 128; }
 inline bool Float(HcclDataType t) { return t == HCCL_DATA_TYPE_FP32 || t == HCCL_DATA_TYPE_FP16 || t == HCCL_DATA_TYPE_BFP16; }
 inline uint64_t SizeOf(HcclDataType t) { return t == HCCL_DATA_TYPE_FP32 ? 4 : 2; }
+// From one row to the next, in elements; 0: no gap.  Beyond 2^40 lies no memory, and a negative number taken for an unsigned one does.
+inline bool Stride(uint64_t stride, uint64_t least) { return stride == 0 || (stride >= least && stride <= uint64_t(1) << 40); }
 inline bool Scaled(HcclAmdScaleType s) { return s == HCCL_AMD_SCALE_FP32 || s == HCCL_AMD_SCALE_E8M0; }
 inline bool Aligned(const void *p, uint64_t to) { return reinterpret_cast<uintptr_t>(p) % to == 0; }
 inline bool AlignedTo(HcclDataType t, const void *p) { return Aligned(p, SizeOf(t)); }

@@ -273,7 +273,7 @@ HcclResult HcclAmdExpertPack(const void *x, HcclDataType type, uint64_t tokens, 
     }
     EXPERTS_CHK_PTR(x);
     EXPERTS_CHK_PTR(out);
-    EXPERTS_CHK(xStride == 0 || xStride >= width);
+    EXPERTS_CHK(Stride(xStride, width));
     EXPERTS_CHK(AlignedTo(type, x) && Aligned(rowOf, 4));
     PackArgs a{};
     a.x = x;
@@ -286,7 +286,7 @@ HcclResult HcclAmdExpertPack(const void *x, HcclDataType type, uint64_t tokens, 
     a.topK = int(topK);
     const hipStream_t on = static_cast<hipStream_t>(stream);
     if (scaleType == HCCL_AMD_SCALE_NONE) {
-        EXPERTS_CHK(outStride == 0 || outStride >= width);
+        EXPERTS_CHK(Stride(outStride, width));
         EXPERTS_CHK(AlignedTo(type, out));
         a.outStride = int64_t(outStride == 0 ? width : outStride);
         a.pieces = int((width + kPiece - 1) / kPiece);
@@ -301,8 +301,8 @@ HcclResult HcclAmdExpertPack(const void *x, HcclDataType type, uint64_t tokens, 
     EXPERTS_CHK(ScaleAligned(scaleType, scales));
     a.outStride = int64_t(outStride == 0 ? Up128(width) : outStride);
     a.scaleStride = int64_t(scaleStride == 0 ? Blocks(width) : scaleStride);
-    EXPERTS_CHK(uint64_t(a.outStride) >= Up128(width) && a.outStride % 16 == 0 && Aligned(out, 16));
-    EXPERTS_CHK(uint64_t(a.scaleStride) >= Blocks(width));
+    EXPERTS_CHK(Stride(outStride, Up128(width)) && outStride % 16 == 0 && Aligned(out, 16));
+    EXPERTS_CHK(Stride(scaleStride, Blocks(width)));
     a.padded = int(Up128(width));
     a.pieces = (a.padded + kPiece - 1) / kPiece;
     a.waves = int64_t(tokens) * a.pieces;
@@ -332,8 +332,8 @@ HcclResult HcclAmdExpertCombine(const void *x, HcclDataType type, uint64_t rows,
         EXPERTS_CHK_PTR(x);
     }
     EXPERTS_CHK_PTR(y);
-    EXPERTS_CHK(xStride == 0 || xStride >= width);
-    EXPERTS_CHK(yStride == 0 || yStride >= width);
+    EXPERTS_CHK(Stride(xStride, width));
+    EXPERTS_CHK(Stride(yStride, width));
     EXPERTS_CHK(AlignedTo(type, x) && AlignedTo(type, y) && Aligned(rowOf, 4) && Aligned(weights, 4));
     CombineArgs a{};
     a.x = x;
@@ -374,9 +374,9 @@ HcclResult HcclAmdExpertCombineGrad(const void *yGrad, uint64_t yGradStride, con
             EXPERTS_CHK_PTR(x);
         }
     }
-    EXPERTS_CHK(xStride == 0 || xStride >= width);
-    EXPERTS_CHK(yGradStride == 0 || yGradStride >= width);
-    EXPERTS_CHK(xGradStride == 0 || xGradStride >= width);
+    EXPERTS_CHK(Stride(xStride, width));
+    EXPERTS_CHK(Stride(yGradStride, width));
+    EXPERTS_CHK(Stride(xGradStride, width));
     EXPERTS_CHK(AlignedTo(type, x) && AlignedTo(type, yGrad) && AlignedTo(type, xGrad));
     EXPERTS_CHK(Aligned(rowOf, 4) && Aligned(weights, 4) && Aligned(weightGrad, 4));
     CombineArgs a{};

@@ -657,9 +657,9 @@ HcclResult HcclAmdBlockMatmul(const void *a, uint64_t aStride, const void *aScal
     p.blocks = int(Blocks(k));
     p.groups = int(groups);
     p.experts = int(experts);
-    EXPERTS_CHK(uint64_t(p.rowPitch) >= Up128(k) && p.rowPitch % 16 == 0 && Aligned(a, 16) && Aligned(w, 16));
-    EXPERTS_CHK(uint64_t(p.rowScalePitch) >= Blocks(k) && ScaleAligned(scaleType, aScales) && ScaleAligned(scaleType, wScales));
-    EXPERTS_CHK(uint64_t(p.outPitch) >= n && AlignedTo(yType, y));
+    EXPERTS_CHK(Stride(aStride, Up128(k)) && aStride % 16 == 0 && Aligned(a, 16) && Aligned(w, 16));
+    EXPERTS_CHK(Stride(aScaleStride, Blocks(k)) && ScaleAligned(scaleType, aScales) && ScaleAligned(scaleType, wScales));
+    EXPERTS_CHK(Stride(yStride, n) && AlignedTo(yType, y));
     EXPERTS_CHK(Aligned(offsets, 4) && Aligned(expertOfGroup, 4));
     p.wideOut = WideOut(yType, n, y, p.outPitch);
     const auto columnsOf = [&](const Form &form) { return (n + form.cols - 1) / form.cols; };

@@ -219,7 +219,7 @@ HcclResult HcclAmdBlockQuantWeights(const void *w, HcclDataType type, uint32_t e
     if (qT != nullptr) {
         EXPERTS_CHK_PTR(scalesT);
     }
-    EXPERTS_CHK(wStride == 0 || wStride >= k);
+    EXPERTS_CHK(Stride(wStride, k));
     EXPERTS_CHK(AlignedTo(type, w) && Aligned(q, 16) && Aligned(qT, 16) && ScaleAligned(scaleType, scales) && ScaleAligned(scaleType, scalesT));
     EXPERTS_CHK(Blocks(n) * Blocks(k) * experts <= (uint64_t(1) << 23));   // workgroups of 256 below 2^32 threads
     TileArgs a{};
@@ -255,7 +255,7 @@ HcclResult HcclAmdBlockQuantColumns(const void *x, HcclDataType type, uint64_t r
     EXPERTS_CHK_PTR(x);
     EXPERTS_CHK_PTR(qT);
     EXPERTS_CHK_PTR(scales);
-    EXPERTS_CHK(xStride == 0 || xStride >= width);
+    EXPERTS_CHK(Stride(xStride, width));
     EXPERTS_CHK(AlignedTo(type, x) && Aligned(qT, 16) && ScaleAligned(scaleType, scales) && Aligned(offsets, 4));
     const uint64_t units = rows / 128 + groups;
     EXPERTS_CHK(Blocks(width) * units <= (uint64_t(1) << 23));

@@ -872,7 +872,7 @@ HcclResult HcclAmdExpertRoute(const void *logits, HcclDataType logitType, uint64
         EXPERTS_CHK_PTR(expertOf);
         EXPERTS_CHK_PTR(weights);
         EXPERTS_CHK_PTR(rowOf);
-        EXPERTS_CHK(logitStride == 0 || logitStride >= experts);
+        EXPERTS_CHK(Stride(logitStride, experts));
         EXPERTS_CHK(AlignedTo(logitType, logits) && Aligned(expertOf, 4) && Aligned(weights, 4) && Aligned(rowOf, 4));
         if (needed != 0) {
             EXPERTS_CHK_PTR(workspace);
@@ -938,8 +938,8 @@ HcclResult HcclAmdExpertRouteGrad(const void *logits, HcclDataType logitType, ui
     EXPERTS_CHK_PTR(expertOf);
     EXPERTS_CHK_PTR(counts);
     EXPERTS_CHK_PTR(logitGrad);
-    EXPERTS_CHK(logitStride == 0 || logitStride >= experts);
-    EXPERTS_CHK(logitGradStride == 0 || logitGradStride >= experts);
+    EXPERTS_CHK(Stride(logitStride, experts));
+    EXPERTS_CHK(Stride(logitGradStride, experts));
     EXPERTS_CHK(AlignedTo(logitType, logits) && AlignedTo(logitType, logitGrad) && Aligned(expertOf, 4) && Aligned(counts, 4));
     EXPERTS_CHK(Aligned(weightGrad, 4) && Aligned(lossGrad, 4));
     RouteGradArgs a{};

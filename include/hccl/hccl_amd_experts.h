@@ -9,7 +9,7 @@
  * All of them: device pointers unless said otherwise, of one GPU; no communicator; the work is queued on `stream` (a
  * hipStream_t, not null) and nothing is allocated, copied or waited for, so a call can be captured into a HIP graph.  An
  * output must not overlap an input or another output.  Same inputs, same bits: no atomics whose order matters.  Strides are
- * in elements, from one row to the next; 0 stands for rows that follow each other without a gap.  Values in 16 bits are
+ * in elements, from one row to the next, 2^40 at most; 0 stands for rows that follow each other without a gap.  Values in 16 bits are
  * widened, everything is summed in 32 bits, and rounded once at the end.  Indices and offsets read from device memory are
  * checked on the device: what points outside is skipped.
  * Errors: HCCL_E_PTR (a null pointer or stream), HCCL_E_PARA (a size, stride or alignment), HCCL_E_NOT_SUPPORT (a type),

@@ -196,6 +196,24 @@ def test_reference_scales():
     assert ref.block_scale(np.float32([0]), ref.E8M0)[0][0] == 127 - 96 - 8
 
 
+@pytest.mark.parametrize("stride", [2 ** 64 - 1024, 2 ** 63, 2 ** 40 + 16])
+def test_strides_that_no_memory_has(stride):
+    """What a negative number becomes on its way to an unsigned one, and anything else beyond 2^40, is refused and not followed."""
+    calls = [("HcclAmdExpertRoute", (P, BF16, 100, 64, 0, 8, 0, None, 1.0, P, P, P, P, P, P, P, 1 << 30, N), (4,)),
+             ("HcclAmdExpertRouteGrad", (P, BF16, 100, 64, 0, 8, 0, None, 1.0, P, P, P, P, P, 0, N), (4, 14)),
+             ("HcclAmdExpertPack", (P, BF16, 10, 300, 0, 2, P, 1, P, 20, 0, P, 0, N), (4, 10, 12)),
+             ("HcclAmdExpertPack", (P, BF16, 10, 300, 0, 2, P, 0, P, 20, 0, None, 0, N), (4, 10)),
+             ("HcclAmdExpertCombine", (P, BF16, 20, 300, 0, 10, 2, P, P, P, 0, N), (4, 10)),
+             ("HcclAmdExpertCombineGrad", (P, 0, P, FP16, 20, 300, 0, 10, 2, P, P, P, 0, P, N), (1, 6, 12)),
+             ("HcclAmdBlockQuantWeights", (P, BF16, 2, 300, 100, 0, 1, P, P, P, P, N), (5,)),
+             ("HcclAmdBlockQuantColumns", (P, BF16, 600, 100, 0, 4, P, 1, P, 1024, P, N), (4,)),
+             ("HcclAmdBlockMatmul", (P, 0, P, 0, 50, 4, P, None, P, P, 4, 100, 300, 1, P, BF16, 0, N), (1, 3, 16))]
+    for fn, args, at in calls:
+        for i in at:
+            assert args[i] == 0
+            assert getattr(H.lib(), fn)(*args[:i], stride, *args[i + 1:]) == PARA, (fn, i)
+
+
 def test_grad_weight_refuses_groups_without_weights():
     """Group g uses weights g: more groups than weights are refused, as the product refuses them."""
     for fn, args in (("HcclAmdBlockMatmulGradWeight", (P, P, P, P, 1024, 50, 100, 300, 1, 5, P, None, 4, P, BF16, 0, N)),
