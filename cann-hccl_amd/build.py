@@ -100,7 +100,8 @@ def build_ranks(force=False):
     hands it and is linked against nothing.  An accelerator only: where it cannot
     be built (no headers of the interpreter, say) the mirror calls through ctypes."""
     src = os.path.join(CSRC, "pyranks.cc")
-    if force or _newer(RANKS, [src]):
+    public = os.path.join(ROOT, "include", "hccl")
+    if force or _newer(RANKS, [src] + [os.path.join(public, f) for f in os.listdir(public)]):   # (it calls by their prototypes)
         try:
             _run(["g++", "-O2", "-std=c++17", "-fPIC", "-shared", "-Wall", "-I", os.path.join(ROOT, "include"),
                   "-I", sysconfig.get_paths()["include"], src, "-o", RANKS])

@@ -1,5 +1,6 @@
 """The experts' operators without a GPU: what they refuse, what they need, the 64-bit reference's gradients against differences."""
 import ctypes
+import importlib.util
 import os
 import re
 
@@ -246,3 +247,24 @@ def test_native_calls_and_ctypes_refuse_alike():
             assert H._expert(0, *args) == -1
         assert H._expert(9) == -1 and H._expert() == -1 and H._expert("0") == -1
         assert H._expert(0, ctypes.c_void_p(P), *refused[1:]) == PTR
+
+
+def test_native_module_is_built_again_when_a_prototype_changes(monkeypatch, tmp_path):
+    """It calls the library by the prototypes in the public headers: newer than the module, any of them has it compiled again."""
+    spec = importlib.util.spec_from_file_location("hccl_build_under_test", os.path.join(ROOT, "cann-hccl_amd", "build.py"))
+    build = importlib.util.module_from_spec(spec)
+    spec.loader.exec_module(build)
+    module, ran = tmp_path / "module.so", []
+    module.write_bytes(b"")
+    monkeypatch.setattr(build, "RANKS", str(module))
+    monkeypatch.setattr(build, "_run", ran.append)
+    times = {}
+    monkeypatch.setattr(build.os.path, "getmtime", lambda p: times.get(os.path.basename(p), 1.0))
+    times["module.so"] = 2.0
+    build.build_ranks()
+    assert not ran
+    for newer in ("pyranks.cc", "hccl_amd_experts.h", "hccl.h", "hccl_types.h"):
+        times[newer] = 3.0
+        build.build_ranks()
+        assert len(ran) == 1 and ran.pop()[0] == "g++", newer
+        del times[newer]
