@@ -155,6 +155,36 @@ def route_grad(r, topk, renorm, loss_scale, weight_grad, loss_grad):
     return out, size
 
 
+def route_finite(logits, topk, renorm, mask, loss_scale, weight_grad, loss_grad):
+    """route() and route_grad() for finite logits of many tokens, all tokens at once."""
+    T, E = logits.shape
+    live = np.ones((T, 1), bool) if mask is None else (mask != 0)[:, None]
+    pick = np.argsort(-logits, axis=1, kind="stable")[:, :topk]      # (of equal ones the lowest expert stays in front)
+    z = np.exp(logits - logits.max(1, keepdims=True))
+    p = np.where(live, z / z.sum(1, keepdims=True), 0)
+    chosen = np.take_along_axis(p, pick, 1)
+    inside = np.where(live, chosen.sum(1, keepdims=True), 1)
+    weights = chosen / inside if renorm else chosen
+    expert = np.where(live, pick, -1).astype(np.int32)
+    counts = np.concatenate([np.bincount(pick[live[:, 0]].reshape(-1), minlength=E), [live.sum()]])
+    rows, tokens = counts[:E].sum(), counts[E]
+    order = np.argsort(np.where(live, pick, E).reshape(-1), kind="stable")
+    row_of = np.empty(T * topk, np.int32)
+    row_of[order] = np.arange(T * topk)
+    row_of = np.where(live, row_of.reshape(T, topk), -1)
+    loss = loss_scale * E * float(np.sum(counts[:E] / rows * (p.sum(0) / tokens)))
+    g = np.broadcast_to(loss_grad * loss_scale * E * counts[:E] / rows / tokens, (T, E)).copy()
+    dw = np.where(live, weight_grad, 0)
+    if not renorm:
+        np.put_along_axis(g, pick, np.take_along_axis(g, pick, 1) + dw, 1)
+    grad = p * (g - (p * g).sum(1, keepdims=True))
+    size = p * (np.abs(g) + (p * np.abs(g)).sum(1, keepdims=True))
+    if renorm:
+        for to, d in ((grad, weights * (dw - (weights * dw).sum(1, keepdims=True))), (size, weights * (np.abs(dw) + (weights * np.abs(dw)).sum(1, keepdims=True)))):
+            np.put_along_axis(to, pick, np.take_along_axis(to, pick, 1) + d, 1)
+    return {"expert": expert, "weights": weights, "row_of": row_of, "counts": counts, "offsets": np.concatenate([[0], np.cumsum(counts[:E])]), "loss": loss}, grad, size
+
+
 # ---- bounds ------------------------------------------------------------------------------------------------------------------
 
 def close(got, want, bound, dtype=torch.float32):

@@ -184,6 +184,23 @@ def test_reference_route_gradient_against_differences(tokens, experts, topk, ren
             assert abs(slope - got[t, e]) < 1e-8 * (1 + np.abs(dw).sum())
 
 
+@pytest.mark.parametrize("renorm", [False, True])
+@pytest.mark.parametrize("masked", [False, True])
+def test_reference_of_many_tokens_is_the_reference(renorm, masked):
+    rng = np.random.default_rng(21)
+    x = rng.integers(-4, 4, (60, 9)) * 0.5                   # ties everywhere, zeros of both signs
+    x[x == 0] *= rng.choice([-1.0, 1.0], (x == 0).sum())
+    mask = (rng.random(60) > 0.3).astype(np.uint8) if masked else None
+    dw, dl = rng.standard_normal((60, 4)), -0.7
+    want = ref.route(x, 4, renorm, mask, 0.3)
+    grad, size = ref.route_grad(want, 4, renorm, 0.3, dw, dl)
+    got, got_grad, got_size = ref.route_finite(x, 4, renorm, mask, 0.3, dw, dl)
+    for k in ("expert", "row_of", "counts", "offsets"):
+        assert np.array_equal(got[k], want[k]), k
+    for a, b in ((got["weights"], want["weights"]), (got["loss"], want["loss"]), (got_grad, grad), (got_size, size)):
+        assert np.allclose(a, b, rtol=1e-13, atol=1e-15)
+
+
 def test_reference_scales():
     """The least power of two that brings a maximum to 448 or below, at the powers' edges; floats next to them."""
     tops = []

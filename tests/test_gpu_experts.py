@@ -143,6 +143,32 @@ def test_route_large(stream):
     assert all(np.array_equal(got[k], again[k]) for k in got) and np.array_equal(grad, grad2)
 
 
+@pytest.mark.parametrize("dtype", ["fp32", "bf16", "fp16"])
+@pytest.mark.parametrize("tokens,experts,topk", [(4200, 127, 7), (4200, 256, 8), (5000, 200, 16), (4500, 65, 2), (6000, 256, 3), (4300, 30, 16), (5000, 64, 8),
+                                                 (70000, 16, 2), (140000, 8, 1), (66000, 256, 8), (17000, 300, 3), (40000, 1024, 4)])
+def test_route_many_tokens(stream, dtype, tokens, experts, topk):
+    """Beyond 4096 tokens, four lanes to a token, with up to 64 experts a lane and lists of every length; beyond 65536 (with more than 256 experts
+    16384) workgroups of several tiles each."""
+    rng = np.random.default_rng(tokens + experts)
+    t = TYPE[dtype]
+    for renorm in (False, True):
+        print("route", dtype, tokens, experts, topk, renorm, flush=True)
+        logits = torch.from_numpy((2 * rng.standard_normal((tokens, experts)) + rng.standard_normal(experts)).astype(np.float32)).to(t)
+        mask = (rng.random(tokens) > 0.2).astype(np.uint8) if renorm else None
+        dw, dl = rng.standard_normal((tokens, topk)).astype(np.float32), 1.25
+        got, grad = run_route(stream, logits, topk, renorm, mask, dw=dw, dl=dl)
+        x = logits.double().numpy()
+        r, want, size = ref.route_finite(x, topk, renorm, mask, 0.01, dw.astype(np.float64), dl)
+        for k in ("expert", "row_of"):
+            assert np.array_equal(got[k], r[k]), k
+        assert np.array_equal(got["counts"][0], r["counts"]) and np.array_equal(got["offsets"][0], r["offsets"])
+        # (as for few tokens: exp's argument, the sum over the experts, the quotient; the loss adds up the tokens as well)
+        rel = (2 * (x.max(1) - x.min(1)).max() + experts + 10) * U
+        assert close(got["weights"], r["weights"], 2 * rel * np.abs(r["weights"]) + 1e-37)
+        assert close(got["loss"][0], [r["loss"]], (rel + (tokens + 2 * experts + 10) * U) * abs(r["loss"]))
+        assert close(grad, want, (4 * rel + 8 * U) * size + 1e-37, t)
+
+
 @pytest.mark.parametrize("dtype", ["fp32", "bf16"])
 @pytest.mark.parametrize("stride,shift", [(0, 1), (61, 0), (64, 3), (72, 0)])
 def test_route_strides(stream, dtype, stride, shift):
@@ -183,6 +209,32 @@ def test_route_masked_places(stream, dtype, renorm):
     # nobody takes part: zeros
     got, grad = run_route(stream, logits, 4, renorm, np.zeros(80, np.uint8), dw=dw, dl=dl)
     assert not got["counts"].any() and not got["offsets"].any() and not got["loss"].any() and not grad.any() and (got["row_of"] == -1).all()
+
+
+@pytest.mark.parametrize("renorm", [False, True])
+@pytest.mark.parametrize("dtype", ["fp32", "bf16", "fp16"])
+@pytest.mark.parametrize("experts", [20, 127])
+def test_route_masked_places_of_many_tokens(stream, dtype, renorm, experts):
+    """The same in the form for many tokens: masked tokens of NaN and infinities, rows of few experts, of none, of the type's lowest value."""
+    t, T = TYPE[dtype], 4200
+    rng = np.random.default_rng(experts)
+    logits = torch.from_numpy(rng.standard_normal((T, experts))).to(t)
+    mask = np.ones(T, np.uint8)
+    for i, v in ((0, float("nan")), (64, float("inf")), (2000, -float("inf")), (T - 1, float("nan"))):
+        logits[i] = v
+        mask[i] = 0
+    logits[1] = -float("inf")
+    logits[2] = -float("inf")
+    logits[2, 3] = 0.5
+    logits[3] = torch.finfo(t).min
+    logits[4, :] = torch.finfo(t).min
+    logits[4, 5] = 1.0
+    logits[T - 2] = -float("inf")
+    logits[T - 2, experts - 2:] = 0.0
+    dw, dl = rng.standard_normal((T, 4)).astype(np.float32), 1.0
+    got, grad = run_route(stream, logits, 4, renorm, mask, dw=dw, dl=dl)
+    assert np.isfinite(got["loss"]).all() and np.isfinite(grad).all()
+    check_route(logits, 4, renorm, mask, got, grad, dw, dl)
 
 
 @pytest.mark.parametrize("dtype", ["fp32", "bf16", "fp16"])
