@@ -99,7 +99,7 @@ __device__ __forceinline__ void StoreFour(T *out, const float (&v)[4], int col, 
 // 16 kRF rows by 16 kCF columns of the result to a workgroup, whose kWaves waves share the blocks out among them, kAhead at a time, and
 // add up through LDS: for few rows, where the weights' bytes are what takes time and as many waves as possible should be reading
 // them, all they need next at once.  8 rows at 8 of 64 experts by 4096 x 2048 (67 MB of weights): 13.3 us, 5.0 TB/s, what a copy
-// reaches; one row by 4096 x 8192 (34 MB): 9 us.
+// reaches; one row by 4096 x 8192 (34 MB): 8 us.
 template <typename T, HcclAmdScaleType kScale, int kRF, int kCF, int kWaves, int kAhead>
 __global__ void __launch_bounds__(64 * kWaves) FewRowsKernel(ProductArgs a)
 {
@@ -315,12 +315,12 @@ __device__ __forceinline__ uint32_t ScaleBits(uint8_t s) { return s; }
 // registers.  The 16-byte pieces of a row lie in LDS in an order that depends on the row (piece p of row r at p ^ (r / 2 % 8)), so that the
 // 16 rows a lane group reads are in different banks; since such a load fills LDS in lane order, it is the lanes' addresses
 // in memory that are swapped.  Scales pass through a register of one thread each.
-// Bound by the matrix unit together with the vector unit: 128 x 128 to a workgroup of four waves takes 128 conversions and, with 32-bit
+// Bound by the matrix unit and the vector unit together: 128 x 128 to a workgroup of four waves takes 128 conversions and, with 32-bit
 // scales, 80 multiplications and sums a wave and step, for 64 products.  256 x 256 to eight waves takes 192 for 128 and all there is of LDS and
-// registers.  Measured: 8192 x 4096 x 8192, scales of powers of two, 256 x 256: 380 us (1.45 PFLOP/s; a library's 16-bit product reaches 1.44),
-// 128 x 128: 443; 32-bit scales 456 (1.2), where 256 x 256 takes 480.  32768 rows of 64 experts by 4096 x 2048, 32-bit scales: 566 us (0.97), a
-// fifth of it tiles that are not full.  The weights' gradient of 16 experts, 16411 rows, 2048 x 4096: 335 us (0.82), of which its 0.5 GB of
-// results take 100.
+// registers.  Measured: 8192 x 4096 x 8192, scales of powers of two, 256 x 256: 383 us (1.44 PFLOP/s, what a library's 16-bit product reaches;
+// matrix unit busy 65 % of the time, vector unit 49 %), 128 x 128: 443; 32-bit scales 456 (1.2), where 256 x 256 takes 480.  32768 rows of 64 experts by
+// 4096 x 2048, 32-bit scales: 563 us (0.98; 49 and 57 %), a ninth of it tiles that are not full.  The weights' gradient of 16 experts, 16411 rows,
+// 2048 x 4096: 337 us (0.82; 37 and 55 %), of which its 0.5 GB of results take 100; added to what is there, 577.
 // (Two waves to a SIMD are asked for: with the registers of one the compiler keeps products apart from what it computes with.)
 // kGrad: the weights' gradient, scales by column too.
 template <typename T, HcclAmdScaleType kScale, bool kGrad, int kRF, int kCF, int kWR, int kWC>

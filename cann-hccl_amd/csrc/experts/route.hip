@@ -14,8 +14,10 @@
 // rows (up to 512 tokens the third does both).  Up to 64 tokens (a decoding step) one launch does it all.
 //
 // Measured: 65536 tokens of 256 experts, eight chosen, 16-bit logits (33.5 MB): 21 us to choose, 7 to add up, 5 for the rows, 20 for the
-// gradient (67 MB).  Choosing is bound by instructions (64 logits a lane, eight medians each), not by the 7 us its bytes take; the
-// rest by the latency of few dependent accesses.  One token: 7 us, the latency of one wave's way through the code.
+// gradient (67 MB); 32-bit logits 49 us in all and 26 for the gradient.  Choosing is bound by vector instructions (their unit is busy 88 % of the
+// time), not by the 7 us its bytes take: 64 logits a lane, 35 instructions each, of which the eight medians are less than a quarter; the others map
+// values, take exponentials and add up.  The gradient keeps that unit busy 56 % of the time and waits on one chain of dependent steps a token; the
+// rest is the latency of few dependent accesses.  One token: 7 us, the latency of one wave's way through the code.
 #include <type_traits>
 
 #include "common.h"

@@ -56,7 +56,7 @@ extern HcclResult HcclAmdExpertRouteWorkspace(uint64_t tokens, uint32_t experts,
  *   offsets[experts + 1]          first row of every expert; at [experts] the number of rows
  *   loss[1]                       lossScale * experts * sum over e of (counts[e] / rows) * (sum of the probabilities of e / tokens that chose);
  *                                 0 without rows
- * A NaN or +inf logit of a token that takes part makes its probabilities, and with them the loss, NaN, as the formula has it.
+ * A NaN or +inf logit of a token that chose any makes all its probabilities, and with them its weights and the loss, NaN, as the formula has it.
  * topK <= experts.  workspace: 16-byte aligned, HcclAmdExpertRouteWorkspace bytes, free for other use once the stream is past the call. */
 extern HcclResult HcclAmdExpertRoute(const void *logits, HcclDataType logitType, uint64_t tokens, uint32_t experts, uint64_t logitStride,
     uint32_t topK, uint32_t renormalise, const uint8_t *tokenMask, float lossScale, int32_t *expertOf, float *weights, int32_t *rowOf,
