@@ -576,14 +576,14 @@ HcclResult Choose(HcclDataType type, HcclAmdScaleType scaleType, F f)
 constexpr uint64_t kMostTiles = uint64_t(1) << 22;   // workgroups of up to 512 below 2^32 threads
 
 // What a product takes in each form, in microseconds: `call`, and for every 256 workgroups, one to a compute unit, `round` and `block` times the
-// blocks of 128 along its sums.  The form that should take least is taken.  The figures are least squares of relative errors over 616 products:
-// 1, 4, 16, 60, 128 groups, 4 to 12000 rows, 300 to 7168 columns, sums of 300 to 8192, and 260 of 1, 8 and 64 groups by 512 to 14336.  What is taken so is
-// 1.4 % slower than the fastest of all on average, in 9 of 876 by more than a quarter.  For instance, columns x sum, us in the order below:
+// blocks of 128 along its sums.  The form that should take least is taken.  The figures are least squares of the relative errors, rounded, over 876
+// products: 1 to 128 groups, 1 to 12000 rows, 300 to 14336 columns, sums of 300 to 8192 values (256 x 256: over 28).  What is taken so is
+// 1.4 % slower than the fastest of all on average, in 9 of the 876 by more than a quarter.  For instance, columns x sum, us in the order below:
 //   one group     4096 x 8192:    1 row    8   20   22   58;   64 rows  38   24   31   60;   256 rows 142   81   54   68;   2048 rows  -   -   -  126
 //                 1408 x 2048:    4 rows   6    7    7   17;   96 rows  16    9   10   19;   800 rows  82   30   24   20
 //   64 groups     4096 x 2048:    8 rows  21   13   14   19;   60 groups, 1408 x 2048: 800 rows 105 42 37 41, 1500 rows 177 64 49 41
 //   256 x 256 against 128 x 128, scales of powers of two, 4096 columns: 2048 rows x 8192 177 and 119, 4096 rows x 8192 190 and 228, 8192 rows x 1024 59
-//                 and 63, x 512 36 and 35.  With 32-bit scales the larger is never faster (8192 x 4096 x 8192: 480 and 444).
+//                 and 63, x 512 36 and 35.  With 32-bit scales the larger is 2 % faster at best, mostly slower (8192 x 4096 x 8192: 480 and 444).
 struct Form {
     uint32_t rows, cols;
     double call, round, block;
