@@ -35,6 +35,8 @@ ALGO_RING, ALGO_MESH, ALGO_RHD, ALGO_PAIRWISE = range(4)
 HCCL_DATA_TYPE_FP8E4M3 = 14          # 8-bit rows of the experts' operators; refused by every collective
 # HcclAmdScaleType (include/hccl/hccl_amd_experts.h)
 HCCL_AMD_SCALE_NONE, HCCL_AMD_SCALE_FP32, HCCL_AMD_SCALE_E8M0 = 0, 1, 2
+# HcclAmdScore
+HCCL_AMD_SCORE_SOFTMAX, HCCL_AMD_SCORE_SIGMOID = 0, 1
 
 # Every symbol include/hccl/hccl.h and include/hccl/hccl_amd_ext.h declare.
 EXPORTS = [
@@ -51,7 +53,15 @@ EXPORTS = [
 EXPERT_EXPORTS = [
     "HcclAmdExpertRouteWorkspace", "HcclAmdExpertRoute", "HcclAmdExpertRouteGrad", "HcclAmdExpertPack", "HcclAmdExpertCombine",
     "HcclAmdExpertCombineGrad", "HcclAmdBlockQuantWeights", "HcclAmdBlockQuantColumns", "HcclAmdBlockMatmul", "HcclAmdBlockMatmulGradWeight",
+    "HcclAmdNormRows", "HcclAmdNormRowsGrad", "HcclAmdExpertGate", "HcclAmdExpertGateGrad", "HcclAmdExpertRouteScored", "HcclAmdExpertRouteScoredGrad",
+    "HcclAmdExpertBias", "HcclAmdGradSquares", "HcclAmdGradClip",
+    "HcclAmdNormRowsGradWorkspace", "HcclAmdExpertRouteScoredWorkspace", "HcclAmdGradSquaresWorkspace",
 ]
+_EXPERT_CALLS = EXPERT_EXPORTS[1:-3]     # those that queue work, in the order of csrc/pyranks.cc
+
+
+class HcclAmdGradTensor(ctypes.Structure):
+    _fields_ = [("in_", ctypes.c_void_p), ("out", ctypes.c_void_p), ("count", ctypes.c_uint64), ("type", ctypes.c_int32), ("reserved", ctypes.c_uint32)]
 
 
 class HcclAmdOpInfo(ctypes.Structure):
@@ -212,6 +222,18 @@ def lib():
     L.HcclAmdBlockQuantColumns.argtypes = [vp, i32, u64, u64, u64, u32, vp, i32, vp, u64, vp, vp]
     L.HcclAmdBlockMatmul.argtypes = [vp, u64, vp, u64, u64, u32, vp, vp, vp, vp, u32, u64, u64, i32, vp, i32, u64, vp]
     L.HcclAmdBlockMatmulGradWeight.argtypes = [vp, vp, vp, vp, u64, u64, u64, u64, i32, u32, vp, vp, u32, vp, i32, u32, vp]
+    L.HcclAmdNormRows.argtypes = [vp, i32, u64, u64, u64, vp, u64, vp, i32, f32, vp, u64, vp, u64, i32, vp, u64, vp, u64, vp]
+    L.HcclAmdNormRowsGradWorkspace.argtypes = [u64, u64, ctypes.POINTER(u64)]
+    L.HcclAmdNormRowsGrad.argtypes = [vp, u64, vp, i32, u64, u64, u64, vp, i32, f32, vp, u64, vp, u64, vp, u32, vp, u64, vp]
+    L.HcclAmdExpertGate.argtypes = [vp, i32, u64, u64, u64, vp, i32, vp, u64, vp, u64, vp]
+    L.HcclAmdExpertGateGrad.argtypes = [vp, u64, vp, i32, u64, u64, u64, vp, vp, u64, vp, u64, vp]
+    L.HcclAmdExpertRouteScoredWorkspace.argtypes = [u64, u32, ctypes.POINTER(u64)]
+    L.HcclAmdExpertRouteScored.argtypes = [vp, i32, u64, u32, u64, i32, vp, u32, u32, u32, u32, u32, f32, vp, vp, vp, vp, vp, vp, vp, u64, vp]
+    L.HcclAmdExpertRouteScoredGrad.argtypes = [vp, i32, u64, u32, u64, i32, u32, u32, f32, vp, vp, vp, u64, vp]
+    L.HcclAmdExpertBias.argtypes = [vp, u32, f32, vp, vp, vp]
+    L.HcclAmdGradSquaresWorkspace.argtypes = [vp, u32, ctypes.POINTER(u64)]
+    L.HcclAmdGradSquares.argtypes = [vp, u32, u32, vp, vp, u64, vp]
+    L.HcclAmdGradClip.argtypes = [vp, u32, vp, f32, vp, vp]
     ranks = _native_ranks(L)
     _call, _expert = (ranks.call, ranks.expert) if ranks else (_through_ctypes, _through_ctypes)
     _lib = L
@@ -237,7 +259,7 @@ def _native_ranks(L):
     except ImportError:
         return None
     ranks.bind(tuple(ctypes.cast(getattr(L, name), ctypes.c_void_p).value for name in _KINDS))
-    ranks.bind_experts(tuple(ctypes.cast(getattr(L, name), ctypes.c_void_p).value for name in EXPERT_EXPORTS[1:]))
+    ranks.bind_experts(tuple(ctypes.cast(getattr(L, name), ctypes.c_void_p).value for name in _EXPERT_CALLS))
     return ranks
 
 
@@ -262,12 +284,12 @@ _expert = _load_and_expert
 
 
 def _expert_call(kind, *args):
-    """One experts' operator, EXPERT_EXPORTS[kind + 1]."""
+    """One experts' operator, _EXPERT_CALLS[kind]."""
     code = _expert(kind, *args)
     if code == -1:
-        code = getattr(lib(), EXPERT_EXPORTS[kind + 1])(*args)
+        code = getattr(lib(), _EXPERT_CALLS[kind])(*args)
     if code != HCCL_SUCCESS:
-        raise HcclError(EXPERT_EXPORTS[kind + 1], code)
+        raise HcclError(_EXPERT_CALLS[kind], code)
 
 
 class HcclError(RuntimeError):
@@ -558,3 +580,85 @@ def block_matmul_grad_weight(y_grad_t, y_grad_scales, x_t, x_scales, columns, ro
                              stream, expert_of_group=None, accumulate=False):
     _expert_call(8, y_grad_t, y_grad_scales, x_t, x_scales, columns, rows, n, k, scale_type, groups, offsets, expert_of_group, experts, w_grad,
                  grad_dtype, 1 if accumulate else 0, stream)
+
+
+def norm_rows(x, dtype, rows, width, stream, residual=None, gain=None, gain_dtype=HCCL_DATA_TYPE_FP32, epsilon=1e-6, sum=None, y=None,
+              scale_type=HCCL_AMD_SCALE_NONE, q=None, scales=None, x_stride=0, residual_stride=0, sum_stride=0, y_stride=0, q_stride=0, scale_stride=0):
+    """Rows and their residual, normed by their root mean square: the sum, y in the rows' type, y as 8-bit rows (scale_type)."""
+    _expert_call(9, x, dtype, rows, width, x_stride, residual, residual_stride, gain, gain_dtype, epsilon, sum, sum_stride, y, y_stride, scale_type, q,
+                 q_stride, scales, scale_stride, stream)
+
+
+def norm_rows_grad_workspace(rows, width):
+    """Bytes of device workspace norm_rows_grad needs for a gain's gradient."""
+    need = ctypes.c_uint64()
+    _check("HcclAmdNormRowsGradWorkspace", lib().HcclAmdNormRowsGradWorkspace(rows, width, ctypes.byref(need)))
+    return need.value
+
+
+def norm_rows_grad(y_grad, sum, dtype, rows, width, x_grad, stream, gain=None, gain_dtype=HCCL_DATA_TYPE_FP32, epsilon=1e-6, sum_grad=None, gain_grad=None,
+                   accumulate=False, workspace=None, workspace_bytes=0, y_grad_stride=0, sum_stride=0, sum_grad_stride=0, x_grad_stride=0):
+    """Gradients of norm_rows, from the sum that it left (x, if there was no residual)."""
+    _expert_call(10, y_grad, y_grad_stride, sum, dtype, rows, width, sum_stride, gain, gain_dtype, epsilon, sum_grad, sum_grad_stride, x_grad, x_grad_stride,
+                 gain_grad, 1 if accumulate else 0, workspace, workspace_bytes, stream)
+
+
+def expert_gate(h, dtype, rows, width, out, stream, used=None, scale_type=HCCL_AMD_SCALE_NONE, scales=None, h_stride=0, out_stride=0, scale_stride=0):
+    """silu(gate) * up of h[rows, 2 * width], in h's type or (scale_type) as 8-bit rows; used: how many rows there are, on the device."""
+    _expert_call(11, h, dtype, rows, width, h_stride, used, scale_type, out, out_stride, scales, scale_stride, stream)
+
+
+def expert_gate_grad(out_grad, h, dtype, rows, width, h_grad, stream, used=None, out=None, out_grad_stride=0, h_stride=0, h_grad_stride=0, out_stride=0):
+    """Gradient of expert_gate, and (out) its result once more."""
+    _expert_call(12, out_grad, out_grad_stride, h, dtype, rows, width, h_stride, used, h_grad, h_grad_stride, out, out_stride, stream)
+
+
+def expert_route_scored_workspace(tokens, experts):
+    """Bytes of device workspace expert_route_scored needs."""
+    need = ctypes.c_uint64()
+    _check("HcclAmdExpertRouteScoredWorkspace", lib().HcclAmdExpertRouteScoredWorkspace(tokens, experts, ctypes.byref(need)))
+    return need.value
+
+
+def expert_route_scored(logits, dtype, tokens, experts, topk, score, expert_of, weights, row_of, counts, offsets, workspace, workspace_bytes, stream,
+                        bias=None, groups=1, groups_kept=1, group_top=2, renorm=False, weight_scale=1.0, mask=None, stride=0):
+    """The topk experts of every token by softmax or sigmoid scores and a bias, out of its best groups, their weights, rows in expert order, counts."""
+    _expert_call(13, logits, dtype, tokens, experts, stride, score, bias, groups, groups_kept, group_top, topk, 1 if renorm else 0, weight_scale, mask,
+                 expert_of, weights, row_of, counts, offsets, workspace, workspace_bytes, stream)
+
+
+def expert_route_scored_grad(logits, dtype, tokens, experts, topk, score, expert_of, weight_grad, logit_grad, stream, renorm=False, weight_scale=1.0,
+                             stride=0, grad_stride=0):
+    _expert_call(14, logits, dtype, tokens, experts, stride, score, topk, 1 if renorm else 0, weight_scale, expert_of, weight_grad, logit_grad, grad_stride,
+                 stream)
+
+
+def expert_bias(counts, experts, rate, bias, new_bias, stream):
+    """A step of the bias towards equal counts; new_bias may be bias."""
+    _expert_call(15, counts, experts, rate, bias, new_bias, stream)
+
+
+def grad_tensors(tensors):
+    """The list that grad_squares and grad_clip take, from (in, out, count, dtype) of every tensor; out may be in, or None for grad_squares alone."""
+    return (HcclAmdGradTensor * len(tensors))(*[HcclAmdGradTensor(a, b, n, t, 0) for a, b, n, t in tensors])
+
+
+def _address(tensors):
+    return ctypes.addressof(tensors) if isinstance(tensors, ctypes.Array) else tensors
+
+
+def grad_squares_workspace(tensors, n):
+    """Bytes of device workspace grad_squares needs for these tensors."""
+    need = ctypes.c_uint64()
+    _check("HcclAmdGradSquaresWorkspace", lib().HcclAmdGradSquaresWorkspace(_address(tensors), n, ctypes.byref(need)))
+    return need.value
+
+
+def grad_squares(tensors, n, squares, workspace, workspace_bytes, stream, accumulate=False):
+    """The sum of the squares of all tensors' elements, in 64 bits (added to what is there with accumulate).  tensors: grad_tensors(), or its address."""
+    _expert_call(16, _address(tensors), n, 1 if accumulate else 0, squares, workspace, workspace_bytes, stream)
+
+
+def grad_clip(tensors, n, squares, max_norm, norm, stream):
+    """Every tensor's out from its in, times max_norm / sqrt(squares) where that is below 1; the norm (None: not wanted)."""
+    _expert_call(17, _address(tensors), n, squares, max_norm, norm, stream)

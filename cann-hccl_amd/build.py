@@ -27,8 +27,8 @@ COMMON = ["-O3", "-std=c++17", "-fPIC", "-ffp-contract=off", "-I", os.path.join(
 DEVICE = ["--offload-arch=gfx950", "-Xclang", "-target-feature", "-Xclang", "-packed-fp32-ops"]
 DTYPES = list(range(12)) + [255]
 DEVICE_SOURCES = ["noalloc.hip"]
-# the operators around the all-to-all-v: a directory of their own, with headers that nothing else reads
-EXPERT_SOURCES = ["route.hip", "exchange.hip", "quant.hip", "product.hip"]
+# the operators around the all-to-all-v and the training step: a directory of their own, with headers that nothing else reads
+EXPERT_SOURCES = ["route_scored.hip", "route.hip", "norm.hip", "exchange.hip", "quant.hip", "product.hip", "gate.hip", "clip.hip"]
 EXPERT_HEADER = "hccl_amd_experts.h"
 HOST_SOURCES = ["plan.cc", "plan_schedules.cc", "plan_lower.cc", "plan_fuse.cc", "plan_template.cc", "ranktable.cc", "exec.cc", "direct.cc", "a2av.cc", "api.cc", "api_rendezvous.cc", "api_comm.cc", "api_ext.cc", "kernels_table.cc"]
 

@@ -1,0 +1,346 @@
+// Gradients of many tensors held to a norm over all of them: HcclAmdGradSquares, HcclAmdGradClip.
+//
+// The tensors' table rides in the kernel arguments, kTensors to a launch; tensors are cut into chunks, counted over the table, and a workgroup finds its
+// chunk's tensor by halving.  Chunks start at 16-byte boundaries of the input, so that every load inside a tensor is aligned whatever its first
+// element is.  Squares are added up in 64 bits: those of 32 bits are exact there, and neither 1e30 nor 1e-30 leaves the range.  A workgroup's sum has
+// its own place in the workspace and a second launch adds the places up in their order: same inputs, same bits.
+#include <type_traits>
+
+#include "sums.h"
+
+namespace hcclamd {
+namespace experts {
+namespace {
+
+constexpr int kThreads = 256;
+constexpr int kEach = 8;                           // neighbouring elements of a lane
+constexpr int kChunk = 16384;                      // elements
+constexpr int kTensors = 120;                      // of a launch: 3840 of the 4096 bytes that arguments may take
+constexpr int kMostSlots = 2048;                   // workgroups of a launch that adds up: eight to a compute unit
+constexpr uint32_t kMaxTensors = 1u << 24;         // of a list: its places are counted in 32 bits
+constexpr uint64_t kMaxCount = uint64_t(1) << 37;  // elements of a tensor; the chunks of a launch are counted in 32 bits
+
+struct Tensor {
+    const void *in;       // moved down to a 16-byte boundary,
+    void *out;            // and as many elements here
+    int64_t last;         // elements from there to the tensor's end
+    int32_t chunk;        // its first chunk's number
+    int16_t type;
+    int16_t lead;         // elements in front of the tensor's first
+};
+static_assert(sizeof(Tensor) == 32, "32 bytes a tensor");
+
+struct Table {
+    Tensor tensor[kTensors];
+    int32_t n, chunks;
+};
+
+__device__ __forceinline__ int Find(const Table &t, int chunk)
+{
+    int lo = 0, hi = t.n;      // tensor[lo].chunk <= chunk < tensor[hi].chunk
+    while (hi - lo > 1) {
+        const int mid = (lo + hi) / 2;
+        if (t.tensor[mid].chunk <= chunk) {
+            lo = mid;
+        } else {
+            hi = mid;
+        }
+    }
+    return lo;
+}
+
+template <typename T>
+__device__ __forceinline__ double Squares(const Tensor &t, int chunk)
+{
+    constexpr int kParts = kChunk / (kThreads * kEach);
+    const T *in = static_cast<const T *>(t.in);
+    const int64_t from = int64_t(chunk - t.chunk) * kChunk;
+    float v[kParts][kEach];
+    if (from >= t.lead && from + kChunk <= t.last) {
+#pragma unroll
+        for (int p = 0; p < kParts; p++) {
+            Load<true, kEach>(in + from + (p * kThreads + int(threadIdx.x)) * kEach, v[p]);
+        }
+    } else {
+#pragma unroll
+        for (int p = 0; p < kParts; p++) {
+            const int64_t at = from + (p * kThreads + int(threadIdx.x)) * kEach;
+            if (at >= t.lead && at + kEach <= t.last) {
+                Load<true, kEach>(in + at, v[p]);
+            } else {
+#pragma unroll
+                for (int i = 0; i < kEach; i++) {
+                    v[p][i] = at + i >= t.lead && at + i < t.last ? float(in[at + i]) : 0.0f;
+                }
+            }
+        }
+    }
+    double sum[2] = {0.0, 0.0};
+#pragma unroll
+    for (int p = 0; p < kParts; p++) {
+#pragma unroll
+        for (int i = 0; i < kEach; i++) {
+            sum[i % 2] = __builtin_fma(double(v[p][i]), double(v[p][i]), sum[i % 2]);
+        }
+    }
+    return sum[0] + sum[1];
+}
+
+__global__ void __launch_bounds__(kThreads) SquaresKernel(Table t, double *slots)
+{
+    __shared__ double parts[kThreads / 64];
+    double sum = 0.0;
+    for (int chunk = blockIdx.x; chunk < t.chunks; chunk += gridDim.x) {
+        const Tensor &of = t.tensor[Find(t, chunk)];
+        switch (of.type) {
+            case HCCL_DATA_TYPE_FP32:
+                sum += Squares<float>(of, chunk);
+                break;
+            case HCCL_DATA_TYPE_FP16:
+                sum += Squares<_Float16>(of, chunk);
+                break;
+            default:
+                sum += Squares<__bf16>(of, chunk);
+                break;
+        }
+    }
+    sum = AddWave(sum);
+    if (threadIdx.x % 64 == 0) {
+        parts[threadIdx.x / 64] = sum;
+    }
+    __syncthreads();
+    if (threadIdx.x == 0) {
+        slots[blockIdx.x] = (parts[0] + parts[1]) + (parts[2] + parts[3]);
+    }
+}
+
+__global__ void __launch_bounds__(1024) AddSlotsKernel(const double *slots, int n, double *squares, bool accumulate)
+{
+    __shared__ double parts[1024 / 64];
+    double sum = 0.0;
+#pragma unroll 4
+    for (int i = threadIdx.x; i < n; i += 1024) {
+        sum += slots[i];
+    }
+    sum = AddWave(sum);
+    if (threadIdx.x % 64 == 0) {
+        parts[threadIdx.x / 64] = sum;
+    }
+    __syncthreads();
+    if (threadIdx.x == 0) {
+        sum = accumulate ? squares[0] : 0.0;
+#pragma unroll
+        for (int i = 0; i < 1024 / 64; i++) {
+            sum += parts[i];
+        }
+        squares[0] = sum;
+    }
+}
+
+template <typename T>
+__device__ __forceinline__ void Scale(const Tensor &t, int chunk, float by)
+{
+    constexpr int kParts = kChunk / (kThreads * kEach);
+    const T *in = static_cast<const T *>(t.in);
+    T *out = static_cast<T *>(t.out);
+    const int64_t from = int64_t(chunk - t.chunk) * kChunk;
+    const bool aligned = reinterpret_cast<uintptr_t>(out) % 16 == 0;
+    if (from >= t.lead && from + kChunk <= t.last) {
+        float v[kParts][kEach];
+#pragma unroll
+        for (int p = 0; p < kParts; p++) {
+            Load<true, kEach>(in + from + (p * kThreads + int(threadIdx.x)) * kEach, v[p]);
+        }
+#pragma unroll
+        for (int p = 0; p < kParts; p++) {
+            const int64_t at = from + (p * kThreads + int(threadIdx.x)) * kEach;
+#pragma unroll
+            for (int i = 0; i < kEach; i++) {
+                v[p][i] *= by;
+            }
+            if (aligned) {
+                Store<true, kEach>(out + at, v[p]);
+            } else {
+                Store<false, kEach>(out + at, v[p]);
+            }
+        }
+        return;
+    }
+    for (int p = 0; p < kParts; p++) {
+        const int64_t at = from + (p * kThreads + int(threadIdx.x)) * kEach;
+        if (at >= t.lead && at + kEach <= t.last) {
+            float v[kEach];
+            Load<true, kEach>(in + at, v);
+#pragma unroll
+            for (int i = 0; i < kEach; i++) {
+                v[i] *= by;
+            }
+            Store<false, kEach>(out + at, v);
+        } else {
+            for (int i = 0; i < kEach; i++) {
+                if (at + i >= t.lead && at + i < t.last) {
+                    out[at + i] = T(float(in[at + i]) * by);
+                }
+            }
+        }
+    }
+}
+
+// The first workgroup of the list's first launch (`norm` not null) leaves the norm.
+__global__ void __launch_bounds__(kThreads) ClipKernel(Table t, const double *squares, float maxNorm, float *norm)
+{
+    const double length = __builtin_sqrt(squares[0]);
+    if (norm != nullptr && blockIdx.x == 0 && threadIdx.x == 0) {
+        norm[0] = float(length);
+    }
+    const bool within = length <= double(maxNorm);        // (not so where the norm is NaN)
+    const float by = within ? 1.0f : float(double(maxNorm) / length);
+    for (int chunk = blockIdx.x; chunk < t.chunks; chunk += gridDim.x) {
+        const Tensor &of = t.tensor[Find(t, chunk)];
+        if (within && of.out == of.in) {
+            continue;
+        }
+        switch (of.type) {
+            case HCCL_DATA_TYPE_FP32:
+                Scale<float>(of, chunk, by);
+                break;
+            case HCCL_DATA_TYPE_FP16:
+                Scale<_Float16>(of, chunk, by);
+                break;
+            default:
+                Scale<__bf16>(of, chunk, by);
+                break;
+        }
+    }
+}
+
+HcclResult Check(const char *fn, const HcclAmdGradTensor *tensors, uint32_t n, bool write)
+{
+    for (uint32_t i = 0; i < n; i++) {
+        const HcclAmdGradTensor &t = tensors[i];
+        if (!Float(t.type)) {
+            HCCL_LOG_ERROR("%s: tensor %u: type not supported", fn, i);
+            return HCCL_E_NOT_SUPPORT;
+        }
+        if (t.count > kMaxCount || t.reserved != 0 || !AlignedTo(t.type, t.in) || (write && !AlignedTo(t.type, t.out))) {
+            HCCL_LOG_ERROR("%s: tensor %u: count or alignment", fn, i);
+            return HCCL_E_PARA;
+        }
+        if (t.count != 0 && (t.in == nullptr || (write && t.out == nullptr))) {
+            HCCL_LOG_ERROR("%s: tensor %u is null", fn, i);
+            return HCCL_E_PTR;
+        }
+    }
+    return HCCL_SUCCESS;
+}
+
+// The next launch's table, from tensor `at` on, which is moved behind it; false: there are no more elements.
+bool Next(const HcclAmdGradTensor *tensors, uint32_t n, uint32_t &at, Table &table)
+{
+    table.n = table.chunks = 0;
+    for (; at < n && table.n < kTensors; at++) {
+        const HcclAmdGradTensor &t = tensors[at];
+        if (t.count == 0) {
+            continue;
+        }
+        const uint64_t unit = SizeOf(t.type), lead = reinterpret_cast<uintptr_t>(t.in) % 16 / unit;
+        Tensor &to = table.tensor[table.n++];
+        to.in = reinterpret_cast<const void *>(reinterpret_cast<uintptr_t>(t.in) - lead * unit);
+        to.out = reinterpret_cast<void *>(reinterpret_cast<uintptr_t>(t.out) - lead * unit);
+        to.last = int64_t(t.count + lead);
+        to.chunk = table.chunks;
+        to.type = int16_t(t.type);
+        to.lead = int16_t(lead);
+        table.chunks += int32_t((t.count + lead + kChunk - 1) / kChunk);
+    }
+    return table.n != 0;
+}
+
+int Slots(const Table &t) { return t.chunks < kMostSlots ? t.chunks : kMostSlots; }
+
+}  // namespace
+}  // namespace experts
+}  // namespace hcclamd
+
+using namespace hcclamd::experts;
+
+extern "C" {
+
+HcclResult HcclAmdGradSquaresWorkspace(const HcclAmdGradTensor *tensors, uint32_t n, uint64_t *bytes)
+{
+    EXPERTS_CHK_PTR(bytes);
+    if (n != 0) {
+        EXPERTS_CHK_PTR(tensors);
+    }
+    const HcclResult r = Check(__func__, tensors, n, false);
+    if (r != HCCL_SUCCESS) {
+        return r;
+    }
+    uint64_t slots = 0;
+    Table table;
+    for (uint32_t at = 0; Next(tensors, n, at, table);) {
+        slots += uint64_t(Slots(table));
+    }
+    *bytes = slots * sizeof(double);
+    return HCCL_SUCCESS;
+}
+
+HcclResult HcclAmdGradSquares(const HcclAmdGradTensor *tensors, uint32_t n, uint32_t accumulate, double *squares, void *workspace,
+    uint64_t workspaceBytes, void *stream)
+{
+    EXPERTS_CHK_PTR(stream);
+    EXPERTS_CHK_PTR(squares);
+    EXPERTS_CHK(Aligned(squares, 8));
+    EXPERTS_CHK(n <= kMaxTensors);
+    uint64_t needed = 0;
+    const HcclResult checked = HcclAmdGradSquaresWorkspace(tensors, n, &needed);
+    if (checked != HCCL_SUCCESS) {
+        return checked;
+    }
+    if (needed != 0) {
+        EXPERTS_CHK_PTR(workspace);
+        EXPERTS_CHK(Aligned(workspace, 16));
+        EXPERTS_CHK(workspaceBytes >= needed);
+    }
+    const hipStream_t on = static_cast<hipStream_t>(stream);
+    double *slots = static_cast<double *>(workspace);
+    int used = 0;
+    Table table;
+    for (uint32_t at = 0; Next(tensors, n, at, table);) {
+        const HcclResult r = Launch("HcclAmdGradSquares", SquaresKernel, uint32_t(Slots(table)), kThreads, 0, on, table, slots + used);
+        if (r != HCCL_SUCCESS) {
+            return r;
+        }
+        used += Slots(table);
+    }
+    return Launch("HcclAmdGradSquares", AddSlotsKernel, 1, 1024, 0, on, static_cast<const double *>(slots), used, squares, accumulate != 0);
+}
+
+HcclResult HcclAmdGradClip(const HcclAmdGradTensor *tensors, uint32_t n, const double *squares, float maxNorm, float *norm, void *stream)
+{
+    EXPERTS_CHK_PTR(stream);
+    EXPERTS_CHK_PTR(squares);
+    EXPERTS_CHK(Aligned(squares, 8) && Aligned(norm, 4));
+    EXPERTS_CHK(maxNorm >= 0.0f);
+    if (n != 0) {
+        EXPERTS_CHK_PTR(tensors);
+    }
+    const HcclResult checked = Check(__func__, tensors, n, true);
+    if (checked != HCCL_SUCCESS) {
+        return checked;
+    }
+    Table table;
+    uint32_t at = 0;
+    while (Next(tensors, n, at, table) || norm != nullptr) {
+        // (no elements at all: the norm is left all the same)
+        const HcclResult r = Launch("HcclAmdGradClip", ClipKernel, uint32_t(table.chunks < 1 ? 1 : table.chunks < (1 << 20) ? table.chunks : 1 << 20), kThreads, 0,
+            static_cast<hipStream_t>(stream), table, squares, maxNorm, norm);
+        if (r != HCCL_SUCCESS) {
+            return r;
+        }
+        norm = nullptr;
+    }
+    return HCCL_SUCCESS;
+}
+
+}  // extern "C"

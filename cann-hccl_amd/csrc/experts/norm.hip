@@ -1,0 +1,496 @@
+// Rows and their residual, normed by their root mean square (HcclAmdNormRows), in their type and as 8-bit rows, and the gradient.
+//
+// With r = (mean s^2 + epsilon)^-1/2, d = dy * gain and n = s r:
+//   y = n * gain      dx = r (d - n mean(d n)) + dsum      dgain = sum over rows of dy * n
+//
+// A row stays in registers between its sums and its results: read once, written once.  64, 256, 512 or 1024 threads to a row, each with one, two or four
+// times eight neighbouring values, so that a lane's accesses are 16 bytes and 16 lanes hold a block of an 8-bit row.  Sums are in 64 bits: a
+// square of 32 bits is exact there, and no row overflows.
+#include <type_traits>
+
+#include "sums.h"
+
+namespace hcclamd {
+namespace experts {
+namespace {
+
+constexpr int kEach = 8;     // neighbouring values of a lane
+
+struct NormArgs {
+    const void *x, *residual, *gain;
+    void *sum, *y, *q, *scales;
+    int64_t xStride, residualStride, sumStride, yStride, qStride, scaleStride;
+    int64_t rows;
+    int width, padded;
+    float epsilon;
+    bool gain32;               // gain is in 32 bits, else in the rows' type
+    bool powers;               // the scales are powers of two
+};
+
+constexpr int BlockOf(int rowThreads) { return rowThreads < 256 ? 256 : rowThreads; }
+
+// The row's sum on all its threads.  `parts`: a place per wave, used by one call between two barriers.
+template <int kRowThreads>
+__device__ __forceinline__ double AddRow(double x, double *parts)
+{
+    x = AddWave(x);
+    if constexpr (kRowThreads > 64) {
+        if (threadIdx.x % 64 == 0) {
+            parts[threadIdx.x / 64] = x;
+        }
+        __syncthreads();
+        x = 0.0;
+#pragma unroll
+        for (int w = 0; w < kRowThreads / 64; w++) {
+            x += parts[w];
+        }
+    }
+    return x;
+}
+
+// gain[at ...], 1 where there is none.
+template <int kHow, typename T>
+__device__ __forceinline__ void LoadGain(const void *gain, bool gain32, int at, int width, float (&g)[kEach])
+{
+    if (gain == nullptr) {
+#pragma unroll
+        for (int i = 0; i < kEach; i++) {
+            g[i] = 1.0f;
+        }
+    } else if (gain32) {
+        LoadPart<kHow, kEach>(static_cast<const float *>(gain), at, width, g);
+    } else {
+        LoadPart<kHow, kEach>(static_cast<const T *>(gain), at, width, g);
+    }
+}
+
+template <HcclAmdScaleType kScale>
+__device__ __forceinline__ void StoreBlock(const float (&v)[kEach], float top, const NormArgs &a, int64_t row, int at)
+{
+    const BlockScale<kScale> scale(top);
+    float s[kEach];
+#pragma unroll
+    for (int i = 0; i < kEach; i++) {
+        s[i] = Scaled8(v[i], scale.times);
+    }
+    if (at < a.padded) {
+        *reinterpret_cast<Word2 *>(static_cast<uint8_t *>(a.q) + row * a.qStride + at) =
+            Word2{Quantise4(s[0], s[1], s[2], s[3]), Quantise4(s[4], s[5], s[6], s[7])};
+        if (threadIdx.x % 16 == 0) {
+            static_cast<typename BlockScale<kScale>::Stored *>(a.scales)[row * a.scaleStride + at / 128] = scale.stored;
+        }
+    }
+}
+
+// kRowThreads threads to a row, each with kChunks times eight values.
+template <typename T, int kRowThreads, int kChunks, bool kEight, int kHow>
+__global__ void __launch_bounds__(BlockOf(kRowThreads)) NormKernel(NormArgs a)
+{
+    constexpr int kRows = BlockOf(kRowThreads) / kRowThreads;
+    __shared__ double parts[kRowThreads / 64];
+    const int l = int(threadIdx.x) % kRowThreads;
+    for (int64_t row = int64_t(blockIdx.x) * kRows + int(threadIdx.x) / kRowThreads; row < a.rows; row += int64_t(gridDim.x) * kRows) {
+        float s[kChunks][kEach], g[kChunks][kEach];
+#pragma unroll
+        for (int c = 0; c < kChunks; c++) {
+            LoadPart<kHow, kEach>(static_cast<const T *>(a.x) + row * a.xStride, (c * kRowThreads + l) * kEach, a.width, s[c]);
+        }
+        if (a.residual != nullptr) {
+            float r[kChunks][kEach];
+#pragma unroll
+            for (int c = 0; c < kChunks; c++) {
+                LoadPart<kHow, kEach>(static_cast<const T *>(a.residual) + row * a.residualStride, (c * kRowThreads + l) * kEach, a.width, r[c]);
+            }
+#pragma unroll
+            for (int c = 0; c < kChunks; c++) {
+#pragma unroll
+                for (int i = 0; i < kEach; i++) {
+                    s[c][i] += r[c][i];
+                }
+            }
+        }
+#pragma unroll
+        for (int c = 0; c < kChunks; c++) {
+            LoadGain<kHow, T>(a.gain, a.gain32, (c * kRowThreads + l) * kEach, a.width, g[c]);
+        }
+        double squares[kChunks];
+#pragma unroll
+        for (int c = 0; c < kChunks; c++) {
+            squares[c] = 0.0;
+#pragma unroll
+            for (int i = 0; i < kEach; i++) {
+                squares[c] = __builtin_fma(double(s[c][i]), double(s[c][i]), squares[c]);
+            }
+        }
+        if (a.sum != nullptr) {
+#pragma unroll
+            for (int c = 0; c < kChunks; c++) {
+                StorePart<kHow, kEach>(static_cast<T *>(a.sum) + row * a.sumStride, (c * kRowThreads + l) * kEach, a.width, s[c]);
+            }
+        }
+        double all = squares[0];
+#pragma unroll
+        for (int c = 1; c < kChunks; c++) {
+            all += squares[c];
+        }
+        all = AddRow<kRowThreads>(all, parts);
+        const float by = float(1.0 / __builtin_sqrt(all / double(a.width) + double(a.epsilon)));
+#pragma unroll
+        for (int c = 0; c < kChunks; c++) {
+            const int at = (c * kRowThreads + l) * kEach;
+            float v[kEach];
+#pragma unroll
+            for (int i = 0; i < kEach; i++) {
+                v[i] = s[c][i] * by * g[c][i];
+            }
+            if (a.y != nullptr) {
+                StorePart<kHow, kEach>(static_cast<T *>(a.y) + row * a.yStride, at, a.width, v);
+            }
+            if constexpr (kEight) {
+                float top = 0.0f;
+#pragma unroll
+                for (int i = 0; i < kEach; i++) {
+                    // (behind the row's end a gain of 1 may meet an infinite factor)
+                    v[i] = kHow == kAligned ? (at < a.width ? v[i] : 0.0f) : (at + i < a.width ? v[i] : 0.0f);
+                    top = __builtin_fmaxf(top, FiniteSize(v[i]));
+                }
+                top = LargestOfNeighbours<16>(top);
+                if (a.powers) {
+                    StoreBlock<HCCL_AMD_SCALE_E8M0>(v, top, a, row, at);
+                } else {
+                    StoreBlock<HCCL_AMD_SCALE_FP32>(v, top, a, row, at);
+                }
+            }
+        }
+        if constexpr (kRowThreads > 64) {
+            __syncthreads();     // before the next row's sums
+        }
+    }
+}
+
+struct NormGradArgs {
+    const void *yGrad, *sum, *gain, *sumGrad;
+    void *xGrad;
+    float *partial;            // [workgroups][width]: sums over a workgroup's rows of dy * n; null: not wanted
+    int64_t yGradStride, sumStride, sumGradStride, xGradStride;
+    int64_t rows;
+    int width;
+    float epsilon;
+    bool gain32;
+};
+
+// A workgroup goes through rows and keeps what they add to the gain's gradient in registers.
+template <typename T, int kRowThreads, int kChunks, int kHow>
+__global__ void __launch_bounds__(BlockOf(kRowThreads)) NormGradKernel(NormGradArgs a)
+{
+    constexpr int kRows = BlockOf(kRowThreads) / kRowThreads;
+    __shared__ double parts[2][kRowThreads / 64];
+    __shared__ float sums[kRows > 1 ? kRows : 1][kRows > 1 ? kRowThreads * kChunks * kEach : 1];
+    const int l = int(threadIdx.x) % kRowThreads, slot = int(threadIdx.x) / kRowThreads;
+    float gain[kChunks][kEach], more[kChunks][kEach];
+#pragma unroll
+    for (int c = 0; c < kChunks; c++) {
+        LoadGain<kHow, T>(a.gain, a.gain32, (c * kRowThreads + l) * kEach, a.width, gain[c]);
+#pragma unroll
+        for (int i = 0; i < kEach; i++) {
+            more[c][i] = 0.0f;
+        }
+    }
+    for (int64_t row = int64_t(blockIdx.x) * kRows + slot; row < a.rows; row += int64_t(gridDim.x) * kRows) {
+        float d[kChunks][kEach], s[kChunks][kEach];
+#pragma unroll
+        for (int c = 0; c < kChunks; c++) {
+            LoadPart<kHow, kEach>(static_cast<const T *>(a.yGrad) + row * a.yGradStride, (c * kRowThreads + l) * kEach, a.width, d[c]);
+            LoadPart<kHow, kEach>(static_cast<const T *>(a.sum) + row * a.sumStride, (c * kRowThreads + l) * kEach, a.width, s[c]);
+        }
+        double squares = 0.0, dots = 0.0;
+#pragma unroll
+        for (int c = 0; c < kChunks; c++) {
+#pragma unroll
+            for (int i = 0; i < kEach; i++) {
+                squares = __builtin_fma(double(s[c][i]), double(s[c][i]), squares);
+                dots = __builtin_fma(double(d[c][i] * gain[c][i]), double(s[c][i]), dots);
+            }
+        }
+        squares = AddWave(squares);
+        dots = AddWave(dots);
+        if constexpr (kRowThreads > 64) {
+            if (threadIdx.x % 64 == 0) {
+                parts[0][threadIdx.x / 64] = squares;
+                parts[1][threadIdx.x / 64] = dots;
+            }
+            __syncthreads();
+            squares = dots = 0.0;
+#pragma unroll
+            for (int w = 0; w < kRowThreads / 64; w++) {
+                squares += parts[0][w];
+                dots += parts[1][w];
+            }
+        }
+        const double length = 1.0 / __builtin_sqrt(squares / double(a.width) + double(a.epsilon));
+        const float by = float(length), mean = float(dots * length / double(a.width));
+#pragma unroll
+        for (int c = 0; c < kChunks; c++) {
+            const int at = (c * kRowThreads + l) * kEach;
+            float out[kEach];
+#pragma unroll
+            for (int i = 0; i < kEach; i++) {
+                const float n = s[c][i] * by;
+                more[c][i] = __builtin_fmaf(d[c][i], n, more[c][i]);
+                out[i] = by * (d[c][i] * gain[c][i] - n * mean);
+            }
+            if (a.xGrad != nullptr) {
+                if (a.sumGrad != nullptr) {
+                    float t[kEach];
+                    LoadPart<kHow, kEach>(static_cast<const T *>(a.sumGrad) + row * a.sumGradStride, at, a.width, t);
+#pragma unroll
+                    for (int i = 0; i < kEach; i++) {
+                        out[i] += t[i];
+                    }
+                }
+                StorePart<kHow, kEach>(static_cast<T *>(a.xGrad) + row * a.xGradStride, at, a.width, out);
+            }
+        }
+        if constexpr (kRowThreads > 64) {
+            __syncthreads();     // before the next row's sums
+        }
+    }
+    if (a.partial == nullptr) {
+        return;
+    }
+    if constexpr (kRows > 1) {
+        // the waves' sums, one behind the other
+#pragma unroll
+        for (int c = 0; c < kChunks; c++) {
+#pragma unroll
+            for (int i = 0; i < kEach; i++) {
+                sums[slot][(c * kRowThreads + l) * kEach + i] = more[c][i];
+            }
+        }
+        __syncthreads();
+        for (int i = threadIdx.x; i < a.width; i += BlockOf(kRowThreads)) {
+            float all = sums[0][i];
+#pragma unroll
+            for (int k = 1; k < kRows; k++) {
+                all += sums[k][i];
+            }
+            a.partial[int64_t(blockIdx.x) * a.width + i] = all;
+        }
+    } else {
+#pragma unroll
+        for (int c = 0; c < kChunks; c++) {
+            StorePart<kAnyhow, kEach>(a.partial + int64_t(blockIdx.x) * a.width, (c * kRowThreads + l) * kEach, a.width, more[c]);
+        }
+    }
+}
+
+constexpr int kGainCols = 16, kGainRuns = 256 / kGainCols;
+
+// gainGrad from the workgroups' sums: 16 columns to a workgroup, 16 runs of workgroups to a column, then the runs in their order.
+__global__ void __launch_bounds__(256) NormGainKernel(const float *partial, int slots, int width, float *gainGrad, bool accumulate)
+{
+    __shared__ float parts[kGainRuns][kGainCols + 1];
+    const int c = int(threadIdx.x) % kGainCols, run = int(threadIdx.x) / kGainCols, at = int(blockIdx.x) * kGainCols + c;
+    float sum = 0.0f;
+    if (at < width) {
+#pragma unroll 8
+        for (int s = run; s < slots; s += kGainRuns) {
+            sum += partial[int64_t(s) * width + at];
+        }
+    }
+    parts[run][c] = sum;
+    __syncthreads();
+    if (run == 0 && at < width) {
+        float all = accumulate ? gainGrad[at] : 0.0f;
+#pragma unroll
+        for (int i = 0; i < kGainRuns; i++) {
+            all += parts[i][c];
+        }
+        gainGrad[at] = all;
+    }
+}
+
+// f(threads to a row, times eight values of a thread), as constants
+template <typename F>
+HcclResult ByWidth(uint64_t width, F f)
+{
+    typedef std::integral_constant<int, 1> One;
+    typedef std::integral_constant<int, 2> Two;
+    typedef std::integral_constant<int, 4> Four;
+    if (width <= 512) {
+        return f(std::integral_constant<int, 64>{}, One{});
+    }
+    if (width <= 1024) {
+        return f(std::integral_constant<int, 64>{}, Two{});
+    }
+    if (width <= 2048) {
+        return f(std::integral_constant<int, 256>{}, One{});
+    }
+    if (width <= 4096) {
+        return f(std::integral_constant<int, 256>{}, Two{});
+    }
+    if (width <= 8192) {
+        return f(std::integral_constant<int, 512>{}, Two{});
+    }
+    return width <= 16384 ? f(std::integral_constant<int, 1024>{}, Two{}) : f(std::integral_constant<int, 1024>{}, Four{});
+}
+
+template <typename F>
+HcclResult ByType(HcclDataType type, F f)
+{
+    return type == HCCL_DATA_TYPE_FP32 ? f(float{}) : type == HCCL_DATA_TYPE_FP16 ? f(_Float16{}) : f(__bf16{});
+}
+
+constexpr uint64_t kMostGradBlocks = 512;   // workgroups that go through rows: two to a compute unit
+
+uint64_t GradBlocks(uint64_t rows, uint64_t width)
+{
+    const uint64_t each = width <= 1024 ? 4 : 1, blocks = (rows + each - 1) / each;
+    return blocks < kMostGradBlocks ? blocks : kMostGradBlocks;
+}
+
+// Whether rows at p can be taken 16 bytes at a time.
+bool Wide(HcclDataType type, const void *p, int64_t stride) { return p == nullptr || (Aligned(p, 16) && uint64_t(stride) * SizeOf(type) % 16 == 0); }
+
+int64_t Between(uint64_t stride, uint64_t width) { return int64_t(stride == 0 ? width : stride); }
+
+}  // namespace
+}  // namespace experts
+}  // namespace hcclamd
+
+using namespace hcclamd::experts;
+
+extern "C" {
+
+HcclResult HcclAmdNormRows(const void *x, HcclDataType type, uint64_t rows, uint64_t width, uint64_t xStride, const void *residual,
+    uint64_t residualStride, const void *gain, HcclDataType gainType, float epsilon, void *sum, uint64_t sumStride, void *y, uint64_t yStride,
+    HcclAmdScaleType scaleType, void *q, uint64_t qStride, void *scales, uint64_t scaleStride, void *stream)
+{
+    EXPERTS_CHK_PTR(stream);
+    EXPERTS_CHK_TYPE(Float(type));
+    EXPERTS_CHK_TYPE(gain == nullptr || gainType == type || gainType == HCCL_DATA_TYPE_FP32);
+    EXPERTS_CHK_TYPE(scaleType == HCCL_AMD_SCALE_NONE || Scaled(scaleType));
+    EXPERTS_CHK(rows <= kMaxSize && width <= HCCL_AMD_MAX_NORM_WIDTH);
+    EXPERTS_CHK(epsilon >= 0.0f);
+    if (rows == 0 || width == 0 || (sum == nullptr && y == nullptr && scaleType == HCCL_AMD_SCALE_NONE)) {
+        return HCCL_SUCCESS;
+    }
+    EXPERTS_CHK_PTR(x);
+    EXPERTS_CHK(Stride(xStride, width) && Stride(residualStride, width) && Stride(sumStride, width) && Stride(yStride, width));
+    EXPERTS_CHK(AlignedTo(type, x) && AlignedTo(type, residual) && AlignedTo(type, sum) && AlignedTo(type, y));
+    EXPERTS_CHK(gain == nullptr || AlignedTo(gainType, gain));
+    NormArgs a{};
+    a.x = x;
+    a.residual = residual;
+    a.gain = gain;
+    a.sum = sum;
+    a.y = y;
+    a.xStride = Between(xStride, width);
+    a.residualStride = Between(residualStride, width);
+    a.sumStride = Between(sumStride, width);
+    a.yStride = Between(yStride, width);
+    a.rows = int64_t(rows);
+    a.width = int(width);
+    a.padded = int(Up128(width));
+    a.epsilon = epsilon;
+    a.gain32 = gainType == HCCL_DATA_TYPE_FP32;
+    EXPERTS_CHK(sum == nullptr || ((sum != x || a.sumStride == a.xStride) && (sum != residual || a.sumStride == a.residualStride)));
+    const bool eight = scaleType != HCCL_AMD_SCALE_NONE;
+    if (eight) {
+        EXPERTS_CHK_PTR(q);
+        EXPERTS_CHK_PTR(scales);
+        EXPERTS_CHK(Stride(qStride, Up128(width)) && qStride % 16 == 0 && Aligned(q, 16));
+        EXPERTS_CHK(Stride(scaleStride, Blocks(width)) && ScaleAligned(scaleType, scales));
+        a.q = q;
+        a.scales = scales;
+        a.qStride = Between(qStride, Up128(width));
+        a.scaleStride = Between(scaleStride, Blocks(width));
+        a.powers = scaleType == HCCL_AMD_SCALE_E8M0;
+    } else {
+        EXPERTS_CHK(q == nullptr && scales == nullptr);
+    }
+    const bool wide = width % kEach == 0 && Wide(type, x, a.xStride) && Wide(type, residual, a.residualStride) && Wide(type, sum, a.sumStride) &&
+        Wide(type, y, a.yStride) && Aligned(gain, 16);
+    return ByType(type, [&](auto of) {
+        return ByWidth(width, [&](auto threads, auto chunks) {
+            typedef decltype(of) T;
+            constexpr int kThreads = decltype(threads)::value, kChunks = decltype(chunks)::value, kBlock = BlockOf(kThreads), kRows = kBlock / kThreads;
+            const int64_t blocks = (a.rows + kRows - 1) / kRows;
+            const auto go = [&](auto kernel) {
+                return Launch("HcclAmdNormRows", kernel, uint32_t(blocks < (1 << 20) ? blocks : 1 << 20), kBlock, 0, static_cast<hipStream_t>(stream), a);
+            };
+            return eight ? (wide ? go(NormKernel<T, kThreads, kChunks, true, kAligned>) : go(NormKernel<T, kThreads, kChunks, true, kAnyhow>))
+                         : (wide ? go(NormKernel<T, kThreads, kChunks, false, kAligned>) : go(NormKernel<T, kThreads, kChunks, false, kAnyhow>));
+        });
+    });
+}
+
+HcclResult HcclAmdNormRowsGradWorkspace(uint64_t rows, uint64_t width, uint64_t *bytes)
+{
+    EXPERTS_CHK_PTR(bytes);
+    EXPERTS_CHK(rows <= kMaxSize && width <= HCCL_AMD_MAX_NORM_WIDTH);
+    *bytes = GradBlocks(rows, width) * width * sizeof(float);
+    return HCCL_SUCCESS;
+}
+
+HcclResult HcclAmdNormRowsGrad(const void *yGrad, uint64_t yGradStride, const void *sum, HcclDataType type, uint64_t rows, uint64_t width,
+    uint64_t sumStride, const void *gain, HcclDataType gainType, float epsilon, const void *sumGrad, uint64_t sumGradStride, void *xGrad,
+    uint64_t xGradStride, float *gainGrad, uint32_t accumulate, void *workspace, uint64_t workspaceBytes, void *stream)
+{
+    EXPERTS_CHK_PTR(stream);
+    EXPERTS_CHK_TYPE(Float(type));
+    EXPERTS_CHK_TYPE(gain == nullptr || gainType == type || gainType == HCCL_DATA_TYPE_FP32);
+    EXPERTS_CHK(rows <= kMaxSize && width <= HCCL_AMD_MAX_NORM_WIDTH);
+    EXPERTS_CHK(epsilon >= 0.0f);
+    if (width == 0 || (xGrad == nullptr && gainGrad == nullptr) || (rows == 0 && gainGrad == nullptr)) {
+        return HCCL_SUCCESS;
+    }
+    EXPERTS_CHK(Aligned(gainGrad, 4));
+    const hipStream_t on = static_cast<hipStream_t>(stream);
+    const uint64_t blocks = GradBlocks(rows, width);
+    if (rows != 0) {
+        EXPERTS_CHK_PTR(yGrad);
+        EXPERTS_CHK_PTR(sum);
+        EXPERTS_CHK(Stride(yGradStride, width) && Stride(sumStride, width) && Stride(sumGradStride, width) && Stride(xGradStride, width));
+        EXPERTS_CHK(AlignedTo(type, yGrad) && AlignedTo(type, sum) && AlignedTo(type, sumGrad) && AlignedTo(type, xGrad));
+        EXPERTS_CHK(gain == nullptr || AlignedTo(gainType, gain));
+        NormGradArgs a{};
+        a.yGrad = yGrad;
+        a.sum = sum;
+        a.gain = gain;
+        a.sumGrad = sumGrad;
+        a.xGrad = xGrad;
+        a.yGradStride = Between(yGradStride, width);
+        a.sumStride = Between(sumStride, width);
+        a.sumGradStride = Between(sumGradStride, width);
+        a.xGradStride = Between(xGradStride, width);
+        a.rows = int64_t(rows);
+        a.width = int(width);
+        a.epsilon = epsilon;
+        a.gain32 = gainType == HCCL_DATA_TYPE_FP32;
+        EXPERTS_CHK(xGrad == nullptr || ((xGrad != yGrad || a.xGradStride == a.yGradStride) && (xGrad != sumGrad || a.xGradStride == a.sumGradStride)));
+        if (gainGrad != nullptr) {
+            EXPERTS_CHK_PTR(workspace);
+            EXPERTS_CHK(Aligned(workspace, 16));
+            EXPERTS_CHK(workspaceBytes >= blocks * width * sizeof(float));
+            a.partial = static_cast<float *>(workspace);
+        }
+        const bool wide = width % kEach == 0 && Wide(type, yGrad, a.yGradStride) && Wide(type, sum, a.sumStride) && Wide(type, sumGrad, a.sumGradStride) &&
+            Wide(type, xGrad, a.xGradStride) && Aligned(gain, 16);
+        const HcclResult r = ByType(type, [&](auto of) {
+            return ByWidth(width, [&](auto threads, auto chunks) {
+                typedef decltype(of) T;
+                constexpr int kThreads = decltype(threads)::value, kChunks = decltype(chunks)::value;
+                const auto go = [&](auto kernel) { return Launch("HcclAmdNormRowsGrad", kernel, uint32_t(blocks), BlockOf(kThreads), 0, on, a); };
+                return wide ? go(NormGradKernel<T, kThreads, kChunks, kAligned>) : go(NormGradKernel<T, kThreads, kChunks, kAnyhow>);
+            });
+        });
+        if (r != HCCL_SUCCESS || gainGrad == nullptr) {
+            return r;
+        }
+    }
+    return Launch("HcclAmdNormRowsGrad", NormGainKernel, uint32_t((width + kGainCols - 1) / kGainCols), 256, 0, on,
+        static_cast<const float *>(workspace), int(blocks), int(width), gainGrad, accumulate != 0);
+}
+
+}  // extern "C"

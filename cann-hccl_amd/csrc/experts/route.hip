@@ -20,32 +20,19 @@
 // rest is the latency of few dependent accesses.  One token: 7 us, the latency of one wave's way through the code.
 #include <type_traits>
 
-#include "common.h"
+#include "rows.h"
 
 namespace hcclamd {
 namespace experts {
 namespace {
 
-constexpr int kThreads = 256;
 constexpr uint32_t kNone = 0xffffffffu;
-constexpr uint64_t kMaxTokens = uint64_t(1) << 25;
 
-struct RouteArgs {
+struct RouteArgs : RowsArgs {
     const void *logits;
     const uint8_t *mask;
-    int32_t *expertOf;
     float *weights;
-    int32_t *rowOf;
-    int32_t *counts;
-    int32_t *offsets;
-    float *loss;
-    int32_t *blockCounts;  // [blocks][experts + 1]: rows per expert; last column: tokens that chose
-    float *blockSums;      // [blocks][experts]: sum of probabilities
-    float *sums;           // [experts]
     int64_t stride;
-    int tokens, experts, topK;
-    int blocks, tiles;     // workgroups; tiles of each
-    float lossScale;
     bool renormalise;
 };
 
@@ -206,121 +193,6 @@ template <typename T, int K>
 using List = std::conditional_t<sizeof(T) == 2, WordList<K>, PairList<K>>;
 
 // ---- sums ------------------------------------------------------------------------------------------------
-
-// Adds up over the lanes whose numbers agree above the lowest bits: kLanes neighbouring lanes, a power of two up to 64.
-template <int kLanes>
-__device__ __forceinline__ float AddNeighbours(float x)
-{
-#pragma unroll
-    for (int d = 1; d < kLanes; d <<= 1) {
-        x += __shfl_xor(x, d, 64);
-    }
-    return x;
-}
-
-// A row of 16 lanes turned by kBy.
-template <int kBy>
-__device__ __forceinline__ float Turned(float x)
-{
-    return __int_as_float(__builtin_amdgcn_update_dpp(0, __float_as_int(x), 0x120 + kBy, 0xf, 0xf, true));
-}
-
-// The same over 16 lanes without LDS.
-template <>
-__device__ __forceinline__ float AddNeighbours<16>(float x)
-{
-    x += Turned<8>(x);
-    x += Turned<4>(x);
-    x += Turned<2>(x);
-    x += Turned<1>(x);
-    return x;
-}
-
-// The largest, NaN being less than everything.
-__device__ __forceinline__ float Larger(float a, float b) { return b > a ? b : a; }
-
-template <int kLanes>
-__device__ __forceinline__ float LargestOfNeighbours(float x)
-{
-    if constexpr (kLanes == 16) {
-        x = Larger(x, Turned<8>(x));
-        x = Larger(x, Turned<4>(x));
-        x = Larger(x, Turned<2>(x));
-        x = Larger(x, Turned<1>(x));
-    } else {
-#pragma unroll
-        for (int d = 1; d < kLanes; d <<= 1) {
-            x = Larger(x, __shfl_xor(x, d, 64));
-        }
-    }
-    return x;
-}
-
-// Exclusive prefix sums of n <= 1024 values in LDS, in place, by kThreads threads; returns the total.  `part`: a word per wave.
-template <int kThreads>
-__device__ __forceinline__ int Scan(int *values, int n, int *part)
-{
-    const int per = (n + kThreads - 1) / kThreads, from = min(n, int(threadIdx.x) * per), to = min(n, from + per);
-    int mine = 0;
-    for (int i = from; i < to; i++) {
-        mine += values[i];
-    }
-    const int lane = int(threadIdx.x) % 64;
-    int sum = mine;
-#pragma unroll
-    for (int d = 1; d < 64; d <<= 1) {
-        const int other = __shfl_up(sum, d, 64);
-        sum += lane >= d ? other : 0;
-    }
-    if (lane == 63) {
-        part[threadIdx.x / 64] = sum;
-    }
-    __syncthreads();
-    int at = sum - mine, total = 0;
-    for (int w = 0; w < kThreads / 64; w++) {
-        at += w < int(threadIdx.x) / 64 ? part[w] : 0;
-        total += part[w];
-    }
-    for (int i = from; i < to; i++) {
-        const int v = values[i];
-        values[i] = at;
-        at += v;
-    }
-    __syncthreads();
-    return total;
-}
-
-// counts[experts + 1], offsets and the loss (`write`) from per-expert counts and sums in LDS; afterwards `count` holds the offsets.
-template <int kThreads>
-__device__ __forceinline__ void Finish(const RouteArgs &a, int *count, const float *sum, int tokens, int *part, float *partSum, bool write)
-{
-    float load = 0.0f;
-    for (int e = threadIdx.x; e < a.experts && write; e += kThreads) {
-        load += float(count[e]) * sum[e];
-        a.counts[e] = count[e];
-    }
-    load = AddNeighbours<64>(load);
-    if (threadIdx.x % 64 == 0) {
-        partSum[threadIdx.x / 64] = load;
-    }
-    __syncthreads();
-    const int rows = Scan<kThreads>(count, a.experts, part);
-    if (!write) {
-        return;
-    }
-    for (int e = threadIdx.x; e < a.experts; e += kThreads) {
-        a.offsets[e] = count[e];
-    }
-    if (threadIdx.x == 0) {
-        float all = 0.0f;
-        for (int w = 0; w < kThreads / 64; w++) {
-            all += partSum[w];
-        }
-        a.counts[a.experts] = tokens;
-        a.offsets[a.experts] = rows;
-        a.loss[0] = rows == 0 ? 0.0f : a.lossScale * float(a.experts) * (all / float(rows) / float(tokens));
-    }
-}
 
 // One step of adding up over lanes and sharing out the sums: of 2 kHalf values a lane keeps the half that its bit names, and adds what
 // its partner, whose bit is the other one, has of it.  kDpp: how lanes are exchanged.
@@ -493,7 +365,7 @@ __global__ void __launch_bounds__(kThreads) RouteKernel(RouteArgs a)
         if (a.blocks == 1 && tile + 1 == a.tiles) {
             // a single workgroup: its places become rows at once
             AddWaves(sum, E);
-            Finish<kThreads>(a, count, sum, *routed, part, partSum, true);
+            Finish<kThreads, true>(a, count, sum, *routed, part, partSum, true);
         }
         if (token < a.tokens) {
 #pragma unroll
@@ -524,112 +396,6 @@ __global__ void __launch_bounds__(kThreads) RouteKernel(RouteArgs a)
     }
 }
 
-constexpr int kMostBlocks = 1024, kScanCols = 8, kScanRuns = kThreads / kScanCols, kScanEach = kMostBlocks / kScanRuns;
-
-// Adds up the workgroups' counts and probabilities, eight experts (columns) to a workgroup and 32 runs of rows to an expert, all of a run
-// on its way at once, and leaves in blockCounts what lies in front of every workgroup.  Column `experts` holds the tokens that chose.
-__global__ void __launch_bounds__(kThreads) ScanKernel(RouteArgs a)
-{
-    __shared__ int parts[kScanRuns][kScanCols + 1];
-    __shared__ float partSums[kScanRuns][kScanCols + 1];
-    const int c = int(threadIdx.x) % kScanCols, run = int(threadIdx.x) / kScanCols, e = int(blockIdx.x) * kScanCols + c;
-    const int64_t width = a.experts + 1;
-    const int per = (a.blocks + kScanRuns - 1) / kScanRuns, from = run * per;
-    int n[kScanEach], all = 0;
-    float p[kScanEach], sum = 0.0f;
-#pragma unroll
-    for (int i = 0; i < kScanEach; i++) {
-        const bool in = i < per && from + i < a.blocks;
-        n[i] = in && e <= a.experts ? a.blockCounts[(from + i) * width + e] : 0;
-        p[i] = in && e < a.experts ? a.blockSums[int64_t(from + i) * a.experts + e] : 0.0f;
-    }
-#pragma unroll
-    for (int i = 0; i < kScanEach; i++) {
-        all += n[i];
-        sum += p[i];
-    }
-    parts[run][c] = all;
-    partSums[run][c] = sum;
-    __syncthreads();
-    int before = 0;
-    all = 0;
-    sum = 0.0f;
-#pragma unroll
-    for (int i = 0; i < kScanRuns; i++) {
-        before += i < run ? parts[i][c] : 0;
-        all += parts[i][c];
-        sum += partSums[i][c];
-    }
-    if (e > a.experts) {
-        return;
-    }
-#pragma unroll
-    for (int i = 0; i < kScanEach; i++) {
-        if (i < per && from + i < a.blocks) {
-            a.blockCounts[(from + i) * width + e] = before;
-            before += n[i];
-        }
-    }
-    if (run == 0) {
-        a.counts[e] = all;
-        if (e < a.experts) {
-            a.sums[e] = sum;
-        }
-    }
-}
-
-// Every choice's row: its expert's first row, the rows of the workgroups before its own, its place in its own.  kAll: every workgroup adds up
-// the table of counts itself, and no launch has done so before.
-template <bool kAll>
-__global__ void __launch_bounds__(kThreads) RowsKernel(RouteArgs a, int tokensEach)
-{
-    extern __shared__ uint32_t lds[];
-    const int E = a.experts, block = int(blockIdx.x);
-    int *count = reinterpret_cast<int *>(lds);                           // [experts + 1]
-    float *sum = reinterpret_cast<float *>(count + E + 1);               // [experts]
-    int *before = reinterpret_cast<int *>(sum + E);                      // [experts]
-    int *part = before + E;                                              // [waves]
-    float *partSum = reinterpret_cast<float *>(part + kThreads / 64);    // [waves]
-    for (int e = threadIdx.x; e <= E; e += kThreads) {
-        int all = 0, front = 0;
-        float p = 0.0f;
-        if constexpr (kAll) {
-#pragma unroll 8
-            for (int b = 0; b < a.blocks; b++) {
-                const int n = a.blockCounts[int64_t(b) * (E + 1) + e];
-                all += n;
-                front += b < block ? n : 0;
-            }
-            if (block == 0 && e < E) {
-#pragma unroll 8
-                for (int b = 0; b < a.blocks; b++) {
-                    p += a.blockSums[int64_t(b) * E + e];
-                }
-            }
-        } else {
-            all = a.counts[e];
-            front = a.blockCounts[int64_t(block) * (E + 1) + e];
-            p = block == 0 && e < E ? a.sums[e] : 0.0f;
-        }
-        count[e] = all;
-        if (e < E) {
-            sum[e] = p;
-            before[e] = front;
-        }
-    }
-    __syncthreads();
-    const int tokens = count[E];
-    Finish<kThreads>(a, count, sum, tokens, part, partSum, block == 0);
-    const int64_t first = int64_t(block) * tokensEach * a.topK;
-    const int64_t last = min(first + int64_t(tokensEach) * a.topK, int64_t(a.tokens) * a.topK);
-    for (int64_t i = first + threadIdx.x; i < last; i += kThreads) {
-        const int e = a.expertOf[i];
-        if (e >= 0) {
-            a.rowOf[i] += count[e] + before[e];
-        }
-    }
-}
-
 struct RouteGradArgs {
     const void *logits;
     const uint8_t *mask;
@@ -643,13 +409,6 @@ struct RouteGradArgs {
     float lossScale;
     bool renormalise;
 };
-
-// Keeps the compiler from moving LDS operations of one wave's lanes past each other.
-__device__ __forceinline__ void Ordered()
-{
-    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
-    __builtin_amdgcn_wave_barrier();
-}
 
 // kLanes lanes to a token (at least as many as it has choices), kEach experts to a lane, in vectors of four that the lanes of a token
 // take in turn.  A workgroup goes through tokens, what it knows of the experts stays in registers.  What the weights' gradients add at
@@ -775,19 +534,6 @@ __global__ void __launch_bounds__(kThreads) RouteGradKernel(RouteGradArgs a)
 // Tokens of a tile: 64 with four lanes to a token, 16 with sixteen.  Sixteen lanes where a lane would have more than 64 experts,
 // and for few tokens, where the time is one lane's.
 int TileOf(uint64_t tokens, uint32_t experts) { return experts > 256 || tokens <= 64 * 64 ? 16 : 64; }
-
-// Workgroups: at most 1024, four to a compute unit, each with as many tiles as that takes.
-int TilesOf(uint64_t tokens, int tile)
-{
-    const uint64_t tiles = (tokens + uint64_t(tile) - 1) / uint64_t(tile);
-    return tiles == 0 ? 1 : tiles <= 4 ? int(tiles) : int((tiles + kMostBlocks - 1) / kMostBlocks);
-}
-
-int BlocksOf(uint64_t tokens, int tile)
-{
-    const uint64_t each = uint64_t(tile) * uint64_t(TilesOf(tokens, tile));
-    return tokens == 0 ? 1 : int((tokens + each - 1) / each);
-}
 
 template <typename T, int K, int kLanes, int kChunks>
 HcclResult LaunchRoute(const RouteArgs &a, bool wide, hipStream_t stream)
@@ -915,13 +661,13 @@ HcclResult HcclAmdExpertRoute(const void *logits, HcclDataType logitType, uint64
     // 256 experts 13 instead of 15; with more of them that reading takes as long as a launch of its own.
     const bool few = a.blocks <= 32;
     if (!few) {
-        r = Launch("HcclAmdExpertRoute", ScanKernel, experts / kScanCols + 1, kThreads, 0, on, a);
+        r = Launch("HcclAmdExpertRoute", ScanKernel<true>, experts / kScanCols + 1, kThreads, 0, on, RowsArgs(a));
         if (r != HCCL_SUCCESS) {
             return r;
         }
     }
-    return Launch("HcclAmdExpertRoute", few ? RowsKernel<true> : RowsKernel<false>, uint32_t(a.blocks), kThreads,
-        4 * (3 * size_t(experts) + 1 + 2 * (kThreads / 64)), on, a, tile * a.tiles);
+    return Launch("HcclAmdExpertRoute", few ? RowsKernel<true, true> : RowsKernel<false, true>, uint32_t(a.blocks), kThreads,
+        RowsLds(a.experts), on, RowsArgs(a), tile * a.tiles);
 }
 
 HcclResult HcclAmdExpertRouteGrad(const void *logits, HcclDataType logitType, uint64_t tokens, uint32_t experts, uint64_t logitStride,

@@ -1,0 +1,92 @@
+// Sums and maxima over neighbouring lanes, and the order of a wave's LDS operations.
+#pragma once
+#include "common.h"
+
+namespace hcclamd {
+namespace experts {
+
+// Adds up over the lanes whose numbers agree above the lowest bits: kLanes neighbouring lanes, a power of two up to 64.
+template <int kLanes>
+__device__ __forceinline__ float AddNeighbours(float x)
+{
+#pragma unroll
+    for (int d = 1; d < kLanes; d <<= 1) {
+        x += __shfl_xor(x, d, 64);
+    }
+    return x;
+}
+
+// A row of 16 lanes turned by kBy.
+template <int kBy>
+__device__ __forceinline__ float Turned(float x)
+{
+    return __int_as_float(__builtin_amdgcn_update_dpp(0, __float_as_int(x), 0x120 + kBy, 0xf, 0xf, true));
+}
+
+// The same over 16 lanes without LDS.
+template <>
+__device__ __forceinline__ float AddNeighbours<16>(float x)
+{
+    x += Turned<8>(x);
+    x += Turned<4>(x);
+    x += Turned<2>(x);
+    x += Turned<1>(x);
+    return x;
+}
+
+// The largest, NaN being less than everything.
+__device__ __forceinline__ float Larger(float a, float b) { return b > a ? b : a; }
+
+template <int kLanes>
+__device__ __forceinline__ float LargestOfNeighbours(float x)
+{
+    if constexpr (kLanes == 16) {
+        x = Larger(x, Turned<8>(x));
+        x = Larger(x, Turned<4>(x));
+        x = Larger(x, Turned<2>(x));
+        x = Larger(x, Turned<1>(x));
+    } else {
+#pragma unroll
+        for (int d = 1; d < kLanes; d <<= 1) {
+            x = Larger(x, __shfl_xor(x, d, 64));
+        }
+    }
+    return x;
+}
+
+template <int kBy>
+__device__ __forceinline__ double Turned(double x)
+{
+    const uint64_t bits = __builtin_bit_cast(uint64_t, x);
+    const uint32_t low = uint32_t(__builtin_amdgcn_update_dpp(0, int(uint32_t(bits)), 0x120 + kBy, 0xf, 0xf, true));
+    const uint32_t high = uint32_t(__builtin_amdgcn_update_dpp(0, int(uint32_t(bits >> 32)), 0x120 + kBy, 0xf, 0xf, true));
+    return __builtin_bit_cast(double, uint64_t(high) << 32 | low);
+}
+
+__device__ __forceinline__ double FromLane(double x, int lane)
+{
+    const uint64_t bits = __builtin_bit_cast(uint64_t, x);
+    const uint32_t low = uint32_t(__builtin_amdgcn_readlane(int(uint32_t(bits)), lane));
+    const uint32_t high = uint32_t(__builtin_amdgcn_readlane(int(uint32_t(bits >> 32)), lane));
+    return __builtin_bit_cast(double, uint64_t(high) << 32 | low);
+}
+
+// Over all lanes of a wave, which all have to be there: rows of 16 by turning them, then the four rows.
+__device__ __forceinline__ double AddWave(double x)
+{
+    x += Turned<8>(x);
+    x += Turned<4>(x);
+    x += Turned<2>(x);
+    x += Turned<1>(x);
+    return (FromLane(x, 0) + FromLane(x, 16)) + (FromLane(x, 32) + FromLane(x, 48));
+}
+
+// Keeps the compiler from moving LDS operations of one wave's lanes past each other.
+__device__ __forceinline__ void Ordered()
+{
+    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+    __builtin_amdgcn_wave_barrier();
+}
+
+}  // namespace experts
+}  // namespace hcclamd

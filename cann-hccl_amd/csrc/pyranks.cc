@@ -6,7 +6,7 @@
 // per collective: 8-rank all-reduce of 8 KiB 7.6 us through ctypes, 4.4 us here; 64-rank all-to-all-v of short blocks,
 // tables as numpy arrays, 80 us and 29 us.
 //
-// The experts' operators (hccl_amd_experts.h) are single calls of up to 18 arguments, whose conversion by ctypes costs more than
+// The experts' operators (hccl_amd_experts.h) are single calls of up to 22 arguments, whose conversion by ctypes costs more than
 // the launch: expert() makes them in the same way.  A call that packs 64 tokens takes 3.4 us of the host through ctypes, 2.8 us here.
 //
 // Whatever this loop does not recognise (other sequence or pointer types than lists or tuples of integers, None and
@@ -49,7 +49,7 @@ struct Functions {
 static_assert(sizeof(Functions) == KIND_COUNT * sizeof(void *), "one function per kind");
 Functions g_fn = {};
 
-// the experts' operators, in the order of the mirror's EXPERT_EXPORTS without its first (a query)
+// the experts' operators, in the order of the mirror's EXPERT_EXPORTS without the queries of workspaces
 struct ExpertFunctions {
     decltype(&HcclAmdExpertRoute) route;
     decltype(&HcclAmdExpertRouteGrad) routeGrad;
@@ -60,6 +60,15 @@ struct ExpertFunctions {
     decltype(&HcclAmdBlockQuantColumns) quantColumns;
     decltype(&HcclAmdBlockMatmul) matmul;
     decltype(&HcclAmdBlockMatmulGradWeight) matmulGradWeight;
+    decltype(&HcclAmdNormRows) normRows;
+    decltype(&HcclAmdNormRowsGrad) normRowsGrad;
+    decltype(&HcclAmdExpertGate) gate;
+    decltype(&HcclAmdExpertGateGrad) gateGrad;
+    decltype(&HcclAmdExpertRouteScored) routeScored;
+    decltype(&HcclAmdExpertRouteScoredGrad) routeScoredGrad;
+    decltype(&HcclAmdExpertBias) bias;
+    decltype(&HcclAmdGradSquares) gradSquares;
+    decltype(&HcclAmdGradClip) gradClip;
 };
 constexpr long kExpertKinds = sizeof(ExpertFunctions) / sizeof(void *);
 ExpertFunctions g_expert = {};
@@ -288,6 +297,15 @@ PyObject *Expert(PyObject *, PyObject *const *args, Py_ssize_t nargs)
             case 6: res = Forward(g_expert.quantColumns, a, n); break;
             case 7: res = Forward(g_expert.matmul, a, n); break;
             case 8: res = Forward(g_expert.matmulGradWeight, a, n); break;
+            case 9: res = Forward(g_expert.normRows, a, n); break;
+            case 10: res = Forward(g_expert.normRowsGrad, a, n); break;
+            case 11: res = Forward(g_expert.gate, a, n); break;
+            case 12: res = Forward(g_expert.gateGrad, a, n); break;
+            case 13: res = Forward(g_expert.routeScored, a, n); break;
+            case 14: res = Forward(g_expert.routeScoredGrad, a, n); break;
+            case 15: res = Forward(g_expert.bias, a, n); break;
+            case 16: res = Forward(g_expert.gradSquares, a, n); break;
+            case 17: res = Forward(g_expert.gradClip, a, n); break;
             default: break;
         }
     }

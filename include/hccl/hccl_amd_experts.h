@@ -1,14 +1,19 @@
-/* Operators of an expert-parallel layer, next to HcclAlltoAllV.  Nothing here exists in the reference.
+/* Operators of an expert-parallel layer, next to HcclAlltoAllV, and of its training step, next to HcclAllReduce.  Nothing here exists in
+ * the reference.
  *
  *   HcclAmdExpertRoute      logits -> experts, weights, per-expert counts, rows in expert order, balance loss
  *   HcclAmdExpertPack       tokens -> rows in expert order (an all-to-all-v's send buffer), copied or in 8 bits
  *   HcclAmdBlockMatmul      8-bit rows, group by group, times their experts' 8-bit weights
  *   HcclAmdExpertCombine    rows -> tokens, weighted and summed
+ *   HcclAmdNormRows         rows + residual, normed by their root mean square, in their type and as 8-bit rows
+ *   HcclAmdExpertRouteScored, HcclAmdExpertBias   experts by sigmoid or softmax scores, a balancing bias, in groups
+ *   HcclAmdExpertGate       silu(gate) * up between two products, in the rows' type or as 8-bit rows
+ *   HcclAmdGradSquares, HcclAmdGradClip   gradients of many tensors held to a norm over all of them (and all ranks)
  *   ...Grad, HcclAmdBlockMatmulGradWeight, HcclAmdBlockQuant...   their gradients and what these read
  *
  * All of them: device pointers unless said otherwise, of one GPU; no communicator; the work is queued on `stream` (a
  * hipStream_t, not null) and nothing is allocated, copied or waited for, so a call can be captured into a HIP graph.  An
- * output must not overlap an input or another output.  Same inputs, same bits: no atomics whose order matters.  Strides are
+ * output must not overlap an input or another output, except where a call says that the two may be the same.  Same inputs, same bits: no atomics whose order matters.  Strides are
  * in elements, from one row to the next, 2^40 at most; 0 stands for rows that follow each other without a gap.  Values in 16 bits are
  * widened, everything is summed in 32 bits, and rounded once at the end.  Indices and offsets read from device memory are
  * checked on the device: what points outside is skipped.
@@ -35,6 +40,8 @@ extern "C" {
 #define HCCL_AMD_MAX_EXPERTS 1024u   /* of a router */
 #define HCCL_AMD_MAX_GROUPS 4096u    /* groups of rows, and weights, of one product */
 #define HCCL_AMD_MAX_TOPK 16u
+#define HCCL_AMD_MAX_EXPERT_GROUPS 64u   /* groups of experts of a router */
+#define HCCL_AMD_MAX_NORM_WIDTH 32768u   /* of a row that is normed */
 
 typedef enum HcclAmdScaleTypeDef {
     HCCL_AMD_SCALE_NONE = 0,
@@ -123,6 +130,102 @@ extern HcclResult HcclAmdBlockMatmul(const void *a, uint64_t aStride, const void
 extern HcclResult HcclAmdBlockMatmulGradWeight(const void *yGradT, const void *yGradScales, const void *xT, const void *xScales,
     uint64_t columns, uint64_t rows, uint64_t n, uint64_t k, HcclAmdScaleType scaleType, uint32_t groups, const int32_t *offsets,
     const int32_t *expertOfGroup, uint32_t experts, void *wGrad, HcclDataType gradType, uint32_t accumulate, void *stream);
+
+/* s = x + residual (x alone if residual is NULL), y = s * gain / sqrt(mean of s^2 over the row + epsilon).
+ *   x, residual[rows][...]        FP32, FP16 or BFP16, sum and y alike; widened, and s and y stay in 32 bits until they are rounded once for
+ *                                 each output.  The squares are summed in 64 bits: no row overflows
+ *   gain[width]                   gainType: FP32, or the rows' type; NULL: all 1
+ *   sum[rows][sumStride]          s; NULL: not wanted; may be x or residual, of the same stride
+ *   y[rows][yStride]              NULL: not wanted
+ *   q[rows][qStride], scales      8-bit rows of y as it is in 32 bits (see above), ceil(width / 128) scales to a row; both NULL with
+ *                                 HCCL_AMD_SCALE_NONE
+ * epsilon: 0 or more.  width <= HCCL_AMD_MAX_NORM_WIDTH, rows < 2^31. */
+extern HcclResult HcclAmdNormRows(const void *x, HcclDataType type, uint64_t rows, uint64_t width, uint64_t xStride, const void *residual,
+    uint64_t residualStride, const void *gain, HcclDataType gainType, float epsilon, void *sum, uint64_t sumStride, void *y, uint64_t yStride,
+    HcclAmdScaleType scaleType, void *q, uint64_t qStride, void *scales, uint64_t scaleStride, void *stream);
+
+/* Bytes of device workspace that HcclAmdNormRowsGrad needs for gainGrad (host pointer `bytes`). */
+extern HcclResult HcclAmdNormRowsGradWorkspace(uint64_t rows, uint64_t width, uint64_t *bytes);
+
+/* Gradients of HcclAmdNormRows from yGrad and from sumGrad (NULL: none), what reaches the sum from elsewhere; `sum` as the forward call
+ * left it (x, if there was no residual).
+ *   xGrad[rows][xGradStride]      of x and of residual alike; NULL: not wanted; may be yGrad or sumGrad, of the same stride
+ *   gainGrad[width]               32 bits (added to what is there with `accumulate`); NULL: not wanted, no workspace then
+ * workspace: 16-byte aligned, HcclAmdNormRowsGradWorkspace bytes, free for other use once the stream is past the call. */
+extern HcclResult HcclAmdNormRowsGrad(const void *yGrad, uint64_t yGradStride, const void *sum, HcclDataType type, uint64_t rows, uint64_t width,
+    uint64_t sumStride, const void *gain, HcclDataType gainType, float epsilon, const void *sumGrad, uint64_t sumGradStride, void *xGrad,
+    uint64_t xGradStride, float *gainGrad, uint32_t accumulate, void *workspace, uint64_t workspaceBytes, void *stream);
+
+/* a[r][i] = g / (1 + exp(-g)) * u with g = h[r][i], u = h[r][width + i]: what stands between an expert's two products.
+ *   h[rows][hStride]              2 * width to a row; FP32, FP16 or BFP16
+ *   used[1]                       how many rows there are, on the device (a receive buffer's offsets[groups], say), brought into [0, rows];
+ *                                 NULL: all.  Rows behind them are left as they are, in every output
+ *   scaleType NONE                out[rows][outStride] in h's type
+ *   FP32, E8M0                    8-bit rows (see above) of a as it is in 32 bits, and scales[rows][scaleStride], ceil(width / 128) to a row */
+extern HcclResult HcclAmdExpertGate(const void *h, HcclDataType type, uint64_t rows, uint64_t width, uint64_t hStride, const int32_t *used,
+    HcclAmdScaleType scaleType, void *out, uint64_t outStride, void *scales, uint64_t scaleStride, void *stream);
+
+/* Gradient of HcclAmdExpertGate, and a once more for the gradient of the weights behind it, for those who did not keep it.
+ *   hGrad[rows][hGradStride]      2 * width to a row; NULL: not wanted; may be h, of the same stride
+ *   a[rows][aStride]              in h's type; NULL: not wanted; may be aGrad, of the same stride */
+extern HcclResult HcclAmdExpertGateGrad(const void *aGrad, uint64_t aGradStride, const void *h, HcclDataType type, uint64_t rows, uint64_t width,
+    uint64_t hStride, const int32_t *used, void *hGrad, uint64_t hGradStride, void *a, uint64_t aStride, void *stream);
+
+typedef enum HcclAmdScoreDef {
+    HCCL_AMD_SCORE_SOFTMAX = 0,
+    HCCL_AMD_SCORE_SIGMOID = 1
+} HcclAmdScore;
+
+/* Chooses topK experts for every token by their scores, s = softmax(logits) over all experts or 1 / (1 + exp(-logits)), and counts them.
+ *   logits, tokenMask, expertOf, rowOf, counts, offsets    as in HcclAmdExpertRoute
+ *   bias[experts]                 added to the scores for the choice alone, in 64 bits; NULL: none.  -inf or NaN: never chosen
+ *   groups, groupsKept, groupTop  the experts are `groups` groups of as many neighbours each; a token's experts come from its groupsKept best groups,
+ *                                 by the sum of a group's groupTop (1 or 2) largest s + bias.  groups = groupsKept = 1: from all of them
+ *   weights[tokens][topK]         weightScale * s, with `renormalise` weightScale * s / (sum of the chosen s): without the bias; 0 where expertOf is -1
+ * Largest s + bias first, worked out in 64 bits, ties to the lowest group and expert.  A logit of -inf or NaN is never chosen, and nor is a group
+ * without any that can be; in a softmax a NaN or +inf logit makes the weights of its token's others NaN, as the formula has it.
+ * topK <= groupsKept * (experts / groups).  workspace: 16-byte aligned, HcclAmdExpertRouteScoredWorkspace bytes, free for other use once the stream
+ * is past the call. */
+extern HcclResult HcclAmdExpertRouteScoredWorkspace(uint64_t tokens, uint32_t experts, uint64_t *bytes);
+extern HcclResult HcclAmdExpertRouteScored(const void *logits, HcclDataType logitType, uint64_t tokens, uint32_t experts, uint64_t logitStride,
+    HcclAmdScore score, const float *bias, uint32_t groups, uint32_t groupsKept, uint32_t groupTop, uint32_t topK, uint32_t renormalise,
+    float weightScale, const uint8_t *tokenMask, int32_t *expertOf, float *weights, int32_t *rowOf, int32_t *counts, int32_t *offsets,
+    void *workspace, uint64_t workspaceBytes, void *stream);
+
+/* Gradient of the logits from weightGrad[tokens][topK]; expertOf as HcclAmdExpertRouteScored left it.  Every logit's gradient is written; those of
+ * tokens that chose nothing are zero, and so are, but for a softmax that is not renormalised, those of experts that were not chosen.  (The bias
+ * only chooses: it has no gradient.) */
+extern HcclResult HcclAmdExpertRouteScoredGrad(const void *logits, HcclDataType logitType, uint64_t tokens, uint32_t experts, uint64_t logitStride,
+    HcclAmdScore score, uint32_t topK, uint32_t renormalise, float weightScale, const int32_t *expertOf, const float *weightGrad, void *logitGrad,
+    uint64_t logitGradStride, void *stream);
+
+/* newBias[e] = bias[e] + rate where counts[e] is below the mean of all experts' counts, - rate where it is above it.  counts[experts] may be one router's or
+ * the sum of all ranks' (HcclAllReduce, INT32).  newBias may be bias. */
+extern HcclResult HcclAmdExpertBias(const int32_t *counts, uint32_t experts, float rate, const float *bias, float *newBias, void *stream);
+
+/* A tensor of gradients: `count` elements behind each other (FP32, FP16 or BFP16), aligned to one.  Lists of these are host memory, read during the
+ * call. */
+typedef struct HcclAmdGradTensorDef {
+    const void *in;
+    void *out;             /* HcclAmdGradClip writes here; may be `in` */
+    uint64_t count;
+    HcclDataType type;
+    uint32_t reserved;     /* 0 */
+} HcclAmdGradTensor;
+
+/* Bytes of device workspace that HcclAmdGradSquares needs (host pointer `bytes`). */
+extern HcclResult HcclAmdGradSquaresWorkspace(const HcclAmdGradTensor *tensors, uint32_t n, uint64_t *bytes);
+
+/* squares[0] = the sum of the squares of all elements of all tensors (added to what is there with `accumulate`), in 64 bits throughout: neither
+ * large nor small gradients leave its range.  Where each rank has part of the gradients, HcclAllReduce (FP64, sum) of the ranks' squares comes next.
+ * workspace: 16-byte aligned, HcclAmdGradSquaresWorkspace bytes, free for other use once the stream is past the call. */
+extern HcclResult HcclAmdGradSquares(const HcclAmdGradTensor *tensors, uint32_t n, uint32_t accumulate, double *squares, void *workspace,
+    uint64_t workspaceBytes, void *stream);
+
+/* With norm = sqrt(squares[0]): out = in * (maxNorm / norm) where norm > maxNorm, else out = in (nothing is read or written then where they are the
+ * same).  maxNorm / norm is rounded to 32 bits once, each product once more to the tensor's type.  norm[1]: written, in 32 bits; NULL: not wanted.  As
+ * the formula has it, a NaN among the gradients makes all of them NaN, an infinity the finite ones 0 and itself NaN: norm[0] says so. */
+extern HcclResult HcclAmdGradClip(const HcclAmdGradTensor *tensors, uint32_t n, const double *squares, float maxNorm, float *norm, void *stream);
 
 #ifdef __cplusplus
 }
