@@ -196,14 +196,40 @@ __global__ void __launch_bounds__(BlockOf(kRowThreads)) NormGradKernel(NormGradA
             more[c][i] = 0.0f;
         }
     }
-    for (int64_t row = int64_t(blockIdx.x) * kRows + slot; row < a.rows; row += int64_t(gridDim.x) * kRows) {
+    const int64_t step = int64_t(gridDim.x) * kRows;
+    int64_t row = int64_t(blockIdx.x) * kRows + slot;
+    T nextD[kChunks][kEach], nextS[kChunks][kEach];
+    const auto load = [&]() {
+        if (row < a.rows) {
+#pragma unroll
+            for (int c = 0; c < kChunks; c++) {
+                LoadPart<kHow, kEach>(static_cast<const T *>(a.yGrad) + row * a.yGradStride, (c * kRowThreads + l) * kEach, a.width, nextD[c], T(0.0f));
+                LoadPart<kHow, kEach>(static_cast<const T *>(a.sum) + row * a.sumStride, (c * kRowThreads + l) * kEach, a.width, nextS[c], T(0.0f));
+            }
+        }
+    };
+    load();
+    while (row < a.rows) {
         float d[kChunks][kEach], s[kChunks][kEach];
+        T arrived[kChunks][kEach];
+        double squares = 0.0, dots = 0.0;
 #pragma unroll
         for (int c = 0; c < kChunks; c++) {
-            LoadPart<kHow, kEach>(static_cast<const T *>(a.yGrad) + row * a.yGradStride, (c * kRowThreads + l) * kEach, a.width, d[c]);
-            LoadPart<kHow, kEach>(static_cast<const T *>(a.sum) + row * a.sumStride, (c * kRowThreads + l) * kEach, a.width, s[c]);
+#pragma unroll
+            for (int i = 0; i < kEach; i++) {
+                d[c][i] = float(nextD[c][i]);
+                s[c][i] = float(nextS[c][i]);
+            }
         }
-        double squares = 0.0, dots = 0.0;
+#pragma unroll
+        for (int c = 0; c < kChunks; c++) {
+            if (a.sumGrad != nullptr) {
+                LoadPart<kHow, kEach>(static_cast<const T *>(a.sumGrad) + row * a.sumGradStride, (c * kRowThreads + l) * kEach, a.width, arrived[c], T(0.0f));
+            }
+        }
+        const int64_t here = row;
+        row += step;
+        load();       // the next row is on its way while this one is summed up
 #pragma unroll
         for (int c = 0; c < kChunks; c++) {
 #pragma unroll
@@ -238,17 +264,10 @@ __global__ void __launch_bounds__(BlockOf(kRowThreads)) NormGradKernel(NormGradA
                 const float n = s[c][i] * by;
                 more[c][i] = __builtin_fmaf(d[c][i], n, more[c][i]);
                 out[i] = by * (d[c][i] * gain[c][i] - n * mean);
+                out[i] += a.sumGrad != nullptr ? float(arrived[c][i]) : 0.0f;
             }
             if (a.xGrad != nullptr) {
-                if (a.sumGrad != nullptr) {
-                    float t[kEach];
-                    LoadPart<kHow, kEach>(static_cast<const T *>(a.sumGrad) + row * a.sumGradStride, at, a.width, t);
-#pragma unroll
-                    for (int i = 0; i < kEach; i++) {
-                        out[i] += t[i];
-                    }
-                }
-                StorePart<kHow, kEach>(static_cast<T *>(a.xGrad) + row * a.xGradStride, at, a.width, out);
+                StorePart<kHow, kEach>(static_cast<T *>(a.xGrad) + here * a.xGradStride, at, a.width, out);
             }
         }
         if constexpr (kRowThreads > 64) {
@@ -341,12 +360,11 @@ HcclResult ByType(HcclDataType type, F f)
     return type == HCCL_DATA_TYPE_FP32 ? f(float{}) : type == HCCL_DATA_TYPE_FP16 ? f(_Float16{}) : f(__bf16{});
 }
 
-constexpr uint64_t kMostGradBlocks = 512;   // workgroups that go through rows: two to a compute unit
-
+// Workgroups that go through rows: what makes 16 waves to a compute unit.
 uint64_t GradBlocks(uint64_t rows, uint64_t width)
 {
-    const uint64_t each = width <= 1024 ? 4 : 1, blocks = (rows + each - 1) / each;
-    return blocks < kMostGradBlocks ? blocks : kMostGradBlocks;
+    const uint64_t each = width <= 1024 ? 4 : 1, blocks = (rows + each - 1) / each, most = width <= 4096 ? 1024 : width <= 8192 ? 512 : 256;
+    return blocks < most ? blocks : most;
 }
 
 // Whether rows at p can be taken 16 bytes at a time.

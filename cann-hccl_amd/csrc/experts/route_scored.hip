@@ -6,7 +6,7 @@
 //   softmax, renormalised   dx_j = w_j (dw_j - sum_i (w_i / c) dw_i)  over the chosen ones; the others' gradients are zero
 //   softmax                 dx_e = s_e (c dw_e - sum_i c s_i dw_i)    over all experts, dw_e = 0 where e was not chosen
 //
-// 16 lanes to a token (64 beyond 256 experts), its logits in registers.  Scores next to each other decide which expert a token goes to, and the choice
+// 8, 16 or 64 lanes to a token, its logits in registers.  Scores next to each other decide which expert a token goes to, and the choice
 // is that of 64 bits; but it is made in 32 wherever these are enough.  A score and its bias become a whole number of 22 bits, a word of that and
 // the expert goes into sorted lists by one median of three per entry, and the lists of a token's lanes are merged.  What the 22 bits are off by at most
 // is known, so that a choice is settled unless, at some place that matters, two of them are closer than that and not made from the same logit and
@@ -44,116 +44,132 @@ __device__ __forceinline__ int Anew(int lane)
     return lane;
 }
 
+// The same of a number that all lanes have: masks made from it are two scalar registers each.
+__device__ __forceinline__ int AnewForAll(int n)
+{
+    asm volatile("" : "+s"(n));
+    return n;
+}
+
 // Expert number of element i of lane l: eight neighbours to a lane, then the next lane's.
 template <int kLanes>
 __device__ __forceinline__ int ExpertOf(int i, int l) { return (i / 8 * kLanes + l) * 8 + i % 8; }
 
 // ---- the choice in 64 bits --------------------------------------------------------------------------------
-// One token's, by a whole wave: its experts best first, -1 where there is none.  kEach: a lane's experts, 64 apart.  `of`: a place per group, in LDS.
+// A key and its expert, and which of two is first: the larger, the lower expert of equal ones.
+struct Choice {
+    double key;
+    int expert;
+};
+
+__device__ __forceinline__ bool Before(Choice a, Choice b) { return a.key > b.key || (a.key == b.key && a.expert < b.expert); }
+
+__device__ __forceinline__ Choice First(Choice a, Choice b)
+{
+    const bool take = Before(b, a);
+    return Choice{take ? b.key : a.key, take ? b.expert : a.expert};
+}
+
+template <int kBy>
+__device__ __forceinline__ Choice TurnedChoice(Choice c)
+{
+    return Choice{Turned<kBy>(c.key), __builtin_amdgcn_update_dpp(0, c.expert, 0x120 + kBy, 0xf, 0xf, true)};
+}
+
+__device__ __forceinline__ Choice ChoiceFrom(Choice c, int lane) { return Choice{FromLane(c.key, lane), __builtin_amdgcn_readlane(c.expert, lane)}; }
+
+// Over a whole wave.
+__device__ __forceinline__ Choice FirstOfWave(Choice c)
+{
+    c = First(c, TurnedChoice<8>(c));
+    c = First(c, TurnedChoice<4>(c));
+    c = First(c, TurnedChoice<2>(c));
+    c = First(c, TurnedChoice<1>(c));
+    return First(First(ChoiceFrom(c, 0), ChoiceFrom(c, 16)), First(ChoiceFrom(c, 32), ChoiceFrom(c, 48)));
+}
+
+// One token's, by a whole wave: its experts best first, -1 where there is none.  kEach: a lane's experts, 64 apart.  `keys`: a place per expert, `of`: one per
+// group, in LDS.  Loops, not straight code: this is seldom called, and every instruction has to be fetched then.
 template <int kEach, int K, typename T>
-__device__ __forceinline__ void ChooseExactly(const ScoredArgs &a, const T *row, double *of, int (&chosen)[K])
+__device__ __forceinline__ void ChooseExactly(const ScoredArgs &a, const T *row, double *keys, double *of, int (&chosen)[K])
 {
     const int lane = Anew(int(__lane_id()));
-    float x[kEach];
-    double key[kEach];
-#pragma unroll
-    for (int i = 0; i < kEach; i++) {
-        x[i] = i * 64 + lane < a.experts ? float(row[i * 64 + lane]) : -__builtin_inff();
-    }
+    float top = -__builtin_inff();
+    double sum = 1.0;
     if (a.softmax) {
         // (a NaN is left out, +inf takes all)
-        float top = -__builtin_inff();
-#pragma unroll
-        for (int i = 0; i < kEach; i++) {
-            top = Larger(top, x[i]);
+        for (int e = lane; e < a.experts; e += 64) {
+            top = Larger(top, float(row[e]));
         }
         top = LargestOfNeighbours<64>(top);
-        double sum = 0.0;
-#pragma unroll
-        for (int i = 0; i < kEach; i++) {
-            key[i] = x[i] == top ? 1.0 : x[i] < top ? exp(double(x[i]) - double(top)) : 0.0;
-            sum += key[i];
+        sum = 0.0;
+#pragma unroll 1
+        for (int e = lane; e < a.experts; e += 64) {
+            const float x = float(row[e]);
+            sum += x == top ? 1.0 : x < top ? exp(double(x) - double(top)) : 0.0;
         }
         sum = AddWave(sum);
-#pragma unroll
-        for (int i = 0; i < kEach; i++) {
-            key[i] /= sum;
-        }
-    } else {
-#pragma unroll
-        for (int i = 0; i < kEach; i++) {
-            key[i] = 1.0 / (1.0 + exp(-double(x[i])));
-        }
     }
-#pragma unroll
-    for (int i = 0; i < kEach; i++) {
-        if (a.bias != nullptr) {
-            key[i] += double(a.bias[min(i * 64 + lane, a.experts - 1)]);
-        }
-        key[i] = x[i] > -__builtin_inff() && key[i] > kNever ? key[i] : kNever;
+#pragma unroll 1
+    for (int e = lane; e < a.experts; e += 64) {
+        const float x = float(row[e]);
+        const double p = exp(a.softmax ? (x == top ? 0.0 : double(x) - double(top)) : -double(x));
+        const double key = (a.softmax ? p / sum : 1.0 / (1.0 + p)) + (a.bias != nullptr ? double(a.bias[e]) : 0.0);
+        keys[e] = x > -__builtin_inff() && key > kNever ? key : kNever;
     }
+    Ordered();
+    unsigned long long keep = ~0ull;
     if (a.groups > 1) {
-        for (int g = 0; g < a.groups; g++) {
-            double first = kNever, next = kNever;
-#pragma unroll
-            for (int i = 0; i < kEach; i++) {
-                const bool mine = int(uint32_t(i * 64 + lane) * a.perSize >> 20) == g;
-                const double k = mine ? key[i] : kNever;
-                next = k > first ? first : k > next ? k : next;
-                first = k > first ? k : first;
+        double mine = kNever;
+        if (lane < a.groups) {
+            double next = kNever;
+            int at = lane % a.size;            // (neighbouring lanes begin at different banks)
+#pragma unroll 4
+            for (int i = 0; i < a.size; i++) {
+                const double k = keys[lane * a.size + at];
+                next = k > mine ? mine : k > next ? k : next;
+                mine = k > mine ? k : mine;
+                at = at + 1 == a.size ? 0 : at + 1;
             }
-#pragma unroll
-            for (int d = 1; d < 64; d <<= 1) {
-                const double f = __shfl_xor(first, d, 64), n = __shfl_xor(next, d, 64);
-                const double low = first < f ? first : f, rest = next > n ? next : n;
-                next = low > rest ? low : rest;
-                first = first > f ? first : f;
-            }
-            if (lane == 0) {
-                of[g] = a.second && next > kNever ? first + next : first;
-            }
+            mine = a.second && next > kNever ? mine + next : mine;
+            of[lane] = mine;
         }
         Ordered();
-        const double mine = lane < a.groups ? of[lane] : kNever;
         int before = 0;
+#pragma unroll 4
         for (int o = 0; o < a.groups; o++) {
             const double other = of[o];
             before += other > mine || (other == mine && o < lane) ? 1 : 0;
         }
-        const unsigned long long keep = __ballot(lane < a.groups && before < a.kept);
-        Ordered();
+        keep = __ballot(lane < a.groups && before < a.kept);
+    }
+    double key[kEach];
+#pragma unroll
+    for (int i = 0; i < kEach; i++) {
+        const int e = i * 64 + lane;
+        const uint32_t g = a.groups > 1 ? uint32_t(e) * a.perSize >> 20 : 0;
+        key[i] = e < a.experts && (keep >> (g & 63) & 1) != 0 ? keys[min(e, a.experts - 1)] : kNever;
+    }
+    Ordered();
+    int taken = -1;                            // lane j: the j-th
+#pragma unroll 1
+    for (int j = 0; j < a.topK; j++) {
+        Choice best{kNever, -1};
 #pragma unroll
         for (int i = 0; i < kEach; i++) {
-            const uint32_t g = uint32_t(i * 64 + lane) * a.perSize >> 20;
-            key[i] = (keep >> (g & 63) & 1) != 0 ? key[i] : kNever;
+            const bool take = key[i] > best.key;      // (a lane's experts ascend)
+            best = Choice{take ? key[i] : best.key, take ? i * 64 + lane : best.expert};
+        }
+        best = FirstOfWave(best);
+        taken = lane == j ? best.expert : taken;
+#pragma unroll
+        for (int i = 0; i < kEach; i++) {
+            key[i] = i * 64 + lane == best.expert ? kNever : key[i];
         }
     }
 #pragma unroll
-    for (int j = 0; j < K; j++) {
-        chosen[j] = -1;
-        if (j < a.topK) {
-            double best = kNever;
-            int e = -1;
-#pragma unroll
-            for (int i = 0; i < kEach; i++) {
-                const bool take = key[i] > best;      // (a lane's experts ascend)
-                best = take ? key[i] : best;
-                e = take ? i * 64 + lane : e;
-            }
-#pragma unroll
-            for (int d = 1; d < 64; d <<= 1) {
-                const double other = __shfl_xor(best, d, 64);
-                const int oe = __shfl_xor(e, d, 64);
-                const bool take = other > best || (other == best && oe < e);
-                best = take ? other : best;
-                e = take ? oe : e;
-            }
-            chosen[j] = e;
-#pragma unroll
-            for (int i = 0; i < kEach; i++) {
-                key[i] = i * 64 + lane == e ? kNever : key[i];
-            }
-        }
+    for (int i = 0; i < K; i++) {
+        chosen[i] = __builtin_amdgcn_readlane(taken, i);
     }
 }
 
@@ -163,22 +179,58 @@ __device__ __forceinline__ float LogSigmoid(float x) { return fminf(x, 0.0f) - l
 __device__ __forceinline__ float Sigmoid(float x) { return __builtin_amdgcn_rcpf(1.0f + Exp(-x)); }
 
 // ---- the choice in 32 bits --------------------------------------------------------------------------------
-// A score and its bias as a whole number: 1 + (s + b - least b) * times, below 2^22.  One step is (1 + largest b - least b) / 2^22.  With U = 2^-24, the
-// difference b - least b, the sum and the product are each off by at most 2^22 U = 1/4 step, cutting off takes up to 1.  A sigmoid is off by
+// A score and its bias as a whole number: 1 + (s + b - least b) * times, below 2^22; 0 for an expert that cannot be chosen.  One step is
+// (1 + largest b - least b) / 2^22.  With U = 2^-24, the difference b - least b, its product and the sum with s are each off by at most 2^22 U = 1/4 step,
+// cutting off takes up to 1.  A sigmoid is off by
 //   s (1 - s) (2 U |x| + 2 U)   the power's argument and the power         (|x| s (1 - s) < 0.23)
 //   s (U + 2 U)                 the sum and the reciprocal
-// which is 4 U, 1 step at most: two numbers are off against each other by twice 2.75.  A softmax's power, quotient and product are off by 5 U, and its sum, of 16 to a
-// lane over up to 64 lanes, by 36 U, the same for all of a token's: 46 U, 11.5 steps between two of them, and 3.5 for the rest.
+// which is 4 U, 1 step at most: two numbers are off against each other by twice 2.75.  A softmax's power, quotient and product are off by 5 U, and its sum, of 32 to a
+// lane over 8 lanes or 16 over 64, by 50 U, the same for all of a token's: 60 U, 15 steps between two of them, and 3.5 for the rest.
 constexpr uint32_t kSlackSigmoid = 8, kSlackSoftmax = 24;
 
-// Three bytes of DPP: the other lane of a pair, the other pair of four, the other four of eight, the other eight of sixteen (mirrored, where the
-// lanes of each part are alike).
+// DPP of the other lane of a pair, the other pair of four, the other four of eight, the other eight of sixteen (mirrored, where the lanes of each
+// part are alike).
 constexpr int kOther[4] = {0xb1, 0x4e, 0x141, 0x140};
 
 template <int kWhich>
 __device__ __forceinline__ uint32_t Other(uint32_t x)
 {
     return uint32_t(__builtin_amdgcn_update_dpp(0, int(x), kOther[kWhich], 0xf, 0xf, true));
+}
+
+template <int kWhich>
+__device__ __forceinline__ float Other(float x)
+{
+    return __int_as_float(__builtin_amdgcn_update_dpp(0, __float_as_int(x), kOther[kWhich], 0xf, 0xf, true));
+}
+
+// f(v, the other's) step by step until the kLanes lanes of a token have the same.
+template <int kLanes, typename V, typename F>
+__device__ __forceinline__ V OverLanes(V v, F f)
+{
+    v = f(v, Other<0>(v));
+    v = f(v, Other<1>(v));
+    v = f(v, Other<2>(v));
+    if constexpr (kLanes > 8) {
+        v = f(v, Other<3>(v));
+    }
+    if constexpr (kLanes == 64) {
+        v = f(v, __shfl_xor(v, 16, 64));
+        v = f(v, __shfl_xor(v, 32, 64));
+    }
+    return v;
+}
+
+template <int kLanes, typename V>
+__device__ __forceinline__ V AddLanes(V v)
+{
+    return OverLanes<kLanes>(v, [](V a, V b) { return a + b; });
+}
+
+template <int kLanes>
+__device__ __forceinline__ float LargestOfLanes(float v)
+{
+    return OverLanes<kLanes>(v, [](float a, float b) { return Larger(a, b); });
 }
 
 __device__ __forceinline__ uint32_t Max(uint32_t a, uint32_t b) { return a > b ? a : b; }
@@ -190,6 +242,14 @@ __device__ __forceinline__ uint32_t Median(uint32_t a, uint32_t b, uint32_t c)
     uint32_t m;
     asm("v_med3_u32 %0, %1, %2, %3" : "=v"(m) : "v"(a), "v"(b), "v"(c));
     return m;
+}
+
+// The hardware's conversion: what is below 1, -inf and NaN become 0.
+__device__ __forceinline__ uint32_t Whole(float x)
+{
+    uint32_t n;
+    asm("v_cvt_u32_f32 %0, %1" : "=v"(n) : "v"(x));
+    return n;
 }
 
 // The larger half of two sorted lists: element by element against the other one backwards, which leaves a sequence that rises and falls once, then
@@ -234,82 +294,57 @@ __device__ __forceinline__ void MergeTwo(uint32_t &first, uint32_t &next)
     first = Max(first, f);
 }
 
-template <int kLanes>
-__device__ __forceinline__ uint32_t AddAll(uint32_t x)
-{
-    x += Other<0>(x);
-    x += Other<1>(x);
-    x += Other<2>(x);
-    x += Other<3>(x);
-    if constexpr (kLanes == 64) {
-        x += uint32_t(__shfl_xor(int(x), 16, 64));
-        x += uint32_t(__shfl_xor(int(x), 32, 64));
-    }
-    return x;
-}
-
 // What a launch's biases make of whole numbers.
 struct Steps {
-    float least, times;
+    float times;
     uint32_t slack;      // two numbers this close or closer need not be in their order
     bool fine;           // false: a bias is infinite, everything is chosen in 64 bits
 };
 
-// A lane's biases above the least of all, and what becomes of them.  Called by whole waves, which find out the same.
-template <int kLanes, int kEach>
-__device__ __forceinline__ Steps StepsOf(const ScoredArgs &a, int l, float (&bias)[kEach])
+// The part of the numbers that the biases make, -inf where the bias is -inf or NaN, into LDS.  Called by all waves, which find out the same.
+template <int kMost>
+__device__ __forceinline__ Steps StepsOf(const ScoredArgs &a, float *part)
 {
-    Steps s{0.0f, 0.0f, a.softmax ? kSlackSoftmax : kSlackSigmoid, true};
-    float least = 0.0f, most = 0.0f;
+    Steps s{float((1 << 22) - 4), a.softmax ? kSlackSoftmax : kSlackSigmoid, true};
+    float least = __builtin_inff(), most = -__builtin_inff();
     if (a.bias != nullptr) {
         bool infinite = false;
-        least = __builtin_inff();
-        most = -__builtin_inff();
-#pragma unroll
-        for (int i = 0; i < kEach; i++) {
-            const int e = ExpertOf<kLanes>(i, l);
-            const float b = a.bias[min(e, a.experts - 1)];
-            bias[i] = b > -__builtin_inff() && e < a.experts ? b : -__builtin_inff();
+        for (int e = int(threadIdx.x) % 64; e < a.experts; e += 64) {
+            const float b = a.bias[e];
             infinite = infinite || b == __builtin_inff();
-            most = Larger(most, bias[i]);
-            least = bias[i] > -__builtin_inff() && bias[i] < least ? bias[i] : least;
+            most = Larger(most, b);
+            least = b > -__builtin_inff() && b < least ? b : least;
         }
-#pragma unroll
-        for (int d = 1; d < kLanes; d <<= 1) {
-            most = Larger(most, __shfl_xor(most, d, 64));
-            const float other = __shfl_xor(least, d, 64);
-            least = other < least ? other : least;
-        }
+        most = LargestOfLanes<64>(most);
+        least = -LargestOfLanes<64>(-least);
         s.fine = __ballot(infinite) == 0 && most - least < __builtin_inff();
-        least = least <= most ? least : 0.0f;
-        most = most > least ? most : least;
-    } else {
-#pragma unroll
-        for (int i = 0; i < kEach; i++) {
-            bias[i] = ExpertOf<kLanes>(i, l) < a.experts ? 0.0f : -__builtin_inff();
-        }
     }
-#pragma unroll
-    for (int i = 0; i < kEach; i++) {
-        bias[i] -= least;
+    least = least <= most ? least : 0.0f;
+    s.times = s.times / (1.0f + (most > least ? most - least : 0.0f));
+    for (int e = threadIdx.x; e < kMost; e += kThreads) {
+        const float b = a.bias != nullptr && e < a.experts ? a.bias[e] : 0.0f;
+        part[e] = b > -__builtin_inff() ? __builtin_fmaf(b - least, s.times, 1.0f) : -__builtin_inff();
     }
-    s.least = least;
-    s.times = float((1 << 22) - 4) / (1.0f + (most - least));
     return s;
 }
 
-// Whether a group's experts are those of 1, 2, 4, 8 or 16 neighbouring lanes.
-__host__ __device__ constexpr bool Evenly(int size) { return size % 8 == 0 && size <= 128 && (size & (size - 1)) == 0; }
+// Whether a group's experts are those of 1, 2, 4 or 8 neighbouring lanes.
+__host__ __device__ constexpr bool Evenly(int size) { return size % 8 == 0 && size <= 64 && (size & (size - 1)) == 0; }
 
-// Takes out what is not in a token's best groups.  Returns false where 32 bits do not settle it.  `numbers`: a place per expert, `of`: one per group, the
-// token's, in LDS.
-template <int kLanes, int kEach>
-__device__ __forceinline__ bool ChooseGroups(const ScoredArgs &a, uint32_t (&number)[kEach], uint32_t slack, int l, int lane, uint32_t *numbers, uint32_t *of)
+// Takes out what is not in a token's best groups.  Returns false where 32 bits do not settle which these are.  `numbers`: a place per expert, `of`: one per
+// group and 64 more, the token's, in LDS.
+template <int kLanes, int kEach, bool kEvenly>
+__device__ __forceinline__ bool ChooseGroups(const ScoredArgs &a, uint32_t (&number)[kEach], uint32_t slack, int l, uint32_t *numbers, uint32_t *of)
 {
-    bool sure = true;
     constexpr int kChunks = kEach / 8;
-    const int across = a.size / 8;        // lanes that share a group
-    if (Evenly(a.size)) {
+    // a group's number: the sum of its two largest, or the largest; then its place among the groups, so that no two are alike.  A group with
+    // one choice or none left: its sum has a zero in it, which has no number here.
+    const auto leave = [&](uint32_t g, uint32_t first, uint32_t next) {
+        const uint32_t sum = !a.second ? first : next != 0 ? first + next : first != 0 ? (1u << 24) - 1 : 0;
+        of[g] = sum << 6 | (63 - g);
+    };
+    if constexpr (kEvenly) {
+        const int across = a.size / 8;        // lanes that share a group
 #pragma unroll
         for (int c = 0; c < kChunks; c++) {
             uint32_t first = number[c * 8], next = 0;
@@ -327,16 +362,11 @@ __device__ __forceinline__ bool ChooseGroups(const ScoredArgs &a, uint32_t (&num
             if (across > 4) {
                 MergeTwo<2>(first, next);
             }
-            if (across > 8) {
-                MergeTwo<3>(first, next);
-            }
             const int e = (c * kLanes + l) * 8;
-            if (l % across == 0 && e < a.experts) {
-                // (a group with one choice or none left: its sum has another zero, or none)
-                of[uint32_t(e) * a.perSize >> 20] = !a.second ? first : next != 0 ? first + next : first != 0 ? ~0u : 0;
+            if ((l & (across - 1)) == 0 && e < a.experts) {
+                leave(uint32_t(e) * a.perSize >> 20, first, next);
             }
         }
-        Ordered();
     } else {
 #pragma unroll
         for (int c = 0; c < kChunks; c++) {
@@ -358,82 +388,156 @@ __device__ __forceinline__ bool ChooseGroups(const ScoredArgs &a, uint32_t (&num
                 first = Max(first, n);
                 at = at + 1 == a.size ? 0 : at + 1;
             }
-            of[g] = !a.second ? first : next != 0 ? first + next : first != 0 ? ~0u : 0;
-        }
-        Ordered();
-    }
-    const uint32_t room = a.second ? 2 * slack : slack;
-    uint32_t keep[2] = {0, 0};
-    for (int g0 = 0; g0 < a.groups; g0 += kLanes) {
-        const int g = g0 + l;
-        const uint32_t mine = g < a.groups ? of[g] : 0;
-        int before = 0, close = 0;         // groups in front of this one; those that might be
-        for (int o = 0; o < a.groups; o++) {
-            const uint32_t other = of[o];
-            before += other > mine || (other == mine && o < g) ? 1 : 0;
-            close += other + room >= mine && other <= mine + room ? 1 : 0;
-        }
-        // (a group is close to itself) settled where no group it is not sure of decides whether it is kept
-        const bool kept = mine != 0 && before < a.kept;
-        sure = sure && (mine == 0 || (mine != ~0u && (close == 1 || before + close <= a.kept || before - close >= a.kept)));
-        const unsigned long long bits = __ballot(kept);
-        if constexpr (kLanes == 64) {
-            keep[0] = uint32_t(bits);
-            keep[1] = uint32_t(bits >> 32);
-        } else {
-            const uint32_t part = uint32_t(bits >> (lane & 48)) & 0xffff;
-            keep[0] |= g0 < 32 ? part << (g0 & 16) : 0;
-            keep[1] |= g0 < 32 ? 0 : part << (g0 & 16);
+            leave(uint32_t(g), first, next);
         }
     }
     Ordered();
+    // the number of the last group that is kept: those that reach it are
+    uint32_t least = ~0u, most = 0;      // of the kept ones' numbers, of the others'
+#pragma unroll 1
+    for (int g = l; g < a.groups; g += kLanes) {
+        const uint32_t mine = of[g];
+        int before = 0;
+#pragma unroll 1
+        for (int o = 0; o < a.groups; o += 4) {
+            // (places behind the last group's hold 0)
+            const Word4 four = *reinterpret_cast<const Word4 *>(of + o);
 #pragma unroll
-    for (int i = 0; i < kEach; i++) {
-        const uint32_t g = uint32_t(ExpertOf<kLanes>(i, l)) * a.perSize >> 20;
-        const uint32_t word = g < 32 ? keep[0] : keep[1];
-        number[i] = (word >> (g & 31) & 1) != 0 ? number[i] : 0;
+            for (int i = 0; i < 4; i++) {
+                before += four[i] > mine ? 1 : 0;
+            }
+        }
+        const bool kept = mine >= 64 && before < a.kept;
+        least = kept ? Min(least, mine) : least;
+        most = kept ? most : Max(most, mine);
+        // (one choice among the two that are summed: not settled)
+        most = a.second && mine >> 6 == (1u << 24) - 1 ? ~0u : most;
     }
-    return sure;
+    least = OverLanes<kLanes>(least, [](uint32_t x, uint32_t y) { return Min(x, y); });
+    most = OverLanes<kLanes>(most, [](uint32_t x, uint32_t y) { return Max(x, y); });
+    const auto kept = [&](int e) { return e < a.experts && of[uint32_t(e) * a.perSize >> 20] >= least; };
+#pragma unroll
+    for (int c = 0; c < kChunks; c++) {
+        if constexpr (kEvenly) {
+            const bool use = kept((c * kLanes + l) * 8);
+#pragma unroll
+            for (int i = 0; i < 8; i++) {
+                number[c * 8 + i] = use ? number[c * 8 + i] : 0;
+            }
+        } else {
+#pragma unroll
+            for (int i = 0; i < 8; i++) {
+                number[c * 8 + i] = kept((c * kLanes + l) * 8 + i) ? number[c * 8 + i] : 0;
+            }
+        }
+    }
+    Ordered();
+    return most < 64 || least >> 6 > (most >> 6) + (a.second ? 2 * slack : slack);
 }
 
-// The choice in 32 bits.  Returns false where they do not settle it, on some of the token's lanes.
-template <int kLanes, int kEach, int K, typename T>
-__device__ __forceinline__ bool ChooseFast(const ScoredArgs &a, const Steps &steps, const float (&x)[kEach], const float (&bias)[kEach], const T *row, bool in, int l,
-    int lane, uint32_t *numbers, uint32_t *of, int (&chosen)[K])
+// The keys in 64 bits of two experts of a lane's token.
+template <int kLanes, typename T>
+__device__ __forceinline__ void Keys(const ScoredArgs &a, const T *row, float top, int l, Choice &own, Choice &more)
+{
+    const int at = min(own.expert, a.experts - 1), next = min(more.expert, a.experts - 1);
+    double x = double(float(row[at])), y = double(float(row[next])), total = 1.0;
+    const double b = a.bias != nullptr ? double(a.bias[at]) : 0.0, c = a.bias != nullptr ? double(a.bias[next]) : 0.0;
+    if (a.softmax) {
+        total = 0.0;
+#pragma unroll 1
+        for (int i = l; i < a.experts; i += kLanes) {
+            const float v = float(row[i]);
+            total += v <= top ? exp(double(v) - double(top)) : 0.0;
+        }
+#pragma unroll 1
+        for (int d = 1; d < kLanes; d <<= 1) {
+            total += __shfl_xor(total, d, 64);
+        }
+        x = double(top) - x;
+        y = double(top) - y;
+    }
+    const double p = exp(-x), q = exp(-y);
+    own.key = (a.softmax ? p / total : 1.0 / (1.0 + p)) + b;
+    more.key = (a.softmax ? q / total : 1.0 / (1.0 + q)) + c;
+}
+
+// Whether all that reach the border and are not the token's own are made from the same logit and bias as the last of its own, and none of its own that is close
+// to its neighbour from others than that: such experts tie in 64 bits too, and go by their numbers.  `mine`: lane j has the j-th.
+template <int kLanes, int kEach, typename T>
+__device__ __forceinline__ bool Ties(const ScoredArgs &a, const T *row, const uint32_t (&number)[kEach], uint32_t mine, uint32_t border, uint32_t room, int l, int lane)
+{
+    const int e = min(int(1023u - (mine & 1023u)), a.experts - 1);
+    const float logit = float(row[e]), b = a.bias != nullptr ? a.bias[e] : 0.0f;
+    const int from = lane - l + a.topK - 1;
+    const float lastLogit = __shfl(logit, from, 64), lastBias = __shfl(b, from, 64);
+    const uint32_t next = uint32_t(__shfl_down(int(mine), 1, 64));
+    const float nextLogit = __shfl_down(logit, 1, 64), nextBias = __shfl_down(b, 1, 64);
+    const uint32_t pairs = AddLanes<kLanes>(l + 1 < a.topK && mine - next <= room && !(logit == nextLogit && b == nextBias) ? 1u : 0u);
+    const uint32_t listed = AddLanes<kLanes>(l < a.topK && mine >= border && !(logit == lastLogit && b == lastBias) ? 1u : 0u);
+    uint32_t others = 0;
+#pragma unroll
+    for (int i = 0; i < kEach; i++) {
+        if (number[i] >= border) {
+            const int at = ExpertOf<kLanes>(i, l);
+            others += !(float(row[at]) == lastLogit && (a.bias == nullptr || a.bias[at] == lastBias)) ? 1 : 0;
+        }
+    }
+    return pairs == 0 && AddLanes<kLanes>(others) == listed;
+}
+
+// The choice in 32 bits.  Returns false where they do not settle it, on some of the token's lanes.  Of a softmax also the row's largest logit and the sum of
+// the powers, NaN where a logit is NaN or +inf.
+template <int kLanes, int kEach, int K, bool kEvenly, typename T>
+__device__ __forceinline__ bool ChooseFast(const ScoredArgs &a, const Steps &steps, const float (&x)[kEach], const float *part, const T *row, bool in, int l,
+    int lane, uint32_t *numbers, uint32_t *of, int (&chosen)[K], float &top, float &sum)
 {
     uint32_t number[kEach];
+    float s[kEach], by = steps.times, largest = -__builtin_inff();
+#pragma unroll
+    for (int i = 0; i < kEach; i++) {
+        largest = __builtin_fmaxf(largest, x[i]);      // (leaves NaN out)
+    }
     if (a.softmax) {
-        float top = -__builtin_inff(), sum = 0.0f, s[kEach];
+        bool bad = false;
 #pragma unroll
         for (int i = 0; i < kEach; i++) {
-            top = Larger(top, x[i]);
+            bad = bad || !(x[i] < __builtin_inff());
         }
-        top = LargestOfNeighbours<kLanes>(top);
+        top = OverLanes<kLanes>(largest, [](float u, float v) { return __builtin_fmaxf(u, v); });
+        sum = 0.0f;
 #pragma unroll
         for (int i = 0; i < kEach; i++) {
-            s[i] = x[i] == top ? 1.0f : x[i] < top ? Exp(x[i] - top) : 0.0f;
+            // (+inf takes all, a NaN is left out)
+            s[i] = Exp(x[i] == top ? 0.0f : x[i] - top);
+            s[i] = x[i] <= top ? s[i] : 0.0f;
             sum += s[i];
         }
-        const float by = 1.0f / AddNeighbours<kLanes>(sum);
-#pragma unroll
-        for (int i = 0; i < kEach; i++) {
-            number[i] = 1 + uint32_t((s[i] * by + bias[i]) * steps.times);
-        }
+        sum = AddLanes<kLanes>(sum);
+        by = steps.times / sum;
+        sum = AddLanes<kLanes>(bad ? 1.0f : 0.0f) > 0.0f ? __builtin_nanf("") : sum;
     } else {
 #pragma unroll
         for (int i = 0; i < kEach; i++) {
-            number[i] = 1 + uint32_t((Sigmoid(x[i]) + bias[i]) * steps.times);
+            s[i] = Sigmoid(x[i]);
         }
     }
-    // (bias[i]: above the least one, -inf where the expert is never chosen)
 #pragma unroll
-    for (int i = 0; i < kEach; i++) {
-        number[i] = x[i] > -__builtin_inff() && bias[i] >= 0.0f ? number[i] : 0;
+    for (int c = 0; c < kEach / 8; c++) {
+        float p[8];
+        Load<true, 8>(part + (c * kLanes + l) * 8, p);
+#pragma unroll
+        for (int i = 0; i < 8; i++) {
+            // (0 * x is NaN where the logit is infinite or NaN)
+            number[c * 8 + i] = Whole(__builtin_fmaf(s[c * 8 + i], by, __builtin_fmaf(x[c * 8 + i], 0.0f, p[i])));
+        }
     }
-    bool sure = true;
+    bool sure = !(largest == __builtin_inff());       // (+inf can be chosen, but not like this)
     if (a.groups > 1) {
-        sure = ChooseGroups<kLanes, kEach>(a, number, steps.slack, l, lane, numbers, of);
+        const bool settled = ChooseGroups<kLanes, kEach, kEvenly>(a, number, steps.slack, l, numbers, of);
+        sure = sure && settled;
     }
+    // a word is a number and the expert, complemented; below kLeast there is no choice in it
+    constexpr uint32_t kLeast = 1024;
     uint32_t best[K];
 #pragma unroll
     for (int i = 0; i < K; i++) {
@@ -441,17 +545,21 @@ __device__ __forceinline__ bool ChooseFast(const ScoredArgs &a, const Steps &ste
     }
 #pragma unroll
     for (int i = 0; i < kEach; i++) {
-        number[i] = number[i] != 0 ? number[i] << 10 | (1023u - uint32_t(ExpertOf<kLanes>(i, l))) : 0;
+        number[i] = number[i] << 10 | (1023u - uint32_t(ExpertOf<kLanes>(i, l)));
 #pragma unroll
         for (int k = K - 1; k > 0; k--) {
-            best[k] = Median(best[k - 1], best[k], number[i]);
+            if (k <= i) {      // (the first ones meet empty places)
+                best[k] = k < i ? Median(best[k - 1], best[k], number[i]) : Min(best[k - 1], number[i]);
+            }
         }
         best[0] = Max(best[0], number[i]);
     }
     MergeOther<0>(best);
     MergeOther<1>(best);
     MergeOther<2>(best);
-    MergeOther<3>(best);
+    if constexpr (kLanes > 8) {
+        MergeOther<3>(best);
+    }
     if constexpr (kLanes == 64) {
 #pragma unroll 1
         for (int d = 16; d < 64; d <<= 1) {
@@ -465,68 +573,84 @@ __device__ __forceinline__ bool ChooseFast(const ScoredArgs &a, const Steps &ste
     }
     // places that are too close: among the chosen ones, and at the border
     const uint32_t room = (steps.slack + 1) << 10;
-    uint32_t last = 0;
-    bool close = false;
+    uint32_t last = 0, gap = ~0u;
 #pragma unroll
     for (int i = 0; i < K; i++) {
         last = i + 1 == a.topK ? best[i] : last;
         if (i + 1 < K) {
-            close = close || (i + 1 < a.topK && best[i] - best[i + 1] <= room);
+            gap = i + 1 < a.topK ? Min(gap, best[i] - best[i + 1]) : gap;
         }
     }
-    const uint32_t border = last > room ? last - room : 1;
-    uint32_t above = 0;
+    uint32_t beyond = ~0u;        // how far below the last one the next of the others is (those above it wrap round)
 #pragma unroll
     for (int i = 0; i < kEach; i++) {
-        above += number[i] >= border ? 1 : 0;
+        beyond = Min(beyond, last - 1 - number[i]);
     }
-    above = AddAll<kLanes>(above);
-    close = close || above != uint32_t(a.topK);
-    if (__ballot(in && close) != 0) {
-        // what is made from the same logit and bias ties in 64 bits too, and goes by its number; the others do not
-        const bool has = l < a.topK;
+    beyond = OverLanes<kLanes>(beyond, [](uint32_t u, uint32_t v) { return Min(u, v); });
+    const bool close = in && sure && (gap <= room || beyond < room);
+    sure = sure && last >= kLeast;
+    if (__ballot(close) != 0) {
+        // lane j has the j-th
         uint32_t mine = 0;
 #pragma unroll
         for (int i = 0; i < K; i++) {
             mine = l == i ? best[i] : mine;
         }
-        const int e = mine != 0 ? int(1023u - (mine & 1023u)) : 0;
-        const float logit = mine != 0 ? float(row[e]) : 0.0f, b = mine != 0 && a.bias != nullptr ? a.bias[e] : 0.0f;
-        const int from = lane - l + a.topK - 1;
-        const float lastLogit = __shfl(logit, from, 64), lastBias = __shfl(b, from, 64);
-        const uint32_t next = uint32_t(__shfl_down(int(mine), 1, 64));
-        const float nextLogit = __shfl_down(logit, 1, 64), nextBias = __shfl_down(b, 1, 64);
-        const bool pair = l + 1 < a.topK && mine - next <= room && !(logit == nextLogit && b == nextBias);
-        const uint32_t listed = AddAll<kLanes>(has && !(logit == lastLogit && b == lastBias) ? 1 : 0);
-        uint32_t others = 0;
+        const uint32_t border = last >= kLeast + room ? last - room : kLeast, extra = last - 1 - beyond;      // the next of the others
+        uint32_t above = 0;
 #pragma unroll
         for (int i = 0; i < kEach; i++) {
-            // (the biases themselves: two of them may be as far above the least, in 32 bits)
-            const float own = a.bias != nullptr ? a.bias[min(ExpertOf<kLanes>(i, l), a.experts - 1)] : 0.0f;
-            others += number[i] >= border && !(x[i] == lastLogit && own == lastBias) ? 1 : 0;
+            above += number[i] >= border ? 1 : 0;
         }
-        others = AddAll<kLanes>(others);
-        sure = sure && !pair && last != 0 && others == listed;
+        above = AddLanes<kLanes>(above);
+        const bool few = sure && above <= uint32_t(a.topK) + 1;
+        if (__ballot(close && !few) != 0) {
+            const bool ties = Ties<kLanes>(a, row, number, mine, border, room, l, lane);
+            sure = sure && (!close || few || ties);
+        }
+        if (__ballot(close && few) != 0) {
+            // between these and one more by their keys in 64 bits
+            Choice own{kNever, int(1023u - (mine & 1023u))}, more{kNever, int(1023u - (extra & 1023u))};
+            Keys<kLanes>(a, row, top, l, own, more);
+            // (without another one within reach its key says nothing)
+            more.key = above > uint32_t(a.topK) ? more.key : kNever;
+            int place = 0;
+            for (int i = 0; i < a.topK; i++) {
+                const Choice other{__shfl(own.key, lane - l + i, 64), __shfl(own.expert, lane - l + i, 64)};
+                place += Before(other, own) ? 1 : 0;
+            }
+            // the one more moves back what it goes before, and goes where they were
+            const bool after = l < a.topK && Before(more, own);
+            const int moved = int(AddLanes<kLanes>(after ? 1u : 0u));
+            place += after ? 1 : 0;
+#pragma unroll
+            for (int i = 0; i < K; i++) {
+                const uint32_t word = AddLanes<kLanes>(l < a.topK && place == i ? mine : 0u);
+                best[i] = close && few && i < a.topK ? (moved > 0 && i == a.topK - moved ? extra : word) : best[i];
+            }
+        }
     }
 #pragma unroll
     for (int i = 0; i < K; i++) {
-        chosen[i] = i < a.topK && in && best[i] != 0 ? int(1023u - (best[i] & 1023u)) : -1;
+        chosen[i] = i < a.topK && in && best[i] >= kLeast ? int(1023u - (best[i] & 1023u)) : -1;
     }
     return sure || !in;
 }
 
-template <typename T, int K, int kLanes, int kEach, int kHow>
-__global__ void __launch_bounds__(kThreads, kLanes == 64 ? 2 : 4) ScoredKernel(ScoredArgs a)
+template <typename T, int K, int kLanes, int kEach, bool kEvenly>
+__global__ void __launch_bounds__(kThreads, kLanes == 64 ? 2 : 4) ScoredKernel(ScoredArgs args)
 {
+    ScoredArgs a = args;
     constexpr int kWaveTokens = 64 / kLanes, kTile = kWaveTokens * kThreads / 64;
     extern __shared__ uint32_t lds[];
     const int E = a.experts;
     uint32_t *chose = lds;                                                // [experts]: one bit per token of the tile
     int *count = reinterpret_cast<int *>(chose + E);                      // [experts]: rows of the tiles so far
-    int *part = count + E;                                                // [waves]
-    int *routed = part + kThreads / 64;                                   // [1]
-    __shared__ double groupScores[kThreads / 64][HCCL_AMD_MAX_EXPERT_GROUPS];
-    __shared__ uint32_t groupNumbers[kTile][HCCL_AMD_MAX_EXPERT_GROUPS];
+    int *parts = count + E;                                               // [waves]
+    int *routed = parts + kThreads / 64;                                  // [1]
+    __shared__ double groupKeys[kThreads / 64][HCCL_AMD_MAX_EXPERT_GROUPS];
+    __shared__ double keys[kThreads / 64][kLanes * kEach];
+    __shared__ __align__(16) uint32_t groupNumbers[kTile][HCCL_AMD_MAX_EXPERT_GROUPS];
     uint32_t *numbers = reinterpret_cast<uint32_t *>(routed + 1);         // [tokens of the tile][experts], for groups that lanes do not share evenly
 
     const int wave = int(threadIdx.x) / 64;
@@ -537,10 +661,14 @@ __global__ void __launch_bounds__(kThreads, kLanes == 64 ? 2 : 4) ScoredKernel(S
     if (threadIdx.x == 0) {
         *routed = 0;
     }
-    float bias[kEach];
-    const Steps steps = StepsOf<kLanes, kEach>(a, int(threadIdx.x) % kLanes, bias);
+    for (int i = threadIdx.x; i < kTile * int(HCCL_AMD_MAX_EXPERT_GROUPS); i += kThreads) {
+        groupNumbers[0][i] = 0;
+    }
+    __shared__ __align__(16) float part[kLanes * kEach];
+    const Steps steps = StepsOf<kLanes * kEach>(a, part);
     __syncthreads();
     for (int tile = 0; tile < a.tiles; tile++) {
+        a.topK = AnewForAll(args.topK);
         const int lane = Anew(int(threadIdx.x) % 64), l = lane % kLanes, r = wave * kWaveTokens + lane / kLanes;
         const int token = (int(blockIdx.x) * a.tiles + tile) * kTile + r;
         const bool in = token < a.tokens && (a.mask == nullptr || a.mask[token] != 0);
@@ -550,26 +678,26 @@ __global__ void __launch_bounds__(kThreads, kLanes == 64 ? 2 : 4) ScoredKernel(S
 #pragma unroll
         for (int c = 0; c < kEach / 8; c++) {
             float v[8];
-            LoadPart<kHow, 8>(row, (c * kLanes + l) * 8, a.tokens > 0 ? E : 0, v, -__builtin_inff());
+            LoadPart<kAnyhow, 8>(row, (c * kLanes + l) * 8, a.tokens > 0 ? E : 0, v, -__builtin_inff());
 #pragma unroll
             for (int i = 0; i < 8; i++) {
                 x[c * 8 + i] = v[i];
             }
         }
         int chosen[K];
-        const bool settled = ChooseFast<kLanes, kEach, K>(a, steps, x, bias, row, in, l, lane, numbers + r * E, groupNumbers[r], chosen);
+        float top = 0.0f, total = 0.0f;
+        const bool settled = ChooseFast<kLanes, kEach, K, kEvenly>(a, steps, x, part, row, in, l, lane, numbers + r * E, groupNumbers[r], chosen, top, total);
         const bool sure = steps.fine && settled;
-        const unsigned long long lanes = kLanes == 64 ? ~0ull : 0xffffull << (lane & 48);
         unsigned long long unsure = __ballot(in && !sure);
         while (unsure != 0) {
             const int which = (__ffsll(unsure) - 1) / kLanes, whose = (int(blockIdx.x) * a.tiles + tile) * kTile + wave * kWaveTokens + which;
             int exactly[K];
-            ChooseExactly<kLanes * kEach / 64, K>(a, static_cast<const T *>(a.logits) + int64_t(whose) * a.stride, groupScores[wave], exactly);
+            ChooseExactly<kLanes * kEach / 64, K>(a, static_cast<const T *>(a.logits) + int64_t(whose) * a.stride, keys[wave], groupKeys[wave], exactly);
 #pragma unroll
             for (int i = 0; i < K; i++) {
                 chosen[i] = lane / kLanes == which ? exactly[i] : chosen[i];
             }
-            unsure &= ~(kLanes == 64 ? ~0ull : 0xffffull << which * 16);
+            unsure &= ~(kLanes == 64 ? ~0ull : ((1ull << kLanes % 64) - 1) << which * kLanes);
         }
         // lane j of a token has its j-th choice
         int mine = -1;
@@ -579,35 +707,28 @@ __global__ void __launch_bounds__(kThreads, kLanes == 64 ? 2 : 4) ScoredKernel(S
         }
         const float logit = mine >= 0 ? float(row[mine]) : -__builtin_inff();
         float w;
+        constexpr int kHold = kLanes < 16 ? kLanes : 16;      // lanes that hold choices
         if (a.softmax) {
-            float top = -__builtin_inff(), total = 0.0f;
-            bool bad = false;
-#pragma unroll
-            for (int i = 0; i < kEach; i++) {
-                top = Larger(top, x[i]);
-                bad = bad || !(x[i] < __builtin_inff());
-            }
-            top = LargestOfNeighbours<kLanes>(top);
-#pragma unroll
-            for (int i = 0; i < kEach; i++) {
-                total += Exp(x[i] - top);
-            }
-            total = AddNeighbours<kLanes>(total);
-            if (a.renormalise) {
-                top = LargestOfNeighbours<16>(logit);
-            }
-            w = mine >= 0 ? Exp(logit - top) : 0.0f;
-            w /= a.renormalise ? AddNeighbours<16>(w) : total;
+            const float topChosen = LargestOfLanes<kHold>(logit);
+            w = mine >= 0 ? Exp(logit - (a.renormalise ? topChosen : top)) : 0.0f;
+            const float inside = AddLanes<kHold>(w);
+            w /= a.renormalise ? inside : total;
             // (a NaN or +inf in the row: the weights are NaN, chosen or not by these)
-            const unsigned long long rows = __ballot(bad);
-            w = (rows & lanes) != 0 ? __builtin_nanf("") : w;
-        } else if (a.renormalise) {
-            // by logarithms: the scores of very negative logits are 0 in 32 bits, their ratios are not
-            const float s = mine >= 0 ? LogSigmoid(logit) : -__builtin_inff(), top = LargestOfNeighbours<16>(s);
-            w = mine >= 0 ? Exp(s - top) : 0.0f;
-            w /= AddNeighbours<16>(w);
+            w = total > 0.0f ? w : __builtin_nanf("");
         } else {
             w = Sigmoid(logit);
+            if (a.renormalise) {
+                // scores below 2^-115 lose bits in 32, their ratios do not: by logarithms there
+                float log = w;
+                const bool far = mine >= 0 && logit < -80.0f;
+                if (__ballot(far) != 0) {
+                    log = mine >= 0 ? LogSigmoid(logit) : -__builtin_inff();
+                    const float top = LargestOfLanes<kHold>(log);
+                    w = Exp(log - top);
+                }
+                w = mine >= 0 ? w : 0.0f;
+                w /= AddLanes<kHold>(w);
+            }
         }
         if (mine >= 0 && l == 0) {
             atomicAdd(routed, 1);   // a whole number: the order does not matter
@@ -636,7 +757,7 @@ __global__ void __launch_bounds__(kThreads, kLanes == 64 ? 2 : 4) ScoredKernel(S
         const bool last = a.blocks == 1 && tile + 1 == a.tiles;
         if (last) {
             // a single workgroup: its places become rows at once
-            Finish<kThreads, false>(a, count, nullptr, *routed, part, nullptr, true);
+            Finish<kThreads, false>(a, count, nullptr, *routed, parts, nullptr, true);
         }
         if (writes) {
             a.rowOf[at] = place < 0 ? -1 : place + (last ? count[mine] : 0);
@@ -785,29 +906,48 @@ __global__ void __launch_bounds__(kThreads) BiasKernel(const int32_t *counts, in
     }
 }
 
-// Tokens of a tile: four a wave with 16 lanes to each, one with 64.
-int TileOf(uint32_t experts) { return experts <= 256 ? 16 : 4; }
+// Lanes to a token.
+int LanesOf(uint64_t tokens, uint32_t experts, uint32_t topK) { return experts > 256 ? 64 : topK > 8 || tokens <= 4096 ? 16 : 8; }
 
-template <typename T, int K, int kLanes, int kEach>
-HcclResult LaunchScored(const ScoredArgs &a, bool wide, hipStream_t stream)
+int TileOf(uint64_t tokens, uint32_t experts, uint32_t topK) { return kThreads / LanesOf(tokens, experts, topK); }
+
+// Tiles to a workgroup: one, until there are as many workgroups as the launches behind take.  (64 tokens by four workgroups and a launch that joins them take
+// 13 us, by one workgroup 18.)
+int TilesEach(uint64_t tokens, int tile)
 {
-    const size_t lds = 4 * (2 * size_t(a.experts) + kThreads / 64 + 1 + (Evenly(a.size) ? 0 : kThreads / kLanes * size_t(a.experts)));
-    const auto go = [&](auto kernel) { return Launch("HcclAmdExpertRouteScored", kernel, uint32_t(a.blocks), kThreads, lds, stream, a); };
-    return wide ? go(ScoredKernel<T, K, kLanes, kEach, kAligned>) : go(ScoredKernel<T, K, kLanes, kEach, kAnyhow>);
+    const uint64_t tiles = (tokens + uint64_t(tile) - 1) / uint64_t(tile);
+    return tiles == 0 ? 1 : int((tiles + kMostBlocks - 1) / kMostBlocks);
 }
 
-template <typename T, int K>
-HcclResult LaunchScoredShape(const ScoredArgs &a, bool wide, hipStream_t stream)
+int Workgroups(uint64_t tokens, int tile)
 {
-    return a.experts <= 128   ? LaunchScored<T, K, 16, 8>(a, wide, stream)
-           : a.experts <= 256 ? LaunchScored<T, K, 16, 16>(a, wide, stream)
-                              : LaunchScored<T, K, 64, 16>(a, wide, stream);
+    const uint64_t each = uint64_t(tile) * uint64_t(TilesEach(tokens, tile));
+    return tokens == 0 ? 1 : int((tokens + each - 1) / each);
+}
+
+template <typename T, int K, int kLanes, int kEach>
+HcclResult LaunchScored(const ScoredArgs &a, hipStream_t stream)
+{
+    const size_t lds = 4 * (2 * size_t(a.experts) + kThreads / 64 + 1 + (a.groups == 1 || Evenly(a.size) ? 0 : kThreads / kLanes * size_t(a.experts)));
+    const auto go = [&](auto kernel) { return Launch("HcclAmdExpertRouteScored", kernel, uint32_t(a.blocks), kThreads, lds, stream, a); };
+    return a.groups == 1 || Evenly(a.size) ? go(ScoredKernel<T, K, kLanes, kEach, true>) : go(ScoredKernel<T, K, kLanes, kEach, false>);
 }
 
 template <typename T>
-HcclResult LaunchScoredType(const ScoredArgs &a, bool wide, hipStream_t stream)
+HcclResult LaunchScoredType(const ScoredArgs &a, int lanes, hipStream_t stream)
 {
-    return a.topK <= 8 ? LaunchScoredShape<T, 8>(a, wide, stream) : LaunchScoredShape<T, 16>(a, wide, stream);
+    if (lanes == 8) {
+        return a.experts <= 64    ? LaunchScored<T, 8, 8, 8>(a, stream)
+               : a.experts <= 128 ? LaunchScored<T, 8, 8, 16>(a, stream)
+                                  : LaunchScored<T, 8, 8, 32>(a, stream);
+    }
+    if (lanes == 64) {
+        return a.topK <= 8 ? LaunchScored<T, 8, 64, 16>(a, stream) : LaunchScored<T, 16, 64, 16>(a, stream);
+    }
+    if (a.topK <= 8) {
+        return a.experts <= 128 ? LaunchScored<T, 8, 16, 8>(a, stream) : LaunchScored<T, 8, 16, 16>(a, stream);
+    }
+    return a.experts <= 128 ? LaunchScored<T, 16, 16, 8>(a, stream) : LaunchScored<T, 16, 16, 16>(a, stream);
 }
 
 template <typename T, bool kDense, int kHow>
@@ -835,7 +975,9 @@ HcclResult HcclAmdExpertRouteScoredWorkspace(uint64_t tokens, uint32_t experts, 
     EXPERTS_CHK_PTR(bytes);
     EXPERTS_CHK(experts >= 1 && experts <= HCCL_AMD_MAX_EXPERTS);
     EXPERTS_CHK(tokens <= kMaxTokens);
-    const uint64_t blocks = uint64_t(BlocksOf(tokens, TileOf(experts)));
+    // (whatever topK will be)
+    const uint64_t few = uint64_t(Workgroups(tokens, TileOf(tokens, experts, 1))), many = uint64_t(Workgroups(tokens, TileOf(tokens, experts, HCCL_AMD_MAX_TOPK)));
+    const uint64_t blocks = few > many ? few : many;
     *bytes = blocks == 1 ? 0 : 4 * blocks * (uint64_t(experts) + 1);
     return HCCL_SUCCESS;
 }
@@ -872,7 +1014,7 @@ HcclResult HcclAmdExpertRouteScored(const void *logits, HcclDataType logitType, 
             EXPERTS_CHK(workspaceBytes >= needed);
         }
     }
-    const int tile = TileOf(experts);
+    const int tile = TileOf(tokens, experts, topK);
     ScoredArgs a{};
     a.logits = logits;
     a.mask = tokenMask;
@@ -894,14 +1036,13 @@ HcclResult HcclAmdExpertRouteScored(const void *logits, HcclDataType logitType, 
     a.tokens = int(tokens);
     a.experts = int(experts);
     a.topK = int(topK);
-    a.tiles = TilesOf(tokens, tile);
-    a.blocks = BlocksOf(tokens, tile);       // no token: the one workgroup writes the zeros
+    a.tiles = TilesEach(tokens, tile);
+    a.blocks = Workgroups(tokens, tile);       // no token: the one workgroup writes the zeros
     a.blockCounts = static_cast<int32_t *>(workspace);
     const hipStream_t on = static_cast<hipStream_t>(stream);
-    const bool wide = experts % 8 == 0 && Aligned(logits, 16) && uint64_t(a.stride) * SizeOf(logitType) % 16 == 0;
-    HcclResult r = logitType == HCCL_DATA_TYPE_FP32   ? LaunchScoredType<float>(a, wide, on)
-                   : logitType == HCCL_DATA_TYPE_FP16 ? LaunchScoredType<_Float16>(a, wide, on)
-                                                      : LaunchScoredType<__bf16>(a, wide, on);
+    HcclResult r = logitType == HCCL_DATA_TYPE_FP32   ? LaunchScoredType<float>(a, kThreads / tile, on)
+                   : logitType == HCCL_DATA_TYPE_FP16 ? LaunchScoredType<_Float16>(a, kThreads / tile, on)
+                                                      : LaunchScoredType<__bf16>(a, kThreads / tile, on);
     if (r != HCCL_SUCCESS || a.blocks == 1) {
         return r;
     }
