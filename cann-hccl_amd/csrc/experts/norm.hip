@@ -3,8 +3,8 @@
 // With r = (mean s^2 + epsilon)^-1/2, d = dy * gain and n = s r:
 //   y = n * gain      dx = r (d - n mean(d n)) + dsum      dgain = sum over rows of dy * n
 //
-// A row stays in registers between its sums and its results: read once, written once.  64, 256, 512 or 1024 threads to a row, each with one, two or four
-// times eight neighbouring values, so that a lane's accesses are 16 bytes and 16 lanes hold a block of an 8-bit row.  Sums are in 64 bits: a
+// A row stays in registers between its sums and its results: read once, written once.  64 to 1024 threads to a row, each with eight neighbouring values (16 or 32
+// beyond 8192), so that a lane's accesses are 16 bytes and 16 lanes hold a block of an 8-bit row.  Sums are in 64 bits: a
 // square of 32 bits is exact there, and no row overflows.
 #include <type_traits>
 
@@ -27,7 +27,8 @@ struct NormArgs {
     bool powers;               // the scales are powers of two
 };
 
-constexpr int BlockOf(int rowThreads) { return rowThreads < 256 ? 256 : rowThreads; }
+// A wave to a row: four rows to a workgroup.  More than one: a row to a workgroup, whose waves meet twice a row.
+constexpr int BlockOf(int rowThreads) { return rowThreads == 64 ? 256 : rowThreads; }
 
 // The row's sum on all its threads.  `parts`: a place per wave, used by one call between two barriers.
 template <int kRowThreads>
@@ -229,7 +230,9 @@ __global__ void __launch_bounds__(BlockOf(kRowThreads)) NormGradKernel(NormGradA
         }
         const int64_t here = row;
         row += step;
-        load();       // the next row is on its way while this one is summed up
+        if constexpr (kChunks == 1) {
+            load();       // the next row is on its way while this one is summed up (more chunks leave no registers for that)
+        }
 #pragma unroll
         for (int c = 0; c < kChunks; c++) {
 #pragma unroll
@@ -272,6 +275,9 @@ __global__ void __launch_bounds__(BlockOf(kRowThreads)) NormGradKernel(NormGradA
         }
         if constexpr (kRowThreads > 64) {
             __syncthreads();     // before the next row's sums
+        }
+        if constexpr (kChunks > 1) {
+            load();
         }
     }
     if (a.partial == nullptr) {
@@ -340,16 +346,16 @@ HcclResult ByWidth(uint64_t width, F f)
         return f(std::integral_constant<int, 64>{}, One{});
     }
     if (width <= 1024) {
-        return f(std::integral_constant<int, 64>{}, Two{});
+        return f(std::integral_constant<int, 128>{}, One{});
     }
     if (width <= 2048) {
         return f(std::integral_constant<int, 256>{}, One{});
     }
     if (width <= 4096) {
-        return f(std::integral_constant<int, 256>{}, Two{});
+        return f(std::integral_constant<int, 512>{}, One{});
     }
     if (width <= 8192) {
-        return f(std::integral_constant<int, 512>{}, Two{});
+        return f(std::integral_constant<int, 1024>{}, One{});
     }
     return width <= 16384 ? f(std::integral_constant<int, 1024>{}, Two{}) : f(std::integral_constant<int, 1024>{}, Four{});
 }
@@ -363,7 +369,8 @@ HcclResult ByType(HcclDataType type, F f)
 // Workgroups that go through rows: what makes 16 waves to a compute unit.
 uint64_t GradBlocks(uint64_t rows, uint64_t width)
 {
-    const uint64_t each = width <= 1024 ? 4 : 1, blocks = (rows + each - 1) / each, most = width <= 4096 ? 1024 : width <= 8192 ? 512 : 256;
+    const uint64_t each = width <= 512 ? 4 : 1, blocks = (rows + each - 1) / each;
+    const uint64_t most = width <= 512 ? 1024 : width <= 1024 ? 2048 : width <= 2048 ? 1024 : width <= 4096 ? 512 : 256;
     return blocks < most ? blocks : most;
 }
 
