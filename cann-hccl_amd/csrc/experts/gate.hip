@@ -44,9 +44,12 @@ __global__ void __launch_bounds__(kThreads) GateKernel(GateArgs a)
         const int64_t row = w / a.pieces;
         const int at = int(w % a.pieces) * kPiece + int(threadIdx.x % 64) * kEach;
         const T *h = static_cast<const T *>(a.h) + row * a.hStride;
+        T gates[kEach], ups[kEach];
+        Fetch<kWide, kEach>(h, at, a.width, gates);
+        Fetch<kWide, kEach>(h + a.width, at, a.width, ups);
         float g[kEach], u[kEach];
-        LoadPart<kWide, kEach>(h, at, a.width, g);
-        LoadPart<kWide, kEach>(h + a.width, at, a.width, u);
+        Settle<kWide, kEach>(gates, at, a.width, g);
+        Settle<kWide, kEach>(ups, at, a.width, u);
 #pragma unroll
         for (int i = 0; i < kEach; i++) {
             u[i] *= g[i] * Sigmoid(g[i]);
@@ -84,12 +87,16 @@ __global__ void __launch_bounds__(kThreads) GateGradKernel(GateArgs a)
         const int64_t row = w / a.pieces;
         const int at = int(w % a.pieces) * kPiece + int(threadIdx.x % 64) * kEach;
         const T *h = static_cast<const T *>(a.h) + row * a.hStride;
-        float g[kEach], u[kEach], d[kEach];
-        LoadPart<kWide, kEach>(h, at, a.width, g);
-        LoadPart<kWide, kEach>(h + a.width, at, a.width, u);
+        T gates[kEach], ups[kEach], grads[kEach] = {};
+        Fetch<kWide, kEach>(h, at, a.width, gates);
+        Fetch<kWide, kEach>(h + a.width, at, a.width, ups);
         if (a.hGrad != nullptr) {
-            LoadPart<kWide, kEach>(static_cast<const T *>(a.aGrad) + row * a.aGradStride, at, a.width, d);
+            Fetch<kWide, kEach>(static_cast<const T *>(a.aGrad) + row * a.aGradStride, at, a.width, grads);
         }
+        float g[kEach], u[kEach], d[kEach];
+        Settle<kWide, kEach>(gates, at, a.width, g);
+        Settle<kWide, kEach>(ups, at, a.width, u);
+        Settle<kWide, kEach>(grads, at, a.width, d);
         float v[kEach], dg[kEach], du[kEach];
 #pragma unroll
         for (int i = 0; i < kEach; i++) {

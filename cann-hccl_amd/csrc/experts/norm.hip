@@ -30,6 +30,23 @@ struct NormArgs {
 // A wave to a row: four rows to a workgroup.  More than one: a row to a workgroup, whose waves meet twice a row.
 constexpr int BlockOf(int rowThreads) { return rowThreads == 64 ? 256 : rowThreads; }
 
+// The sum of kWaves places, a power of two up to 16, on all lanes: each reads one, and they are added up as AddWave does.
+template <int kWaves>
+__device__ __forceinline__ double AddParts(const double *parts)
+{
+    double x = parts[threadIdx.x % kWaves];
+    if constexpr (kWaves > 8) {
+        x += Turned<8>(x);
+    }
+    if constexpr (kWaves > 4) {
+        x += Turned<4>(x);
+    }
+    if constexpr (kWaves > 2) {
+        x += Turned<2>(x);
+    }
+    return x + Turned<1>(x);
+}
+
 // The row's sum on all its threads.  `parts`: a place per wave, used by one call between two barriers.
 template <int kRowThreads>
 __device__ __forceinline__ double AddRow(double x, double *parts)
@@ -40,11 +57,7 @@ __device__ __forceinline__ double AddRow(double x, double *parts)
             parts[threadIdx.x / 64] = x;
         }
         __syncthreads();
-        x = 0.0;
-#pragma unroll
-        for (int w = 0; w < kRowThreads / 64; w++) {
-            x += parts[w];
-        }
+        x = AddParts<kRowThreads / 64>(parts);
     }
     return x;
 }
@@ -59,9 +72,13 @@ __device__ __forceinline__ void LoadGain(const void *gain, bool gain32, int at, 
             g[i] = 1.0f;
         }
     } else if (gain32) {
-        LoadPart<kHow, kEach>(static_cast<const float *>(gain), at, width, g);
+        float v[kEach];
+        Fetch<kHow, kEach>(static_cast<const float *>(gain), at, width, v);
+        Settle<kHow, kEach>(v, at, width, g);
     } else {
-        LoadPart<kHow, kEach>(static_cast<const T *>(gain), at, width, g);
+        T v[kEach];
+        Fetch<kHow, kEach>(static_cast<const T *>(gain), at, width, v);
+        Settle<kHow, kEach>(v, at, width, g);
     }
 }
 
@@ -92,21 +109,28 @@ __global__ void __launch_bounds__(BlockOf(kRowThreads)) NormKernel(NormArgs a)
     const int l = int(threadIdx.x) % kRowThreads;
     for (int64_t row = int64_t(blockIdx.x) * kRows + int(threadIdx.x) / kRowThreads; row < a.rows; row += int64_t(gridDim.x) * kRows) {
         float s[kChunks][kEach], g[kChunks][kEach];
-#pragma unroll
-        for (int c = 0; c < kChunks; c++) {
-            LoadPart<kHow, kEach>(static_cast<const T *>(a.x) + row * a.xStride, (c * kRowThreads + l) * kEach, a.width, s[c]);
-        }
-        if (a.residual != nullptr) {
-            float r[kChunks][kEach];
+        {
+            T x[kChunks][kEach], r[kChunks][kEach];
 #pragma unroll
             for (int c = 0; c < kChunks; c++) {
-                LoadPart<kHow, kEach>(static_cast<const T *>(a.residual) + row * a.residualStride, (c * kRowThreads + l) * kEach, a.width, r[c]);
+                Fetch<kHow, kEach>(static_cast<const T *>(a.x) + row * a.xStride, (c * kRowThreads + l) * kEach, a.width, x[c]);
+            }
+            if (a.residual != nullptr) {
+#pragma unroll
+                for (int c = 0; c < kChunks; c++) {
+                    Fetch<kHow, kEach>(static_cast<const T *>(a.residual) + row * a.residualStride, (c * kRowThreads + l) * kEach, a.width, r[c]);
+                }
             }
 #pragma unroll
             for (int c = 0; c < kChunks; c++) {
+                Settle<kHow, kEach>(x[c], (c * kRowThreads + l) * kEach, a.width, s[c]);
+                if (a.residual != nullptr) {
+                    float v[kEach];
+                    Settle<kHow, kEach>(r[c], (c * kRowThreads + l) * kEach, a.width, v);
 #pragma unroll
-                for (int i = 0; i < kEach; i++) {
-                    s[c][i] += r[c][i];
+                    for (int i = 0; i < kEach; i++) {
+                        s[c][i] += v[i];
+                    }
                 }
             }
         }
@@ -204,8 +228,8 @@ __global__ void __launch_bounds__(BlockOf(kRowThreads)) NormGradKernel(NormGradA
         if (row < a.rows) {
 #pragma unroll
             for (int c = 0; c < kChunks; c++) {
-                LoadPart<kHow, kEach>(static_cast<const T *>(a.yGrad) + row * a.yGradStride, (c * kRowThreads + l) * kEach, a.width, nextD[c], T(0.0f));
-                LoadPart<kHow, kEach>(static_cast<const T *>(a.sum) + row * a.sumStride, (c * kRowThreads + l) * kEach, a.width, nextS[c], T(0.0f));
+                Fetch<kHow, kEach>(static_cast<const T *>(a.yGrad) + row * a.yGradStride, (c * kRowThreads + l) * kEach, a.width, nextD[c]);
+                Fetch<kHow, kEach>(static_cast<const T *>(a.sum) + row * a.sumStride, (c * kRowThreads + l) * kEach, a.width, nextS[c]);
             }
         }
     };
@@ -216,16 +240,13 @@ __global__ void __launch_bounds__(BlockOf(kRowThreads)) NormGradKernel(NormGradA
         double squares = 0.0, dots = 0.0;
 #pragma unroll
         for (int c = 0; c < kChunks; c++) {
-#pragma unroll
-            for (int i = 0; i < kEach; i++) {
-                d[c][i] = float(nextD[c][i]);
-                s[c][i] = float(nextS[c][i]);
-            }
+            Settle<kHow, kEach>(nextD[c], (c * kRowThreads + l) * kEach, a.width, d[c]);
+            Settle<kHow, kEach>(nextS[c], (c * kRowThreads + l) * kEach, a.width, s[c]);
         }
 #pragma unroll
         for (int c = 0; c < kChunks; c++) {
             if (a.sumGrad != nullptr) {
-                LoadPart<kHow, kEach>(static_cast<const T *>(a.sumGrad) + row * a.sumGradStride, (c * kRowThreads + l) * kEach, a.width, arrived[c], T(0.0f));
+                Fetch<kHow, kEach>(static_cast<const T *>(a.sumGrad) + row * a.sumGradStride, (c * kRowThreads + l) * kEach, a.width, arrived[c]);
             }
         }
         const int64_t here = row;
@@ -249,25 +270,23 @@ __global__ void __launch_bounds__(BlockOf(kRowThreads)) NormGradKernel(NormGradA
                 parts[1][threadIdx.x / 64] = dots;
             }
             __syncthreads();
-            squares = dots = 0.0;
-#pragma unroll
-            for (int w = 0; w < kRowThreads / 64; w++) {
-                squares += parts[0][w];
-                dots += parts[1][w];
-            }
+            squares = AddParts<kRowThreads / 64>(parts[0]);
+            dots = AddParts<kRowThreads / 64>(parts[1]);
         }
         const double length = 1.0 / __builtin_sqrt(squares / double(a.width) + double(a.epsilon));
         const float by = float(length), mean = float(dots * length / double(a.width));
 #pragma unroll
         for (int c = 0; c < kChunks; c++) {
             const int at = (c * kRowThreads + l) * kEach;
-            float out[kEach];
+            float out[kEach], other[kEach] = {};
+            if (a.sumGrad != nullptr) {
+                Settle<kHow, kEach>(arrived[c], at, a.width, other);
+            }
 #pragma unroll
             for (int i = 0; i < kEach; i++) {
                 const float n = s[c][i] * by;
                 more[c][i] = __builtin_fmaf(d[c][i], n, more[c][i]);
-                out[i] = by * (d[c][i] * gain[c][i] - n * mean);
-                out[i] += a.sumGrad != nullptr ? float(arrived[c][i]) : 0.0f;
+                out[i] = by * (d[c][i] * gain[c][i] - n * mean) + other[i];
             }
             if (a.xGrad != nullptr) {
                 StorePart<kHow, kEach>(static_cast<T *>(a.xGrad) + here * a.xGradStride, at, a.width, out);
