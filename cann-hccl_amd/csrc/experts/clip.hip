@@ -1,7 +1,7 @@
 // Gradients of many tensors held to a norm over all of them: HcclAmdGradSquares, HcclAmdGradClip.
 //
-// The tensors' table rides in the kernel arguments, kTensors to a launch; tensors are cut into chunks, counted over the table, and a workgroup finds its
-// chunk's tensor by halving.  Chunks start at 16-byte boundaries of the input, so that every load inside a tensor is aligned whatever its first
+// The tensors' table rides in the kernel arguments, up to 120 to a launch; tensors are cut into chunks, counted over the table, and a wave finds its
+// chunk's tensor by looking at all of them at once.  Chunks start at 16-byte boundaries of the input, so that every load inside a tensor is aligned whatever its first
 // element is.  Squares are added up in 64 bits: those of 32 bits are exact there, and neither 1e30 nor 1e-30 leaves the range.  A workgroup's sum has
 // its own place in the workspace and a second launch adds the places up in their order: same inputs, same bits.
 #include <type_traits>
@@ -14,8 +14,9 @@ namespace {
 
 constexpr int kThreads = 256;
 constexpr int kEach = 8;                           // neighbouring elements of a lane
-constexpr int kChunk = 16384;                      // elements
-constexpr int kTensors = 120;                      // of a launch: 3840 of the 4096 bytes that arguments may take
+constexpr int kPart = kThreads * kEach;            // elements that a workgroup takes at once
+constexpr int kShort = 1, kLong = 8;               // such parts of a chunk
+constexpr int kFew = 32, kMany = 120;              // tensors of a launch; 120 take 3840 of the 4096 bytes that arguments may
 constexpr int kMostSlots = 2048;                   // workgroups of a launch that adds up: eight to a compute unit
 constexpr uint32_t kMaxTensors = 1u << 24;         // of a list: its places are counted in 32 bits
 constexpr uint64_t kMaxCount = uint64_t(1) << 37;  // elements of a tensor; the chunks of a launch are counted in 32 bits
@@ -30,63 +31,80 @@ struct Tensor {
 };
 static_assert(sizeof(Tensor) == 32, "32 bytes a tensor");
 
+template <int kTensors>
 struct Table {
     Tensor tensor[kTensors];
     int32_t n, chunks;
 };
 
-__device__ __forceinline__ int Find(const Table &t, int chunk)
+// The tensor that `chunk` is of: as many as begin at or before it, less one.  Called by whole waves.
+template <int kTensors>
+__device__ __forceinline__ int Find(const Table<kTensors> &t, int chunk)
 {
-    int lo = 0, hi = t.n;      // tensor[lo].chunk <= chunk < tensor[hi].chunk
-    while (hi - lo > 1) {
-        const int mid = (lo + hi) / 2;
-        if (t.tensor[mid].chunk <= chunk) {
-            lo = mid;
-        } else {
-            hi = mid;
-        }
+    int found = -1;
+#pragma unroll
+    for (int i = 0; i < kTensors; i += 64) {
+        const int at = i + int(__lane_id());
+        found += __popcll(__ballot(at < t.n && t.tensor[at < kTensors ? at : 0].chunk <= chunk));
     }
-    return lo;
+    return __builtin_amdgcn_readfirstlane(found);
 }
 
+// One of a lane's parts at the ends of a tensor, zeros outside.
 template <typename T>
-__device__ __forceinline__ double Squares(const Tensor &t, int chunk)
+__device__ __forceinline__ void LoadEdge(const Tensor &t, int64_t at, float (&v)[kEach])
 {
-    constexpr int kParts = kChunk / (kThreads * kEach);
     const T *in = static_cast<const T *>(t.in);
-    const int64_t from = int64_t(chunk - t.chunk) * kChunk;
-    float v[kParts][kEach];
-    if (from >= t.lead && from + kChunk <= t.last) {
 #pragma unroll
-        for (int p = 0; p < kParts; p++) {
-            Load<true, kEach>(in + from + (p * kThreads + int(threadIdx.x)) * kEach, v[p]);
-        }
-    } else {
-#pragma unroll
-        for (int p = 0; p < kParts; p++) {
-            const int64_t at = from + (p * kThreads + int(threadIdx.x)) * kEach;
-            if (at >= t.lead && at + kEach <= t.last) {
-                Load<true, kEach>(in + at, v[p]);
-            } else {
-#pragma unroll
-                for (int i = 0; i < kEach; i++) {
-                    v[p][i] = at + i >= t.lead && at + i < t.last ? float(in[at + i]) : 0.0f;
-                }
-            }
-        }
+    for (int i = 0; i < kEach; i++) {
+        v[i] = 0.0f;
     }
-    double sum[2] = {0.0, 0.0};
-#pragma unroll
-    for (int p = 0; p < kParts; p++) {
+    if (at >= t.lead && at + kEach <= t.last) {
+        Load<true, kEach>(in + at, v);
+    } else if (at + kEach > t.lead && at < t.last) {
 #pragma unroll
         for (int i = 0; i < kEach; i++) {
-            sum[i % 2] = __builtin_fma(double(v[p][i]), double(v[p][i]), sum[i % 2]);
+            v[i] = at + i >= t.lead && at + i < t.last ? float(in[at + i]) : 0.0f;
+        }
+    }
+}
+
+template <typename T, int kParts>
+__device__ __forceinline__ double Squares(const Tensor &t, int chunk)
+{
+    const T *in = static_cast<const T *>(t.in);
+    const int64_t from = int64_t(chunk - t.chunk) * (kParts * kPart) + int(threadIdx.x) * kEach;
+    const int64_t whole = int64_t(chunk - t.chunk) * (kParts * kPart);
+    double sum[2] = {0.0, 0.0};
+    const auto add = [&](const float (&v)[kEach]) {
+#pragma unroll
+        for (int i = 0; i < kEach; i++) {
+            sum[i % 2] = __builtin_fma(double(v[i]), double(v[i]), sum[i % 2]);
+        }
+    };
+    if (whole >= t.lead && whole + kParts * kPart <= t.last) {
+        float v[kParts][kEach];
+#pragma unroll
+        for (int p = 0; p < kParts; p++) {
+            Load<true, kEach>(in + from + p * kPart, v[p]);
+        }
+#pragma unroll
+        for (int p = 0; p < kParts; p++) {
+            add(v[p]);
+        }
+    } else {
+#pragma unroll 1
+        for (int p = 0; p < kParts && whole + p * kPart < t.last; p++) {
+            float v[kEach];
+            LoadEdge<T>(t, from + p * kPart, v);
+            add(v);
         }
     }
     return sum[0] + sum[1];
 }
 
-__global__ void __launch_bounds__(kThreads) SquaresKernel(Table t, double *slots)
+template <int kTensors, int kParts>
+__global__ void __launch_bounds__(kThreads) SquaresKernel(Table<kTensors> t, double *slots)
 {
     __shared__ double parts[kThreads / 64];
     double sum = 0.0;
@@ -94,13 +112,13 @@ __global__ void __launch_bounds__(kThreads) SquaresKernel(Table t, double *slots
         const Tensor &of = t.tensor[Find(t, chunk)];
         switch (of.type) {
             case HCCL_DATA_TYPE_FP32:
-                sum += Squares<float>(of, chunk);
+                sum += Squares<float, kParts>(of, chunk);
                 break;
             case HCCL_DATA_TYPE_FP16:
-                sum += Squares<_Float16>(of, chunk);
+                sum += Squares<_Float16, kParts>(of, chunk);
                 break;
             default:
-                sum += Squares<__bf16>(of, chunk);
+                sum += Squares<__bf16, kParts>(of, chunk);
                 break;
         }
     }
@@ -137,49 +155,48 @@ __global__ void __launch_bounds__(1024) AddSlotsKernel(const double *slots, int 
     }
 }
 
-template <typename T>
+template <typename T, int kParts>
 __device__ __forceinline__ void Scale(const Tensor &t, int chunk, float by)
 {
-    constexpr int kParts = kChunk / (kThreads * kEach);
     const T *in = static_cast<const T *>(t.in);
     T *out = static_cast<T *>(t.out);
-    const int64_t from = int64_t(chunk - t.chunk) * kChunk;
+    const int64_t whole = int64_t(chunk - t.chunk) * (kParts * kPart), from = whole + int(threadIdx.x) * kEach;
     const bool aligned = reinterpret_cast<uintptr_t>(out) % 16 == 0;
-    if (from >= t.lead && from + kChunk <= t.last) {
+    const auto store = [&](int64_t at, float (&v)[kEach]) {
+#pragma unroll
+        for (int i = 0; i < kEach; i++) {
+            v[i] *= by;
+        }
+        if (aligned) {
+            Store<true, kEach>(out + at, v);
+        } else {
+            Store<false, kEach>(out + at, v);
+        }
+    };
+    if (whole >= t.lead && whole + kParts * kPart <= t.last) {
         float v[kParts][kEach];
 #pragma unroll
         for (int p = 0; p < kParts; p++) {
-            Load<true, kEach>(in + from + (p * kThreads + int(threadIdx.x)) * kEach, v[p]);
+            Load<true, kEach>(in + from + p * kPart, v[p]);
         }
 #pragma unroll
         for (int p = 0; p < kParts; p++) {
-            const int64_t at = from + (p * kThreads + int(threadIdx.x)) * kEach;
-#pragma unroll
-            for (int i = 0; i < kEach; i++) {
-                v[p][i] *= by;
-            }
-            if (aligned) {
-                Store<true, kEach>(out + at, v[p]);
-            } else {
-                Store<false, kEach>(out + at, v[p]);
-            }
+            store(from + p * kPart, v[p]);
         }
         return;
     }
-    for (int p = 0; p < kParts; p++) {
-        const int64_t at = from + (p * kThreads + int(threadIdx.x)) * kEach;
+#pragma unroll 1
+    for (int p = 0; p < kParts && whole + p * kPart < t.last; p++) {
+        const int64_t at = from + p * kPart;
+        float v[kEach];
+        LoadEdge<T>(t, at, v);
         if (at >= t.lead && at + kEach <= t.last) {
-            float v[kEach];
-            Load<true, kEach>(in + at, v);
+            store(at, v);
+        } else if (at + kEach > t.lead && at < t.last) {
 #pragma unroll
             for (int i = 0; i < kEach; i++) {
-                v[i] *= by;
-            }
-            Store<false, kEach>(out + at, v);
-        } else {
-            for (int i = 0; i < kEach; i++) {
                 if (at + i >= t.lead && at + i < t.last) {
-                    out[at + i] = T(float(in[at + i]) * by);
+                    out[at + i] = T(v[i] * by);
                 }
             }
         }
@@ -187,7 +204,8 @@ __device__ __forceinline__ void Scale(const Tensor &t, int chunk, float by)
 }
 
 // The first workgroup of the list's first launch (`norm` not null) leaves the norm.
-__global__ void __launch_bounds__(kThreads) ClipKernel(Table t, const double *squares, float maxNorm, float *norm)
+template <int kTensors, int kParts>
+__global__ void __launch_bounds__(kThreads) ClipKernel(Table<kTensors> t, const double *squares, float maxNorm, float *norm)
 {
     const double length = __builtin_sqrt(squares[0]);
     if (norm != nullptr && blockIdx.x == 0 && threadIdx.x == 0) {
@@ -202,13 +220,13 @@ __global__ void __launch_bounds__(kThreads) ClipKernel(Table t, const double *sq
         }
         switch (of.type) {
             case HCCL_DATA_TYPE_FP32:
-                Scale<float>(of, chunk, by);
+                Scale<float, kParts>(of, chunk, by);
                 break;
             case HCCL_DATA_TYPE_FP16:
-                Scale<_Float16>(of, chunk, by);
+                Scale<_Float16, kParts>(of, chunk, by);
                 break;
             default:
-                Scale<__bf16>(of, chunk, by);
+                Scale<__bf16, kParts>(of, chunk, by);
                 break;
         }
     }
@@ -235,8 +253,10 @@ HcclResult Check(const char *fn, const HcclAmdGradTensor *tensors, uint32_t n, b
 }
 
 // The next launch's table, from tensor `at` on, which is moved behind it; false: there are no more elements.
-bool Next(const HcclAmdGradTensor *tensors, uint32_t n, uint32_t &at, Table &table)
+template <int kTensors>
+bool Next(const HcclAmdGradTensor *tensors, uint32_t n, int parts, uint32_t &at, Table<kTensors> &table)
 {
+    const uint64_t chunk = uint64_t(parts) * kPart;
     table.n = table.chunks = 0;
     for (; at < n && table.n < kTensors; at++) {
         const HcclAmdGradTensor &t = tensors[at];
@@ -251,12 +271,65 @@ bool Next(const HcclAmdGradTensor *tensors, uint32_t n, uint32_t &at, Table &tab
         to.chunk = table.chunks;
         to.type = int16_t(t.type);
         to.lead = int16_t(lead);
-        table.chunks += int32_t((t.count + lead + kChunk - 1) / kChunk);
+        table.chunks += int32_t((t.count + lead + chunk - 1) / chunk);
     }
     return table.n != 0;
 }
 
-int Slots(const Table &t) { return t.chunks < kMostSlots ? t.chunks : kMostSlots; }
+int Slots(int chunks) { return chunks < kMostSlots ? chunks : kMostSlots; }
+
+// Parts of a chunk: as many as load well together, one where the chunks would not be enough for two workgroups to each compute unit.
+int PartsOf(const HcclAmdGradTensor *tensors, uint32_t n)
+{
+    uint64_t parts = 0;
+    for (uint32_t i = 0; i < n && parts < 512 * kLong; i++) {
+        parts += (tensors[i].count + kPart - 1) / kPart;
+    }
+    return parts < 512 * kLong ? kShort : kLong;
+}
+
+template <int kTensors, int kParts>
+HcclResult Squares(const HcclAmdGradTensor *tensors, uint32_t n, double *slots, int *used, hipStream_t on)
+{
+    Table<kTensors> table;
+    for (uint32_t at = 0; Next(tensors, n, kParts, at, table);) {
+        const int some = Slots(table.chunks);
+        const HcclResult r = Launch("HcclAmdGradSquares", SquaresKernel<kTensors, kParts>, uint32_t(some), kThreads, 0, on, table, slots + *used);
+        if (r != HCCL_SUCCESS) {
+            return r;
+        }
+        *used += some;
+    }
+    return HCCL_SUCCESS;
+}
+
+template <int kTensors, int kParts>
+HcclResult Clip(const HcclAmdGradTensor *tensors, uint32_t n, const double *squares, float maxNorm, float *norm, hipStream_t on)
+{
+    Table<kTensors> table;
+    uint32_t at = 0;
+    while (Next(tensors, n, kParts, at, table) || norm != nullptr) {
+        // (no elements at all: the norm is left all the same)
+        const int blocks = table.chunks < 1 ? 1 : table.chunks < (1 << 20) ? table.chunks : 1 << 20;
+        const HcclResult r = Launch("HcclAmdGradClip", ClipKernel<kTensors, kParts>, uint32_t(blocks), kThreads, 0, on, table, squares, maxNorm, norm);
+        if (r != HCCL_SUCCESS) {
+            return r;
+        }
+        norm = nullptr;
+    }
+    return HCCL_SUCCESS;
+}
+
+// f(tensors of a launch, parts of a chunk), as constants.  A list of up to 32 tensors takes a launch with room for these alone: its arguments are a quarter
+// as long.
+template <typename F>
+HcclResult ByList(const HcclAmdGradTensor *tensors, uint32_t n, F f)
+{
+    const auto byParts = [&](auto room) {
+        return PartsOf(tensors, n) == kShort ? f(room, std::integral_constant<int, kShort>{}) : f(room, std::integral_constant<int, kLong>{});
+    };
+    return n <= kFew ? byParts(std::integral_constant<int, kFew>{}) : byParts(std::integral_constant<int, kMany>{});
+}
 
 }  // namespace
 }  // namespace experts
@@ -277,9 +350,10 @@ HcclResult HcclAmdGradSquaresWorkspace(const HcclAmdGradTensor *tensors, uint32_
         return r;
     }
     uint64_t slots = 0;
-    Table table;
-    for (uint32_t at = 0; Next(tensors, n, at, table);) {
-        slots += uint64_t(Slots(table));
+    const int parts = PartsOf(tensors, n);
+    Table<kMany> table;
+    for (uint32_t at = 0; Next(tensors, n, parts, at, table);) {
+        slots += uint64_t(Slots(table.chunks));
     }
     *bytes = slots * sizeof(double);
     return HCCL_SUCCESS;
@@ -305,13 +379,11 @@ HcclResult HcclAmdGradSquares(const HcclAmdGradTensor *tensors, uint32_t n, uint
     const hipStream_t on = static_cast<hipStream_t>(stream);
     double *slots = static_cast<double *>(workspace);
     int used = 0;
-    Table table;
-    for (uint32_t at = 0; Next(tensors, n, at, table);) {
-        const HcclResult r = Launch("HcclAmdGradSquares", SquaresKernel, uint32_t(Slots(table)), kThreads, 0, on, table, slots + used);
-        if (r != HCCL_SUCCESS) {
-            return r;
-        }
-        used += Slots(table);
+    const HcclResult r = ByList(tensors, n, [&](auto room, auto parts) {
+        return Squares<decltype(room)::value, decltype(parts)::value>(tensors, n, slots, &used, on);
+    });
+    if (r != HCCL_SUCCESS) {
+        return r;
     }
     return Launch("HcclAmdGradSquares", AddSlotsKernel, 1, 1024, 0, on, static_cast<const double *>(slots), used, squares, accumulate != 0);
 }
@@ -329,18 +401,10 @@ HcclResult HcclAmdGradClip(const HcclAmdGradTensor *tensors, uint32_t n, const d
     if (checked != HCCL_SUCCESS) {
         return checked;
     }
-    Table table;
-    uint32_t at = 0;
-    while (Next(tensors, n, at, table) || norm != nullptr) {
-        // (no elements at all: the norm is left all the same)
-        const HcclResult r = Launch("HcclAmdGradClip", ClipKernel, uint32_t(table.chunks < 1 ? 1 : table.chunks < (1 << 20) ? table.chunks : 1 << 20), kThreads, 0,
-            static_cast<hipStream_t>(stream), table, squares, maxNorm, norm);
-        if (r != HCCL_SUCCESS) {
-            return r;
-        }
-        norm = nullptr;
-    }
-    return HCCL_SUCCESS;
+    const hipStream_t on = static_cast<hipStream_t>(stream);
+    return ByList(tensors, n, [&](auto room, auto parts) {
+        return Clip<decltype(room)::value, decltype(parts)::value>(tensors, n, squares, maxNorm, norm, on);
+    });
 }
 
 }  // extern "C"

@@ -33,8 +33,17 @@ __device__ __forceinline__ int64_t Rows(const GateArgs &a)
     return a.used == nullptr ? a.rows : min(int64_t(max(a.used[0], 0)), a.rows);
 }
 
-// 1 / (1 + exp(-g)), by the hardware's power of two and reciprocal, each good to a unit in the last place.
-__device__ __forceinline__ float Sigmoid(float g) { return __builtin_amdgcn_rcpf(1.0f + __builtin_amdgcn_exp2f(g * -1.44269504088896340736f)); }
+// 1 / (1 + exp(-g)), good to a unit and a half in the last place: what rounding loses of the power's argument comes back as a factor, what the hardware's
+// reciprocal loses by one step of Newton's (65536 rows of 2048 values to 8 bits take 116 us with these, 113 without).  Below -87 it is 0 (2e-38 at most, and the
+// power would leave the range).
+__device__ __forceinline__ float Sigmoid(float g)
+{
+    const float x = __builtin_amdgcn_fmed3f(g, -87.0f, 87.0f), t = x * -0x1.715476p+0f;
+    const float lost = __builtin_fmaf(x, -0x1.4ae0cp-26f, __builtin_fmaf(x, -0x1.715476p+0f, -t));      // log2(e) in two parts
+    const float d = __builtin_fmaf(__builtin_amdgcn_exp2f(t), __builtin_fmaf(lost, 0x1.62e43p-1f, 1.0f), 1.0f);
+    const float r = __builtin_amdgcn_rcpf(d);
+    return g < -87.0f ? 0.0f : __builtin_fmaf(__builtin_fmaf(-d, r, 1.0f), r, r);
+}
 
 template <typename T, HcclAmdScaleType kScale, bool kWide>
 __global__ void __launch_bounds__(kThreads) GateKernel(GateArgs a)
