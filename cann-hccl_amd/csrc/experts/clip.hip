@@ -15,7 +15,7 @@ namespace {
 constexpr int kThreads = 256;
 constexpr int kEach = 8;                           // neighbouring elements of a lane
 constexpr int kPart = kThreads * kEach;            // elements that a workgroup takes at once
-constexpr int kShort = 1, kLong = 8;               // such parts of a chunk
+constexpr int kShort = 1, kLong = 4;               // such parts of a chunk
 constexpr int kFew = 32, kMany = 120;              // tensors of a launch; 120 take 3840 of the 4096 bytes that arguments may
 constexpr int kMostSlots = 2048;                   // workgroups of a launch that adds up: eight to a compute unit
 constexpr uint32_t kMaxTensors = 1u << 24;         // of a list: its places are counted in 32 bits

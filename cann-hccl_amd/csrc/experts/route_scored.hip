@@ -186,7 +186,8 @@ __device__ __forceinline__ float Sigmoid(float x) { return __builtin_amdgcn_rcpf
 //   s (U + 2 U)                 the sum and the reciprocal
 // which is 4 U, 1 step at most: two numbers are off against each other by twice 2.75.  A softmax's power, quotient and product are off by 5 U, and its sum, of 32 to a
 // lane over 8 lanes or 16 over 64, by 50 U, the same for all of a token's: 60 U, 15 steps between two of them, and 3.5 for the rest.
-constexpr uint32_t kSlackSigmoid = 8, kSlackSoftmax = 24;
+// (What 64 bits would change is within these, cut off to whole numbers; sums of two are off by twice as much.)
+constexpr uint32_t kSlackSigmoid = 5, kSlackSoftmax = 18;
 
 // DPP of the other lane of a pair, the other pair of four, the other four of eight, the other eight of sixteen (mirrored, where the lanes of each
 // part are alike).
@@ -432,7 +433,7 @@ __device__ __forceinline__ bool ChooseGroups(const ScoredArgs &a, uint32_t (&num
         }
     }
     Ordered();
-    return most < 64 || least >> 6 > (most >> 6) + (a.second ? 2 * slack : slack);
+    return most < 64 || least >> 6 > (most >> 6) + (a.second ? 2 * slack + 1 : slack);
 }
 
 // The keys in 64 bits of two experts of a lane's token.
