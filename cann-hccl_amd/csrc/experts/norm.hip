@@ -328,16 +328,16 @@ __global__ void __launch_bounds__(BlockOf(kRowThreads)) NormGradKernel(NormGradA
     }
 }
 
-constexpr int kGainCols = 16, kGainRuns = 256 / kGainCols;
+constexpr int kGainCols = 16, kGainRuns = 64, kGainThreads = kGainCols * kGainRuns;
 
-// gainGrad from the workgroups' sums: 16 columns to a workgroup, 16 runs of workgroups to a column, then the runs in their order.
-__global__ void __launch_bounds__(256) NormGainKernel(const float *partial, int slots, int width, float *gainGrad, bool accumulate)
+// gainGrad from the workgroups' sums: 16 columns to a workgroup, 64 runs of workgroups to a column, then the runs in their order.
+__global__ void __launch_bounds__(kGainThreads) NormGainKernel(const float *partial, int slots, int width, float *gainGrad, bool accumulate)
 {
     __shared__ float parts[kGainRuns][kGainCols + 1];
     const int c = int(threadIdx.x) % kGainCols, run = int(threadIdx.x) / kGainCols, at = int(blockIdx.x) * kGainCols + c;
     float sum = 0.0f;
     if (at < width) {
-#pragma unroll 8
+#pragma unroll 16
         for (int s = run; s < slots; s += kGainRuns) {
             sum += partial[int64_t(s) * width + at];
         }
@@ -533,7 +533,7 @@ HcclResult HcclAmdNormRowsGrad(const void *yGrad, uint64_t yGradStride, const vo
             return r;
         }
     }
-    return Launch("HcclAmdNormRowsGrad", NormGainKernel, uint32_t((width + kGainCols - 1) / kGainCols), 256, 0, on,
+    return Launch("HcclAmdNormRowsGrad", NormGainKernel, uint32_t((width + kGainCols - 1) / kGainCols), kGainThreads, 0, on,
         static_cast<const float *>(workspace), int(blocks), int(width), gainGrad, accumulate != 0);
 }
 
