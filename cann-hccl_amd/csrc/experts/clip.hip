@@ -19,7 +19,7 @@ constexpr int kShort = 1, kLong = 4;               // such parts of a chunk
 constexpr int kFew = 32, kMany = 120;              // tensors of a launch; 120 take 3840 of the 4096 bytes that arguments may
 constexpr int kMostSlots = 2048;                   // workgroups of a launch that adds up: eight to a compute unit
 constexpr uint32_t kMaxTensors = 1u << 24;         // of a list: its places are counted in 32 bits
-constexpr uint64_t kMaxCount = uint64_t(1) << 37;  // elements of a tensor; the chunks of a launch are counted in 32 bits
+constexpr uint64_t kMaxCount = uint64_t(1) << 36;  // elements of a tensor; the chunks of a launch are counted in 32 bits
 
 struct Tensor {
     const void *in;       // moved down to a 16-byte boundary,

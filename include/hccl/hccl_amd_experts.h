@@ -203,8 +203,8 @@ extern HcclResult HcclAmdExpertRouteScoredGrad(const void *logits, HcclDataType 
  * the sum of all ranks' (HcclAllReduce, INT32).  newBias may be bias. */
 extern HcclResult HcclAmdExpertBias(const int32_t *counts, uint32_t experts, float rate, const float *bias, float *newBias, void *stream);
 
-/* A tensor of gradients: `count` elements behind each other (FP32, FP16 or BFP16), aligned to one.  Lists of these are host memory, read during the
- * call. */
+/* A tensor of gradients: `count` elements (2^36 at most) behind each other (FP32, FP16 or BFP16), aligned to one.  Lists of these, of 2^24 at most, are host
+ * memory, read during the call. */
 typedef struct HcclAmdGradTensorDef {
     const void *in;
     void *out;             /* HcclAmdGradClip writes here; may be `in` */

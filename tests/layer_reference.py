@@ -118,3 +118,24 @@ def route_grad(x, r, kind, topk, renorm, scale, dw):
 def bias_step(counts, rate, bias):
     n = counts.astype(np.int64)
     return (bias + np.float32(rate) * np.sign(n.sum() - len(n) * n).astype(np.float32)).astype(np.float32)
+
+
+def route_many(x, kind, bias, groups, kept, group_top, topk, renorm, scale):
+    """route() for finite logits of many tokens, all tokens at once."""
+    T, E = x.shape
+    s = scores(x, kind)
+    key = s + (0 if bias is None else bias)
+    of = -np.sort(-key.reshape(T, groups, -1), axis=2)[:, :, :group_top]
+    of = of[:, :, 0] + (of[:, :, 1] if of.shape[2] > 1 else 0)
+    use = np.argsort(-of, axis=1, kind="stable")[:, :kept]                 # (of equal ones the lowest stays in front)
+    keep = np.zeros((T, groups), bool)
+    np.put_along_axis(keep, use, True, 1)
+    key = np.where(np.repeat(keep, E // groups, 1), key, -np.inf)
+    expert = np.argsort(-key, axis=1, kind="stable")[:, :topk]
+    p = np.take_along_axis(s, expert, 1)
+    counts = np.concatenate([np.bincount(expert.reshape(-1), minlength=E), [T]])
+    order = np.argsort(expert.reshape(-1), kind="stable")
+    row_of = np.empty(T * topk, np.int32)
+    row_of[order] = np.arange(T * topk)
+    return {"expert": expert, "weights": scale * p / (p.sum(1, keepdims=True) if renorm else 1), "row_of": row_of.reshape(T, topk), "counts": counts,
+            "offsets": np.concatenate([[0], np.cumsum(counts[:E])]), "scores": s}

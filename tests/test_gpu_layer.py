@@ -442,6 +442,32 @@ def test_route_next_to_each_other(stream, kind):
         check_route(x, kind, bias, groups, kept, 2, 8, True, 1.0, None, None, got, None)
 
 
+@pytest.mark.parametrize("tokens,experts,groups,kept,top,topk,dtype", [
+    (4097, 30, 5, 2, 2, 4, "fp32"), (5000, 64, 8, 3, 2, 6, "bf16"), (4500, 100, 1, 1, 1, 8, "fp16"), (6001, 128, 4, 2, 1, 8, "bf16"), (4999, 200, 10, 4, 2, 7, "fp32"),
+    (5001, 256, 8, 4, 2, 8, "bf16"), (4200, 256, 1, 1, 1, 3, "fp32"), (4100, 256, 8, 4, 2, 12, "bf16"), (70001, 16, 4, 2, 2, 2, "bf16"), (5003, 320, 5, 2, 2, 8, "fp16"),
+])
+@pytest.mark.parametrize("kind", ["sigmoid", "softmax"])
+@pytest.mark.parametrize("data", ["spread", "close"])
+def test_route_large(stream, tokens, experts, groups, kept, top, topk, dtype, kind, data):
+    """Every layout for many tokens, several tiles to a workgroup; and scores so close to each other that many choices take 64 bits."""
+    print("route large", tokens, experts, groups, kept, top, topk, dtype, kind, data, flush=True)
+    x = draw(experts, tokens, experts, dtype=TYPE[dtype], scale=1.5)
+    if data == "close":
+        # logits of a few values, biases a few steps of 2^-24 apart: next to each other, not equal
+        x = torch.round(x.float() * 2).clamp(-2, 2).mul(0.5).to(x.dtype)
+        if dtype == "fp32":
+            x += draw(9, tokens, experts).sign() * 2.0 ** -21
+    rng = np.random.default_rng(topk)
+    step = 2.0 ** -24 if data == "close" else 1e-3
+    bias = (0.25 + rng.integers(-20, 20, experts) * step).astype(np.float32)
+    got, _ = run_route(stream, x, kind, bias, groups, kept, top, topk, True, 1.0, None)
+    r = ref.route_many(f64(x), kind, bias.astype(np.float64), groups, kept, top, topk, True, 1.0)
+    for k in ("expert", "row_of"):
+        assert np.array_equal(got[k], r[k]), (k, int((got[k] != r[k]).any(1).sum()))
+    assert np.array_equal(got["counts"][0], r["counts"]) and np.array_equal(got["offsets"][0], r["offsets"])
+    assert near(got["weights"], r["weights"], (3 * 2 * np.abs(f64(x)).max() + experts + 24) * U * r["weights"])
+
+
 @pytest.mark.parametrize("kind", ["sigmoid", "softmax"])
 def test_route_nothing_left(stream, kind):
     """Masked tokens that hold anything, rows of -inf or NaN, groups without an expert, experts that the bias switches off, infinite logits."""
@@ -482,6 +508,23 @@ def test_route_strides_and_shared_words(stream):
         for kind in ("sigmoid", "softmax"):
             got, grad = run_route(stream, x, kind, None, 4, 2, 1, 4, False, 1.0, None, dw, stride, shift)
             check_route(x, kind, None, 4, 2, 1, 4, False, 1.0, None, dw, got, grad)
+
+
+def test_route_grad_many_tokens(stream):
+    """Gradients of more tokens than workgroups take at once, experts in every layout."""
+    for experts, topk, dtype in ((64, 4, torch.bfloat16), (200, 8, torch.float32), (500, 3, torch.float16)):
+        x = draw(experts, 9000, experts, dtype=dtype)
+        dw = np.random.default_rng(2).standard_normal((9000, topk)).astype(np.float32)
+        for kind in ("sigmoid", "softmax"):
+            for renorm in (True, False):
+                got, grad = run_route(stream, x, kind, None, 1, 1, 1, topk, renorm, 1.5, None, dw)
+                r = ref.route_many(f64(x), kind, None, 1, 1, 1, topk, renorm, 1.5)
+                assert np.array_equal(got["expert"], r["expert"])
+                some = np.concatenate([np.arange(50), np.arange(8000, 8050), np.arange(8950, 9000)])
+                r = {k: v[some] for k, v in r.items() if k in ("expert", "weights", "scores")}
+                want, size = ref.route_grad(f64(x)[some], r, kind, topk, renorm, 1.5, dw[some])
+                rel = (3 * 2 * np.abs(f64(x)).max() + experts + 24) * U
+                assert near(grad[some], want, 3 * rel * size + 1e-37, dtype), (experts, kind, renorm)
 
 
 def test_route_grad_skips_bad_experts(stream):

@@ -244,3 +244,17 @@ def test_reference_route_gradient(kind, renorm, tokens, experts, groups, kept, t
 def test_reference_bias():
     counts = np.array([5, 0, 3, 4, 3], np.int32)      # mean 3
     assert np.array_equal(ref.bias_step(counts, 0.5, np.zeros(5, np.float32)), np.float32([-0.5, 0.5, 0, -0.5, 0]))
+
+
+@pytest.mark.parametrize("kind", ["sigmoid", "softmax"])
+@pytest.mark.parametrize("groups,kept,top,topk", [(1, 1, 1, 5), (4, 2, 2, 3), (6, 3, 1, 4)])
+def test_reference_of_many_tokens_is_the_reference(kind, groups, kept, top, topk):
+    rng = np.random.default_rng(groups)
+    x = rng.integers(-4, 4, (60, 12)) * 0.5                   # ties everywhere
+    bias = rng.integers(-1, 2, 12) * 0.25
+    for renorm in (False, True):
+        a = ref.route(x, kind, bias, groups, kept, top, topk, renorm, 1.5, None)
+        b = ref.route_many(x, kind, bias, groups, kept, top, topk, renorm, 1.5)
+        for k in ("expert", "row_of", "counts", "offsets"):
+            assert np.array_equal(a[k], b[k]), k
+        assert np.allclose(a["weights"], b["weights"], rtol=1e-13)
