@@ -88,10 +88,18 @@ __device__ __forceinline__ Choice FirstOfWave(Choice c)
     return First(First(ChoiceFrom(c, 0), ChoiceFrom(c, 16)), First(ChoiceFrom(c, 32), ChoiceFrom(c, 48)));
 }
 
-// One token's, by a whole wave: its experts best first, -1 where there is none.  kEach: a lane's experts, 64 apart.  `keys`: a place per expert, `of`: one per
-// group, in LDS.  Loops, not straight code: this is seldom called, and every instruction has to be fetched then.
-template <int kEach, int K, typename T>
-__device__ __forceinline__ void ChooseExactly(const ScoredArgs &a, const T *row, double *keys, double *of, int (&chosen)[K])
+// What it takes of a launch's arguments: by value, since it is a function of its own, whose registers those that do not call it need not hold free.
+struct ExactArgs {
+    const float *bias;
+    int experts, topK, groups, kept, size;
+    uint32_t perSize;
+    bool softmax, second;
+};
+
+// One token's, by a whole wave: lane j has the j-th expert, best first, -1 where there is none.  kEach: a lane's experts, 64 apart.  `keys`: a place per expert,
+// `of`: one per group, in LDS.  Loops, not straight code: this is seldom called, and every instruction has to be fetched then.
+template <int kEach, typename T>
+__device__ __attribute__((noinline)) int ChooseExactly(ExactArgs a, const T *row, double *keys, double *of)
 {
     const int lane = Anew(int(__lane_id()));
     float top = -__builtin_inff();
@@ -167,10 +175,7 @@ __device__ __forceinline__ void ChooseExactly(const ScoredArgs &a, const T *row,
             key[i] = i * 64 + lane == best.expert ? kNever : key[i];
         }
     }
-#pragma unroll
-    for (int i = 0; i < K; i++) {
-        chosen[i] = __builtin_amdgcn_readlane(taken, i);
-    }
+    return taken;
 }
 
 // log of the sigmoid
@@ -493,12 +498,22 @@ __device__ __forceinline__ bool ChooseFast(const ScoredArgs &a, const Steps &ste
     int lane, uint32_t *numbers, uint32_t *of, int (&chosen)[K], float &top, float &sum)
 {
     uint32_t number[kEach];
-    float s[kEach], by = steps.times, largest = -__builtin_inff();
+    float largest = -__builtin_inff();
 #pragma unroll
     for (int i = 0; i < kEach; i++) {
         largest = __builtin_fmaxf(largest, x[i]);      // (leaves NaN out)
     }
+    // from eight scores, in units of `by`, NaN where the logit is infinite or NaN
+    const auto make = [&](int c, const float (&s)[8], float by) {
+        float p[8];
+        Load<true, 8>(part + (c * kLanes + l) * 8, p);
+#pragma unroll
+        for (int i = 0; i < 8; i++) {
+            number[c * 8 + i] = Whole(__builtin_fmaf(s[i], by, p[i]));
+        }
+    };
     if (a.softmax) {
+        float s[kEach];
         bool bad = false;
 #pragma unroll
         for (int i = 0; i < kEach; i++) {
@@ -512,24 +527,29 @@ __device__ __forceinline__ bool ChooseFast(const ScoredArgs &a, const Steps &ste
             s[i] = Exp(x[i] == top ? 0.0f : x[i] - top);
             s[i] = x[i] <= top ? s[i] : 0.0f;
             sum += s[i];
+            s[i] = __builtin_fmaf(x[i], 0.0f, s[i]);
         }
         sum = AddLanes<kLanes>(sum);
-        by = steps.times / sum;
+        const float by = steps.times / sum;
         sum = AddLanes<kLanes>(bad ? 1.0f : 0.0f) > 0.0f ? __builtin_nanf("") : sum;
+#pragma unroll
+        for (int c = 0; c < kEach / 8; c++) {
+            float eight[8];
+#pragma unroll
+            for (int i = 0; i < 8; i++) {
+                eight[i] = s[c * 8 + i];
+            }
+            make(c, eight, by);
+        }
     } else {
 #pragma unroll
-        for (int i = 0; i < kEach; i++) {
-            s[i] = Sigmoid(x[i]);
-        }
-    }
+        for (int c = 0; c < kEach / 8; c++) {
+            float s[8];
 #pragma unroll
-    for (int c = 0; c < kEach / 8; c++) {
-        float p[8];
-        Load<true, 8>(part + (c * kLanes + l) * 8, p);
-#pragma unroll
-        for (int i = 0; i < 8; i++) {
-            // (0 * x is NaN where the logit is infinite or NaN)
-            number[c * 8 + i] = Whole(__builtin_fmaf(s[c * 8 + i], by, __builtin_fmaf(x[c * 8 + i], 0.0f, p[i])));
+            for (int i = 0; i < 8; i++) {
+                s[i] = __builtin_fmaf(x[c * 8 + i], 0.0f, Sigmoid(x[c * 8 + i]));
+            }
+            make(c, s, steps.times);
         }
     }
     bool sure = !(largest == __builtin_inff());       // (+inf can be chosen, but not like this)
@@ -692,11 +712,12 @@ __global__ void __launch_bounds__(kThreads, kLanes == 64 ? 2 : 4) ScoredKernel(S
         unsigned long long unsure = __ballot(in && !sure);
         while (unsure != 0) {
             const int which = (__ffsll(unsure) - 1) / kLanes, whose = (int(blockIdx.x) * a.tiles + tile) * kTile + wave * kWaveTokens + which;
-            int exactly[K];
-            ChooseExactly<kLanes * kEach / 64, K>(a, static_cast<const T *>(a.logits) + int64_t(whose) * a.stride, keys[wave], groupKeys[wave], exactly);
+            const int taken = ChooseExactly<kLanes * kEach / 64, T>(ExactArgs{a.bias, a.experts, a.topK, a.groups, a.kept, a.size, a.perSize, a.softmax, a.second},
+                static_cast<const T *>(a.logits) + int64_t(whose) * a.stride, keys[wave], groupKeys[wave]);
 #pragma unroll
             for (int i = 0; i < K; i++) {
-                chosen[i] = lane / kLanes == which ? exactly[i] : chosen[i];
+                const int exactly = __builtin_amdgcn_readlane(taken, i);
+                chosen[i] = lane / kLanes == which ? exactly : chosen[i];
             }
             unsure &= ~(kLanes == 64 ? ~0ull : ((1ull << kLanes % 64) - 1) << which * kLanes);
         }
