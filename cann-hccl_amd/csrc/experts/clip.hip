@@ -4,6 +4,10 @@
 // chunk's tensor by looking at all of them at once.  Chunks start at 16-byte boundaries of the input, so that every load inside a tensor is aligned whatever its first
 // element is.  Squares are added up in 64 bits: those of 32 bits are exact there, and neither 1e30 nor 1e-30 leaves the range.  A workgroup's sum has
 // its own place in the workspace and a second launch adds the places up in their order: same inputs, same bits.
+//
+// Bytes moved bound both: 2^30 values in 16 bits (2.1 GB) are added up in 360 us, 6.0 TB/s, and scaled in 710 us, 6.0 TB/s, where a large copy reaches
+// 5.15.  Four parts of 2048 elements to a chunk leave room for eight waves to a SIMD, so that all 2048 workgroups run at once; with eight parts
+// seven do, and the last eighth waited (1190 us for both instead of 1096).  Twenty short tensors: 2.9 us, 1.6 and 3.4, a launch's own time each.
 #include <type_traits>
 
 #include "sums.h"
@@ -234,6 +238,10 @@ __global__ void __launch_bounds__(kThreads) ClipKernel(Table<kTensors> t, const 
 
 HcclResult Check(const char *fn, const HcclAmdGradTensor *tensors, uint32_t n, bool write)
 {
+    if (n > kMaxTensors) {
+        HCCL_LOG_ERROR("%s: %u tensors", fn, n);
+        return HCCL_E_PARA;
+    }
     for (uint32_t i = 0; i < n; i++) {
         const HcclAmdGradTensor &t = tensors[i];
         if (!Float(t.type)) {
@@ -365,7 +373,6 @@ HcclResult HcclAmdGradSquares(const HcclAmdGradTensor *tensors, uint32_t n, uint
     EXPERTS_CHK_PTR(stream);
     EXPERTS_CHK_PTR(squares);
     EXPERTS_CHK(Aligned(squares, 8));
-    EXPERTS_CHK(n <= kMaxTensors);
     uint64_t needed = 0;
     const HcclResult checked = HcclAmdGradSquaresWorkspace(tensors, n, &needed);
     if (checked != HCCL_SUCCESS) {

@@ -10,7 +10,14 @@
 // is that of 64 bits; but it is made in 32 wherever these are enough.  A score and its bias become a whole number of 22 bits, a word of that and
 // the expert goes into sorted lists by one median of three per entry, and the lists of a token's lanes are merged.  What the 22 bits are off by at most
 // is known, so that a choice is settled unless, at some place that matters, two of them are closer than that and not made from the same logit and
-// bias (which tie in any precision).  Waves with an unsettled token choose again in 64 bits.
+// bias (which tie in any precision).  Of an unsettled token the chosen ones and the next are put in order by their keys in 64 bits; where that does not
+// settle it either -- its groups are too close, or several experts at the border -- a whole wave chooses for it in 64 bits.
+//
+// Measured: 65536 tokens of 256 experts in eight groups, eight chosen, 16-bit logits (33.5 MB): 34 us to choose, 6 to add up, 5 for the rows, 10 for the
+// gradient, 4 for the bias.  Choosing is bound by vector instructions: about 35 for each expert, of which eight are medians and eight what a power and a reciprocal
+// take.  One token in 300 has choices closer than 32 bits hold (3 us of the 34), one in 2000 groups that are (4 us, since the others wait); with
+// everything in 64 bits it took 240 us.  Eight lanes to a token spend fewer instructions on merging than sixteen (46 us against 51 with all launches),
+// sixteen are quicker where there are few tokens.
 #include <type_traits>
 
 #include "rows.h"

@@ -392,6 +392,7 @@ ROUTES = [
     (1, 1, 1, 1, 1, 1, "fp32"), (1, 256, 8, 4, 2, 8, "bf16"), (5, 8, 2, 1, 1, 2, "fp16"), (16, 64, 8, 3, 2, 6, "bf16"), (17, 60, 4, 2, 2, 6, "fp32"),
     (33, 126, 9, 4, 1, 5, "fp16"), (70, 160, 8, 3, 2, 16, "fp32"), (100, 129, 3, 2, 2, 7, "bf16"), (200, 255, 5, 5, 2, 3, "fp32"), (9, 257, 1, 1, 1, 8, "bf16"),
     (13, 1024, 64, 7, 2, 16, "fp32"), (6, 1000, 10, 1, 2, 10, "fp16"), (300, 256, 1, 1, 2, 8, "fp32"), (64, 128, 64, 5, 2, 4, "bf16"), (40, 12, 12, 5, 2, 5, "fp32"),
+    (21, 1024, 2, 1, 2, 8, "fp32"), (7, 1020, 4, 2, 2, 16, "bf16"), (4, 1024, 1, 1, 1, 16, "bf16"),
 ]
 
 
