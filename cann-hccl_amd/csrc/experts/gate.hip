@@ -3,7 +3,7 @@
 // With t = 1 / (1 + exp(-g)):   a = g t u      dg = da u t (1 + g (1 - t))      du = da g t
 //
 // A wave takes a row's piece of 512 values, eight neighbouring ones to a lane: 16 lanes hold a block of an 8-bit row.  Every value is read once and
-// written once, and bytes moved bound both kernels: 65536 rows of 2048 values to 8 bits (0.67 GB) 116 us, 5.8 TB/s, where a large copy reaches 5.15; 14770 rows of
+// written once, and bytes moved bound both kernels: 65536 rows of 2048 values to 8 bits (0.67 GB) 115 us, 5.9 TB/s, where a large copy reaches 5.15; 14769 rows of
 // 4095, off every boundary, 70 us (4.3 TB/s), their gradient 127 us (5.7 TB/s).
 #include <type_traits>
 
@@ -34,16 +34,13 @@ __device__ __forceinline__ int64_t Rows(const GateArgs &a)
     return a.used == nullptr ? a.rows : min(int64_t(max(a.used[0], 0)), a.rows);
 }
 
-// 1 / (1 + exp(-g)), good to a unit and a half in the last place: what rounding loses of the power's argument comes back as a factor, what the hardware's
-// reciprocal loses by one step of Newton's (65536 rows of 2048 values to 8 bits take 116 us with these, 113 without).  Below -87 it is 0 (2e-38 at most, and the
-// power would leave the range).
+// 1 / (1 + exp(-g)), good to two units in the last place: what rounding loses of the power's argument comes back as a factor; the power and the reciprocal
+// are the hardware's, a unit each.  Beyond 10000 the power is infinite or 0 whatever is lost.
 __device__ __forceinline__ float Sigmoid(float g)
 {
-    const float x = __builtin_amdgcn_fmed3f(g, -87.0f, 87.0f), t = x * -0x1.715476p+0f;
+    const float x = __builtin_amdgcn_fmed3f(g, -10000.0f, 10000.0f), t = x * -0x1.715476p+0f;
     const float lost = __builtin_fmaf(x, -0x1.4ae0cp-26f, __builtin_fmaf(x, -0x1.715476p+0f, -t));      // log2(e) in two parts
-    const float d = __builtin_fmaf(__builtin_amdgcn_exp2f(t), __builtin_fmaf(lost, 0x1.62e43p-1f, 1.0f), 1.0f);
-    const float r = __builtin_amdgcn_rcpf(d);
-    return g < -87.0f ? 0.0f : __builtin_fmaf(__builtin_fmaf(-d, r, 1.0f), r, r);
+    return __builtin_amdgcn_rcpf(__builtin_fmaf(__builtin_amdgcn_exp2f(t), __builtin_fmaf(lost, 0x1.62e43p-1f, 1.0f), 1.0f));
 }
 
 template <typename T, HcclAmdScaleType kScale, bool kWide>
@@ -67,22 +64,12 @@ __global__ void __launch_bounds__(kThreads) GateKernel(GateArgs a)
         if constexpr (kScale == HCCL_AMD_SCALE_NONE) {
             StorePart<kWide, kEach>(static_cast<T *>(a.out) + row * a.outStride, at, a.width, u);
         } else {
-            float top = 0.0f;
-#pragma unroll
-            for (int i = 0; i < kEach; i++) {
-                top = __builtin_fmaxf(top, FiniteSize(u[i]));
-            }
-            const BlockScale<kScale> scale(LargestOfNeighbours<16>(top));
-            float s[kEach];
-#pragma unroll
-            for (int i = 0; i < kEach; i++) {
-                s[i] = Scaled8(u[i], scale.times);
-            }
+            typename BlockScale<kScale>::Stored scale;
+            const Word2 q = QuantiseBlock<kScale>(u, scale);
             if (at < a.padded) {
-                *reinterpret_cast<Word2 *>(static_cast<uint8_t *>(a.out) + row * a.outStride + at) =
-                    Word2{Quantise4(s[0], s[1], s[2], s[3]), Quantise4(s[4], s[5], s[6], s[7])};
+                *reinterpret_cast<Word2 *>(static_cast<uint8_t *>(a.out) + row * a.outStride + at) = q;
                 if (threadIdx.x % 16 == 0) {
-                    static_cast<typename BlockScale<kScale>::Stored *>(a.scales)[row * a.scaleStride + at / 128] = scale.stored;
+                    static_cast<typename BlockScale<kScale>::Stored *>(a.scales)[row * a.scaleStride + at / 128] = scale;
                 }
             }
         }

@@ -88,19 +88,14 @@ __device__ __forceinline__ void LoadGain(const void *gain, bool gain32, int at, 
 }
 
 template <HcclAmdScaleType kScale>
-__device__ __forceinline__ void StoreBlock(const float (&v)[kEach], float top, const NormArgs &a, int64_t row, int at)
+__device__ __forceinline__ void StoreBlock(float (&v)[kEach], const NormArgs &a, int64_t row, int at)
 {
-    const BlockScale<kScale> scale(top);
-    float s[kEach];
-#pragma unroll
-    for (int i = 0; i < kEach; i++) {
-        s[i] = Scaled8(v[i], scale.times);
-    }
+    typename BlockScale<kScale>::Stored scale;
+    const Word2 q = QuantiseBlock<kScale>(v, scale);
     if (at < a.padded) {
-        *reinterpret_cast<Word2 *>(static_cast<uint8_t *>(a.q) + row * a.qStride + at) =
-            Word2{Quantise4(s[0], s[1], s[2], s[3]), Quantise4(s[4], s[5], s[6], s[7])};
+        *reinterpret_cast<Word2 *>(static_cast<uint8_t *>(a.q) + row * a.qStride + at) = q;
         if (threadIdx.x % 16 == 0) {
-            static_cast<typename BlockScale<kScale>::Stored *>(a.scales)[row * a.scaleStride + at / 128] = scale.stored;
+            static_cast<typename BlockScale<kScale>::Stored *>(a.scales)[row * a.scaleStride + at / 128] = scale;
         }
     }
 }
@@ -177,18 +172,15 @@ __global__ void __launch_bounds__(BlockOf(kRowThreads)) NormKernel(NormArgs a)
                 StorePart<kHow, kEach>(static_cast<T *>(a.y) + row * a.yStride, at, a.width, v);
             }
             if constexpr (kEight) {
-                float top = 0.0f;
 #pragma unroll
                 for (int i = 0; i < kEach; i++) {
                     // (behind the row's end a gain of 1 may meet an infinite factor)
                     v[i] = kHow == kAligned ? (at < a.width ? v[i] : 0.0f) : (at + i < a.width ? v[i] : 0.0f);
-                    top = __builtin_fmaxf(top, FiniteSize(v[i]));
                 }
-                top = LargestOfNeighbours<16>(top);
                 if (a.powers) {
-                    StoreBlock<HCCL_AMD_SCALE_E8M0>(v, top, a, row, at);
+                    StoreBlock<HCCL_AMD_SCALE_E8M0>(v, a, row, at);
                 } else {
-                    StoreBlock<HCCL_AMD_SCALE_FP32>(v, top, a, row, at);
+                    StoreBlock<HCCL_AMD_SCALE_FP32>(v, a, row, at);
                 }
             }
         }

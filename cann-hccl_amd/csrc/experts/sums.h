@@ -81,6 +81,32 @@ __device__ __forceinline__ double AddWave(double x)
     return (FromLane(x, 0) + FromLane(x, 16)) + (FromLane(x, 32) + FromLane(x, 48));
 }
 
+// A block of 128 values, eight to each of 16 lanes, in 8 bits, and its scale.  Where all of a wave's are finite, as they mostly are, nothing looks at each of
+// them (four of 28 instructions a value in the gate, whose vector unit is busy most of the time).  Called by whole waves.
+template <HcclAmdScaleType kScale>
+__device__ __forceinline__ Word2 QuantiseBlock(float (&v)[8], typename BlockScale<kScale>::Stored &stored)
+{
+    float top = 0.0f;
+#pragma unroll
+    for (int i = 0; i < 8; i++) {
+        top = __builtin_fmaxf(top, __builtin_fabsf(v[i]));      // (leaves NaN out)
+    }
+    top = LargestOfNeighbours<16>(top);
+    if (__ballot(!(top < __builtin_inff())) != 0) {
+        top = 0.0f;
+#pragma unroll
+        for (int i = 0; i < 8; i++) {
+            top = __builtin_fmaxf(top, FiniteSize(v[i]));
+            v[i] = Scaled8(v[i], 1.0f);
+        }
+        top = LargestOfNeighbours<16>(top);
+    }
+    const BlockScale<kScale> scale(top);
+    stored = scale.stored;
+    return Word2{Quantise4(v[0] * scale.times, v[1] * scale.times, v[2] * scale.times, v[3] * scale.times),
+        Quantise4(v[4] * scale.times, v[5] * scale.times, v[6] * scale.times, v[7] * scale.times)};
+}
+
 // Keeps the compiler from moving LDS operations of one wave's lanes past each other.
 __device__ __forceinline__ void Ordered()
 {

@@ -334,6 +334,23 @@ def test_gate_far_values(stream):
     assert np.isfinite(dh.numpy()[0, :9][[0, 1, 2, 3, 4, 5, 10 - 4]]).all()
 
 
+@pytest.mark.parametrize("kind", [1, 2])
+def test_gate_not_finite_in_8_bits(stream, kind):
+    """Infinities and NaN become the type's NaN in their own place and leave their block's scale alone."""
+    g, u = draw(1, 40, 300), draw(2, 40, 300)
+    u[3, 5], u[3, 290], g[7, 130], u[9], g[11] = float("inf"), float("nan"), float("nan"), float("-inf"), float("inf")
+    h = torch.cat([g, u], 1)
+    ins, q = put(h), Out(40, 384, torch.uint8)
+    scales = Out(40, 3, torch.float32 if kind == 1 else torch.uint8)
+    ready()
+    H.expert_gate(ins.ptr, dt(h.dtype), 40, 300, q.ptr, stream.cuda_stream, scale_type=kind, scales=scales.ptr)
+    stream.synchronize()
+    with np.errstate(all="ignore"):
+        want = ref.gate(f64(g), f64(u))
+    assert (~np.isfinite(want)).sum() >= 600
+    check_eight(q.get().cpu().numpy(), scales.get().cpu().numpy(), kind, want, float(rel_gate(5.0)))
+
+
 def test_gate_in_place(stream):
     h, da = draw(1, 40, 1300, dtype=torch.float16).cuda(), draw(2, 40, 650, dtype=torch.float16).cuda()
     dh, a = torch.empty_like(h), torch.empty_like(da)
