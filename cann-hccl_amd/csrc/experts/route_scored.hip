@@ -344,8 +344,8 @@ __device__ __forceinline__ Steps StepsOf(const ScoredArgs &a, float *part)
 // Whether a group's experts are those of 1, 2, 4 or 8 neighbouring lanes.
 __host__ __device__ constexpr bool Evenly(int size) { return size % 8 == 0 && size <= 64 && (size & (size - 1)) == 0; }
 
-// Takes out what is not in a token's best groups.  Returns false where 32 bits do not settle which these are.  `numbers`: a place per expert, `of`: one per
-// group and 64 more, the token's, in LDS.
+// Takes out what is not in a token's best groups.  Returns false where 32 bits do not settle which these are.  In LDS, the token's own: `numbers`,
+// a place per expert; `of`, 64 places for groups.
 template <int kLanes, int kEach, bool kEvenly>
 __device__ __forceinline__ bool ChooseGroups(const ScoredArgs &a, uint32_t (&number)[kEach], uint32_t slack, int l, uint32_t *numbers, uint32_t *of)
 {
@@ -495,7 +495,8 @@ __device__ __forceinline__ bool Ties(const ScoredArgs &a, const T *row, const ui
             others += !(float(row[at]) == lastLogit && (a.bias == nullptr || a.bias[at] == lastBias)) ? 1 : 0;
         }
     }
-    return pairs == 0 && AddLanes<kLanes>(others) == listed;
+    others = AddLanes<kLanes>(others);
+    return pairs == 0 && others == listed;
 }
 
 // The choice in 32 bits.  Returns false where they do not settle it, on some of the token's lanes.  Of a softmax also the row's largest logit and the sum of
@@ -747,13 +748,12 @@ __global__ void __launch_bounds__(kThreads, kLanes == 64 ? 2 : 4) ScoredKernel(S
         } else {
             w = Sigmoid(logit);
             if (a.renormalise) {
-                // scores below 2^-115 lose bits in 32, their ratios do not: by logarithms there
-                float log = w;
+                // scores below 2^-115 lose bits in 32, their ratios do not: by logarithms there, all of such a token's and no other's
                 const bool far = mine >= 0 && logit < -80.0f;
                 if (__ballot(far) != 0) {
-                    log = mine >= 0 ? LogSigmoid(logit) : -__builtin_inff();
-                    const float top = LargestOfLanes<kHold>(log);
-                    w = Exp(log - top);
+                    const float some = AddLanes<kHold>(far ? 1.0f : 0.0f), log = mine >= 0 ? LogSigmoid(logit) : -__builtin_inff();
+                    const float largest = LargestOfLanes<kHold>(log);
+                    w = some > 0.0f ? Exp(log - largest) : w;
                 }
                 w = mine >= 0 ? w : 0.0f;
                 w /= AddLanes<kHold>(w);
@@ -783,22 +783,16 @@ __global__ void __launch_bounds__(kThreads, kLanes == 64 ? 2 : 4) ScoredKernel(S
             chose[e] = 0;
         }
         __syncthreads();
-        const bool last = a.blocks == 1 && tile + 1 == a.tiles;
-        if (last) {
+        const bool alone = a.blocks == 1;      // (with a single tile, as TilesEach has it)
+        if (alone) {
             // a single workgroup: its places become rows at once
             Finish<kThreads, false>(a, count, nullptr, *routed, parts, nullptr, true);
         }
         if (writes) {
-            a.rowOf[at] = place < 0 ? -1 : place + (last ? count[mine] : 0);
+            a.rowOf[at] = place < 0 ? -1 : place + (alone ? count[mine] : 0);
         }
     }
     if (a.blocks == 1) {
-        for (int i = threadIdx.x; i < (a.tiles - 1) * kTile * a.topK; i += kThreads) {   // the tiles before the last one
-            const int e = a.expertOf[i];
-            if (e >= 0) {
-                a.rowOf[i] += count[e];
-            }
-        }
         return;
     }
     for (int e = threadIdx.x; e < E; e += kThreads) {

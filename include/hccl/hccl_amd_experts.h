@@ -139,7 +139,8 @@ extern HcclResult HcclAmdBlockMatmulGradWeight(const void *yGradT, const void *y
  *   y[rows][yStride]              NULL: not wanted
  *   q[rows][qStride], scales      8-bit rows of y as it is in 32 bits (see above), ceil(width / 128) scales to a row; both NULL with
  *                                 HCCL_AMD_SCALE_NONE
- * epsilon: 0 or more.  width <= HCCL_AMD_MAX_NORM_WIDTH, rows < 2^31. */
+ * epsilon: 0 or more; with 0 the factor of a row whose root mean square is below 2^-127 (zeros, and next to them) is infinite.
+ * width <= HCCL_AMD_MAX_NORM_WIDTH, rows < 2^31. */
 extern HcclResult HcclAmdNormRows(const void *x, HcclDataType type, uint64_t rows, uint64_t width, uint64_t xStride, const void *residual,
     uint64_t residualStride, const void *gain, HcclDataType gainType, float epsilon, void *sum, uint64_t sumStride, void *y, uint64_t yStride,
     HcclAmdScaleType scaleType, void *q, uint64_t qStride, void *scales, uint64_t scaleStride, void *stream);

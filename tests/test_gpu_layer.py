@@ -519,6 +519,18 @@ def test_route_nothing_left(stream, kind):
             assert not grad[[0, 1, 2, 11]].any()
 
 
+@pytest.mark.parametrize("topk", [6, 12])
+def test_route_weights_are_a_tokens_own(stream, topk):
+    """Scores near the end of 32 bits in one token change no bit of its neighbours' weights."""
+    x = draw(8, 64, 32, scale=2.0)
+    got, _ = run_route(stream, x, "sigmoid", None, 1, 1, 1, topk, True, 1.0, None)
+    x[5::8] = -100 + x[5::8]
+    apart, _ = run_route(stream, x, "sigmoid", None, 1, 1, 1, topk, True, 1.0, None)
+    others = np.arange(64) % 8 != 5
+    assert np.array_equal(got["weights"][others], apart["weights"][others]) and np.array_equal(got["expert"][others], apart["expert"][others])
+    check_route(x, "sigmoid", None, 1, 1, 1, topk, True, 1.0, None, None, apart, None)
+
+
 def test_route_strides_and_shared_words(stream):
     for dtype, stride, shift in (("bf16", 72, 0), ("bf16", 67, 1), ("fp32", 65, 1), ("fp16", 64, 8)):
         x = draw(9, 50, 64, dtype=TYPE[dtype])
