@@ -696,6 +696,7 @@ __global__ void __launch_bounds__(kThreads, kLanes == 64 ? 2 : 4) ScoredKernel(S
     __shared__ __align__(16) float part[kLanes * kEach];
     const Steps steps = StepsOf<kLanes * kEach>(a, part);
     __syncthreads();
+    int rank = -1, taken = -1;      // the last tile's
     for (int tile = 0; tile < a.tiles; tile++) {
         a.topK = AnewForAll(args.topK);
         const int lane = Anew(int(threadIdx.x) % 64), l = lane % kLanes, r = wave * kWaveTokens + lane / kLanes;
@@ -720,11 +721,11 @@ __global__ void __launch_bounds__(kThreads, kLanes == 64 ? 2 : 4) ScoredKernel(S
         unsigned long long unsure = __ballot(in && !sure);
         while (unsure != 0) {
             const int which = (__ffsll(unsure) - 1) / kLanes, whose = (int(blockIdx.x) * a.tiles + tile) * kTile + wave * kWaveTokens + which;
-            const int taken = ChooseExactly<kLanes * kEach / 64, T>(ExactArgs{a.bias, a.experts, a.topK, a.groups, a.kept, a.size, a.perSize, a.softmax, a.second},
+            const int best = ChooseExactly<kLanes * kEach / 64, T>(ExactArgs{a.bias, a.experts, a.topK, a.groups, a.kept, a.size, a.perSize, a.softmax, a.second},
                 static_cast<const T *>(a.logits) + int64_t(whose) * a.stride, keys[wave], groupKeys[wave]);
 #pragma unroll
             for (int i = 0; i < K; i++) {
-                const int exactly = __builtin_amdgcn_readlane(taken, i);
+                const int exactly = __builtin_amdgcn_readlane(best, i);
                 chosen[i] = lane / kLanes == which ? exactly : chosen[i];
             }
             unsure &= ~(kLanes == 64 ? ~0ull : ((1ull << kLanes % 64) - 1) << which * kLanes);
@@ -783,16 +784,19 @@ __global__ void __launch_bounds__(kThreads, kLanes == 64 ? 2 : 4) ScoredKernel(S
             chose[e] = 0;
         }
         __syncthreads();
-        const bool alone = a.blocks == 1;      // (with a single tile, as TilesEach has it)
-        if (alone) {
-            // a single workgroup: its places become rows at once
-            Finish<kThreads, false>(a, count, nullptr, *routed, parts, nullptr, true);
-        }
         if (writes) {
-            a.rowOf[at] = place < 0 ? -1 : place + (alone ? count[mine] : 0);
+            a.rowOf[at] = place;
         }
+        rank = writes ? place : -1;
+        taken = mine;
     }
     if (a.blocks == 1) {
+        // a single workgroup, which has a single tile: its places become rows at once
+        Finish<kThreads, false>(a, count, nullptr, *routed, parts, nullptr, true);
+        if (rank >= 0) {
+            const int lane = int(threadIdx.x) % 64;
+            a.rowOf[(wave * kWaveTokens + lane / kLanes) * a.topK + lane % kLanes] = rank + count[taken];
+        }
         return;
     }
     for (int e = threadIdx.x; e < E; e += kThreads) {
