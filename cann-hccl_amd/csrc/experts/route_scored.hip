@@ -198,7 +198,9 @@ __device__ __forceinline__ float Sigmoid(float x) { return __builtin_amdgcn_rcpf
 //   s (U + 2 U)                 the sum and the reciprocal
 // which is 4 U, 1 step at most: two numbers are off against each other by twice 2.75.  A softmax's power, quotient and product are off by 5 U, and its sum, of 32 to a
 // lane over 8 lanes or 16 over 64, by 50 U, the same for all of a token's: 60 U, 15 steps between two of them, and 3.5 for the rest.
-// (What 64 bits would change is within these, cut off to whole numbers; sums of two are off by twice as much.)
+// (What 64 bits would change is within these, cut off to whole numbers; sums of two are off by twice as much.)  Two numbers further apart than that are of scores that
+// are a step and a half apart at least.  In 64 bits a score next to a bias b loses up to 2^-53 |b|, which the difference of biases here does not: from |b| = 2^24
+// times the biases' range on, a 128th of a step, nothing is settled here, since equal large biases make scores equal there that are not here.
 constexpr uint32_t kSlackSigmoid = 5, kSlackSoftmax = 18;
 
 // DPP of the other lane of a pair, the other pair of four, the other four of eight, the other eight of sixteen (mirrored, where the lanes of each
@@ -311,7 +313,7 @@ __device__ __forceinline__ void MergeTwo(uint32_t &first, uint32_t &next)
 struct Steps {
     float times;
     uint32_t slack;      // two numbers this close or closer need not be in their order
-    bool fine;           // false: a bias is infinite, everything is chosen in 64 bits
+    bool fine;           // false: a bias is infinite or too large, everything is chosen in 64 bits
 };
 
 // The part of the numbers that the biases make, -inf where the bias is -inf or NaN, into LDS.  Called by all waves, which find out the same.
@@ -330,7 +332,8 @@ __device__ __forceinline__ Steps StepsOf(const ScoredArgs &a, float *part)
         }
         most = LargestOfLanes<64>(most);
         least = -LargestOfLanes<64>(-least);
-        s.fine = __ballot(infinite) == 0 && most - least < __builtin_inff();
+        const float size = __builtin_fmaxf(__builtin_fabsf(most), __builtin_fabsf(least)), range = most - least;
+        s.fine = __ballot(infinite) == 0 && range < __builtin_inff() && !(least <= most && size > 0x1p24f * (1.0f + range));
     }
     least = least <= most ? least : 0.0f;
     s.times = s.times / (1.0f + (most > least ? most - least : 0.0f));
