@@ -45,7 +45,8 @@ constexpr double kNever = -__builtin_inf();
 
 // No instruction.  The compiler forgets what it knows of a lane's number, and works out what follows from it where it is needed instead of keeping
 // it in registers over all tiles (64 of them and more): 43.0 us instead of 46.2 for 65536 tokens.
-__device__ __forceinline__ int Anew(int lane)
+template <typename V>
+__device__ __forceinline__ V Anew(V lane)
 {
     asm volatile("" : "+v"(lane));
     return lane;
@@ -185,9 +186,7 @@ __device__ __attribute__((noinline)) int ChooseExactly(ExactArgs a, const T *row
     return taken;
 }
 
-// log of the sigmoid
-__device__ __forceinline__ float LogSigmoid(float x) { return fminf(x, 0.0f) - log1pf(Exp(-__builtin_fabsf(x))); }
-
+// For the choice in 32 bits, which knows what it is off by.
 __device__ __forceinline__ float Sigmoid(float x) { return __builtin_amdgcn_rcpf(1.0f + Exp(-x)); }
 
 // ---- the choice in 32 bits --------------------------------------------------------------------------------
@@ -246,6 +245,28 @@ template <int kLanes>
 __device__ __forceinline__ float LargestOfLanes(float v)
 {
     return OverLanes<kLanes>(v, [](float a, float b) { return Larger(a, b); });
+}
+
+// For weights and gradients: t = 1 / (1 + exp(-|x|)) and exp(-|x|) t, the sigmoids of |x| and -|x|.
+struct Sigmoids {
+    float large, small;
+    __device__ __forceinline__ explicit Sigmoids(float x)
+    {
+        const float e = Power(-__builtin_fabsf(x), 0.0f);
+        large = 1.0f / (1.0f + e);
+        small = e * large;
+    }
+};
+
+// A lane's share of its token's chosen scores, all of the token's by one factor, which is such that the largest is neither 0 nor infinite however small
+// the scores are: with m the largest chosen logit exp(x - m), of a sigmoid exp(min(x, 0) - min(m, 0)) / (1 + exp(-|x|)).  0 where nothing is `chosen`.
+template <int kLanes>
+__device__ __forceinline__ float Share(float logit, bool chosen, bool softmax)
+{
+    const float x = softmax ? logit : __builtin_fminf(logit, 0.0f);
+    const Difference d(x, LargestOfLanes<kLanes>(chosen ? x : -__builtin_inff()));
+    const float s = Power(d.high, d.low);
+    return chosen ? softmax ? s : s * Sigmoids(logit).large : 0.0f;
 }
 
 __device__ __forceinline__ uint32_t Max(uint32_t a, uint32_t b) { return a > b ? a : b; }
@@ -531,16 +552,30 @@ __device__ __forceinline__ bool ChooseFast(const ScoredArgs &a, const Steps &ste
             bad = bad || !(x[i] < __builtin_inff());
         }
         top = OverLanes<kLanes>(largest, [](float u, float v) { return __builtin_fmaxf(u, v); });
-        sum = 0.0f;
+        // (+inf takes all, a NaN is left out)
+        float sums[4] = {};
+        if (a.renormalise) {
+#pragma unroll
+            for (int i = 0; i < kEach; i++) {
+                s[i] = Exp(x[i] == top ? 0.0f : x[i] - top);
+            }
+        } else {
+            // (their sum divides the weights: powers that lose nothing of their arguments; where the largest is infinite, NaN, which says nothing then: -inf
+            // leaves no choice, with +inf the weights are NaN and 64 bits choose)
+            const float most = Anew(top);      // (the differences are not worked out in front of both branches, where registers would have to hold them)
+#pragma unroll
+            for (int i = 0; i < kEach; i++) {
+                const Difference d(x[i], most);
+                s[i] = Power(d.high, d.low);
+            }
+        }
 #pragma unroll
         for (int i = 0; i < kEach; i++) {
-            // (+inf takes all, a NaN is left out)
-            s[i] = Exp(x[i] == top ? 0.0f : x[i] - top);
             s[i] = x[i] <= top ? s[i] : 0.0f;
-            sum += s[i];
+            sums[i % 4] += s[i];
             s[i] = __builtin_fmaf(x[i], 0.0f, s[i]);
         }
-        sum = AddLanes<kLanes>(sum);
+        sum = AddLanes<kLanes>((sums[0] + sums[1]) + (sums[2] + sums[3]));
         const float by = steps.times / sum;
         sum = AddLanes<kLanes>(bad ? 1.0f : 0.0f) > 0.0f ? __builtin_nanf("") : sum;
 #pragma unroll
@@ -742,27 +777,18 @@ __global__ void __launch_bounds__(kThreads, kLanes == 64 ? 2 : 4) ScoredKernel(S
         const float logit = mine >= 0 ? float(row[mine]) : -__builtin_inff();
         float w;
         constexpr int kHold = kLanes < 16 ? kLanes : 16;      // lanes that hold choices
-        if (a.softmax) {
-            const float topChosen = LargestOfLanes<kHold>(logit);
-            w = mine >= 0 ? Exp(logit - (a.renormalise ? topChosen : top)) : 0.0f;
-            const float inside = AddLanes<kHold>(w);
-            w /= a.renormalise ? inside : total;
-            // (a NaN or +inf in the row: the weights are NaN, chosen or not by these)
-            w = total > 0.0f ? w : __builtin_nanf("");
+        if (a.renormalise) {
+            w = Share<kHold>(logit, mine >= 0, a.softmax);
+            w /= AddLanes<kHold>(w);
+        } else if (a.softmax) {
+            const Difference d(logit, top);
+            w = Power(d.high, d.low) / total;
         } else {
-            w = Sigmoid(logit);
-            if (a.renormalise) {
-                // scores below 2^-115 lose bits in 32, their ratios do not: by logarithms there, all of such a token's and no other's
-                const bool far = mine >= 0 && logit < -80.0f;
-                if (__ballot(far) != 0) {
-                    const float some = AddLanes<kHold>(far ? 1.0f : 0.0f), log = mine >= 0 ? LogSigmoid(logit) : -__builtin_inff();
-                    const float largest = LargestOfLanes<kHold>(log);
-                    w = some > 0.0f ? Exp(log - largest) : w;
-                }
-                w = mine >= 0 ? w : 0.0f;
-                w /= AddLanes<kHold>(w);
-            }
+            const Sigmoids s(logit);
+            w = logit < 0.0f ? s.small : s.large;
         }
+        // (a NaN or +inf in a softmax's row: the weights are NaN, chosen or not by these)
+        w = !a.softmax || total > 0.0f ? w : __builtin_nanf("");
         if (mine >= 0 && l == 0) {
             atomicAdd(routed, 1);   // a whole number: the order does not matter
         }
@@ -859,11 +885,13 @@ __global__ void __launch_bounds__(kThreads) ScoredGradKernel(ScoredGradArgs a)
             top = LargestOfNeighbours<kLanes>(top);
 #pragma unroll
             for (int i = 0; i < kEach; i++) {
-                x[i] = Exp(x[i] - top);
+                const Difference d(x[i], top);
+                x[i] = Power(d.high, d.low);
                 sum += x[i];
             }
             const float by = 1.0f / AddNeighbours<kLanes>(sum);
-            more = chosen >= 0 ? Exp(logit - top) * by * dw : 0.0f;
+            const Difference d(logit, top);
+            more = chosen >= 0 ? Power(d.high, d.low) * by * dw : 0.0f;
             const float dot = AddNeighbours<kLanes>(more);
 #pragma unroll
             for (int c = 0; c < kEach / 8; c++) {
@@ -877,19 +905,16 @@ __global__ void __launch_bounds__(kThreads) ScoredGradKernel(ScoredGradArgs a)
                 mine[chosen] += more;
             }
         } else {
+            // (what crosses lanes stands outside of what only some of them do; 1 - s is the sigmoid of -x)
+            const Sigmoids of(logit);
             if (a.renormalise) {
-                const float key = chosen < 0 ? -__builtin_inff() : a.softmax ? logit : LogSigmoid(logit);
-                const float top = LargestOfNeighbours<16>(key);      // (what crosses lanes stands outside of what only some of them do)
-                float w = chosen >= 0 ? Exp(key - top) : 0.0f;
-                const float sum = AddNeighbours<16>(w);
-                w = chosen >= 0 ? w / sum : 0.0f;
-                const float mean = AddNeighbours<16>(w * dw);
+                const float share = Share<16>(logit, chosen >= 0, a.softmax), w = share / AddNeighbours<16>(share);
+                const float mean = AddNeighbours<16>(chosen >= 0 ? w * dw : 0.0f);
                 more = w * (dw - mean);
+                more = a.softmax ? more : more * (logit < 0.0f ? of.large : of.small);
             } else {
-                more = Sigmoid(logit) * dw;
+                more = of.large * of.small * dw;
             }
-            // (1 - s is the sigmoid of -x)
-            more = a.softmax ? more : more * Sigmoid(-logit);
             if (chosen >= 0) {
                 mine[chosen] = more;
             }

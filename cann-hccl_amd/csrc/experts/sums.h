@@ -107,6 +107,27 @@ __device__ __forceinline__ Word2 QuantiseBlock(float (&v)[8], typename BlockScal
         Quantise4(v[4] * scale.times, v[5] * scale.times, v[6] * scale.times, v[7] * scale.times)};
 }
 
+// a - b in two parts: what rounding takes from the first is the second.
+struct Difference {
+    float high, low;
+    __device__ __forceinline__ Difference(float a, float b) : high(a - b), low(0.0f)
+    {
+        const float back = high - a;
+        low = (a - (high - back)) - (b + back);
+    }
+};
+
+// exp(x + more) for x <= 0, `more` being what rounding took from x: good to two units in the last place where it is 2^-126 or more, 0 below.  What rounding the
+// power's argument loses (2^-24 of it, 29 units at x = -40) comes back with the power, which is the hardware's.  A NaN stays; -inf needs no `more`.
+__device__ __forceinline__ float Power(float x, float more)
+{
+    more = x < -10000.0f ? 0.0f : more;
+    x = x < -10000.0f ? -10000.0f : x;
+    const float t = x * 0x1.715476p+0f, p = __builtin_amdgcn_exp2f(t);
+    const float lost = __builtin_fmaf(x, 0x1.4ae0cp-26f, __builtin_fmaf(x, 0x1.715476p+0f, -t));      // log2(e) in two parts
+    return __builtin_fmaf(p, __builtin_fmaf(lost, 0x1.62e43p-1f, more), p);
+}
+
 // Keeps the compiler from moving LDS operations of one wave's lanes past each other.
 __device__ __forceinline__ void Ordered()
 {

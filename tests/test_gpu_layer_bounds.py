@@ -38,3 +38,41 @@ def test_route_large_biases(stream, kind, groups, kept, experts, size):
             r = ref.route_many(f64(x), kind, bias.astype(np.float64), groups, kept, top, 6, True, 1.0)
             for k in ("expert", "row_of"):
                 assert np.array_equal(got[k], r[k]), (k, int((got[k] != r[k]).any(1).sum()))
+
+
+def few_left(seed, tokens, experts, dtype):
+    """Eight logits of each token between -80 and 0, -inf at its other experts."""
+    rng = np.random.default_rng(seed)
+    at = np.argsort(rng.random((tokens, experts)), axis=1)[:, :8]
+    x = np.full((tokens, experts), -np.inf, np.float32)
+    np.put_along_axis(x, at, rng.uniform(-80, 0, (tokens, 8)).astype(np.float32), 1)
+    return torch.from_numpy(x).to(dtype)
+
+
+@pytest.mark.parametrize("tokens,experts", [(300, 8), (4200, 64), (300, 100), (4200, 128), (4200, 256), (300, 256), (300, 600)])
+@pytest.mark.parametrize("dtype", ["fp32", "bf16"])
+@pytest.mark.parametrize("kind", ["sigmoid", "softmax"])
+@pytest.mark.parametrize("renorm", [False, True])
+def test_route_weights_of_small_scores(stream, tokens, experts, dtype, kind, renorm):
+    """Weights and gradients are as exact for scores of 1e-30 as for those next to 1.
+
+    A power is within 3 U: its argument loses nothing, the hardware's power 2 U, the product of the two one more.  With e = exp(-|x|), 1 / (1 + e) is within 3.5 U (half
+    of e's, sum, quotient) and e / (1 + e) within 6 (e's, sum, quotient, product).
+      weights    sigmoid 6;  renormalised: a share is a power times 1 / (1 + e), 7.5, four sums on top for eight of them, the quotient: 20
+                 softmax: the power's 3, the sum's 3 + 13 (eight to each of four sums of a lane, then 2 and 3 levels; 16 to 64 lanes 4 + 2 + 6), the quotient: 20
+                 renormalised: 3 for the share, 7 for the sum, 1: 11;  all of them one more for the scale
+      gradients, of their magnitudes
+                 sigmoid: 6 + 3.5, two products, the scale: 12.5
+                 softmax: power 3, inverse of the sum 3 + 16 + 6 + 1, product: 30; times a sum over the chosen, 32 and 6, and product: 69, sum 70, scale 71
+                 renormalised, with w's 20 (sigmoid) or 11: the mean w's and 5, the difference and two products 3, 1 - s 7, scale: 56 and 31"""
+    x = few_left(experts + tokens, tokens, experts, TYPE[dtype])
+    dw = np.random.default_rng(1).standard_normal((tokens, 8)).astype(np.float32)
+    got, grad = run_route(stream, x, kind, None, 1, 1, 1, 8, renorm, 1.5, None, dw)
+    r = ref.route_many(f64(x), kind, None, 1, 1, 1, 8, renorm, 1.5)
+    assert np.array_equal(got["expert"], r["expert"])
+    weights = {("sigmoid", False): 7, ("sigmoid", True): 21, ("softmax", False): 21, ("softmax", True): 12}[kind, renorm]
+    assert near(got["weights"], r["weights"], weights * U * r["weights"] + 2.0 ** -126)
+    some = slice(0, 300)
+    want, size = ref.route_grad(f64(x)[some], {k: r[k][some] for k in ("expert", "weights", "scores")}, kind, 8, renorm, 1.5, dw[some])
+    rel = {("sigmoid", False): 12.5, ("sigmoid", True): 56, ("softmax", False): 71, ("softmax", True): 31}[kind, renorm]
+    assert near(grad[some], want, rel * U * size + 2.0 ** -120, x.dtype)
