@@ -197,7 +197,9 @@ extern HcclResult HcclAmdExpertRouteScored(const void *logits, HcclDataType logi
 
 /* Gradient of the logits from weightGrad[tokens][topK]; expertOf as HcclAmdExpertRouteScored left it.  Every logit's gradient is written; those of
  * tokens that chose nothing are zero, and so are, but for a softmax that is not renormalised, those of experts that were not chosen.  (The bias
- * only chooses: it has no gradient.) */
+ * only chooses: it has no gradient.)  A NaN or +inf logit makes all gradients of its token NaN in a softmax that is not renormalised.  In one that is, only
+ * the chosen logits are read: +inf among them makes their gradients NaN, and of a NaN or +inf among the others, which made the weights NaN, the gradients
+ * have what weightGrad has. */
 extern HcclResult HcclAmdExpertRouteScoredGrad(const void *logits, HcclDataType logitType, uint64_t tokens, uint32_t experts, uint64_t logitStride,
     HcclAmdScore score, uint32_t topK, uint32_t renormalise, float weightScale, const int32_t *expertOf, const float *weightGrad, void *logitGrad,
     uint64_t logitGradStride, void *stream);

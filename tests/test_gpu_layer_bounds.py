@@ -76,3 +76,34 @@ def test_route_weights_of_small_scores(stream, tokens, experts, dtype, kind, ren
     want, size = ref.route_grad(f64(x)[some], {k: r[k][some] for k in ("expert", "weights", "scores")}, kind, 8, renorm, 1.5, dw[some])
     rel = {("sigmoid", False): 12.5, ("sigmoid", True): 56, ("softmax", False): 71, ("softmax", True): 31}[kind, renorm]
     assert near(grad[some], want, rel * U * size + 2.0 ** -120, x.dtype)
+
+
+@pytest.mark.parametrize("tokens,experts", [(40, 24), (4200, 24), (40, 200), (40, 300)])
+@pytest.mark.parametrize("kind", ["sigmoid", "softmax"])
+@pytest.mark.parametrize("renorm", [False, True])
+def test_route_grad_of_tokens_that_are_not_finite(stream, tokens, experts, kind, renorm):
+    """NaN and +inf, chosen and not: what their tokens' gradients are, and that the other tokens' are as ever."""
+    inf, nan = float("inf"), float("nan")
+    x, bias = draw(4, tokens, experts), np.zeros(experts, np.float32)
+    bias[7] = -np.inf                                      # never chosen
+    x[3, 5], x[5, 5], x[9, 7], x[11, 5], x[11, 6] = nan, inf, inf, inf, inf
+    dw = np.random.default_rng(1).standard_normal((tokens, 4)).astype(np.float32)
+    got, grad = run_route(stream, x, kind, bias, 1, 1, 1, 4, renorm, 1.5, None, dw)
+    y = f64(x)
+    r = ref.route(y, kind, bias, 1, 1, 1, 4, renorm, 1.5, None)
+    assert np.array_equal(got["expert"], r["expert"]) and (r["expert"] >= 0).all()
+    assert np.array_equal(np.isnan(got["weights"]), np.isnan(r["weights"]))
+    if kind == "softmax":
+        assert np.isnan(r["weights"]).all(1).nonzero()[0].tolist() == [3, 5, 9, 11]
+    if kind == "softmax" and renorm:
+        chosen = np.take_along_axis(y, r["expert"].astype(np.int64), 1)
+        with np.errstate(invalid="ignore"):
+            w = np.exp(chosen - chosen.max(1, keepdims=True))
+        r["weights"] = 1.5 * w / w.sum(1, keepdims=True)   # without the others
+    want, size = ref.route_grad(y, r, kind, 4, renorm, 1.5, dw)
+    if kind == "softmax" and not renorm:
+        want[[3, 5, 9, 11]] = np.nan
+    nans = {("softmax", False): 4 * experts, ("softmax", True): 8}.get((kind, renorm), 0)
+    assert np.isnan(want).sum() == nans and np.array_equal(np.isnan(grad), np.isnan(want))
+    # (the bound of the test above, for the largest of its forms)
+    assert near(grad, want, 71 * U * np.nan_to_num(size) + 2.0 ** -120)
