@@ -118,7 +118,7 @@ struct Difference {
 };
 
 // exp(x + more) for x <= 0, `more` being what rounding took from x: good to two units in the last place where it is 2^-126 or more, 0 below.  What rounding the
-// power's argument loses (2^-24 of it, 29 units at x = -40) comes back with the power, which is the hardware's.  A NaN stays; -inf needs no `more`.
+// power's argument loses (up to 2^-24 of it: 22 * 2^-24 of the power at x = -40) comes back with the power, which is the hardware's.  A NaN stays; -inf needs no `more`.
 __device__ __forceinline__ float Power(float x, float more)
 {
     more = x < -10000.0f ? 0.0f : more;

@@ -9,7 +9,8 @@ import torch
 import layer_reference as ref
 from experts_reference import U
 from hccl_loader import load
-from test_gpu_layer import TYPE, draw, f64, near, run_route
+from test_gpu_experts import Out, dt
+from test_gpu_layer import TYPE, draw, f64, near, put, ready, run_route
 
 pytestmark = pytest.mark.gpu
 H = load()
@@ -107,3 +108,52 @@ def test_route_grad_of_tokens_that_are_not_finite(stream, tokens, experts, kind,
     assert np.isnan(want).sum() == nans and np.array_equal(np.isnan(grad), np.isnan(want))
     # (the bound of the test above, for the largest of its forms)
     assert near(grad, want, 71 * U * np.nan_to_num(size) + 2.0 ** -120)
+
+
+# ---- gate ---------------------------------------------------------------------------------------------------------------------
+
+def run_gate(stream, g, u, da):
+    """a, a once more, dh, all in 32 bits."""
+    rows, width = g.shape
+    ins, das = put(torch.cat([g, u], 1)), put(da)
+    a, again, dh = Out(rows, width, torch.float32), Out(rows, width, torch.float32), Out(rows, 2 * width, torch.float32)
+    ready()
+    H.expert_gate(ins.ptr, dt(g.dtype), rows, width, a.ptr, stream.cuda_stream)
+    H.expert_gate_grad(das.ptr, ins.ptr, dt(g.dtype), rows, width, dh.ptr, stream.cuda_stream, out=again.ptr)
+    stream.synchronize()
+    return a.numpy(), again.numpy(), dh.numpy()[:, :width], dh.numpy()[:, width:]
+
+
+@pytest.mark.parametrize("low,high", [(-1, 1), (-10, 0), (0, 8), (8, 17), (17, 60), (-40, -10), (-87, -40), (-110, -87)])
+@pytest.mark.parametrize("width", [512, 501])
+def test_gate_is_as_exact_everywhere(stream, low, high, width):
+    """With E = exp(-g), t = 1 / (1 + E): the power 2 U, its factor 1, the sum 1, the reciprocal 2, t 6 in all.  a and du have two products more.  1 - t is E t where g > 0 (3 for E,
+    a product, 6 for t, a product: 11), else 7; 1 + g (1 - t) multiplies that by g (one more), and the sum, t's 6 and three products are 10."""
+    g = torch.rand(200, width, generator=torch.Generator().manual_seed(low + 200)) * (high - low) + low
+    u, da = draw(1, 200, width), draw(2, 200, width)
+    a, again, dg, du = run_gate(stream, g, u, da)
+    g, u, da = f64(g), f64(u), f64(da)
+    want_g, want_u, size_g, size_u = ref.gate_grad(da, g, u)
+    least = 2.0 ** -125 * (1 + np.abs(g)) * (1 + np.abs(u)) * (1 + np.abs(da))      # what a sigmoid below 2^-126 that is 0 makes
+    assert near(a, ref.gate(g, u), 8 * U * np.abs(ref.gate(g, u)) + least) and np.array_equal(a, again)
+    assert near(du, want_u, 8 * U * size_u + least)
+    part = np.abs(g) * ref.sigmoid(-g)
+    assert near(dg, want_g, (10 + 12 * part / (1 + part)) * U * size_g + least)
+
+
+def test_gate_far_and_not_finite(stream):
+    """Gates beyond the power's range, infinities and NaN: results and both gradients are the formula's, as it comes out in 64 bits and is rounded to 32."""
+    inf, nan = float("inf"), float("nan")
+    g = torch.tensor([[0.0, -0.0, 90.0, -90.0, 200.0, -200.0, 3e38, -3e38, inf, -inf, nan, 1e-30, -1e-30, 1e5, -1e5, 1.0, 1.0, 1.0, 0.0, 0.0]])
+    u = torch.full_like(g, 2.0)
+    u[0, 15:] = torch.tensor([inf, -inf, nan, inf, nan])
+    a, again, dg, du = run_gate(stream, g, u, torch.ones_like(g))
+    with np.errstate(all="ignore"):
+        want = ref.gate(f64(g), f64(u))
+        want_g, want_u, _, _ = ref.gate_grad(np.ones(g.shape), f64(g), f64(u))
+        # in 64 bits t is not 0 at -200, and its product with 3e38 no infinity
+        for got, w in ((a, want), (again, want), (dg, want_g), (du, want_u)):
+            w = w.astype(np.float32).astype(np.float64)
+            assert np.array_equal(np.isnan(got), np.isnan(w)) and np.array_equal(np.isposinf(got), np.isposinf(w)) and np.array_equal(np.isneginf(got), np.isneginf(w))
+            fine = np.isfinite(w)
+            assert near(got[fine], w[fine], 22 * U * np.abs(w[fine]) + 2.0 ** -117)
