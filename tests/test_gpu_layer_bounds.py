@@ -10,7 +10,7 @@ import layer_reference as ref
 from experts_reference import U
 from hccl_loader import load
 from test_gpu_experts import Out, dt
-from test_gpu_layer import TYPE, draw, f64, near, put, ready, run_route
+from test_gpu_layer import TYPE, draw, f64, grad_norm, near, put, ready, run_route
 
 pytestmark = pytest.mark.gpu
 H = load()
@@ -157,3 +157,22 @@ def test_gate_far_and_not_finite(stream):
             assert np.array_equal(np.isnan(got), np.isnan(w)) and np.array_equal(np.isposinf(got), np.isposinf(w)) and np.array_equal(np.isneginf(got), np.isneginf(w))
             fine = np.isfinite(w)
             assert near(got[fine], w[fine], 22 * U * np.abs(w[fine]) + 2.0 ** -117)
+
+
+# ---- norm ---------------------------------------------------------------------------------------------------------------------
+
+@pytest.mark.parametrize("rows,width", [(20000, 64), (40000, 512), (20000, 1000), (10000, 2001), (8000, 4096), (6000, 8192), (3000, 16384), (1200, 32767)])
+@pytest.mark.parametrize("start", [False, True])
+def test_gain_gradient_of_many_rows(stream, rows, width, start):
+    """Terms of one sign, where every sum's rounding shows.  A term has the roundings of the row's factor and of two products, a workgroup's sum one, the result one: 5 U, and
+    beyond 8192 columns one for each row of a workgroup, of which there are 256.  As a whole the terms' roundings, thousands that are independent, leave little, and the workgroups'
+    as much: the result's own, 3^-1/2 U on average, has to be most of it."""
+    s, dy = draw(1, rows, width).abs(), draw(2, rows, width).abs()
+    before = draw(3, width).abs() if start else None
+    _, dgain = grad_norm(stream, dy, s, None, 1e-6, None, want_dx=False, start=before)
+    v = s.cuda().double()
+    n = v * (v.square().mean(1, keepdim=True) + float(np.float32(1e-6))).rsqrt()
+    want = (dy.cuda().double() * n).sum(0).cpu().numpy() + (f64(before) if start else 0)
+    off = np.abs(dgain.numpy()[0] - want) / want
+    assert off.max() <= (5 + (-(-rows // 256) if width > 8192 else 0)) * U
+    assert (off ** 2).mean() ** 0.5 <= U
