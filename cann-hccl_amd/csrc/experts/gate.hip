@@ -3,7 +3,7 @@
 // With t = 1 / (1 + exp(-g)):   a = g t u      dg = da u t (1 + g (1 - t))      du = da g t
 //
 // A wave takes a row's piece of 512 values, eight neighbouring ones to a lane: 16 lanes hold a block of an 8-bit row.  Every value is read once and
-// written once, and bytes moved bound both kernels: 65536 rows of 2048 values to 8 bits (0.67 GB) 115 us, 5.9 TB/s, where a large copy reaches 5.15; 14769 rows of
+// written once, and bytes moved bound both kernels: 65536 rows of 2048 values to 8 bits (0.67 GB) 113 us, 5.9 TB/s, where a large copy reaches 5.15; 14769 rows of
 // 4095, off every boundary, 70 us (4.3 TB/s), their gradient 127 us (5.7 TB/s).
 #include <type_traits>
 

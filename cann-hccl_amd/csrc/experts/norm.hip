@@ -3,14 +3,19 @@
 // With r = (mean s^2 + epsilon)^-1/2, d = dy * gain and n = s r:
 //   y = n * gain      dx = r (d - n mean(d n)) + dsum      dgain = sum over rows of dy * n
 //
-// A row stays in registers between its sums and its results: read once, written once.  64 to 1024 threads to a row, each with eight neighbouring values (16 or 32
-// beyond 8192), so that a lane's accesses are 16 bytes and 16 lanes hold a block of an 8-bit row.  Sums are in 64 bits: a
-// square of 32 bits is exact there, and no row overflows.
+// Up to 8192 columns a row stays in registers between its sums and its results: read once, written once.  64 to 1024 threads to a row, each with eight neighbouring
+// values (16 or 32 beyond 8192), so that a lane's accesses are 16 bytes and 16 lanes hold a block of an 8-bit row.  Sums are in 64 bits: a square of 32 bits is
+// exact there, and no row overflows.
 //
 // Bytes moved bound them, where a large copy reaches 5.15 TB/s: 16384 rows of 8192 values with residual and sum (1.07 GB) 177 us, 6.0 TB/s, their gradient
-// (1.07 GB) 202 us, 5.3 TB/s, and 5 us to add up the gain's.  8192 rows of 4096 to 8 bits (0.24 GB) 51 us, 4.6 TB/s.  More values to a thread, fewer
+// (1.07 GB) 199 us, 5.4 TB/s, the 5 us that add up the gain's included.  8192 rows of 4096 to 8 bits (0.24 GB) 50 us, 4.7 TB/s.  More values to a thread, fewer
 // threads to a row were slower: 16 and 512 for rows of 8192 411 us in all instead of 383.  Rows of 2001 values, off every boundary (5003 of them):
-// 13.5 us, 22 and 6; 16384 of them 102 us in all, of 2000 values 84.  One row of 8192: 4 us, the latency of loads, sums and a launch.
+// 13.7 us, 22 and 6; 16384 of them 102 us in all, of 2000 values 84.  One row of 8192: 4 us, the latency of loads, sums and a launch.
+//
+// Where something else bounds them (16 bits, residual and sum): rows that do not fill a wave's 512 columns, which pays for each of them whole: 262144 rows of 128 80 us, 3.4 TB/s, the
+// gradient 133, 2.0, by vector instructions.  And rows that do not fit the registers: forward above 16384 columns (2 to 29 registers to scratch), gradient above 8192 (5 to 11 at 16384
+// and 242 to 358 at 32768, 91 to 991 off boundaries), which then fetches no row ahead either: 2048 rows of 16384 49 us and 78 (5.5 and 3.5 TB/s), of 32768 105 and 381 (5.1 and
+// 1.4), of 16383 61 and 143, of 32767 143 and 610.
 #include <type_traits>
 
 #include "sums.h"
@@ -386,7 +391,8 @@ HcclResult ByType(HcclDataType type, F f)
     return type == HCCL_DATA_TYPE_FP32 ? f(float{}) : type == HCCL_DATA_TYPE_FP16 ? f(_Float16{}) : f(__bf16{});
 }
 
-// Workgroups that go through rows: what makes 16 waves to a compute unit.
+// Workgroups that go through rows: what makes 16 waves to a compute unit, each of which leaves sums of its own.  Twice as many took 126 us for the gradient of 262144 rows of 128
+// (instead of 133), but 50 for 65536 of 512 (47), 64 for 32768 of 1024 (53), 56 for 16384 of 2048 (50), 108 of 4096 (105), 204 of 8192 (198); half as many 157, 51, 61, 59, 130, 350.
 uint64_t GradBlocks(uint64_t rows, uint64_t width)
 {
     const uint64_t each = width <= 512 ? 4 : 1, blocks = (rows + each - 1) / each;

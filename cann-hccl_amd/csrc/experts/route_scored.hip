@@ -13,11 +13,13 @@
 // bias (which tie in any precision).  Of an unsettled token the chosen ones and the next are put in order by their keys in 64 bits; where that does not
 // settle it either -- its groups are too close, or several experts at the border -- a whole wave chooses for it in 64 bits.
 //
-// Measured: 65536 tokens of 256 experts in eight groups, eight chosen, 16-bit logits (33.5 MB): 33 us to choose, 6 to add up, 5 for the rows, 10 for the
-// gradient, 4 for the bias.  Choosing is bound by vector instructions: about 35 for each expert, of which eight are medians and eight what a power and a reciprocal
-// take.  One token in 300 has choices closer than 32 bits hold (3 us of the 33), one in 2000 groups that are (4 us, since the others wait); with
-// everything in 64 bits it took 240 us.  Eight lanes to a token spend fewer instructions on merging than sixteen (43 us against 49 with all launches),
-// sixteen are quicker where there are few tokens.
+// Measured: 65536 tokens of 256 experts in eight groups, eight chosen, 16-bit logits (33.5 MB): 34 us to choose, 6 to add up, 4 for the rows, 10 for the
+// gradient, 2 for the bias.  Choosing spends about 35 vector instructions on each expert, of which eight are medians and eight what a power and a reciprocal take: they
+// keep the vector units busy for 59 % of the time, and waves wait for 40 % of theirs, since a tile's logits are not fetched before the one in front is done.  One token in 300 has choices
+// closer than 32 bits hold (3 us of the 34), one in 2000 groups that are (4 us, since the others wait); with everything in 64 bits it took 240 us, which is also what a finite bias
+// 1e4 away from the others makes of it (64 us for all launches instead of 44 where it is 100 away, 105 at 1000).  Eight lanes to a token spend fewer instructions on merging than
+// sixteen (43 us against 49 with all launches), sixteen are quicker where there are few tokens.  Above 256 experts there is one layout, a wave to a token with 16 experts to a lane, whatever
+// share of them is there: 65536 tokens of 257, 384, 512 and 1024 experts 142, 135, 138 and 168 us with all launches, in eight groups of 40, 48, 64 and 128 231, 245, 167 and 437.
 #include <type_traits>
 
 #include "rows.h"
@@ -961,13 +963,15 @@ __global__ void __launch_bounds__(kThreads) BiasKernel(const int32_t *counts, in
     }
 }
 
-// Lanes to a token.
+// Lanes to a token.  All launches, with eight lanes and with sixteen, 60 experts (fp32, softmax) and 256 (16 bits, sigmoid): 2048 tokens 18.1 and 17.2 us, 18.3 and 17.2; 4097 18.4
+// and 17.5, 20.0 and 19.1; 6500 18.5 and 18.1, 21.7 and 21.9; 8192 18.6 and 18.2, 22.0 and 22.3; 16384 19.6 and 21.6, 24.4 and 26.0; 32768 22.8 and 30.0, 31.1 and 34.1.  (Between 4097 tokens and about 7000
+// sixteen would be up to 5 % quicker.)
 int LanesOf(uint64_t tokens, uint32_t experts, uint32_t topK) { return experts > 256 ? 64 : topK > 8 || tokens <= 4096 ? 16 : 8; }
 
 int TileOf(uint64_t tokens, uint32_t experts, uint32_t topK) { return kThreads / LanesOf(tokens, experts, topK); }
 
 // Tiles to a workgroup: one, until there are as many workgroups as the launches behind take.  (64 tokens by four workgroups and a launch that joins them take
-// 13 us, by one workgroup 18.)
+// 11 us; by one workgroup and no such launch they took 18 when four took 13.)
 int TilesEach(uint64_t tokens, int tile)
 {
     const uint64_t tiles = (tokens + uint64_t(tile) - 1) / uint64_t(tile);

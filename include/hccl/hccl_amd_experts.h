@@ -180,8 +180,9 @@ typedef enum HcclAmdScoreDef {
 /* Chooses topK experts for every token by their scores, s = softmax(logits) over all experts or 1 / (1 + exp(-logits)), and counts them.
  *   logits, tokenMask, expertOf, rowOf, counts, offsets    as in HcclAmdExpertRoute
  *   bias[experts]                 added to the scores for the choice alone, in 64 bits; NULL: none.  -inf or NaN: never chosen, and the way to
- *                                 switch an expert off: biases that are far apart or far from 0 (1e4 and more) are chosen by as
- *                                 well, but take 64 bits for most tokens, which is several times as slow
+ *                                 switch an expert off: finite biases that are far apart (100 and more) do as well, but then more
+ *                                 tokens take 64 bits; all of them where biases are 1e4 apart or 2^24
+ *                                 from 0, which is five times as slow
  *   groups, groupsKept, groupTop  the experts are `groups` groups of as many neighbours each; a token's experts come from its groupsKept best groups,
  *                                 by the sum of a group's groupTop (1 or 2) largest s + bias.  groups = groupsKept = 1: from all of them
  *   weights[tokens][topK]         weightScale * s, with `renormalise` weightScale * s / (sum of the chosen s): without the bias; 0 where expertOf is -1
